@@ -609,6 +609,56 @@ int bgtq_decode_combined_noalloc(const BgtqDecodePlan* plan_host, const BgtqHead
                 const float* v_rot, void* out, int64_t o_sb, int64_t o_sh, float* lse_out,
                 int32_t* status, void* stream);
 
+/* ---- paged 4-bit cache ------------------------------------------------------
+ * A cache without calibration for batches whose sequences have lengths of their own.  No counterpart in the reference (its caches are
+ * contiguous, one length for the batch).  A pool of pages; a page holds page_tokens tokens (a multiple of 16) of every KV head; page p of
+ * head h starts at pages + p * page_stride + h * head_stride BYTES (16-byte aligned) and is page_tokens / 16 units of 2304 bytes:
+ *   [0, 1024)     K codes: token t of the unit, half-word W (0..31) at 64 t + 2 W
+ *   [1024, 2048)  V codes: at 1024 + 128 (t / 2) + 4 W + 2 (t % 2)
+ *   [2048, 2176)  K scales, bf16: token t, group g (0..3) at 2048 + 8 t + 2 g;   [2176, 2304)  V scales
+ * Nibble n of half-word W is the code of dim 32 n + W plus 8; group n is dims 32 n .. 32 n + 31; value = code * scale, exact in fp16.
+ * A token's slot is page * page_tokens + place in the page.
+ * All entry points below launch programmatic dependents that wait on the device before they read or write anything; they may be captured
+ * in a graph.  status (optional device int32): left alone when all is well; 1 a bounded wait ran out (the output is incomplete), 2 a slot
+ * or position outside its range (that row was not stored, or reads as zeros), 4 a page number outside the pool in the table, for a
+ * position below the sequence's length (its tokens were left out). */
+#define BGTQ_PAGED_BF16 1         /* q, k, v and outputs are bf16 instead of fp16 */
+#define BGTQ_PAGED_F32 2          /* bgtq_paged_read: fp32 outputs */
+#define BGTQ_PAGED_CAUSAL 4       /* bgtq_paged_attend with cu_q: query i sees the tokens up to its own position */
+
+/* Quantise and store n_tok tokens.  k / v element (i, h, d) at k + i * k_st + h * k_sh + d (strides multiples of 4 elements, 8-byte
+ * aligned); token i goes to slot slots[i], nowhere when that is negative; the slots of a call are distinct.  rope_cos / rope_sin (may both
+ * be NULL): fp32 tables, row p at + p * rope_st (a multiple of 4), 64 entries; dims d and d + 64 of k, and of q, are turned by row
+ * positions[i] in fp32: x' = x cos - y sin, y' = y cos + x sin, nothing fused, K quantised from the fp32 result.  q (NULL and n_q = 0 to
+ * leave it out; needs the tables): rotated queries, rounded once, to q_out (n_tok, n_q, 128) contiguous.
+ * scale_g = bf16(max |x| of the group / 7) held in [2^-17, 9344]; code = x / scale to the nearest, ties to even, held in [-7, 7].
+ * A NaN makes its group NaN (scale 0x7fff, codes 0); what lies beyond 65408 saturates. */
+int bgtq_paged_append(uint8_t* pages, int64_t page_stride, int64_t head_stride, int32_t n_pages, int32_t page_tokens, const int64_t* slots,
+                const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh,
+                const void* q, int64_t q_st, int64_t q_sh, void* q_out,
+                const float* rope_cos, const float* rope_sin, int64_t rope_st, const int64_t* positions, int32_t n_positions,
+                int32_t n_tok, int32_t n_kv, int32_t n_q, int32_t flags, int32_t* status, void* stream);
+
+/* The values of n_tok slots -> k, v (n_tok, n_kv, 128) contiguous, fp16 (exact), bf16 or fp32; zeros for a negative slot. */
+int bgtq_paged_read(const uint8_t* pages, int64_t page_stride, int64_t head_stride, int32_t n_pages, int32_t page_tokens,
+                const int64_t* slots, int32_t n_tok, int32_t n_kv, void* k, void* v, int32_t flags, int32_t* status, void* stream);
+
+/* Attention of few query rows per sequence over the first seq_lens[b] tokens of each sequence (held to the table's capacity):
+ * token t of sequence b lies in page table[b * table_stride + t / page_tokens].  cu_q NULL: row b of q (n_seq, n_q, 128) is sequence b's
+ * one query, n_tok = n_seq.  Otherwise rows cu_q[b] .. cu_q[b + 1] - 1 of q (n_tok, n_q, 128) are its last positions, and with
+ * BGTQ_PAGED_CAUSAL row i of n sees the first seq_lens[b] - n + 1 + i tokens.  A row that sees none is zeros, its lse -inf; rows
+ * behind cu_q[n_seq] are left as they were.  lse (optional, (n_tok, n_q) fp32): natural logarithm of the sum of exponentials.
+ * n_q / n_kv <= 8.  max_q, max_tokens: no sequence has more rows, more tokens (they size the launch; one that has is still attended
+ * whole).  workspace:
+ * bgtq_paged_workspace_bytes(...) of the same arguments, 16-byte aligned, of no other call that may run at the same time. */
+int64_t bgtq_paged_workspace_bytes(int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv, int32_t max_q,
+                int64_t max_tokens);
+int bgtq_paged_attend(const void* q, int64_t q_st, int64_t q_sh, const uint8_t* pages, int64_t page_stride, int64_t head_stride,
+                int32_t n_pages, int32_t page_tokens, const int32_t* table, int64_t table_stride, int32_t table_cols,
+                const int32_t* seq_lens, const int32_t* cu_q, int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv,
+                int32_t max_q, int64_t max_tokens, float scale, int32_t flags, void* workspace, int64_t workspace_bytes,
+                void* out, int64_t o_st, int64_t o_sh, float* lse, int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,338 @@
+"""GPU: the paged 4-bit cache against plain operations: stored bytes bit for bit, attention against 64 bits within the bound that
+tests/paged_reference.py derives."""
+import math
+
+import pytest
+import torch
+
+import paged_reference as R
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+TYPES = [torch.float16, torch.bfloat16]
+
+
+def _tables(n):
+    angle = torch.arange(n, dtype=torch.float64)[:, None] * 10000.0 ** (-torch.arange(64, dtype=torch.float64) / 64)
+    return angle.cos().float(), angle.sin().float()
+
+
+def _noise(gen, *shape):
+    return torch.randn(*shape, generator=gen)
+
+
+def _case(gen, n_kv, page, lens, spare=2, dtype=torch.float16):
+    """Pages holding sequences of these lengths in shuffled order, everything else in them all ones (codes 7, scales NaN)."""
+    from blockgtq_b200 import page_bytes, paged_kv4_append
+    width = max(1, max(-(-t // page) for t in lens)) + 1
+    n_pages = sum(-(-t // page) for t in lens) + spare
+    order = torch.randperm(n_pages, generator=gen).tolist()
+    table, slots = torch.full((len(lens), width), -7, dtype=torch.int32), []
+    for b, t in enumerate(lens):
+        for i in range(-(-t // page)):
+            table[b, i] = order.pop()
+        slots.append(torch.tensor([int(table[b, i // page]) * page + i % page for i in range(t)], dtype=torch.int64))
+    pages = torch.full((n_pages, n_kv, page_bytes(page)), 255, dtype=torch.uint8, device=DEV)
+    flat = torch.cat(slots)
+    k = _noise(gen, len(flat), n_kv, 128) * torch.exp(_noise(gen, 1, n_kv, 128))
+    v = _noise(gen, len(flat), n_kv, 128) * torch.exp(2 * _noise(gen, len(flat), 1, 1))
+    paged_kv4_append(pages, flat.to(DEV), k.to(dtype).to(DEV), v.to(dtype).to(DEV))
+    return pages, table, slots
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,n_kv,n_q,page,rope", [(1, 1, 1, 16, True), (3, 2, 14, 16, True), (37, 8, 32, 64, True), (64, 3, 3, 48, False), (258, 2, 4, 128, True)])
+def test_append_stores_the_plain_quantisers_bytes(dtype, n, n_kv, n_q, page, rope):
+    from blockgtq_b200 import page_bytes, paged_kv4_append, paged_kv4_read
+    gen = torch.Generator().manual_seed(n)
+    n_pages = -(-n // page) + 2
+    slots = torch.randperm(n_pages * page, generator=gen)[:n]
+    if n == 64:
+        slots = torch.arange(n) + 5                       # neighbours, from an odd one on
+    if n > 2:
+        slots[1] = -1
+    k, v, q = (_noise(gen, n, h, 128).to(dtype) for h in (n_kv, n_kv, n_q))
+    if n > 30:
+        k[2, 0, 32:64] = 0
+        v[3, 0, :32] = 3.5
+        v[3, 0, 5] = 7.0                                  # x / scale = 3.5: a tie, to the even code
+        v[4, n_kv - 1, 7] = math.inf
+        v[5, 0, 40] = math.nan
+        k[6, 0] *= 1e-6
+        k[7, 0] *= 3000
+    cos, sin = _tables(300)
+    positions = torch.randint(0, 300, (n,), generator=gen)
+    background = torch.randint(0, 256, (n_pages, n_kv, page_bytes(page)), generator=gen, dtype=torch.uint8)
+    want = background.clone()
+    k_in = R.rotated(k, cos, sin, positions) if rope else k.float()
+    for i in range(n):
+        if slots[i] >= 0:
+            R.write(want, int(slots[i]), k_in[i], v[i].float())
+    pages = background.to(DEV)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    extra = dict(q=q.to(DEV), cos=cos.to(DEV), sin=sin.to(DEV), positions=positions.to(DEV)) if rope else {}
+    got_q = paged_kv4_append(pages, slots.to(DEV), k.to(DEV), v.to(DEV), status=status, **extra)
+    assert (pages.cpu() != want).sum() == 0 and status.item() == 0
+    if rope:
+        assert torch.equal(got_q.cpu(), R.rotated(q, cos, sin, positions).to(dtype))
+    else:
+        assert got_q is None
+    for t in (torch.float16, torch.float32, torch.bfloat16):
+        gk, gv = paged_kv4_read(pages, slots.to(DEV), dtype=t)
+        there = slots >= 0
+        wk, wv, _, _ = R.read(want, slots[there])
+        for g, w in ((gk, wk), (gv, wv)):
+            assert g.dtype == t and not g.cpu()[~there].any()
+            assert torch.equal(g.cpu()[there].nan_to_num(123.0), w.to(t).nan_to_num(123.0))
+
+
+def test_append_takes_rows_of_any_stride_and_a_layer_of_a_pool():
+    from blockgtq_b200 import page_bytes, paged_kv4_append
+    gen = torch.Generator().manual_seed(5)
+    n, n_kv, n_q = 9, 2, 4
+    qkv = _noise(gen, n, n_q + 2 * n_kv, 128).half()
+    cos, sin = _tables(50)
+    wide = torch.cat([cos, sin], 1).to(DEV)
+    pos, slots = torch.arange(n) + 20, torch.arange(n) + 3
+    pool = torch.zeros(2, 3, n_kv, page_bytes(16), dtype=torch.uint8, device=DEV)
+    dev = qkv.to(DEV)
+    q, k, v = dev[:, :n_q], dev[:, n_q:n_q + n_kv], dev[:, n_q + n_kv:]
+    got = paged_kv4_append(pool[1], slots.to(DEV), k, v, q=q, cos=wide[:, :64], sin=wide[:, 64:], positions=pos.to(DEV))
+    odd = torch.zeros(n, n_kv, 131, dtype=torch.float16, device=DEV)[:, :, 3:]             # rows that no wide load can take
+    odd.copy_(v)
+    other = torch.zeros_like(pool)
+    paged_kv4_append(other[1], slots.to(DEV), k.transpose(0, 1).contiguous().transpose(0, 1), odd, cos=wide[:, :64], sin=wide[:, 64:], positions=pos.to(DEV))
+    want = torch.zeros(3, n_kv, page_bytes(16), dtype=torch.uint8)
+    kr = R.rotated(qkv[:, n_q:n_q + n_kv], cos, sin, pos)
+    for i in range(n):
+        R.write(want, int(slots[i]), kr[i], qkv[i, n_q + n_kv:].float())
+    assert torch.equal(pool[1].cpu(), want) and torch.equal(other[1].cpu(), want) and not pool[0].any()
+    assert torch.equal(got.cpu(), R.rotated(qkv[:, :n_q], cos, sin, pos).half())
+
+
+def test_slots_and_positions_out_of_range_are_reported_and_store_nothing():
+    from blockgtq_b200 import page_bytes, paged_kv4_append, paged_kv4_read
+    pages = torch.zeros(2, 1, page_bytes(16), dtype=torch.uint8, device=DEV)
+    rows = torch.ones(1, 1, 128, dtype=torch.float16, device=DEV)
+    cos, sin = (x.to(DEV) for x in _tables(4))
+    def one(slot, position):
+        status = torch.zeros(1, dtype=torch.int32, device=DEV)
+        paged_kv4_append(pages, torch.tensor([slot], device=DEV), rows, rows, cos=cos, sin=sin, positions=torch.tensor([position], device=DEV), status=status)
+        return status.item()
+    assert one(32, 0) == 2 and one(1 << 40, 0) == 2 and not pages.any()
+    assert one(-1, 99) == 0 and not pages.any()
+    assert one(0, 4) == 2 and not pages[0, 0, :64].any()          # the key; the value has no angle
+    assert one(0, 3) == 0 and pages[0, 0, :64].any()
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    k, v = paged_kv4_read(pages, torch.tensor([32, 0], device=DEV), status=status)
+    assert status.item() == 2 and not k[0].any() and k[1].any()
+
+
+def _check(got, lse, ref, rows):
+    out, want_lse, tol, tol_lse = ref
+    g = got[rows].double().cpu()
+    assert torch.isfinite(g).all()
+    off = (g - out).abs()                                     # (a row that sees nothing has a bound of zero)
+    assert (off <= tol).all(), ((off - tol).max(), off.max())
+    if lse is not None:
+        l = lse[rows].double().cpu()
+        assert torch.equal(l == -math.inf, want_lse == -math.inf)
+        f = torch.isfinite(want_lse)
+        assert ((l - want_lse).abs()[f] <= tol_lse[f]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n_kv,gqa,page,lens", [
+    (1, 1, 16, [1]), (2, 4, 64, [0, 1, 15, 16, 17]), (2, 8, 16, [33, 0, 0, 300]), (1, 7, 48, [500, 31, 32]), (8, 2, 128, [257, 129]),
+    (1, 3, 32, [2000]), (4, 1, 64, [63, 64, 65, 640])])
+def test_decode_against_64_bits(dtype, n_kv, gqa, page, lens):
+    from blockgtq_b200 import paged_kv4_decode_attention
+    gen = torch.Generator().manual_seed(sum(lens) + gqa)
+    pages, table, slots = _case(gen, n_kv, page, lens, dtype=dtype)
+    q = (_noise(gen, len(lens), n_kv * gqa, 128) * 1.5).to(dtype)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    out, lse = paged_kv4_decode_attention(q.to(DEV), pages, table.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV), return_lse=True, status=status)
+    assert status.item() == 0 and out.dtype == dtype
+    host = pages.cpu()
+    for b, t in enumerate(lens):
+        _check(out, lse, R.attention(q[b:b + 1], host, slots[b], [t], 1 / math.sqrt(128)), slice(b, b + 1))
+
+
+@pytest.mark.parametrize("magnitude", [1e-30, 1e-3, 3e3, 1e30])
+def test_decode_of_bf16_queries_of_any_magnitude(magnitude):
+    from blockgtq_b200 import paged_kv4_decode_attention
+    gen = torch.Generator().manual_seed(3)
+    pages, table, slots = _case(gen, 2, 16, [70])
+    q = (_noise(gen, 1, 4, 128) * magnitude).bfloat16()
+    scale = 0.1 / magnitude
+    out, lse = paged_kv4_decode_attention(q.to(DEV), pages, table.to(DEV), torch.tensor([70], dtype=torch.int32, device=DEV), scale=scale, return_lse=True)
+    _check(out, lse, R.attention(q, pages.cpu(), slots[0], [70], torch.tensor(scale).item()), slice(0, 1))
+
+
+def test_decode_of_many_sequences_and_of_one_long_one_cut_between_ctas():
+    from blockgtq_b200 import paged_kv4_decode_attention
+    gen = torch.Generator().manual_seed(11)
+    lens = [int(x) for x in torch.randint(0, 40, (700,), generator=gen)]
+    lens[350] = 9000
+    pages, table, slots = _case(gen, 1, 16, lens)
+    q = _noise(gen, len(lens), 2, 128).half()
+    out, lse = paged_kv4_decode_attention(q.to(DEV), pages, table.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV), return_lse=True)
+    host = pages.cpu()
+    for b in [0, 1, 2, 3, 255, 256, 257, 349, 350, 351, 511, 512, 699]:
+        _check(out, lse, R.attention(q[b:b + 1], host, slots[b], [lens[b]], 1 / math.sqrt(128)), slice(b, b + 1))
+
+
+PREFILLS = [
+    # n_kv, gqa, page, (tokens, queries) per sequence
+    (1, 1, 16, [(1, 1)]), (2, 4, 64, [(5, 5), (70, 3), (16, 16)]), (1, 7, 32, [(40, 9), (0, 0), (33, 33)]), (2, 8, 16, [(130, 1), (131, 40)]),
+    (1, 2, 128, [(300, 300)]), (1, 3, 16, [(5, 9), (0, 4), (20, 2)])]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n_kv,gqa,page,seqs", PREFILLS)
+def test_prefill_against_64_bits(dtype, n_kv, gqa, page, seqs, causal):
+    from blockgtq_b200 import paged_kv4_prefill_attention
+    lens, counts = [t for t, _ in seqs], [n for _, n in seqs]
+    gen = torch.Generator().manual_seed(sum(lens) + gqa)
+    pages, table, slots = _case(gen, n_kv, page, lens, dtype=dtype)
+    n, behind = sum(counts), 3
+    q = (_noise(gen, n + behind, n_kv * gqa, 128) * 1.5).to(dtype)
+    ends = [sum(counts[:i]) for i in range(len(counts) + 1)]
+    out = torch.full((n + behind, n_kv * gqa, 128), 77.0, dtype=dtype, device=DEV)
+    got, lse = paged_kv4_prefill_attention(q.to(DEV), pages, table.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV),
+                                           torch.tensor(ends, dtype=torch.int32, device=DEV), max_q_len=max(counts), max_seq_len=max(lens),
+                                           causal=causal, return_lse=True, out=out)
+    assert got is out and (out[n:] == 77).all()
+    host = pages.cpu()
+    for b, (t, m) in enumerate(seqs):
+        seen = [t - m + 1 + i if causal else t for i in range(m)]
+        _check(out, lse, R.attention(q[ends[b]:ends[b + 1]], host, slots[b], seen, 1 / math.sqrt(128)), slice(ends[b], ends[b + 1]))
+
+
+def test_a_page_number_outside_the_pool_leaves_its_tokens_out():
+    from blockgtq_b200 import paged_kv4_decode_attention
+    gen = torch.Generator().manual_seed(2)
+    pages, table, slots = _case(gen, 1, 16, [40, 40])
+    q = _noise(gen, 2, 2, 128).half()
+    for bad in (-1, pages.shape[0], 1 << 30):
+        t = table.clone()
+        t[0, 1] = bad
+        status = torch.zeros(1, dtype=torch.int32, device=DEV)
+        out, lse = paged_kv4_decode_attention(q.to(DEV), pages, t.to(DEV), torch.tensor([40, 40], dtype=torch.int32, device=DEV), return_lse=True, status=status)
+        assert status.item() == 4
+        left = torch.cat([slots[0][:16], slots[0][32:]])
+        _check(out, lse, R.attention(q[:1], pages.cpu(), left, [24], 1 / math.sqrt(128)), slice(0, 1))
+        _check(out, lse, R.attention(q[1:], pages.cpu(), slots[1], [40], 1 / math.sqrt(128)), slice(1, 2))
+
+
+def test_a_length_beyond_the_table_is_held_to_it():
+    from blockgtq_b200 import paged_kv4_decode_attention
+    gen = torch.Generator().manual_seed(2)
+    pages, table, slots = _case(gen, 1, 16, [32])
+    q = _noise(gen, 1, 2, 128).half()
+    for t in (33, 1 << 30, -5):
+        out, lse = paged_kv4_decode_attention(q.to(DEV), pages, table[:, :2].to(DEV), torch.tensor([t], dtype=torch.int32, device=DEV), return_lse=True)
+        _check(out, lse, R.attention(q, pages.cpu(), slots[0], [min(32, t)], 1 / math.sqrt(128)), slice(0, 1))
+
+
+def test_no_number_in_a_row_shows_and_in_a_hidden_place_does_not():
+    from blockgtq_b200 import paged_kv4_append, paged_kv4_decode_attention, paged_kv4_prefill_attention
+    gen = torch.Generator().manual_seed(9)
+    pages, table, slots = _case(gen, 1, 16, [40])
+    k, v = (_noise(gen, 1, 1, 128).half() for _ in range(2))
+    v[0, 0, 33] = math.nan                                     # group 1 of V of token 39
+    paged_kv4_append(pages, slots[0][39:].to(DEV), k.to(DEV), v.to(DEV))
+    q = _noise(gen, 4, 2, 128).half().to(DEV)
+    def run(t):
+        return paged_kv4_decode_attention(q[:1], pages, table.to(DEV), torch.tensor([t], dtype=torch.int32, device=DEV))
+    assert torch.isfinite(run(39)).all()
+    nan = run(40).isnan()[0]
+    assert nan[:, 32:64].all() and not nan[:, :32].any() and not nan[:, 64:].any()
+    out = paged_kv4_prefill_attention(q, pages, table.to(DEV), torch.tensor([40], dtype=torch.int32, device=DEV), torch.tensor([0, 4], dtype=torch.int32, device=DEV))
+    assert torch.isfinite(out[:3]).all() and out[3, :, 32:64].isnan().all()
+    k[0, 0, 0] = math.nan
+    paged_kv4_append(pages, slots[0][39:].to(DEV), k.to(DEV), torch.zeros_like(v).to(DEV))
+    assert run(40).isnan().all() and torch.isfinite(run(39)).all()
+
+
+def test_steps_of_the_cache_from_prompt_to_decode_on_another_stream():
+    """Prompts, chunks behind them and single tokens through PagedKV4Cache, sequences coming and going, against 64 bits."""
+    from blockgtq_b200 import PagedKV4Cache
+    gen = torch.Generator().manual_seed(21)
+    L, n_q, n_kv = 2, 4, 2
+    cache = PagedKV4Cache(L, n_q, n_kv, n_pages=40, max_seq_len=200, page_size=16, device=DEV)
+    cos, sin = _tables(200)
+    rope = (cos.to(DEV), sin.to(DEV))
+    a, b = cache.add_sequence(), cache.add_sequence()
+    stream = torch.cuda.Stream(DEV)
+    def step(seqs, counts):
+        n = sum(counts)
+        cache.begin_step(seqs, counts)
+        for layer in range(L):
+            q, k, v = (_noise(gen, n, h, 128).half() for h in (n_q, n_kv, n_kv))
+            out = cache.append_and_attend(layer, q.to(DEV), k.to(DEV), v.to(DEV), rope=rope)
+            at, host = 0, cache.pages[layer].cpu()
+            positions = torch.cat([torch.arange(cache.seq_len(s) - c, cache.seq_len(s)) for s, c in zip(seqs, counts)])
+            qr = R.rotated(q, cos, sin, positions).half()
+            for s, c in zip(seqs, counts):
+                t = cache.seq_len(s)
+                slots = torch.tensor([cache._seqs[s][1][i // 16] * 16 + i % 16 for i in range(t)])
+                _check(out, None, R.attention(qr[at:at + c], host, slots, [t - c + 1 + i for i in range(c)], 1 / math.sqrt(128)), slice(at, at + c))
+                at += c
+        cache.check_status()
+    with torch.cuda.stream(stream):
+        step([a, b], [37, 5])
+        step([b, a], [1, 1])
+        step([a], [20])
+        cache.free_sequence(a)
+        c = cache.add_sequence()
+        step([c, b], [50, 4])
+        step([b, c], [1, 1])
+    torch.cuda.current_stream().wait_stream(stream)
+
+
+def test_a_captured_step_follows_the_lengths():
+    from blockgtq_b200 import paged_kv4_append, paged_kv4_decode_attention
+    gen = torch.Generator().manual_seed(31)
+    lens = [60, 7, 0]
+    pages, table, slots = _case(gen, 2, 16, [t + 20 for t in lens])
+    table, table_dev = table, table.to(DEV)
+    cos, sin = _tables(200)
+    rope = dict(cos=cos.to(DEV), sin=sin.to(DEV))
+    q, k, v = (torch.zeros(3, h, 128, dtype=torch.float16, device=DEV) for h in (8, 2, 2))
+    n = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    slot, pos = torch.zeros(3, dtype=torch.int64, device=DEV), torch.zeros(3, dtype=torch.int64, device=DEV)
+    def layer():
+        qr = paged_kv4_append(pages, slot, k, v, q=q, positions=pos, **rope)
+        return paged_kv4_decode_attention(qr, pages, table_dev, n, return_lse=True)
+    slot.fill_(-1)
+    layer()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = layer()
+    for i in range(3):
+        fresh = [_noise(gen, 3, h, 128).half() for h in (8, 2, 2)]
+        for x, y in zip((q, k, v), fresh):
+            x.copy_(y)
+        pos.copy_(torch.tensor([t + i for t in lens]))
+        slot.copy_(torch.tensor([int(slots[b][t + i]) for b, t in enumerate(lens)]))
+        n.copy_(torch.tensor([t + i + 1 for t in lens], dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        host, qr = pages.cpu(), R.rotated(fresh[0], cos, sin, pos.cpu()).half()
+        for b, t in enumerate(lens):
+            _check(out, lse, R.attention(qr[b:b + 1], host, slots[b], [t + i + 1], 1 / math.sqrt(128)), slice(b, b + 1))
+
+
+def test_results_do_not_change_from_call_to_call():
+    from blockgtq_b200 import paged_kv4_decode_attention
+    gen = torch.Generator().manual_seed(41)
+    lens = [1500, 3, 900]
+    pages, table, _ = _case(gen, 2, 16, lens)
+    q = _noise(gen, 3, 8, 128).half().to(DEV)
+    args = (q, pages, table.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV))
+    first = paged_kv4_decode_attention(*args)
+    for _ in range(5):
+        assert torch.equal(first, paged_kv4_decode_attention(*args))
