@@ -29,7 +29,7 @@ DEC_CLUSTER_SHIFT = 8
 PF_NO_TCGEN05 = 16
 COMBINE_PROGRAMMATIC = 1
 STEP_Q_ROTATED = 1
-PAGED_BF16, PAGED_F32, PAGED_CAUSAL = 1, 2, 4
+PAGED_BF16, PAGED_F32, PAGED_CAUSAL, PAGED_FORM_SHIFT = 1, 2, 4, 8
 
 
 class HeadDesc(C.Structure):
@@ -149,7 +149,7 @@ _SIGNATURES = {
     "bgtq_paged_append": (C.c_int, [_vp, _i64, _i64, _i32, _i32, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp,
                                     _vp, _vp, _i64, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp]),
     "bgtq_paged_read": (C.c_int, [_vp, _i64, _i64, _i32, _i32, _vp, _i32, _i32, _vp, _vp, _i32, _vp, _vp]),
-    "bgtq_paged_workspace_bytes": (C.c_int64, [_i32, _i32, _i32, _i32, _i32, _i64]),
+    "bgtq_paged_workspace_bytes": (C.c_int64, [_i32, _i32, _i32, _i32, _i32, _i64, _i32]),
     "bgtq_paged_attend": (C.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _i32, _i32, _vp, _i64, _i32, _vp, _vp, _i32, _i32, _i32, _i32,
                                     _i32, _i64, _f32, _i32, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp]),
     "bgtq_combine_publish": (C.c_int, [_vp, _vp, _i32, _vp, _i32, _i32, _i32, _vp, _i64, _i64, _vp, _i32, _i32, _vp, _vp,

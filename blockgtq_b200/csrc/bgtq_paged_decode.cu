@@ -3,20 +3,23 @@
 //     S[t, col] = sum_g ks[t, g] * (sum_{d in g} q[col, d] (u[t, d] - 8)),   P = 2^(S f - M),
 //     O[d, col] = sum_t P[t, col] vs[t, g(d)] (u[t, d] - 8),   out = O / sum_t P
 //
-// A column is one query row: a query head of the KV head's group in a decode step, (position, head) pairs of a chunk.  K's codes
-// go to the tensor cores as they lie, as subnormal fp16 numbers u * 2^-20, and the eights are the accumulators' start; V's become
-// u - 8 first (1024 + u or 1024 + 16 u by a mask, then one exact fp16 operation), because sums over tokens that carry the eights would lose
-// them again to the accumulators' rounding.  Subnormal operands are aligned by their exponent field, not by their leading bit: u * 2^-24
-// (one shift less per two pairs) cost S ten bits, u * 2^-20 costs six of twenty-four.  The K scales multiply the groups' sums, the
-// V scales the weights.  Nothing is rounded but P * vs (fp16, as the product's operand; sums, maxima, scales and accumulators are fp32).
-// Queries are brought to [2^13, 2^14) by a power of two each, so that bf16 queries of any magnitude are exact in fp16 too.
+// A column is one query row: a query head of the KV head's group in a decode step, (position, head) pairs of a chunk.  Codes become
+// u - 8 in fp16: a mask makes 1024 + u or 1024 + 16 u of two of them at once, one exact operation the rest.  (As subnormal numbers, u * 2^-24
+// without that operation, with the eights in the accumulators' start or in a product of their own: operands are aligned by their exponent
+// field, not by their leading bit, which cost ten bits of the sums; and over tokens the eights take theirs of the accumulators.)  The K scales
+// multiply the groups' sums, the V scales the weights.  Nothing is rounded but P * vs (fp16, as the product's operand; sums, maxima, scales
+// and accumulators are fp32).  Queries are brought to [2^13, 2^14) by a power of two each, so that bf16 queries of any
+// magnitude are exact in fp16 too.
 //
 // P * vs <= 2^14 holds for every magnitude of V: a column's reference M is the running maximum of S f + log2(max_g vs), minus 6, and moves
 // (O rescaled) only when a value exceeds it by 2^14.
 //
-// Work: the 32-token batches of all (sequence, block of columns, KV head) triples form one list, cut evenly over the CTAs; a CTA's
-// eight warps take batches in turn, each with a ring of bulk copies of its own.  At a triple's end the warps' states are merged in shared
-// memory; triples cut between CTAs are merged by a second launch.
+// Work, in one of two forms:
+//   split    the 32-token batches of all (sequence, block of columns, KV head) triples form one list, each triple padded to whole rounds
+//            of eight, and the list is cut evenly over the CTAs.  Triples cut between CTAs are merged by a second launch.
+//   cluster  a cluster of 1 to 8 CTAs per triple, which merge their shares in distributed shared memory: no list, no second launch.
+// In a CTA eight warps take batches in turn, each with a ring of bulk copies of its own (the next triple's first ones travel while this
+// one's states are merged in shared memory).
 #include "bgtq_paged_common.cuh"
 
 namespace bgtq {
@@ -25,8 +28,7 @@ namespace {
 constexpr int kPdWarps = 8, kPdThreads = 32 * kPdWarps;
 constexpr int kBatchTok = 32;
 constexpr int kBatchBytes = kBatchTok / kUnitTok * kUnitBytes;
-constexpr int kPdStages = 3;
-constexpr int kMinBatches = kPdWarps;             // a CTA's least share: one batch per warp
+constexpr int kPdStages = 2;
 constexpr float kLift = 6.f, kReach = 14.f;       // log2 of P * vs at a reference's setting, and where it moves
 constexpr int kOutRow = 132;                      // floats between columns of a warp's state in shared memory
 
@@ -38,7 +40,8 @@ struct PdParams {
     int64_t tb_st;
     const int32_t* lens;
     const int32_t* cu_q;             // null: one query row per sequence
-    int32_t table_cols, n_seq, n_tok, n_q, n_kv, gqa, causal, n_cta;
+    int32_t table_cols, n_seq, n_tok, n_q, n_kv, gqa, causal;
+    int32_t n_cta;                   // split: CTAs;  cluster: column blocks of a sequence that have a cluster of their own
     float scale_log2;
     void* out;
     int64_t o_st, o_sh;
@@ -46,6 +49,13 @@ struct PdParams {
     float* part_o;                   // (2 n_cta, columns, 128)
     float2* part_ml;                 // (2 n_cta, columns): reference, denominator
     int32_t* status;
+};
+
+// How a call is launched.
+struct PdForm {
+    int nt, n_cta, n_rank, blocks_of_seq;       // n_rank: CTAs of a triple's cluster, 0: the split form
+    int64_t triples;
+    bool merge;                                 // split: triples may be cut (those of one round never are)
 };
 
 struct SeqInfo {
@@ -65,9 +75,11 @@ __device__ __forceinline__ SeqInfo pd_seq(const PdParams& P, int i) {
     }
     return s;
 }
+__device__ __forceinline__ uint32_t pd_batches(const SeqInfo& s) { return (uint32_t)((s.len + kBatchTok - 1) / kBatchTok); }
+__device__ __forceinline__ uint32_t pd_padded(const SeqInfo& s) { return (pd_batches(s) + kPdWarps - 1) / kPdWarps * kPdWarps; }
 template <int NT>
 __device__ __forceinline__ uint32_t pd_work(const PdParams& P, const SeqInfo& s) {
-    return (uint32_t)((s.len + kBatchTok - 1) / kBatchTok) * (uint32_t)P.n_kv * (uint32_t)((s.n * P.gqa + 8 * NT - 1) / (8 * NT));
+    return pd_padded(s) * (uint32_t)P.n_kv * (uint32_t)((s.n * P.gqa + 8 * NT - 1) / (8 * NT));
 }
 
 struct ScanSmem {
@@ -98,49 +110,71 @@ __device__ __forceinline__ uint32_t block_scan(ScanSmem& S, uint32_t w) {
     return before + x - w;
 }
 
-// Total of the list and, for the position that `at` makes of it, the sequence that it lies in and where that one starts.
+// Total of the list and, for the position that `at` makes of it, the sequence that it lies in (-1: none) and where that one starts.  Up to 128
+// sequences are looked over by every warp for itself, without a barrier.
 template <int NT, typename At>
 __device__ __forceinline__ void pd_find(const PdParams& P, ScanSmem& S, uint32_t& total, int& seq, uint32_t& start, At at) {
     const int tid = threadIdx.x, step = blockDim.x;
+    if (P.n_seq <= 128) {
+        const int lane = tid & 31;
+        uint32_t w[4], mine = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[i] = 4 * lane + i < P.n_seq ? pd_work<NT>(P, pd_seq(P, 4 * lane + i)) : 0u;
+            mine += w[i];
+        }
+        uint32_t before = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, before, d);
+            if (lane >= d) before += y;
+        }
+        total = __shfl_sync(0xffffffffu, before, 31);
+        before -= mine;
+        const uint32_t want = at(total);
+        const uint32_t who = __ballot_sync(0xffffffffu, before <= want && want - before < mine);
+        uint32_t first = before;
+        int found = 4 * lane;
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            if (found == 4 * lane + i && want - first >= w[i]) {
+                first += w[i];
+                ++found;
+            }
+        seq = who ? __shfl_sync(0xffffffffu, found, __ffs(who) - 1) : -1;
+        start = __shfl_sync(0xffffffffu, first, who ? __ffs(who) - 1 : 0);
+        return;
+    }
     if (tid == 0) S.seq = -1;
-    uint32_t w = 0, before = 0, sum = 0;
+    uint32_t sum = 0;
     for (int base = 0; base < P.n_seq; base += step) {
         const int i = base + tid;
-        w = i < P.n_seq ? pd_work<NT>(P, pd_seq(P, i)) : 0u;
-        before = sum + block_scan(S, w);
+        block_scan(S, i < P.n_seq ? pd_work<NT>(P, pd_seq(P, i)) : 0u);
         __syncthreads();
         sum += S.total;
         __syncthreads();
     }
     total = sum;
     const uint32_t want = at(total);
-    if (P.n_seq <= step) {
-        if (w && before <= want && want - before < w) {
-            S.seq = tid;
+    sum = 0;
+    for (int base = 0; base < P.n_seq; base += step) {
+        const int i = base + tid;
+        const uint32_t w = i < P.n_seq ? pd_work<NT>(P, pd_seq(P, i)) : 0u;
+        const uint32_t before = sum + block_scan(S, w);
+        if (before <= want && want - before < w) {
+            S.seq = i;
             S.start = before;
         }
-    } else {
-        sum = 0;
-        for (int base = 0; base < P.n_seq; base += step) {
-            const int i = base + tid;
-            w = i < P.n_seq ? pd_work<NT>(P, pd_seq(P, i)) : 0u;
-            before = sum + block_scan(S, w);
-            if (w && before <= want && want - before < w) {
-                S.seq = i;
-                S.start = before;
-            }
-            __syncthreads();
-            sum += S.total;
-            __syncthreads();
-        }
+        __syncthreads();
+        sum += S.total;
+        __syncthreads();
     }
-    __syncthreads();
     seq = S.seq;
     start = S.start;
 }
 
 __device__ __forceinline__ uint32_t pd_share(uint32_t total, int n_cta) {
-    return max((uint32_t)kMinBatches, (total + n_cta - 1) / n_cta);
+    return ((total + n_cta - 1) / n_cta + kPdWarps - 1) / kPdWarps * kPdWarps;
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -150,7 +184,7 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ float lg2(float x) {
     float y;
-    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
@@ -163,41 +197,44 @@ __device__ __forceinline__ uint2 lds64(uint32_t a) {
     asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
     return v;
 }
-// D = A B + C with the column sums' start in C (rows alike)
-__device__ __forceinline__ void mma_from(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2], float c0, float c1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
-        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(c0), "f"(c1));
+// Two constants that one instruction takes beside a mask or a factor: held in registers (two of them cannot be immediates).
+struct Magic {
+    uint32_t k1024, m72;            // fp16 pairs
+};
+__device__ __forceinline__ Magic pd_magic() {
+    Magic m;
+    asm volatile("mov.b32 %0, 0x64006400;" : "=r"(m.k1024));
+    asm volatile("mov.b32 %0, 0xd480d480;" : "=r"(m.m72));
+    return m;
 }
-// The pair of codes of group G in a word as fp16: u * 2^-20
+// The pair of codes of group G in a word, w8 = w >> 8: u - 8 as fp16
 template <int G>
-__device__ __forceinline__ uint32_t k_codes(uint32_t w) {
-    return (G == 0 ? w << 4 : G == 1 ? w : G == 2 ? w >> 4 : w >> 8) & 0x00f000f0u;
-}
-// u - 8
-template <int G>
-__device__ __forceinline__ uint32_t v_codes(uint32_t w) {
-    const uint32_t x = G >= 2 ? w >> 8 : w;
-    uint32_t d;
-    if (G & 1) asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"((x & 0x00f000f0u) | 0x64006400u), "r"(0x2c002c00u), "r"(0xd480d480u));   // / 16 - 72
-    else asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"((x & 0x000f000fu) | 0x64006400u), "r"(0x64086408u));                             // - 1032
+__device__ __forceinline__ uint32_t codes(const Magic& m, uint32_t w, uint32_t w8) {
+    uint32_t x, d;
+    if (G & 1) {
+        asm("lop3.b32 %0, %1, 0x00f000f0, %2, 0xEA;" : "=r"(x) : "r"(G >= 2 ? w8 : w), "r"(m.k1024));        // 1024 + 16 u
+        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(x), "r"(0x2c002c00u), "r"(m.m72));               // / 16 - 72
+    } else {
+        asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xEA;" : "=r"(x) : "r"(G >= 2 ? w8 : w), "r"(m.k1024));        // 1024 + u
+        asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(0xe408e408u));                                // - 1032
+    }
     return d;
 }
 
 template <int NT>
 struct PdSmem {
-    __align__(128) uint8_t ring[kPdWarps][kPdStages][kBatchBytes];       // at a triple's end: the warps' states
-    __align__(8) uint64_t full[kPdWarps][kPdStages];
+    __align__(128) uint8_t ring[kPdWarps][kPdStages][kBatchBytes];
+    __align__(16) float o[kPdWarps][8 * NT][kOutRow];        // the warps' states at a triple's end
     float2 ml[kPdWarps][8 * NT];
+    __align__(8) uint64_t full[kPdWarps][kPdStages];
     ScanSmem scan;
+    // cluster form: [rank][8 NT columns][128] and [rank][8 NT] (reference, denominator) follow
 };
 
-// One column block's queries as the products' operands, the accumulators' starts, and the factor from sums to logits.
+// One column block's queries as the products' operands, and the factor from sums to logits (columns 2 c, 2 c + 1).
 template <int NT>
 struct Query {
-    uint32_t b[NT][4][4];            // [group][k-step half: words 0, 1 | 2, 3]
-    float c[NT][4][2];               // -8 * sum of the group's operand, columns 2 c and 2 c + 1
+    uint32_t b[NT][4][4];            // [group][words 0, 1 | 2, 3]
     float f[NT][2];
 };
 
@@ -228,24 +265,12 @@ __device__ __forceinline__ void pd_query(const PdParams& P, Query<NT>& Q, const 
         const int ex = (int)(__float_as_uint(top) >> 23) - 127;
         const int e = top > 0.f && ex < 128 ? 13 - ex : 0;
         const float up0 = __uint_as_float((uint32_t)(127 + e / 2) << 23), up1 = __uint_as_float((uint32_t)(127 + e - e / 2) << 23);
-        const int fe = 20 - e;                                                         // (-120 .. 134, in two steps)
+        const int fe = -e;                                                             // (-140 .. 114, in two steps)
         const float fac = P.scale_log2 * __uint_as_float((uint32_t)(127 + fe / 2) << 23) * __uint_as_float((uint32_t)(127 + fe - fe / 2) << 23);
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            float sum = 0.f;
+        for (int g = 0; g < 4; ++g)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t w = pack_half2(x[g][2 * i] * up0 * up1, x[g][2 * i + 1] * up0 * up1);
-                Q.b[nt][g][i] = w;
-                const float2 v = PgType<__half>::up(w);
-                sum += v.x + v.y;
-            }
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            sum *= -8.f * 9.5367431640625e-7f;                                      // 2^-20
-            Q.c[nt][g][0] = __shfl_sync(0xffffffffu, sum, 8 * c);                   // (lane 4 * column holds column's)
-            Q.c[nt][g][1] = __shfl_sync(0xffffffffu, sum, 8 * c + 4);
-        }
+            for (int i = 0; i < 4; ++i) Q.b[nt][g][i] = pack_half2(x[g][2 * i] * up0 * up1, x[g][2 * i + 1] * up0 * up1);
         Q.f[nt][0] = __shfl_sync(0xffffffffu, fac, 8 * c);
         Q.f[nt][1] = __shfl_sync(0xffffffffu, fac, 8 * c + 4);
     }
@@ -260,9 +285,9 @@ struct State {
 template <int N> struct Int { static constexpr int value = N; };
 template <typename F> __device__ __forceinline__ void each_group(F f) { f(Int<0>{}); f(Int<1>{}); f(Int<2>{}); f(Int<3>{}); }
 
-// 16 tokens at shared address u.  kEdge: some of them (tokens from `left` on of the sequence, from lim[] on of a column) are hidden.
+// 16 tokens at shared address u.  kEdge: some of them (tokens from len on of the sequence, from lim[] on of a column) are hidden.
 template <int NT, bool kEdge>
-__device__ __forceinline__ void pd_unit(uint32_t u, const Query<NT>& Q, State<NT>& st, int r, int c, int t0, int len, const int (&lim)[NT][2]) {
+__device__ __forceinline__ void pd_unit(uint32_t u, const Magic& mg, const Query<NT>& Q, State<NT>& st, int r, int c, int t0, int len, const int (&lim)[NT][2]) {
     float s[NT][4];
     {
         const uint32_t kb = u + r * 64 + c * 16;
@@ -270,15 +295,16 @@ __device__ __forceinline__ void pd_unit(uint32_t u, const Query<NT>& Q, State<NT
         const uint2 ka = lds64(u + kUnitKs + r * 8), kc = lds64(u + kUnitKs + 64 + r * 8);
         const float sa[4] = {pg_lo(ka.x), pg_hi(ka.x), pg_lo(ka.y), pg_hi(ka.y)};
         const float sc[4] = {pg_lo(kc.x), pg_hi(kc.x), pg_lo(kc.y), pg_hi(kc.y)};
+        const uint4 x8 = make_uint4(x.x >> 8, x.y >> 8, x.z >> 8, x.w >> 8), y8 = make_uint4(y.x >> 8, y.y >> 8, y.z >> 8, y.w >> 8);
         each_group([&](auto gi) {
             constexpr int g = decltype(gi)::value;
-            const uint32_t a0[4] = {k_codes<g>(x.x), k_codes<g>(y.x), k_codes<g>(x.y), k_codes<g>(y.y)};
-            const uint32_t a1[4] = {k_codes<g>(x.z), k_codes<g>(y.z), k_codes<g>(x.w), k_codes<g>(y.w)};
+            const uint32_t a0[4] = {codes<g>(mg, x.x, x8.x), codes<g>(mg, y.x, y8.x), codes<g>(mg, x.y, x8.y), codes<g>(mg, y.y, y8.y)};
+            const uint32_t a1[4] = {codes<g>(mg, x.z, x8.z), codes<g>(mg, y.z, y8.z), codes<g>(mg, x.w, x8.w), codes<g>(mg, y.w, y8.w)};
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float acc[4];
                 const uint32_t b0[2] = {Q.b[nt][g][0], Q.b[nt][g][1]}, b1[2] = {Q.b[nt][g][2], Q.b[nt][g][3]};
-                mma_from(acc, a0, b0, Q.c[nt][g][0], Q.c[nt][g][1]);
+                mma_16816_z(acc, a0, b0);
                 mma_16816(acc, a1, b1);
                 if (g == 0) {
                     s[nt][0] = acc[0] * sa[g]; s[nt][1] = acc[1] * sa[g];
@@ -346,10 +372,11 @@ __device__ __forceinline__ void pd_unit(uint32_t u, const Query<NT>& Q, State<NT
         }
     const uint32_t vb = u + kUnitV + c * 128 + r * 16;
     const uint4 x = lds128(vb), y = lds128(vb + 512);
+    const uint4 x8 = make_uint4(x.x >> 8, x.y >> 8, x.z >> 8, x.w >> 8), y8 = make_uint4(y.x >> 8, y.y >> 8, y.z >> 8, y.w >> 8);
     each_group([&](auto gi) {
         constexpr int g = decltype(gi)::value;
-        const uint32_t a0[4] = {v_codes<g>(x.x), v_codes<g>(x.y), v_codes<g>(y.x), v_codes<g>(y.y)};
-        const uint32_t a1[4] = {v_codes<g>(x.z), v_codes<g>(x.w), v_codes<g>(y.z), v_codes<g>(y.w)};
+        const uint32_t a0[4] = {codes<g>(mg, x.x, x8.x), codes<g>(mg, x.y, x8.y), codes<g>(mg, y.x, y8.x), codes<g>(mg, y.y, y8.y)};
+        const uint32_t a1[4] = {codes<g>(mg, x.z, x8.z), codes<g>(mg, x.w, x8.w), codes<g>(mg, y.z, y8.z), codes<g>(mg, y.w, y8.w)};
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             float w[4] = {p[nt][0] * ha[g], p[nt][1] * ha[g], p[nt][2] * hc[g], p[nt][3] * hc[g]};
@@ -376,122 +403,212 @@ __device__ __forceinline__ void pd_write(const PdParams& P, const SeqInfo& s, in
     if (P.lse && lane == 0) P.lse[(int64_t)(s.q0 + pos) * P.n_q + hq] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945309f;
 }
 
-template <int NT, typename T>
+// A run of batches of one triple.
+struct Segment {
+    SeqInfo s;
+    int seq, cb, h, first, n;        // first batch, batches
+    bool whole;                      // all of the triple's
+};
+// A warp's copies of its batches of a segment: first + warp, + 8, ...
+struct Copies {
+    const uint8_t* from;             // lane i: unit i % 2 of batch 16 * block + i / 2, null: not there
+    int issued, n;
+    uint32_t have;                   // two bits per stage: which of its units are there
+};
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+    return a;
+}
+
+template <int NT, typename T, bool kCluster>
 __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(const PdParams P) {
     extern __shared__ __align__(128) uint8_t smem_raw[];
     PdSmem<NT>& S = *reinterpret_cast<PdSmem<NT>*>(smem_raw);
     constexpr int kCols = 8 * NT;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, c = lane & 3;
-    if (tid < kPdWarps * kPdStages) mbar_init(&S.full[0][0] + tid, 1);
-    if (tid == 0) mbar_fence_init();
+    if (lane < kPdStages) {                // each warp waits on its own
+        mbar_init(&S.full[warp][lane], 1);
+        mbar_fence_init();
+    }
+    __syncwarp();
+    uint32_t rank = 0, n_rank = 1;
+    if (kCluster) {
+        asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+        asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(n_rank));
+        if (n_rank > 1) cluster_arrive();            // a CTA's shared memory may be written once that CTA runs
+    }
     grid_launch_dependents();
     grid_dependency_wait();
-    uint32_t total, seq_start, share = 0;
-    int seq;
-    pd_find<NT>(P, S.scan, total, seq, seq_start, [&](uint32_t t) {
-        share = pd_share(t, P.n_cta);
-        return (uint32_t)blockIdx.x * share;
-    });
-    const uint64_t begin = (uint64_t)blockIdx.x * share;
-    if (begin >= total || seq < 0) return;
-    uint32_t pos = (uint32_t)begin;
-    const uint32_t end = (uint32_t)min((uint64_t)total, begin + share);
-    uint32_t issued = 0, taken = 0;        // this warp's copies so far
+
+    Segment g;
+    uint32_t pos = 0, end = 0, begin = 0, seq_start = 0;
+    // split: the segment that starts at pos
+    auto at_pos = [&]() {
+        const uint32_t nb = pd_batches(g.s), np = pd_padded(g.s), triple = (pos - seq_start) / np, first = (pos - seq_start) - triple * np;
+        const uint32_t count = min(np - first, end - pos);
+        g.cb = (int)(triple / P.n_kv);
+        g.h = (int)(triple - (uint32_t)g.cb * P.n_kv);
+        g.first = (int)first;
+        g.n = (int)(min(first + count, nb) - first);
+        g.whole = first == 0 && count == np;
+        return count;
+    };
+    // cluster: this CTA's share of the triple
+    auto share_of = [&]() {
+        const uint32_t nb = pd_batches(g.s), per = pd_padded(g.s) / kPdWarps, a = per * rank / n_rank * kPdWarps, b = per * (rank + 1) / n_rank * kPdWarps;
+        g.first = (int)a;
+        g.n = (int)(min(b, nb) - min(a, nb));
+        g.whole = true;
+    };
+    uint32_t count = 0;
+    if (kCluster) {
+        const uint32_t t = blockIdx.x / n_rank, per_seq = (uint32_t)P.n_kv * P.n_cta;
+        g.seq = (int)(t / per_seq);
+        const uint32_t in_seq = t - (uint32_t)g.seq * per_seq;
+        g.cb = (int)(in_seq / P.n_kv);
+        g.h = (int)(in_seq - (uint32_t)g.cb * P.n_kv);
+        g.s = pd_seq(P, g.seq);
+        if (g.cb * kCols >= g.s.n * P.gqa) {         // (the whole cluster)
+            if (n_rank > 1) cluster_wait();
+            return;
+        }
+        share_of();
+    } else {
+        // rows of sequences that have none of their tokens cached
+        for (int i = blockIdx.x; i < P.n_seq; i += P.n_cta) {
+            const SeqInfo s = pd_seq(P, i);
+            if (s.len > 0) continue;
+            for (int row = warp; row < s.n * P.n_q; row += kPdWarps) {
+                const int qp = row / P.n_q, hq = row - qp * P.n_q;
+                *reinterpret_cast<uint2*>(reinterpret_cast<T*>(P.out) + (int64_t)(s.q0 + qp) * P.o_st + hq * P.o_sh + 4 * lane) = make_uint2(0, 0);
+                if (P.lse && lane == 0) P.lse[(int64_t)(s.q0 + qp) * P.n_q + hq] = -INFINITY;
+            }
+        }
+        uint32_t total, share = 0;
+        pd_find<NT>(P, S.scan, total, g.seq, seq_start, [&](uint32_t t) {
+            share = pd_share(t, P.n_cta);
+            return (uint32_t)blockIdx.x * share;
+        });
+        if ((uint64_t)blockIdx.x * share >= total || g.seq < 0) return;
+        begin = pos = blockIdx.x * share;
+        end = (uint32_t)min((uint64_t)total, (uint64_t)begin + share);
+        g.s = pd_seq(P, g.seq);
+        if (g.s.len == 0) return;                    // (row ranges that do not follow one another: the list is not one then)
+        count = at_pos();
+    }
+
+    uint32_t phases = 0;                   // of this warp's stages
     bool ok = true;
+    const Magic mg = pd_magic();
     const uint32_t ring0 = smem_u32(S.ring[warp][0]);
     const uint64_t policy = l2_evict_first_policy();
-
-    SeqInfo s = pd_seq(P, seq);
-    while (pos < end) {
-        const uint32_t nb = (uint32_t)((s.len + kBatchTok - 1) / kBatchTok);
-        if (nb == 0) break;              // (row ranges that do not follow one another: the list is not one then)
-        const uint32_t triple = (pos - seq_start) / nb, first = (pos - seq_start) - triple * nb;
-        const uint32_t count = min(nb - first, end - pos);
-        const int cb = (int)(triple / P.n_kv), h = (int)(triple - (uint32_t)cb * P.n_kv);
-        // columns' limits
-        int lim[NT][2], lim_min = INT_MAX, lim_max = 0;
+    auto issue = [&](const Segment& sg, Copies& w, int stage) {
+        const int k = w.issued++;
+        if ((k & 15) == 0) {
+            const int kk = k + (lane >> 1), unit = 2 * (sg.first + warp + kPdWarps * kk) + (lane & 1);
+            w.from = nullptr;
+            if (kk < w.n && unit < (sg.s.len + kUnitTok - 1) / kUnitTok) {
+                const int col = unit / P.pool.units, page = P.table[(int64_t)sg.seq * P.tb_st + col];
+                if (page >= 0 && page < P.pool.n_pages)
+                    w.from = P.pool.pages + (int64_t)page * P.pool.page_stride + (int64_t)sg.h * P.pool.head_stride + (unit - col * P.pool.units) * kUnitBytes;
+                else if (P.status)
+                    *P.status = kStatusBadPage;
+            }
+        }
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(w.from), 2 * (k & 15) + (lane & 1)));
+        const uint32_t there = __ballot_sync(0xffffffffu, src != nullptr) & 3u;
+        uint64_t* bar = &S.full[warp][stage];
+        if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)__popc(there) * kUnitBytes);
+        __syncwarp();
+        if (lane < 2 && src) bulk_g2s_hint(S.ring[warp][stage] + lane * kUnitBytes, src, kUnitBytes, bar, policy);
+        w.have = (w.have & ~(3u << (2 * stage))) | there << (2 * stage);
+    };
+    auto begin_copies = [&](const Segment& sg) {
+        Copies w{nullptr, 0, 0, 0};
+        // batches that no row of the block sees are left out
+        const int last_row = min((sg.cb + 1) * kCols, sg.s.n * P.gqa) - 1;
+        const int lim_max = P.causal ? max(0, sg.s.len - sg.s.n + 1 + last_row / P.gqa) : sg.s.len;
+        const int n = min(sg.n, max(0, (lim_max + kBatchTok - 1) / kBatchTok - sg.first));
+        w.n = max(0, (n - warp + kPdWarps - 1) / kPdWarps);
+        if (ok)
+            while (w.issued < min(w.n, kPdStages)) issue(sg, w, w.issued);
+        return w;
+    };
+    Copies w = begin_copies(g);
+    while (true) {
+        Query<NT> Q;
+        pd_query<NT, T>(P, Q, g.s, g.cb, g.h, r, c);
+        // columns' limits; columns behind the last row compute whatever they like
+        const int n_rows = g.s.n * P.gqa, row0 = g.cb * kCols, behind = g.s.len - g.s.n + 1;
+        int lim[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const int row = cb * kCols + 8 * nt + 2 * c + e, qp = row / P.gqa;
-                lim[nt][e] = qp >= s.n ? 0 : P.causal ? max(0, min(s.len, s.len - s.n + 1 + qp)) : s.len;
+                const int row = row0 + 8 * nt + 2 * c + e;
+                lim[nt][e] = P.causal && row < n_rows ? max(0, behind + row / P.gqa) : g.s.len;
             }
-        {
-            const int row1 = min(cb * kCols + kCols, s.n * P.gqa) - 1;
-            lim_max = P.causal ? max(0, s.len - s.n + 1 + row1 / P.gqa) : s.len;
-            lim_min = row1 + 1 < cb * kCols + kCols ? 0 : P.causal ? max(0, s.len - s.n + 1 + cb * kCols / P.gqa) : s.len;
-        }
-        const int n_batch = min((int)count, max(0, (lim_max + kBatchTok - 1) / kBatchTok - (int)first));
-        const int n_my = (n_batch - warp + kPdWarps - 1) / kPdWarps;      // batches first + warp, + 8, ...
-        const int n_units = (s.len + kUnitTok - 1) / kUnitTok;
-        int page_of = -1;                                                 // lane i: page of unit i % 2 of batch 16 * block + i / 2
-        auto load_pages = [&](int k0) {
-            const int k = k0 + (lane >> 1), unit = 2 * ((int)first + warp + kPdWarps * k) + (lane & 1);
-            page_of = -1;
-            if (k < n_my && unit < n_units) {
-                page_of = P.table[(int64_t)seq * P.tb_st + unit / P.pool.units];
-                if (page_of < 0 || page_of >= P.pool.n_pages) {
-                    page_of = -1;
-                    if (P.status) *P.status = kStatusBadPage;
-                }
-            }
-        };
-        uint32_t have[kPdStages] = {};                                    // which of a stage's two units are there
-        auto issue = [&](int k) {
-            if ((k & 15) == 0) load_pages(k);
-            const int page = __shfl_sync(0xffffffffu, page_of, 2 * (k & 15) + (lane & 1));
-            const uint32_t there = __ballot_sync(0xffffffffu, page >= 0) & 3u;
-            const int stage = issued % kPdStages;
-            uint64_t* bar = &S.full[warp][stage];
-            if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)__popc(there) * kUnitBytes);
-            __syncwarp();
-            if (lane < 2 && page >= 0) {
-                const int unit = 2 * ((int)first + warp + kPdWarps * k) + lane;
-                bulk_g2s_hint(S.ring[warp][stage] + lane * kUnitBytes,
-                              P.pool.pages + (int64_t)page * P.pool.page_stride + (int64_t)h * P.pool.head_stride + (unit % P.pool.units) * kUnitBytes,
-                              kUnitBytes, bar, policy);
-            }
-#pragma unroll
-            for (int i = 0; i < kPdStages; ++i)
-                if (i == stage) have[i] = there;
-            ++issued;
-        };
-        if (ok)
-            for (int k = 0; k < min(n_my, kPdStages); ++k) issue(k);
-        Query<NT> Q;
-        pd_query<NT, T>(P, Q, s, cb, h, r, c);
+        const int lim_min = P.causal ? max(0, behind + row0 / P.gqa) : g.s.len;
         State<NT> st = {};
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) st.m[nt][0] = st.m[nt][1] = -INFINITY;
-        for (int k = 0; k < n_my && ok; ++k) {
-            const int stage = taken % kPdStages;
-            if (!__all_sync(0xffffffffu, mbar_wait_bounded(&S.full[warp][stage], (taken / kPdStages) & 1u))) {
+        int t0 = (g.first + warp) * kBatchTok, stage = 0;
+        for (int k = 0; k < w.n && ok; ++k) {
+            if (!__all_sync(0xffffffffu, mbar_wait_bounded(&S.full[warp][stage], phases >> stage & 1u))) {
                 ok = false;
                 break;
             }
-            ++taken;
-            uint32_t there = 0;
-#pragma unroll
-            for (int i = 0; i < kPdStages; ++i)
-                if (i == stage) there = have[i];
-            const int t0 = ((int)first + warp + kPdWarps * k) * kBatchTok;
-            const uint32_t at = ring0 + stage * kBatchBytes;
+            phases ^= 1u << stage;
+            const uint32_t at = ring0 + stage * kBatchBytes, there = w.have >> (2 * stage) & 3u;
             if (there == 3u && t0 + kBatchTok <= lim_min) {
-                pd_unit<NT, false>(at, Q, st, r, c, t0, s.len, lim);
-                pd_unit<NT, false>(at + kUnitBytes, Q, st, r, c, t0 + kUnitTok, s.len, lim);
+                pd_unit<NT, false>(at, mg, Q, st, r, c, t0, g.s.len, lim);
+                pd_unit<NT, false>(at + kUnitBytes, mg, Q, st, r, c, t0 + kUnitTok, g.s.len, lim);
             } else {
 #pragma unroll 1
                 for (int i = 0; i < 2; ++i)
-                    if (there >> i & 1u) pd_unit<NT, true>(at + i * kUnitBytes, Q, st, r, c, t0 + i * kUnitTok, s.len, lim);
+                    if (there >> i & 1u) pd_unit<NT, true>(at + i * kUnitBytes, mg, Q, st, r, c, t0 + i * kUnitTok, g.s.len, lim);
             }
             __syncwarp();
-            if (k + kPdStages < n_my) issue(k + kPdStages);
+            if (w.issued < w.n) issue(g, w, stage);
+            t0 += kPdWarps * kBatchTok;
+            stage = stage == kPdStages - 1 ? 0 : stage + 1;
         }
-        if (!ok)             // copies in flight land before the ring is used again
-            for (; taken < issued; ++taken) mbar_wait_bounded(&S.full[warp][taken % kPdStages], (taken / kPdStages) & 1u);
-        // ---- the warps' states into shared memory (each into its own ring), merged by column ----
-        float* const mine = reinterpret_cast<float*>(S.ring[warp][0]);
+        if (!ok)             // copies in flight land before the CTA leaves; nothing more is fetched
+            for (int i = 0; i < kPdStages; ++i)
+                if (i < w.issued) mbar_wait_bounded(&S.full[warp][i], phases >> i & 1u);
+        // ---- what comes next, and its first copies ----
+        Segment next = g;
+        bool more = false;
+        uint32_t next_count = 0;
+        const uint32_t this_pos = pos;
+        if (kCluster) {
+            next.cb += P.n_cta;              // (only where a sequence has more rows than the caller said)
+            more = next.cb * kCols < g.s.n * P.gqa;
+        } else {
+            pos += count;
+            while (pos < end && pos - seq_start >= pd_work<NT>(P, next.s)) {
+                if (next.seq + 1 >= P.n_seq) {
+                    pos = end;
+                    break;
+                }
+                seq_start += pd_work<NT>(P, next.s);
+                next.s = pd_seq(P, ++next.seq);
+            }
+            more = pos < end;
+            if (more) {
+                const Segment keep = g;
+                g = next;
+                next_count = at_pos();
+                next = g;
+                g = keep;
+            }
+        }
+        if (more) w = begin_copies(next);
+        // ---- the warps' states merged by column ----
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -504,70 +621,88 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
                 if (r == 0) S.ml[warp][col] = make_float2(st.m[nt][e], l);
 #pragma unroll
                 for (int n = 0; n < 4; ++n)
-                    *reinterpret_cast<float4*>(mine + col * kOutRow + 32 * n + 4 * r) =
+                    *reinterpret_cast<float4*>(&S.o[warp][col][32 * n + 4 * r]) =
                         make_float4(st.o[nt][0][n][e], st.o[nt][0][n][2 + e], st.o[nt][1][n][e], st.o[nt][1][n][2 + e]);
             }
         __syncthreads();
-        const bool whole = first == 0 && count == nb;
+        if (kCluster && n_rank > 1) cluster_wait();          // (every CTA runs, and has read what it got before)
+        const uint32_t xo = smem_u32(smem_raw + sizeof(PdSmem<NT>)), xml = xo + n_rank * kCols * kHD * 4;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int col = 8 * nt + warp;
+            if (row0 + col >= n_rows) continue;
             float m = -INFINITY, l = 0.f;
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int w = 0; w < kPdWarps; ++w) m = fmaxf(m, S.ml[w][col].x);
+            for (int i = 0; i < kPdWarps; ++i) m = fmaxf(m, S.ml[i][col].x);
             const float z = m == -INFINITY ? 0.f : m;
 #pragma unroll
-            for (int w = 0; w < kPdWarps; ++w) {
-                const float2 ml = S.ml[w][col];
+            for (int i = 0; i < kPdWarps; ++i) {
+                const float2 ml = S.ml[i][col];
                 const float f = ex2(ml.x - z);
-                const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(S.ring[w][0]) + col * kOutRow + 4 * lane);
+                const float4 v = *reinterpret_cast<const float4*>(&S.o[i][col][4 * lane]);
                 l = fmaf(f, ml.y, l);
                 o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
             }
-            if (whole) {
-                pd_write<T>(P, s, cb, kCols, col, h, lane, o, m, l);
+            if (kCluster && n_rank > 1) {                    // to the CTA that finishes this column
+                const uint32_t owner = (uint32_t)col % n_rank, row = rank * kCols + col;
+                asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_addr(xo + row * kHD * 4 + 16 * lane, owner)), "f"(o.x),
+                             "f"(o.y), "f"(o.z), "f"(o.w)
+                             : "memory");
+                if (lane == 0)
+                    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(cluster_addr(xml + row * 8, owner)), "f"(m), "f"(l) : "memory");
+            } else if (g.whole) {
+                pd_write<T>(P, g.s, g.cb, kCols, col, g.h, lane, o, m, l);
             } else {
-                const size_t slot = (size_t)(2 * blockIdx.x + (pos == (uint32_t)begin ? 0 : 1)) * kCols + col;
+                const size_t slot = (size_t)(2 * blockIdx.x + (this_pos == begin ? 0 : 1)) * kCols + col;
                 *reinterpret_cast<float4*>(P.part_o + slot * kHD + 4 * lane) = o;
                 if (lane == 0) P.part_ml[slot] = make_float2(m, l);
             }
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // the ring: generic accesses, then bulk copies
-        __syncthreads();
-        pos += count;
-        while (pos < end && pos - seq_start >= pd_work<NT>(P, s)) {
-            if (seq + 1 >= P.n_seq) {
-                pos = end;
-                break;
+        if (kCluster && n_rank > 1) {
+            cluster_arrive();
+            cluster_wait();
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const int col = 8 * nt + warp;
+                if (row0 + col >= n_rows || (uint32_t)col % n_rank != rank) continue;
+                const float* po = reinterpret_cast<const float*>(smem_raw + sizeof(PdSmem<NT>));
+                const float2* pml = reinterpret_cast<const float2*>(po + n_rank * kCols * kHD);
+                float m = -INFINITY, l = 0.f;
+                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (uint32_t i = 0; i < n_rank; ++i) m = fmaxf(m, pml[i * kCols + col].x);
+                const float z = m == -INFINITY ? 0.f : m;
+#pragma unroll 4
+                for (uint32_t i = 0; i < n_rank; ++i) {
+                    const float2 ml = pml[i * kCols + col];
+                    const float f = ex2(ml.x - z);
+                    const float4 v = *reinterpret_cast<const float4*>(po + (i * kCols + col) * kHD + 4 * lane);
+                    l = fmaf(f, ml.y, l);
+                    o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
+                }
+                pd_write<T>(P, g.s, g.cb, kCols, col, g.h, lane, o, m, l);
             }
-            seq_start += pd_work<NT>(P, s);
-            s = pd_seq(P, ++seq);
         }
+        if (!more) break;
+        if (kCluster && n_rank > 1) cluster_arrive();
+        __syncthreads();                                     // (the states are read)
+        g = next;
+        count = next_count;
     }
     if (!ok && lane == 0 && P.status) *P.status = kStatusWaitTimeout;
 }
 
-// Block i: the triple that the end of CTA i's share cuts, if that is its first cut; and the rows of every n_cta-th sequence that has none
-// of its tokens cached.
+// Block (i, col): column col of the triple that the end of CTA i's share cuts, if that is its first cut.  Eight warps share the
+// partials, four of them requested at a time.
 template <int NT, typename T>
-__global__ void __launch_bounds__(512) pg_merge_kernel(const PdParams P) {
+__global__ void __launch_bounds__(256) pg_merge_kernel(const PdParams P) {
     __shared__ ScanSmem scan;
-    __shared__ float4 sum_o[16][32];
-    __shared__ float sum_l[16];
-    constexpr int kCols = 8 * NT, kPer = 16 / 8;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    __shared__ float4 sum_o[8][32];
+    __shared__ float sum_l[8];
+    constexpr int kCols = 8 * NT;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = blockIdx.y;
     grid_launch_dependents();
     grid_dependency_wait();
-    for (int i = blockIdx.x; i < P.n_seq; i += gridDim.x) {
-        const SeqInfo s = pd_seq(P, i);
-        if (s.len > 0) continue;
-        for (int row = warp; row < s.n * P.n_q; row += 16) {
-            const int pos = row / P.n_q, hq = row - pos * P.n_q;
-            *reinterpret_cast<uint2*>(reinterpret_cast<T*>(P.out) + (int64_t)(s.q0 + pos) * P.o_st + hq * P.o_sh + 4 * lane) = make_uint2(0, 0);
-            if (P.lse && lane == 0) P.lse[(int64_t)(s.q0 + pos) * P.n_q + hq] = -INFINITY;
-        }
-    }
     uint32_t total, seq_start, share = 0;
     int seq;
     pd_find<NT>(P, scan, total, seq, seq_start, [&](uint32_t t) {
@@ -577,65 +712,102 @@ __global__ void __launch_bounds__(512) pg_merge_kernel(const PdParams P) {
     const uint64_t cut = ((uint64_t)blockIdx.x + 1) * share;
     if (cut >= total || seq < 0) return;
     const SeqInfo s = pd_seq(P, seq);
-    const uint32_t nb = (uint32_t)((s.len + kBatchTok - 1) / kBatchTok);
-    const uint32_t triple = ((uint32_t)cut - seq_start) / nb, a = seq_start + triple * nb, b = a + nb;
+    if (s.len == 0) return;
+    const uint32_t np = pd_padded(s), triple = ((uint32_t)cut - seq_start) / np, a = seq_start + triple * np, b = a + np;
     if (a == (uint32_t)cut || a + share < (uint32_t)cut) return;              // not cut here, or not for the first time
     const int cb = (int)(triple / P.n_kv), h = (int)(triple - (uint32_t)cb * P.n_kv);
-    const int j0 = blockIdx.x, j1 = min(P.n_cta - 1, (int)((b - 1) / share));                   // CTAs that hold a part of it
-    auto slot_of = [&](int j) { return (size_t)(2 * j + (j == j0 && a != (uint32_t)j0 * share ? 1 : 0)) * kCols; };
-    const int part = warp & (kPer - 1);
-    for (int nt = 0; nt < NT; ++nt) {
-        const int col = 8 * nt + (warp / kPer);
-        float m = -INFINITY;
-        for (int j = j0 + lane; j <= j1; j += 32) m = fmaxf(m, P.part_ml[slot_of(j) + col].x);
+    const int j0 = blockIdx.x, j1 = min(P.n_cta - 1, (int)((b - 1) / share));      // CTAs that hold a part of it
+    const size_t slot0 = (size_t)(2 * j0 + (a != (uint32_t)j0 * share ? 1 : 0)) * kCols + col;
+    auto slot_of = [&](int j) { return j == j0 ? slot0 : (size_t)2 * j * kCols + col; };
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j = j0 + warp; j <= j1; j += 32) {
+        float2 ml[4];
+        float4 v[4];
 #pragma unroll
-        for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-        const float z = m == -INFINITY ? 0.f : m;
-        float l = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int j = j0 + part; j <= j1; j += kPer) {
-            const float2 ml = P.part_ml[slot_of(j) + col];
-            const float4 v = *reinterpret_cast<const float4*>(P.part_o + (slot_of(j) + col) * kHD + 4 * lane);
-            const float f = ex2(ml.x - z);
-            l = fmaf(f, ml.y, l);
-            o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
-        }
-        sum_o[warp][lane] = o;
-        if (lane == 0) sum_l[warp] = l;
-        __syncthreads();
-        if (part == 0) {
-#pragma unroll
-            for (int i = 1; i < kPer; ++i) {
-                const float4 v = sum_o[warp + i][lane];
-                o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
-                l += sum_l[warp + i];
+        for (int i = 0; i < 4; ++i) {
+            const bool there = j + 8 * i <= j1;
+            const size_t slot = there ? slot_of(j + 8 * i) : slot0;
+            ml[i] = P.part_ml[slot];
+            v[i] = *reinterpret_cast<const float4*>(P.part_o + slot * kHD + 4 * lane);
+            if (!there) {
+                ml[i] = make_float2(-INFINITY, 0.f);
+                v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
             }
-            pd_write<T>(P, s, cb, kCols, col, h, lane, o, m, l);
         }
-        __syncthreads();
+        const float top = fmaxf(m, fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)));
+        const float z = top == -INFINITY ? 0.f : top, f0 = ex2(m - z);
+        l *= f0;
+        o.x *= f0; o.y *= f0; o.z *= f0; o.w *= f0;
+        m = top;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float f = ex2(ml[i].x - z);
+            l = fmaf(f, ml[i].y, l);
+            o.x = fmaf(f, v[i].x, o.x); o.y = fmaf(f, v[i].y, o.y); o.z = fmaf(f, v[i].z, o.z); o.w = fmaf(f, v[i].w, o.w);
+        }
     }
+    __shared__ float sum_m[8];
+    sum_o[warp][lane] = o;
+    if (lane == 0) {
+        sum_l[warp] = l;
+        sum_m[warp] = m;
+    }
+    __syncthreads();
+    if (warp) return;
+    m = -INFINITY;
+    l = 0.f;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, sum_m[i]);
+    const float z = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float f = ex2(sum_m[i] - z);
+        const float4 v = sum_o[i][lane];
+        l = fmaf(f, sum_l[i], l);
+        o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
+    }
+    pd_write<T>(P, s, cb, kCols, col, h, lane, o, m, l);
 }
 
 template <int NT, typename T>
-int pd_launch(const PdParams& P, cudaStream_t stream) {
-    const int smem = (int)sizeof(PdSmem<NT>);
-    if (cudaFuncSetAttribute(pg_attend_kernel<NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return BGTQ_E_LAUNCH;
-    if (launch_kernel(pg_attend_kernel<NT, T>, dim3(P.n_cta), dim3(kPdThreads), smem, stream, true, P) != cudaSuccess) return BGTQ_E_LAUNCH;
-    return launch_kernel(pg_merge_kernel<NT, T>, dim3(P.n_cta), dim3(512), 0, stream, true, P) == cudaSuccess ? BGTQ_OK : BGTQ_E_LAUNCH;
+int pd_launch_split(const PdParams& P, bool merge, cudaStream_t stream) {
+    constexpr int smem = (int)sizeof(PdSmem<NT>);
+    const auto kernel = pg_attend_kernel<NT, T, false>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return BGTQ_E_LAUNCH;
+    if (launch_kernel(kernel, dim3(P.n_cta), dim3(kPdThreads), smem, stream, true, P) != cudaSuccess) return BGTQ_E_LAUNCH;
+    if (!merge) return BGTQ_OK;
+    const dim3 grid(P.n_cta - 1, P.cu_q ? 8 * NT : P.gqa);
+    return launch_kernel(pg_merge_kernel<NT, T>, grid, dim3(256), 0, stream, true, P) == cudaSuccess ? BGTQ_OK : BGTQ_E_LAUNCH;
+}
+template <int NT, typename T>
+int pd_launch_cluster(const PdParams& P, int64_t triples, int n_rank, cudaStream_t stream) {
+    const int smem = (int)sizeof(PdSmem<NT>) + (n_rank > 1 ? n_rank * 8 * NT * (kHD * 4 + 8) : 0);
+    const auto kernel = pg_attend_kernel<NT, T, true>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return BGTQ_E_LAUNCH;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(triples * n_rank));
+    cfg.blockDim = dim3(kPdThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = n_rank;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    if (cudaLaunchKernelEx(&cfg, kernel, P) != cudaSuccess || cudaGetLastError() != cudaSuccess) return BGTQ_E_LAUNCH;
+    return BGTQ_OK;
+}
+template <int NT, typename T>
+int pd_launch(const PdParams& P, const PdForm& f, cudaStream_t stream) {
+    return f.n_rank ? pd_launch_cluster<NT, T>(P, f.triples, f.n_rank, stream) : pd_launch_split<NT, T>(P, f.merge, stream);
 }
 
 bool aligned(const void* p, int64_t bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
-
-// CTAs of a launch: as many as are resident at once, no more than there can be shares of sequences of max_tokens.
-int pd_grid(int nt, int64_t blocks, int32_t n_kv, int64_t max_tokens) {
-    int dev = 0, sms = 148;
-    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    const double batches = (double)blocks * n_kv * (double)((max_tokens + kBatchTok - 1) / kBatchTok);
-    if (batches > 2.0e9) return (nt == 1 ? 2 : 1) * sms;
-    const int64_t most = ((int64_t)batches + kMinBatches - 1) / kMinBatches, resident = (nt == 1 ? 2 : 1) * sms;
-    return (int)(most < 1 ? 1 : most < resident ? most : resident);
-}
 
 }  // namespace
 }  // namespace bgtq
@@ -645,17 +817,33 @@ using namespace bgtq;
 // Column tiles of a product: eight query rows are the operand's width; more of them share what is read and unpacked.
 static int pd_tiles(int32_t n_q, int32_t n_kv, int32_t max_q) { return (int64_t)max_q * (n_q / n_kv) <= 8 ? 1 : 2; }
 
-// Column blocks of all sequences, at most.
-static int64_t pd_blocks(int nt, int32_t n_seq, int32_t n_tok, int32_t gqa) {
-    return n_tok <= n_seq ? n_seq : (int64_t)n_tok * gqa / (8 * nt) + n_seq;
+// How a call is launched, from its shape.
+static PdForm pd_form(int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv, int32_t max_q, int64_t max_tokens, int32_t flags) {
+    PdForm f{};
+    int dev = 0, sms = 148;
+    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    const int64_t gqa = n_q / n_kv;
+    f.nt = pd_tiles(n_q, n_kv, max_q);
+    const int64_t cols = 8 * f.nt, rounds = (max_tokens + kPdWarps * kBatchTok - 1) / (kPdWarps * kBatchTok);
+    f.blocks_of_seq = (int)((max_q * gqa + cols - 1) / cols);
+    f.triples = (int64_t)n_seq * n_kv * f.blocks_of_seq;
+    const int64_t resident = (f.nt == 1 ? 2 : 1) * (int64_t)sms;
+    // all sequences' column blocks together, at most
+    const int64_t blocks = n_tok <= n_seq ? n_seq : n_tok * gqa / cols + n_seq;
+    const double most = (double)blocks * n_kv * (double)rounds;
+    f.n_cta = (int)(most < 1 ? 1 : most < (double)resident ? most : (double)resident);
+    const int asked = (flags & BGTQ_PAGED_FORM_MASK) >> BGTQ_PAGED_FORM_SHIFT;
+    if (asked == 15) return f;
+    if (asked) f.n_rank = asked;
+    return f;
 }
 
 extern "C" __attribute__((visibility("default"))) int64_t bgtq_paged_workspace_bytes(int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv,
-                                                                                      int32_t max_q, int64_t max_tokens) {
+                                                                                      int32_t max_q, int64_t max_tokens, int32_t flags) {
     if (n_seq < 0 || n_tok < 0 || n_kv < 1 || n_q < 1 || n_q % n_kv || max_q < 1 || max_tokens < 0) return BGTQ_E_BADARG;
     if (n_q / n_kv > 8) return BGTQ_E_UNSUPPORTED;
-    const int nt = pd_tiles(n_q, n_kv, max_q);
-    return (int64_t)pd_grid(nt, pd_blocks(nt, n_seq, n_tok, n_q / n_kv), n_kv, max_tokens) * 2 * 8 * nt * (kHD * 4 + 8);
+    const PdForm f = pd_form(n_seq, n_tok, n_q, n_kv, max_q, max_tokens, flags);
+    return f.n_rank ? 0 : (int64_t)f.n_cta * 2 * 8 * f.nt * (kHD * 4 + 8);
 }
 
 extern "C" __attribute__((visibility("default"))) int bgtq_paged_attend(
@@ -663,8 +851,9 @@ extern "C" __attribute__((visibility("default"))) int bgtq_paged_attend(
     int32_t page_tokens, const int32_t* table, int64_t table_stride, int32_t table_cols, const int32_t* seq_lens, const int32_t* cu_q,
     int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv, int32_t max_q, int64_t max_tokens, float scale, int32_t flags,
     void* workspace, int64_t workspace_bytes, void* out, int64_t o_st, int64_t o_sh, float* lse, int32_t* status, void* stream) {
+    const int asked = (flags & BGTQ_PAGED_FORM_MASK) >> BGTQ_PAGED_FORM_SHIFT;
     if (n_seq < 0 || n_tok < 0 || n_kv < 1 || n_q < 1 || table_cols < 0 || max_q < 1 || max_tokens < 0 ||
-        (flags & ~(BGTQ_PAGED_BF16 | BGTQ_PAGED_CAUSAL)))
+        (flags & ~(BGTQ_PAGED_BF16 | BGTQ_PAGED_CAUSAL | BGTQ_PAGED_FORM_MASK)) || (asked & (asked - 1) && asked != 15))
         return BGTQ_E_BADARG;
     if (!(scale == scale) || n_q % n_kv) return BGTQ_E_BADARG;
     if (n_q / n_kv > 8) return BGTQ_E_UNSUPPORTED;
@@ -673,22 +862,23 @@ extern "C" __attribute__((visibility("default"))) int bgtq_paged_attend(
     if (!pages || n_pages < 1 || page_tokens < kUnitTok || page_tokens % kUnitTok || !q || !out || !seq_lens || (!table && table_cols > 0))
         return BGTQ_E_BADARG;
     const int64_t cap = (int64_t)table_cols * page_tokens;
-    if (cap > INT32_MAX - 64) return BGTQ_E_TOOBIG;
+    if (cap > INT32_MAX - 512) return BGTQ_E_TOOBIG;
     if (!aligned(pages, 16) || page_stride % 16 || head_stride % 16 || !aligned(q, 16) || q_st % 8 || q_sh % 8 || !aligned(out, 8) || o_st % 4 ||
         o_sh % 4 || !aligned(workspace, 16))
         return BGTQ_E_ALIGN;
-    const int nt = pd_tiles(n_q, n_kv, max_q);
-    const int64_t cols = 8 * nt, blocks = pd_blocks(nt, n_seq, n_tok, n_q / n_kv);
-    if ((double)blocks * n_kv * (double)((cap + kBatchTok - 1) / kBatchTok) > 2.0e9) return BGTQ_E_TOOBIG;      // (the list's 32 bits)
-    const int n_cta = pd_grid(nt, blocks, n_kv, max_tokens);
-    const int64_t need = (int64_t)n_cta * 2 * cols * (kHD * 4 + 8);
-    if (!workspace || workspace_bytes < need) return BGTQ_E_BADARG;
+    PdForm f = pd_form(n_seq, n_tok, n_q, n_kv, max_q, max_tokens, flags);
+    f.merge = cap > kPdWarps * kBatchTok && f.n_cta > 1;
+    const int64_t cols = 8 * f.nt, blocks = n_tok <= n_seq ? n_seq : (int64_t)n_tok * (n_q / n_kv) / cols + n_seq;
+    // the list's positions are 32 bits, and the grid's
+    if ((double)blocks * n_kv * (double)(cap / kBatchTok + kPdWarps) > 2.0e9 || (double)f.triples * 8 > 2.0e9) return BGTQ_E_TOOBIG;
+    const int64_t need = f.n_rank ? 0 : (int64_t)f.n_cta * 2 * cols * (kHD * 4 + 8);
+    if (need && (!workspace || workspace_bytes < need)) return BGTQ_E_BADARG;
     PdParams P{{pages, page_stride, head_stride, n_pages, page_tokens / kUnitTok}, q, q_st, q_sh, table, table_stride, seq_lens, cu_q,
-               table_cols, n_seq, n_tok, n_q, n_kv, n_q / n_kv, !cu_q || (flags & BGTQ_PAGED_CAUSAL) ? 1 : 0, n_cta,
+               table_cols, n_seq, n_tok, n_q, n_kv, n_q / n_kv, !cu_q || (flags & BGTQ_PAGED_CAUSAL) ? 1 : 0, f.n_rank ? f.blocks_of_seq : f.n_cta,
                scale * 1.44269504088896340736f, out, o_st, o_sh, lse, reinterpret_cast<float*>(workspace),
-               reinterpret_cast<float2*>(reinterpret_cast<float*>(workspace) + (int64_t)n_cta * 2 * cols * kHD), status};
+               reinterpret_cast<float2*>(reinterpret_cast<float*>(workspace) + (int64_t)f.n_cta * 2 * cols * kHD), status};
     const cudaStream_t st = (cudaStream_t)stream;
     const bool bf16 = flags & BGTQ_PAGED_BF16;
-    if (nt == 1) return bf16 ? pd_launch<1, __nv_bfloat16>(P, st) : pd_launch<1, __half>(P, st);
-    return bf16 ? pd_launch<2, __nv_bfloat16>(P, st) : pd_launch<2, __half>(P, st);
+    if (f.nt == 1) return bf16 ? pd_launch<1, __nv_bfloat16>(P, f, st) : pd_launch<1, __half>(P, f, st);
+    return bf16 ? pd_launch<2, __nv_bfloat16>(P, f, st) : pd_launch<2, __half>(P, f, st);
 }

@@ -20,6 +20,7 @@ __all__ = ["PAGE_UNIT_BYTES", "page_bytes", "paged_kv4_append", "paged_kv4_read"
 HD = 128
 UNIT = 16                       # tokens of a unit
 PAGE_UNIT_BYTES = 2304          # bytes of a unit of one KV head
+_FORM = 0                       # form of the attention's launch (bgtq.h, BGTQ_PAGED_FORM_SHIFT), 0: the library chooses
 _TYPES = {torch.float16: 0, torch.bfloat16: _lib.PAGED_BF16}
 
 
@@ -147,7 +148,7 @@ def paged_kv4_read(pages, slots, dtype=torch.float16, status=None):
 def _attend(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, causal, scale, return_lse, status, out):
     page = _pool(pages)
     dev, n_kv = pages.device, pages.shape[1]
-    flags = _type_flag(q.dtype, "q") | (_lib.PAGED_CAUSAL if causal else 0)
+    flags = _type_flag(q.dtype, "q") | (_lib.PAGED_CAUSAL if causal else 0) | _FORM << _lib.PAGED_FORM_SHIFT
     q = _rows(q, "q", None, None, q.dtype, dev, 16)
     n, n_q = q.shape[:2]
     if n_q < 1 or n_q % n_kv or n_q // n_kv > 8:
@@ -176,7 +177,7 @@ def _attend(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, causal, sc
     _lib.require_cuda(pages, "pages")
     if n and n_seq:
         with torch.cuda.device(dev):
-            need = lib.bgtq_paged_workspace_bytes(n_seq, n, n_q, n_kv, max_q, max_tokens)
+            need = lib.bgtq_paged_workspace_bytes(n_seq, n, n_q, n_kv, max_q, max_tokens, flags)
             if need < 0:
                 _lib.check(need, "bgtq_paged_workspace_bytes")
             ws = torch.empty(need, dtype=torch.uint8, device=dev)

@@ -625,6 +625,8 @@ int bgtq_decode_combined_noalloc(const BgtqDecodePlan* plan_host, const BgtqHead
 #define BGTQ_PAGED_BF16 1         /* q, k, v and outputs are bf16 instead of fp16 */
 #define BGTQ_PAGED_F32 2          /* bgtq_paged_read: fp32 outputs */
 #define BGTQ_PAGED_CAUSAL 4       /* bgtq_paged_attend with cu_q: query i sees the tokens up to its own position */
+#define BGTQ_PAGED_FORM_SHIFT 8   /* bgtq_paged_attend: 0 the library chooses; 1, 2, 4 or 8 << 8: clusters of so many CTAs per (sequence, KV */
+#define BGTQ_PAGED_FORM_MASK 0xF00  /* head, block of query rows); 15 << 8: one list of work over all CTAs and a launch that merges */
 
 /* Quantise and store n_tok tokens.  k / v element (i, h, d) at k + i * k_st + h * k_sh + d (strides multiples of 4 elements, 8-byte
  * aligned); token i goes to slot slots[i], nowhere when that is negative; the slots of a call are distinct.  rope_cos / rope_sin (may both
@@ -652,7 +654,7 @@ int bgtq_paged_read(const uint8_t* pages, int64_t page_stride, int64_t head_stri
  * whole).  workspace:
  * bgtq_paged_workspace_bytes(...) of the same arguments, 16-byte aligned, of no other call that may run at the same time. */
 int64_t bgtq_paged_workspace_bytes(int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv, int32_t max_q,
-                int64_t max_tokens);
+                int64_t max_tokens, int32_t flags);
 int bgtq_paged_attend(const void* q, int64_t q_st, int64_t q_sh, const uint8_t* pages, int64_t page_stride, int64_t head_stride,
                 int32_t n_pages, int32_t page_tokens, const int32_t* table, int64_t table_stride, int32_t table_cols,
                 const int32_t* seq_lens, const int32_t* cu_q, int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv,

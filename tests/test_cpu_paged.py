@@ -106,10 +106,10 @@ def test_library_refuses_before_it_touches_the_device():
         return lib.bgtq_paged_attend(*a.values())
     assert attend(n_seq=0, n=0) == _lib.OK
     for kw, code in ((dict(nq=3), -1), (dict(nq=18), -2), (dict(n=2), -1), (dict(max_q=2), -1), (dict(max_q=0), -1), (dict(cols=1 << 28), -5),
-                     (dict(q=p + 8), -3), (dict(qst=4), -3), (dict(out=p + 4), -3), (dict(ws=0), -1), (dict(wsb=16), -1), (dict(lens=0), -1),
+                     (dict(q=p + 8), -3), (dict(qst=4), -3), (dict(out=p + 4), -3), (dict(ws=0, flags=15 << 8), -1), (dict(wsb=16, flags=15 << 8), -1), (dict(flags=3 << 8), -1), (dict(lens=0), -1),
                      (dict(table=0), -1), (dict(scale=float("nan")), -1), (dict(flags=2), -1), (dict(pages=p + 1), -3)):
         assert attend(**kw) == code, kw
-    assert lib.bgtq_paged_workspace_bytes(1, 1, 18, 2, 1, 10) == -2 and lib.bgtq_paged_workspace_bytes(1, 1, 3, 2, 1, 10) == -1
+    assert lib.bgtq_paged_workspace_bytes(1, 1, 18, 2, 1, 10, 0) == -2 and lib.bgtq_paged_workspace_bytes(1, 1, 3, 2, 1, 10, 0) == -1
 
 
 def test_values_are_exact_in_half_precision():

@@ -128,6 +128,13 @@ def test_slots_and_positions_out_of_range_are_reported_and_store_nothing():
     assert status.item() == 2 and not k[0].any() and k[1].any()
 
 
+@pytest.fixture(params=["auto", "split", 1, 2, 8])
+def form(request, monkeypatch):
+    """The forms that the attention's launch has; the library chooses one by the call's shape."""
+    from blockgtq_b200 import paged
+    monkeypatch.setattr(paged, "_FORM", {"auto": 0, "split": 15}.get(request.param, request.param))
+
+
 def _check(got, lse, ref, rows):
     out, want_lse, tol, tol_lse = ref
     g = got[rows].double().cpu()
@@ -145,7 +152,7 @@ def _check(got, lse, ref, rows):
 @pytest.mark.parametrize("n_kv,gqa,page,lens", [
     (1, 1, 16, [1]), (2, 4, 64, [0, 1, 15, 16, 17]), (2, 8, 16, [33, 0, 0, 300]), (1, 7, 48, [500, 31, 32]), (8, 2, 128, [257, 129]),
     (1, 3, 32, [2000]), (4, 1, 64, [63, 64, 65, 640])])
-def test_decode_against_64_bits(dtype, n_kv, gqa, page, lens):
+def test_decode_against_64_bits(dtype, n_kv, gqa, page, lens, form):
     from blockgtq_b200 import paged_kv4_decode_attention
     gen = torch.Generator().manual_seed(sum(lens) + gqa)
     pages, table, slots = _case(gen, n_kv, page, lens, dtype=dtype)
@@ -169,7 +176,7 @@ def test_decode_of_bf16_queries_of_any_magnitude(magnitude):
     _check(out, lse, R.attention(q, pages.cpu(), slots[0], [70], torch.tensor(scale).item()), slice(0, 1))
 
 
-def test_decode_of_many_sequences_and_of_one_long_one_cut_between_ctas():
+def test_decode_of_many_sequences_and_of_one_long_one_cut_between_ctas(form):
     from blockgtq_b200 import paged_kv4_decode_attention
     gen = torch.Generator().manual_seed(11)
     lens = [int(x) for x in torch.randint(0, 40, (700,), generator=gen)]
@@ -191,7 +198,7 @@ PREFILLS = [
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n_kv,gqa,page,seqs", PREFILLS)
-def test_prefill_against_64_bits(dtype, n_kv, gqa, page, seqs, causal):
+def test_prefill_against_64_bits(dtype, n_kv, gqa, page, seqs, causal, form):
     from blockgtq_b200 import paged_kv4_prefill_attention
     lens, counts = [t for t, _ in seqs], [n for _, n in seqs]
     gen = torch.Generator().manual_seed(sum(lens) + gqa)
@@ -210,7 +217,7 @@ def test_prefill_against_64_bits(dtype, n_kv, gqa, page, seqs, causal):
         _check(out, lse, R.attention(q[ends[b]:ends[b + 1]], host, slots[b], seen, 1 / math.sqrt(128)), slice(ends[b], ends[b + 1]))
 
 
-def test_a_page_number_outside_the_pool_leaves_its_tokens_out():
+def test_a_page_number_outside_the_pool_leaves_its_tokens_out(form):
     from blockgtq_b200 import paged_kv4_decode_attention
     gen = torch.Generator().manual_seed(2)
     pages, table, slots = _case(gen, 1, 16, [40, 40])
@@ -226,6 +233,20 @@ def test_a_page_number_outside_the_pool_leaves_its_tokens_out():
         _check(out, lse, R.attention(q[1:], pages.cpu(), slots[1], [40], 1 / math.sqrt(128)), slice(1, 2))
 
 
+def test_more_rows_and_tokens_than_the_caller_said_are_attended_all_the_same(form):
+    from blockgtq_b200 import paged_kv4_prefill_attention
+    gen = torch.Generator().manual_seed(17)
+    lens, counts = [700, 90, 300], [40, 7, 1]
+    pages, table, slots = _case(gen, 2, 16, lens)
+    q = _noise(gen, sum(counts), 8, 128).half()
+    ends = [0, 40, 47, 48]
+    out, lse = paged_kv4_prefill_attention(q.to(DEV), pages, table.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV),
+                                           torch.tensor(ends, dtype=torch.int32, device=DEV), max_q_len=2, max_seq_len=16, return_lse=True)
+    host = pages.cpu()
+    for b, (t, m) in enumerate(zip(lens, counts)):
+        _check(out, lse, R.attention(q[ends[b]:ends[b + 1]], host, slots[b], [t - m + 1 + i for i in range(m)], 1 / math.sqrt(128)), slice(ends[b], ends[b + 1]))
+
+
 def test_a_length_beyond_the_table_is_held_to_it():
     from blockgtq_b200 import paged_kv4_decode_attention
     gen = torch.Generator().manual_seed(2)
@@ -236,7 +257,7 @@ def test_a_length_beyond_the_table_is_held_to_it():
         _check(out, lse, R.attention(q, pages.cpu(), slots[0], [min(32, t)], 1 / math.sqrt(128)), slice(0, 1))
 
 
-def test_no_number_in_a_row_shows_and_in_a_hidden_place_does_not():
+def test_no_number_in_a_row_shows_and_in_a_hidden_place_does_not(form):
     from blockgtq_b200 import paged_kv4_append, paged_kv4_decode_attention, paged_kv4_prefill_attention
     gen = torch.Generator().manual_seed(9)
     pages, table, slots = _case(gen, 1, 16, [40])
