@@ -187,15 +187,21 @@ __device__ __forceinline__ float lg2(float x) {
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-    return v;
+// (as in bgtq_common.cuh, but not volatile: the compiler may move them among one another)
+__device__ __forceinline__ void mma_acc(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-    uint2 v;
-    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
-    return v;
+__device__ __forceinline__ void mma_new(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]), "f"(0.f));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t a) {
+    uint32_t d;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
 }
 // Two constants that one instruction takes beside a mask or a factor: held in registers (two of them cannot be immediates).
 struct Magic {
@@ -282,17 +288,17 @@ struct State {
     float m[NT][2], l[NT][2];
 };
 
+template <typename V> __device__ __forceinline__ V at(const uint8_t* p) { return *reinterpret_cast<const V*>(p); }
 template <int N> struct Int { static constexpr int value = N; };
 template <typename F> __device__ __forceinline__ void each_group(F f) { f(Int<0>{}); f(Int<1>{}); f(Int<2>{}); f(Int<3>{}); }
 
-// 16 tokens at shared address u.  kEdge: some of them (tokens from len on of the sequence, from lim[] on of a column) are hidden.
+// 16 tokens at u in shared memory.  kEdge: some of them (tokens from len on of the sequence, from lim[] on of a column) are hidden.
 template <int NT, bool kEdge>
-__device__ __forceinline__ void pd_unit(uint32_t u, const Magic& mg, const Query<NT>& Q, State<NT>& st, int r, int c, int t0, int len, const int (&lim)[NT][2]) {
+__device__ __forceinline__ void pd_unit(const uint8_t* u, const Magic& mg, const Query<NT>& Q, State<NT>& st, int r, int c, int t0, int len, const int (&lim)[NT][2]) {
     float s[NT][4];
     {
-        const uint32_t kb = u + r * 64 + c * 16;
-        const uint4 x = lds128(kb), y = lds128(kb + 512);
-        const uint2 ka = lds64(u + kUnitKs + r * 8), kc = lds64(u + kUnitKs + 64 + r * 8);
+        const uint4 x = at<uint4>(u + r * 64 + c * 16), y = at<uint4>(u + 512 + r * 64 + c * 16);
+        const uint2 ka = at<uint2>(u + kUnitKs + r * 8), kc = at<uint2>(u + kUnitKs + 64 + r * 8);
         const float sa[4] = {pg_lo(ka.x), pg_hi(ka.x), pg_lo(ka.y), pg_hi(ka.y)};
         const float sc[4] = {pg_lo(kc.x), pg_hi(kc.x), pg_lo(kc.y), pg_hi(kc.y)};
         const uint4 x8 = make_uint4(x.x >> 8, x.y >> 8, x.z >> 8, x.w >> 8), y8 = make_uint4(y.x >> 8, y.y >> 8, y.z >> 8, y.w >> 8);
@@ -304,8 +310,8 @@ __device__ __forceinline__ void pd_unit(uint32_t u, const Magic& mg, const Query
             for (int nt = 0; nt < NT; ++nt) {
                 float acc[4];
                 const uint32_t b0[2] = {Q.b[nt][g][0], Q.b[nt][g][1]}, b1[2] = {Q.b[nt][g][2], Q.b[nt][g][3]};
-                mma_16816_z(acc, a0, b0);
-                mma_16816(acc, a1, b1);
+                mma_new(acc, a0, b0);
+                mma_acc(acc, a1, b1);
                 if (g == 0) {
                     s[nt][0] = acc[0] * sa[g]; s[nt][1] = acc[1] * sa[g];
                     s[nt][2] = acc[2] * sc[g]; s[nt][3] = acc[3] * sc[g];
@@ -316,7 +322,7 @@ __device__ __forceinline__ void pd_unit(uint32_t u, const Magic& mg, const Query
             }
         });
     }
-    uint2 va = lds64(u + kUnitVs + r * 8), vc = lds64(u + kUnitVs + 64 + r * 8);
+    uint2 va = at<uint2>(u + kUnitVs + r * 8), vc = at<uint2>(u + kUnitVs + 64 + r * 8);
     if (kEdge) {
         if (t0 + r >= len) va = make_uint2(0, 0);               // what lies behind the sequence may be anything
         if (t0 + 8 + r >= len) vc = make_uint2(0, 0);
@@ -370,8 +376,7 @@ __device__ __forceinline__ void pd_unit(uint32_t u, const Magic& mg, const Query
             p[nt][2 + e] = ex2(fmaf(s[nt][2 + e], Q.f[nt][e], -z));
             st.l[nt][e] += p[nt][e] + p[nt][2 + e];
         }
-    const uint32_t vb = u + kUnitV + c * 128 + r * 16;
-    const uint4 x = lds128(vb), y = lds128(vb + 512);
+    const uint4 x = at<uint4>(u + kUnitV + c * 128 + r * 16), y = at<uint4>(u + kUnitV + 512 + c * 128 + r * 16);
     const uint4 x8 = make_uint4(x.x >> 8, x.y >> 8, x.z >> 8, x.w >> 8), y8 = make_uint4(y.x >> 8, y.y >> 8, y.z >> 8, y.w >> 8);
     each_group([&](auto gi) {
         constexpr int g = decltype(gi)::value;
@@ -384,9 +389,9 @@ __device__ __forceinline__ void pd_unit(uint32_t u, const Magic& mg, const Query
 #pragma unroll
                 for (int e = 0; e < 4; ++e) w[e] = s[nt][e] == -INFINITY ? 0.f : w[e];
             }
-            const uint32_t b[2] = {movmatrix_trans(pack_half2(w[0], w[1])), movmatrix_trans(pack_half2(w[2], w[3]))};
-            mma_16816(st.o[nt][0][g], a0, b);
-            mma_16816(st.o[nt][1][g], a1, b);
+            const uint32_t b[2] = {transposed(pack_half2(w[0], w[1])), transposed(pack_half2(w[2], w[3]))};
+            mma_acc(st.o[nt][0][g], a0, b);
+            mma_acc(st.o[nt][1][g], a1, b);
         }
     });
 }
@@ -504,7 +509,6 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
     uint32_t phases = 0;                   // of this warp's stages
     bool ok = true;
     const Magic mg = pd_magic();
-    const uint32_t ring0 = smem_u32(S.ring[warp][0]);
     const uint64_t policy = l2_evict_first_policy();
     auto issue = [&](const Segment& sg, Copies& w, int stage) {
         const int k = w.issued++;
@@ -563,14 +567,15 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
                 break;
             }
             phases ^= 1u << stage;
-            const uint32_t at = ring0 + stage * kBatchBytes, there = w.have >> (2 * stage) & 3u;
+            const uint8_t* const tile = S.ring[warp][stage];
+            const uint32_t there = w.have >> (2 * stage) & 3u;
             if (there == 3u && t0 + kBatchTok <= lim_min) {
-                pd_unit<NT, false>(at, mg, Q, st, r, c, t0, g.s.len, lim);
-                pd_unit<NT, false>(at + kUnitBytes, mg, Q, st, r, c, t0 + kUnitTok, g.s.len, lim);
+                pd_unit<NT, false>(tile, mg, Q, st, r, c, t0, g.s.len, lim);
+                pd_unit<NT, false>(tile + kUnitBytes, mg, Q, st, r, c, t0 + kUnitTok, g.s.len, lim);
             } else {
 #pragma unroll 1
                 for (int i = 0; i < 2; ++i)
-                    if (there >> i & 1u) pd_unit<NT, true>(at + i * kUnitBytes, mg, Q, st, r, c, t0 + i * kUnitTok, g.s.len, lim);
+                    if (there >> i & 1u) pd_unit<NT, true>(tile + i * kUnitBytes, mg, Q, st, r, c, t0 + i * kUnitTok, g.s.len, lim);
             }
             __syncwarp();
             if (w.issued < w.n) issue(g, w, stage);
