@@ -195,9 +195,12 @@ def lib():
     if built_for != _build.native_abi():
         raise RuntimeError(f"{_build.NATIVE} was built for {built_for}, this is {_build.native_abi()}: rebuild it "
                            "(python -m blockgtq_b200.build --force)")
-    module.bind(*[C.cast(getattr(handle, name), C.c_void_p).value for name in (
-        "bgtq_layer_step", "bgtq_layer_encode", "bgtq_attend", "bgtq_decode_default_splits", "bgtq_encode", "bgtq_rotate_q_rows",
-        "bgtq_prefill", "bgtq_prefill_workspace_bytes")])
+    def addresses(*names):
+        return [C.cast(getattr(handle, name), C.c_void_p).value for name in names]
+
+    module.bind(*addresses("bgtq_layer_step", "bgtq_layer_encode", "bgtq_attend", "bgtq_decode_default_splits", "bgtq_encode",
+                           "bgtq_rotate_q_rows", "bgtq_prefill", "bgtq_prefill_workspace_bytes"))
+    module.bind_paged(*addresses("bgtq_paged_append", "bgtq_paged_read", "bgtq_paged_attend", "bgtq_paged_workspace_bytes"))
     native = module
     _lib = handle
     return _lib

@@ -31,6 +31,12 @@ struct Fns {
     decltype(&bgtq_prefill) prefill;
     decltype(&bgtq_prefill_workspace_bytes) prefill_workspace;
 } F;
+struct PagedFns {
+    decltype(&bgtq_paged_append) paged_append;
+    decltype(&bgtq_paged_read) paged_read;
+    decltype(&bgtq_paged_attend) paged_attend;
+    decltype(&bgtq_paged_workspace_bytes) paged_workspace;
+} G;
 
 PyObject* none() { Py_RETURN_NONE; }
 PyObject* code(int rc) { return PyLong_FromLong(rc); }
@@ -304,18 +310,139 @@ PyObject* prefill(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     return rc == BGTQ_OK ? wrap(std::move(out)) : code(rc);
 }
 
-// bind(addresses in the order of Fns)
-PyObject* bind(PyObject*, PyObject* const* argv, Py_ssize_t n) {
-    if (n != (Py_ssize_t)(sizeof(F) / sizeof(void*))) {
+// ---- the paged 4-bit cache ----
+constexpr int64_t kUnit = 2304;
+
+// The pool: u8 (n_pages, n_kv, page bytes) on the current device, rows on 16-byte boundaries.
+bool pool_ok(const at::Tensor* p) {
+    return is(p, 3, at::kByte) && here(*p) && p->size(0) > 0 && p->size(0) <= INT32_MAX && p->size(1) > 0 && p->size(2) > 0 &&
+           p->size(2) % kUnit == 0 && ((reinterpret_cast<uintptr_t>(p->data_ptr()) | (uint64_t)(p->stride(0) | p->stride(1))) & 15u) == 0;
+}
+int page_tokens(const at::Tensor& p) { return (int)(p.size(2) / kUnit * 16); }
+// rows (n, heads, 128) of a 16-bit type whose addresses are multiples of `bytes`
+bool rows_ok(const at::Tensor* x, at::ScalarType type, int64_t bytes) {
+    return is(x, 3, type) && here(*x) && x->size(2) == kHD && x->size(0) <= INT32_MAX &&
+           ((reinterpret_cast<uintptr_t>(x->data_ptr()) | (uint64_t)(2 * (x->stride(0) | x->stride(1)))) & (uint64_t)(bytes - 1)) == 0;
+}
+bool vec_ok(const at::Tensor* x, at::ScalarType type, int64_t n) { return is(x, 1, type) && here(*x) && x->size(0) == n; }
+bool half_type(const at::Tensor* x) { return x && (x->scalar_type() == at::kHalf || x->scalar_type() == at::kBFloat16); }
+bool status_ok(const at::Tensor* x) { return !x || (x->is_cuda() && here(*x) && x->scalar_type() == at::kInt && x->numel() > 0); }
+int32_t* status_ptr(const at::Tensor* x) { return x ? x->data_ptr<int32_t>() : nullptr; }
+
+// paged_append(pages, slots, k, v, q | None, cos | None, sin | None, positions | None, status | None) -> rotated q | code | None
+PyObject* paged_append(PyObject*, PyObject* const* argv, Py_ssize_t n) {
+    if (n != 9) return none();
+    const Args A{argv};
+    bool bad = false;
+    const at::Tensor *pages = A.tensor(0, bad), *slots = A.tensor(1, bad), *k = A.tensor(2, bad), *v = A.tensor(3, bad), *q = A.tensor(4, bad),
+                     *cs = A.tensor(5, bad), *sn = A.tensor(6, bad), *pos = A.tensor(7, bad), *status = A.tensor(8, bad);
+    if (bad || !pool_ok(pages) || !half_type(k) || !rows_ok(k, k->scalar_type(), 8) || !rows_ok(v, k->scalar_type(), 8) || !status_ok(status))
+        return none();
+    const int64_t m = k->size(0), n_kv = pages->size(1);
+    if (k->size(1) != n_kv || v->size(0) != m || v->size(1) != n_kv || !vec_ok(slots, at::kLong, m)) return none();
+    if (!cs != !sn || !cs != !pos || (q && !cs)) return none();
+    if (cs) {
+        for (const at::Tensor* t : {cs, sn})
+            if (!is(t, 2, at::kFloat) || !here(*t) || t->size(1) != kHD / 2 || t->size(0) < 1 || t->size(0) != cs->size(0) || t->size(0) > INT32_MAX ||
+                t->stride(0) != cs->stride(0) || t->stride(0) % 4 || reinterpret_cast<uintptr_t>(t->data_ptr()) % 16)
+                return none();
+        if (!vec_ok(pos, at::kLong, m)) return none();
+    }
+    if (q && (!rows_ok(q, k->scalar_type(), 8) || q->size(0) != m || q->size(1) < 1)) return none();
+    at::Tensor out;
+    if (q) out = empty(q->sizes(), q->scalar_type(), *q);
+    const int n_q = q ? (int)q->size(1) : 0, flags = k->scalar_type() == at::kBFloat16 ? BGTQ_PAGED_BF16 : 0;
+    void* const st = stream_of(*pages);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = G.paged_append(pages->data_ptr<uint8_t>(), pages->stride(0), pages->stride(1), (int)pages->size(0), page_tokens(*pages),
+                        slots->data_ptr<int64_t>(), k->data_ptr(), k->stride(0), k->stride(1), v->data_ptr(), v->stride(0), v->stride(1),
+                        q ? q->data_ptr() : nullptr, q ? q->stride(0) : 0, q ? q->stride(1) : 0, q ? out.data_ptr() : nullptr,
+                        cs ? cs->data_ptr<float>() : nullptr, cs ? sn->data_ptr<float>() : nullptr, cs ? cs->stride(0) : 0,
+                        cs ? pos->data_ptr<int64_t>() : nullptr, cs ? (int)cs->size(0) : 0, (int)m, (int)n_kv, n_q, flags, status_ptr(status), st);
+    Py_END_ALLOW_THREADS
+    return rc == BGTQ_OK && q ? wrap(std::move(out)) : code(rc);
+}
+
+// paged_read(pages, slots, kind (0 fp16, 1 bf16, 2 fp32), status | None) -> (k, v) | code | None
+PyObject* paged_read(PyObject*, PyObject* const* argv, Py_ssize_t n) {
+    if (n != 4) return none();
+    const Args A{argv};
+    const int kind = A.i32(2);
+    bool bad = false;
+    const at::Tensor *pages = A.tensor(0, bad), *slots = A.tensor(1, bad), *status = A.tensor(3, bad);
+    if (bad || !pool_ok(pages) || !is(slots, 1, at::kLong) || !here(*slots) || slots->size(0) > INT32_MAX || !status_ok(status)) return none();
+    const int64_t m = slots->size(0), n_kv = pages->size(1);
+    const at::ScalarType type = kind == 0 ? at::kHalf : kind == 1 ? at::kBFloat16 : at::kFloat;
+    at::Tensor k = empty({m, n_kv, kHD}, type, *pages), v = empty({m, n_kv, kHD}, type, *pages);
+    void* const st = stream_of(*pages);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = G.paged_read(pages->data_ptr<uint8_t>(), pages->stride(0), pages->stride(1), (int)pages->size(0), page_tokens(*pages),
+                      slots->data_ptr<int64_t>(), (int)m, (int)n_kv, k.data_ptr(), v.data_ptr(),
+                      kind == 0 ? 0 : kind == 1 ? BGTQ_PAGED_BF16 : BGTQ_PAGED_F32, status_ptr(status), st);
+    Py_END_ALLOW_THREADS
+    if (rc != BGTQ_OK) return code(rc);
+    return Py_BuildValue("(NN)", wrap(std::move(k)), wrap(std::move(v)));
+}
+
+// paged_attend(q, pages, block_table, seq_lens, cu_q | None, max_q, max_tokens (< 0: what the table holds), scale, flags, want_lse,
+//              status | None, out | None) -> out | (out, lse) | code | None
+PyObject* paged_attend(PyObject*, PyObject* const* argv, Py_ssize_t n) {
+    if (n != 12) return none();
+    const Args A{argv};
+    const int64_t max_q = A.num(5);
+    int64_t most = A.num(6);
+    const float scale = A.real(7);
+    int flags = A.i32(8);
+    const bool want_lse = A.truth(9);
+    bool bad = false;
+    const at::Tensor *q = A.tensor(0, bad), *pages = A.tensor(1, bad), *table = A.tensor(2, bad), *lens = A.tensor(3, bad), *cu = A.tensor(4, bad),
+                     *status = A.tensor(10, bad), *given = A.tensor(11, bad);
+    if (bad || !pool_ok(pages) || !half_type(q) || !rows_ok(q, q->scalar_type(), 16) || !is(table, 2, at::kInt) || !here(*table) || !status_ok(status))
+        return none();
+    const int64_t m = q->size(0), n_q = q->size(1), n_kv = pages->size(1), n_seq = table->size(0), cap = table->size(1) * page_tokens(*pages);
+    if (m < 1 || n_seq < 1 || n_seq > INT32_MAX || n_q < 1 || n_q % n_kv || n_q / n_kv > 8 || cap > INT32_MAX || !vec_ok(lens, at::kInt, n_seq) ||
+        (cu ? !vec_ok(cu, at::kInt, n_seq + 1) : m != n_seq) || max_q < 1 || max_q > INT32_MAX || scale != scale)
+        return none();
+    if (given && (!rows_ok(given, q->scalar_type(), 8) || given->sizes() != q->sizes())) return none();
+    if (most < 0 || most > cap) most = cap;
+    if (q->scalar_type() == at::kBFloat16) flags |= BGTQ_PAGED_BF16;
+    const int64_t need = G.paged_workspace((int)n_seq, (int)m, (int)n_q, (int)n_kv, (int)max_q, most, flags);
+    if (need < 0) return code((int)need);
+    at::Tensor out = given ? *given : empty(q->sizes(), q->scalar_type(), *q), ws, lse;
+    if (need) ws = empty({need}, at::kByte, *q);
+    if (want_lse) lse = empty({m, n_q}, at::kFloat, *q);
+    void* const st = stream_of(*q);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = G.paged_attend(q->data_ptr(), q->stride(0), q->stride(1), pages->data_ptr<uint8_t>(), pages->stride(0), pages->stride(1),
+                        (int)pages->size(0), page_tokens(*pages), table->data_ptr<int32_t>(), table->stride(0), (int)table->size(1),
+                        lens->data_ptr<int32_t>(), cu ? cu->data_ptr<int32_t>() : nullptr, (int)n_seq, (int)m, (int)n_q, (int)n_kv, (int)max_q, most,
+                        scale, flags, need ? ws.data_ptr() : nullptr, need, out.data_ptr(), out.stride(0), out.stride(1),
+                        want_lse ? lse.data_ptr<float>() : nullptr, status_ptr(status), st);
+    Py_END_ALLOW_THREADS
+    if (rc != BGTQ_OK) return code(rc);
+    PyObject* const o = wrap(std::move(out));
+    return want_lse ? Py_BuildValue("(NN)", o, wrap(std::move(lse))) : o;
+}
+
+template <typename T>
+PyObject* bind_to(T& fns, PyObject* const* argv, Py_ssize_t n) {
+    constexpr Py_ssize_t count = sizeof(T) / sizeof(void*);
+    if (n != count) {
         PyErr_SetString(PyExc_ValueError, "bind: wrong number of addresses");
         return nullptr;
     }
     const Args A{argv};
-    void* fns[sizeof(F) / sizeof(void*)];
-    for (Py_ssize_t i = 0; i < n; ++i) fns[i] = A.ptr<void>((int)i);
-    memcpy(&F, fns, sizeof(F));
+    void* at[count];
+    for (Py_ssize_t i = 0; i < n; ++i) at[i] = A.ptr<void>((int)i);
+    memcpy(&fns, at, sizeof(T));
     return none();
 }
+// bind(addresses in the order of Fns), bind_paged(in the order of PagedFns)
+PyObject* bind(PyObject*, PyObject* const* argv, Py_ssize_t n) { return bind_to(F, argv, n); }
+PyObject* bind_paged(PyObject*, PyObject* const* argv, Py_ssize_t n) { return bind_to(G, argv, n); }
 
 // Library errors raised by torch (an allocation that fails) become Python exceptions.
 template <PyObject* (*FN)(PyObject*, PyObject* const*, Py_ssize_t)>
@@ -337,7 +464,8 @@ PyObject* guarded(PyObject* self, PyObject* const* argv, Py_ssize_t n) {
 
 #define BGTQ_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<name>)), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {BGTQ_METHOD(bind),   BGTQ_METHOD(layer_step),  BGTQ_METHOD(layer_encode), BGTQ_METHOD(encode), BGTQ_METHOD(compress),
-                          BGTQ_METHOD(attend), BGTQ_METHOD(rotate_rows), BGTQ_METHOD(prefill),      {nullptr, nullptr, 0, nullptr}};
+                          BGTQ_METHOD(attend), BGTQ_METHOD(rotate_rows), BGTQ_METHOD(prefill),      BGTQ_METHOD(paged_append), BGTQ_METHOD(paged_read),
+                          BGTQ_METHOD(paged_attend), BGTQ_METHOD(bind_paged), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -15,6 +15,8 @@
 #pragma once
 #include <cuda_bf16.h>
 
+#include <atomic>
+
 #include "bgtq_common.cuh"
 
 namespace bgtq {
@@ -49,5 +51,17 @@ template <> struct PgType<__nv_bfloat16> {
         return d;
     }
 };
+
+// Lets a kernel use this much dynamic shared memory, once per device.
+template <typename K>
+inline bool pg_allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return false;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (bit & done.load(std::memory_order_relaxed)) return true;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return true;
+}
 
 }  // namespace bgtq

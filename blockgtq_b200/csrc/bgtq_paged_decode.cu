@@ -28,7 +28,6 @@ namespace {
 constexpr int kPdWarps = 8, kPdThreads = 32 * kPdWarps;
 constexpr int kBatchTok = 32;
 constexpr int kBatchBytes = kBatchTok / kUnitTok * kUnitBytes;
-constexpr int kPdStages = 2;
 constexpr float kLift = 6.f, kReach = 14.f;       // log2 of P * vs at a reference's setting, and where it moves
 constexpr int kOutRow = 132;                      // floats between columns of a warp's state in shared memory
 
@@ -56,6 +55,7 @@ struct PdForm {
     int nt, n_cta, n_rank, blocks_of_seq;       // n_rank: CTAs of a triple's cluster, 0: the split form
     int64_t triples;
     bool merge;                                 // split: triples may be cut (those of one round never are)
+    bool alone;                                 // cluster: every CTA has an SM for itself
 };
 
 struct SeqInfo {
@@ -227,12 +227,12 @@ __device__ __forceinline__ uint32_t codes(const Magic& m, uint32_t w, uint32_t w
     return d;
 }
 
-template <int NT>
+template <int NT, int kStages>
 struct PdSmem {
-    __align__(128) uint8_t ring[kPdWarps][kPdStages][kBatchBytes];
+    __align__(128) uint8_t ring[kPdWarps][kStages][kBatchBytes];
     __align__(16) float o[kPdWarps][8 * NT][kOutRow];        // the warps' states at a triple's end
     float2 ml[kPdWarps][8 * NT];
-    __align__(8) uint64_t full[kPdWarps][kPdStages];
+    __align__(8) uint64_t full[kPdWarps][kStages];
     ScanSmem scan;
     // cluster form: [rank][8 NT columns][128] and [rank][8 NT] (reference, denominator) follow
 };
@@ -429,13 +429,15 @@ __device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {
     return a;
 }
 
-template <int NT, typename T, bool kCluster>
+// kStages 2: two CTAs on an SM hide each other's latencies.  4: one CTA on an SM, alone with them.
+template <int NT, typename T, bool kCluster, int kStages>
 __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(const PdParams P) {
     extern __shared__ __align__(128) uint8_t smem_raw[];
-    PdSmem<NT>& S = *reinterpret_cast<PdSmem<NT>*>(smem_raw);
+    using Smem = PdSmem<NT, kStages>;
+    Smem& S = *reinterpret_cast<Smem*>(smem_raw);
     constexpr int kCols = 8 * NT;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, c = lane & 3;
-    if (lane < kPdStages) {                // each warp waits on its own
+    if (lane < kStages) {                // each warp waits on its own
         mbar_init(&S.full[warp][lane], 1);
         mbar_fence_init();
     }
@@ -539,7 +541,7 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
         const int n = min(sg.n, max(0, (lim_max + kBatchTok - 1) / kBatchTok - sg.first));
         w.n = max(0, (n - warp + kPdWarps - 1) / kPdWarps);
         if (ok)
-            while (w.issued < min(w.n, kPdStages)) issue(sg, w, w.issued);
+            while (w.issued < min(w.n, kStages)) issue(sg, w, w.issued);
         return w;
     };
     Copies w = begin_copies(g);
@@ -580,10 +582,10 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
             __syncwarp();
             if (w.issued < w.n) issue(g, w, stage);
             t0 += kPdWarps * kBatchTok;
-            stage = stage == kPdStages - 1 ? 0 : stage + 1;
+            stage = stage == kStages - 1 ? 0 : stage + 1;
         }
         if (!ok)             // copies in flight land before the CTA leaves; nothing more is fetched
-            for (int i = 0; i < kPdStages; ++i)
+            for (int i = 0; i < kStages; ++i)
                 if (i < w.issued) mbar_wait_bounded(&S.full[warp][i], phases >> i & 1u);
         // ---- what comes next, and its first copies ----
         Segment next = g;
@@ -631,7 +633,7 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
             }
         __syncthreads();
         if (kCluster && n_rank > 1) cluster_wait();          // (every CTA runs, and has read what it got before)
-        const uint32_t xo = smem_u32(smem_raw + sizeof(PdSmem<NT>)), xml = xo + n_rank * kCols * kHD * 4;
+        const uint32_t xo = smem_u32(smem_raw + sizeof(Smem)), xml = xo + n_rank * kCols * kHD * 4;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int col = 8 * nt + warp;
@@ -671,7 +673,7 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
             for (int nt = 0; nt < NT; ++nt) {
                 const int col = 8 * nt + warp;
                 if (row0 + col >= n_rows || (uint32_t)col % n_rank != rank) continue;
-                const float* po = reinterpret_cast<const float*>(smem_raw + sizeof(PdSmem<NT>));
+                const float* po = reinterpret_cast<const float*>(smem_raw + sizeof(Smem));
                 const float2* pml = reinterpret_cast<const float2*>(po + n_rank * kCols * kHD);
                 float m = -INFINITY, l = 0.f;
                 float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -778,23 +780,26 @@ __global__ void __launch_bounds__(256) pg_merge_kernel(const PdParams P) {
 
 template <int NT, typename T>
 int pd_launch_split(const PdParams& P, bool merge, cudaStream_t stream) {
-    constexpr int smem = (int)sizeof(PdSmem<NT>);
-    const auto kernel = pg_attend_kernel<NT, T, false>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return BGTQ_E_LAUNCH;
+    constexpr int kStages = NT == 1 ? 2 : 4, smem = (int)sizeof(PdSmem<NT, kStages>);
+    const auto kernel = pg_attend_kernel<NT, T, false, kStages>;
+    static std::atomic<uint64_t> allowed{0};
+    if (!pg_allow_smem(kernel, smem, allowed)) return BGTQ_E_LAUNCH;
     if (launch_kernel(kernel, dim3(P.n_cta), dim3(kPdThreads), smem, stream, true, P) != cudaSuccess) return BGTQ_E_LAUNCH;
     if (!merge) return BGTQ_OK;
     const dim3 grid(P.n_cta - 1, P.cu_q ? 8 * NT : P.gqa);
     return launch_kernel(pg_merge_kernel<NT, T>, grid, dim3(256), 0, stream, true, P) == cudaSuccess ? BGTQ_OK : BGTQ_E_LAUNCH;
 }
-template <int NT, typename T>
+template <int NT, typename T, int kStages>
 int pd_launch_cluster(const PdParams& P, int64_t triples, int n_rank, cudaStream_t stream) {
-    const int smem = (int)sizeof(PdSmem<NT>) + (n_rank > 1 ? n_rank * 8 * NT * (kHD * 4 + 8) : 0);
-    const auto kernel = pg_attend_kernel<NT, T, true>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return BGTQ_E_LAUNCH;
+    constexpr int base = (int)sizeof(PdSmem<NT, kStages>), row = 8 * NT * (kHD * 4 + 8);
+    static_assert(base + 8 * row <= 227 * 1024, "a cluster of eight fits");
+    const auto kernel = pg_attend_kernel<NT, T, true, kStages>;
+    static std::atomic<uint64_t> allowed{0};
+    if (!pg_allow_smem(kernel, base + 8 * row, allowed)) return BGTQ_E_LAUNCH;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(triples * n_rank));
     cfg.blockDim = dim3(kPdThreads);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = base + (n_rank > 1 ? n_rank * row : 0);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -809,7 +814,9 @@ int pd_launch_cluster(const PdParams& P, int64_t triples, int n_rank, cudaStream
 }
 template <int NT, typename T>
 int pd_launch(const PdParams& P, const PdForm& f, cudaStream_t stream) {
-    return f.n_rank ? pd_launch_cluster<NT, T>(P, f.triples, f.n_rank, stream) : pd_launch_split<NT, T>(P, f.merge, stream);
+    if (!f.n_rank) return pd_launch_split<NT, T>(P, f.merge, stream);
+    if (NT == 1 && f.alone) return pd_launch_cluster<NT, T, NT == 1 ? 4 : 2>(P, f.triples, f.n_rank, stream);
+    return pd_launch_cluster<NT, T, 2>(P, f.triples, f.n_rank, stream);
 }
 
 bool aligned(const void* p, int64_t bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
@@ -839,7 +846,16 @@ static PdForm pd_form(int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv, i
     f.n_cta = (int)(most < 1 ? 1 : most < (double)resident ? most : (double)resident);
     const int asked = (flags & BGTQ_PAGED_FORM_MASK) >> BGTQ_PAGED_FORM_SHIFT;
     if (asked == 15) return f;
-    if (asked) f.n_rank = asked;
+    // Measured, in microseconds (8 KV heads, 100 to 131072 tokens): a cluster takes 4.4 and 1.45 for each round of its CTAs' warps while every CTA
+    // has an SM for itself, 2.1 where two share one (only without the exchange's memory); the list takes 9, the merging launch among
+    // them, and 2.2 for each round of the CTAs that are resident.
+    int n = 8;
+    while (n > 1 && f.triples * n > sms) n /= 2;
+    if (asked) n = asked;
+    f.alone = f.triples * n <= sms;
+    const double cluster = 4.4 + (f.alone ? 1.45 : 2.1) * (double)((rounds + n - 1) / n);
+    const double split = 9.0 + 2.2 * (double)((most + (double)resident - 1) / (double)resident);
+    if (asked || (f.triples * n <= (n == 1 && f.nt == 1 ? 2 : 1) * sms && cluster < split)) f.n_rank = n;
     return f;
 }
 

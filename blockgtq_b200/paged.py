@@ -21,6 +21,8 @@ HD = 128
 UNIT = 16                       # tokens of a unit
 PAGE_UNIT_BYTES = 2304          # bytes of a unit of one KV head
 _FORM = 0                       # form of the attention's launch (bgtq.h, BGTQ_PAGED_FORM_SHIFT), 0: the library chooses
+_KINDS = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_SCALE = 1.0 / math.sqrt(HD)
 _TYPES = {torch.float16: 0, torch.bfloat16: _lib.PAGED_BF16}
 
 
@@ -77,7 +79,6 @@ def _type_flag(dtype, name):
     return _TYPES[dtype]
 
 
-@_lib.no_grad
 def paged_kv4_append(pages, slots, k, v, q=None, cos=None, sin=None, positions=None, status=None):
     """Quantise k and v (n, n_kv, 128) fp16 or bf16 into the slots of ``pages`` (n_pages, n_kv, page bytes) uint8.
 
@@ -85,6 +86,16 @@ def paged_kv4_append(pages, slots, k, v, q=None, cos=None, sin=None, positions=N
     ``cos`` / ``sin`` (n_positions, 64) fp32 with ``positions`` (n,) int64: k, and ``q`` (n, n_q, 128), go through the rotary
     embedding first (dims d and d + 64 are a pair; fp32, k quantised from the unrounded result).  Returns the rotated q (n, n_q, 128),
     or None without one.  ``status``: optional int32 tensor, set to 2 where a slot or position is out of range (nothing stored)."""
+    r = _lib.host().paged_append(pages, slots, k, v, q, cos, sin, positions, status)
+    if r is None:
+        return _append(pages, slots, k, v, q, cos, sin, positions, status)
+    _lib.done(r, "bgtq_paged_append")
+    return None if q is None else r
+
+
+@torch.no_grad()
+def _append(pages, slots, k, v, q, cos, sin, positions, status):
+    """:func:`paged_kv4_append` for what the extension module leaves: tensors that have to be copied, and errors."""
     page = _pool(pages)
     dev, n_kv = pages.device, pages.shape[1]
     flags = _type_flag(k.dtype, "k")
@@ -125,10 +136,18 @@ def paged_kv4_append(pages, slots, k, v, q=None, cos=None, sin=None, positions=N
     return q_out
 
 
-@_lib.no_grad
 def paged_kv4_read(pages, slots, dtype=torch.float16, status=None):
     """The keys and values that the cache holds for ``slots`` (n,) int64: two tensors (n, n_kv, 128) of fp16 (exact), fp32
-    (exact) or bf16.  A negative slot reads as zeros."""
+    (exact) or bf16.  A negative slot reads as zeros, and so does one out of range, with 2 in ``status``."""
+    kind = _KINDS.get(dtype)
+    r = None if kind is None else _lib.host().paged_read(pages, slots, kind, status)
+    if r is None:
+        return _read(pages, slots, dtype, status)
+    return _lib.done(r, "bgtq_paged_read")
+
+
+@torch.no_grad()
+def _read(pages, slots, dtype, status):
     page = _pool(pages)
     dev, n_kv = pages.device, pages.shape[1]
     if dtype not in (torch.float16, torch.bfloat16, torch.float32):
@@ -146,9 +165,20 @@ def paged_kv4_read(pages, slots, dtype=torch.float16, status=None):
 
 
 def _attend(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, causal, scale, return_lse, status, out):
+    scale = _SCALE if scale is None else float(scale)
+    flags = (_lib.PAGED_CAUSAL if causal else 0) | _FORM << _lib.PAGED_FORM_SHIFT
+    r = _lib.host().paged_attend(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, scale, flags, return_lse, status, out)
+    if r is None:
+        return _attend_any(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, flags, scale, return_lse, status, out)
+    return _lib.done(r, "bgtq_paged_attend", 2)
+
+
+@torch.no_grad()
+def _attend_any(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, flags, scale, return_lse, status, out):
+    """The attention for what the extension module leaves: tensors that have to be copied, empty ones, and errors."""
     page = _pool(pages)
     dev, n_kv = pages.device, pages.shape[1]
-    flags = _type_flag(q.dtype, "q") | (_lib.PAGED_CAUSAL if causal else 0) | _FORM << _lib.PAGED_FORM_SHIFT
+    flags |= _type_flag(q.dtype, "q")
     q = _rows(q, "q", None, None, q.dtype, dev, 16)
     n, n_q = q.shape[:2]
     if n_q < 1 or n_q % n_kv or n_q // n_kv > 8:
@@ -170,7 +200,8 @@ def _attend(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, causal, sc
             or out.data_ptr() % 8:
         raise ValueError("out must be like q, with rows of 8-byte alignment")
     lse = torch.empty(n, n_q, dtype=torch.float32, device=dev) if return_lse else None
-    scale = 1.0 / math.sqrt(HD) if scale is None else float(scale)
+    cap = block_table.shape[1] * page
+    max_tokens = cap if max_tokens < 0 else min(max_tokens, cap)
     if math.isnan(scale):
         raise ValueError("scale is not a number")
     status, lib = _status(status, dev), _lib.lib()
@@ -190,32 +221,37 @@ def _attend(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, causal, sc
     return (out, lse) if return_lse else out
 
 
-@_lib.no_grad
-def paged_kv4_decode_attention(q, pages, block_table, seq_lens, scale=None, return_lse=False, status=None, out=None):
+def paged_kv4_decode_attention(q, pages, block_table, seq_lens, scale=None, return_lse=False, status=None, out=None, max_seq_len=None):
     """One query token of every sequence over its cached tokens: q (B, n_q, 128) fp16 or bf16 -> (B, n_q, 128) of the same type,
     with ``return_lse`` also (B, n_q) fp32, the natural logarithm of each row's sum of exponentials.
 
     ``block_table`` (B, pages per sequence) int32 and ``seq_lens`` (B,) int32: token t of sequence b lies in page ``block_table[b, t // page
     size]``; entries behind the sequence's end are not read.  A sequence without tokens gives zeros and -inf.  Query heads
-    h * n_q / n_kv .. share KV head h, at most 8 of them."""
-    cap = block_table.shape[1] * (pages.shape[2] // PAGE_UNIT_BYTES * UNIT) if block_table.dim() == 2 and pages.dim() == 3 else 0
-    return _attend(q, pages, block_table, seq_lens, None, 1, cap, True, scale, return_lse, status, out)
+    h * n_q / n_kv .. share KV head h, at most 8 of them.  ``max_seq_len``: no sequence is longer (default: what the table holds); it
+    chooses and sizes the launch, not the result."""
+    return _attend(q, pages, block_table, seq_lens, None, 1, _most(max_seq_len), True, scale, return_lse, status, out)
 
 
-@_lib.no_grad
 def paged_kv4_prefill_attention(q, pages, block_table, seq_lens, cu_q, max_q_len=None, max_seq_len=None, causal=True, scale=None,
                                 return_lse=False, status=None, out=None):
     """Several query tokens of every sequence over its cached tokens, their own among them: q (n, n_q, 128), rows ``cu_q[b]`` ..
     ``cu_q[b + 1] - 1`` (``cu_q`` (B + 1,) int32) are the last positions of sequence b, and when ``causal`` each sees the tokens up to itself.
 
     ``max_q_len`` / ``max_seq_len``: no sequence has more query rows / tokens (default: what the shapes allow); they choose and size
-    the launch.  Rows behind ``cu_q[B]`` are not written.  Otherwise as :func:`paged_kv4_decode_attention`."""
-    cap = block_table.shape[1] * (pages.shape[2] // PAGE_UNIT_BYTES * UNIT) if block_table.dim() == 2 and pages.dim() == 3 else 0
-    max_q = max(1, q.shape[0] if max_q_len is None else min(int(max_q_len), q.shape[0]))
-    most = cap if max_seq_len is None else min(int(max_seq_len), cap)
-    if most < 0:
+    the launch, not the result.  Rows behind ``cu_q[B]`` are not written.  Otherwise as :func:`paged_kv4_decode_attention`."""
+    if cu_q is None:
+        raise ValueError("cu_q says which rows are whose")
+    rows = q.shape[0]
+    max_q = max(1, rows if max_q_len is None else min(int(max_q_len), rows))
+    return _attend(q, pages, block_table, seq_lens, cu_q, max_q, _most(max_seq_len), causal, scale, return_lse, status, out)
+
+
+def _most(max_seq_len):
+    if max_seq_len is None:
+        return -1
+    if max_seq_len < 0:
         raise ValueError("max_seq_len must not be negative")
-    return _attend(q, pages, block_table, seq_lens, cu_q, max_q, most, bool(causal), scale, return_lse, status, out)
+    return int(max_seq_len)
 
 
 class PagedKV4Cache:
