@@ -52,6 +52,15 @@ template <> struct PgType<__nv_bfloat16> {
     }
 };
 
+// A query row of largest magnitude `top`: up0 * up1 = 2^e brings it to [2^13, 2^14); returns 2^-e.  A row of zeros, or with an infinity, stays.
+__device__ __forceinline__ float pg_row_scale(float top, float& up0, float& up1) {
+    const int ex = (int)(__float_as_uint(top) >> 23) - 127;
+    const int e = top > 0.f && ex < 128 ? 13 - ex : 0;         // -114 .. 140: in two steps
+    up0 = __uint_as_float((uint32_t)(127 + e / 2) << 23);
+    up1 = __uint_as_float((uint32_t)(127 + e - e / 2) << 23);
+    return __uint_as_float((uint32_t)(127 - e / 2) << 23) * __uint_as_float((uint32_t)(127 - (e - e / 2)) << 23);
+}
+
 // Lets a kernel use this much dynamic shared memory, once per device.
 template <typename K>
 inline bool pg_allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {

@@ -21,6 +21,7 @@
 // In a CTA eight warps take batches in turn, each with a ring of bulk copies of its own (the next triple's first ones travel while this
 // one's states are merged in shared memory).
 #include "bgtq_paged_common.cuh"
+#include "bgtq_paged_prefill.h"
 
 namespace bgtq {
 namespace {
@@ -39,7 +40,7 @@ struct PdParams {
     int64_t tb_st;
     const int32_t* lens;
     const int32_t* cu_q;             // null: one query row per sequence
-    int32_t table_cols, n_seq, n_tok, n_q, n_kv, gqa, causal;
+    int32_t cap, n_seq, n_tok, n_q, n_kv, gqa, causal;
     int32_t n_cta;                   // split: CTAs;  cluster: column blocks of a sequence that have a cluster of their own
     float scale_log2;
     void* out;
@@ -55,6 +56,7 @@ struct PdForm {
     int nt, n_cta, n_rank, blocks_of_seq;       // n_rank: CTAs of a triple's cluster, 0: the split form
     int64_t triples;
     bool merge;                                 // split: triples may be cut (those of one round never are)
+    bool prefill;                               // the tcgen05 form
     bool alone;                                 // cluster: every CTA has an SM for itself
 };
 
@@ -64,8 +66,7 @@ struct SeqInfo {
 
 __device__ __forceinline__ SeqInfo pd_seq(const PdParams& P, int i) {
     SeqInfo s;
-    const int64_t cap = (int64_t)P.table_cols * P.pool.units * kUnitTok;
-    s.len = max(0, (int)min((int64_t)P.lens[i], cap));
+    s.len = max(0, min(P.lens[i], P.cap));
     if (P.cu_q) {
         s.q0 = min(max(P.cu_q[i], 0), P.n_tok);
         s.n = max(0, min(P.cu_q[i + 1], P.n_tok) - s.q0);
@@ -267,12 +268,13 @@ __device__ __forceinline__ void pd_query(const PdParams& P, Query<NT>& Q, const 
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // 2^e with top * 2^e in [2^13, 2^14); a row of zeros, or with an infinity, stays as it is
-        const int ex = (int)(__float_as_uint(top) >> 23) - 127;
-        const int e = top > 0.f && ex < 128 ? 13 - ex : 0;
-        const float up0 = __uint_as_float((uint32_t)(127 + e / 2) << 23), up1 = __uint_as_float((uint32_t)(127 + e - e / 2) << 23);
-        const int fe = -e;                                                             // (-140 .. 114, in two steps)
-        const float fac = P.scale_log2 * __uint_as_float((uint32_t)(127 + fe / 2) << 23) * __uint_as_float((uint32_t)(127 + fe - fe / 2) << 23);
+        float up0, up1;
+        float fac = pg_row_scale(top, up0, up1) * fabsf(P.scale_log2);
+        if (P.scale_log2 < 0.f) up0 = -up0;  // (factors are positive: hidden logits are minus infinity before they meet one)
+        if (P.scale_log2 == 0.f) {
+            up0 = 0.f;
+            fac = 1.f;
+        }
 #pragma unroll
         for (int g = 0; g < 4; ++g)
 #pragma unroll
@@ -829,6 +831,8 @@ using namespace bgtq;
 // Column tiles of a product: eight query rows are the operand's width; more of them share what is read and unpacked.
 static int pd_tiles(int32_t n_q, int32_t n_kv, int32_t max_q) { return (int64_t)max_q * (n_q / n_kv) <= 8 ? 1 : 2; }
 
+constexpr int kPrefillRows = 48;        // rows of a (sequence, KV head) above which the tcgen05 form is the faster one
+
 // How a call is launched, from its shape.
 static PdForm pd_form(int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv, int32_t max_q, int64_t max_tokens, int32_t flags) {
     PdForm f{};
@@ -845,7 +849,8 @@ static PdForm pd_form(int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv, i
     const double most = (double)blocks * n_kv * (double)rounds;
     f.n_cta = (int)(most < 1 ? 1 : most < (double)resident ? most : (double)resident);
     const int asked = (flags & BGTQ_PAGED_FORM_MASK) >> BGTQ_PAGED_FORM_SHIFT;
-    if (asked == 15) return f;
+    f.prefill = asked == 14 || (asked == 0 && max_q * gqa > kPrefillRows);
+    if (f.prefill || asked == 15) return f;
     // Measured, in microseconds (8 KV heads, 100 to 131072 tokens): a cluster takes 4.4 and 1.45 for each round of its CTAs' warps while every CTA
     // has an SM for itself, 2.1 where two share one (only without the exchange's memory); the list takes 9, the merging launch among
     // them, and 2.2 for each round of the CTAs that are resident.
@@ -853,9 +858,10 @@ static PdForm pd_form(int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv, i
     while (n > 1 && f.triples * n > sms) n /= 2;
     if (asked) n = asked;
     f.alone = f.triples * n <= sms;
-    const double cluster = 4.4 + (f.alone ? 1.45 : 2.1) * (double)((rounds + n - 1) / n);
-    const double split = 9.0 + 2.2 * (double)((most + (double)resident - 1) / (double)resident);
-    if (asked || (f.triples * n <= (n == 1 && f.nt == 1 ? 2 : 1) * sms && cluster < split)) f.n_rank = n;
+    const int64_t waves = (f.triples * n + resident - 1) / resident;
+    const double cluster = 4.4 + (f.alone ? 1.45 : 2.1) * (double)(waves * ((rounds + n - 1) / n));
+    const double split = 9.0 + 2.2 * (most + (double)resident - 1) / (double)resident;
+    if (asked || cluster < split) f.n_rank = n;
     return f;
 }
 
@@ -864,6 +870,7 @@ extern "C" __attribute__((visibility("default"))) int64_t bgtq_paged_workspace_b
     if (n_seq < 0 || n_tok < 0 || n_kv < 1 || n_q < 1 || n_q % n_kv || max_q < 1 || max_tokens < 0) return BGTQ_E_BADARG;
     if (n_q / n_kv > 8) return BGTQ_E_UNSUPPORTED;
     const PdForm f = pd_form(n_seq, n_tok, n_q, n_kv, max_q, max_tokens, flags);
+    if (f.prefill) return paged_prefill_workspace(n_seq, n_kv, max_tokens);
     return f.n_rank ? 0 : (int64_t)f.n_cta * 2 * 8 * f.nt * (kHD * 4 + 8);
 }
 
@@ -874,7 +881,7 @@ extern "C" __attribute__((visibility("default"))) int bgtq_paged_attend(
     void* workspace, int64_t workspace_bytes, void* out, int64_t o_st, int64_t o_sh, float* lse, int32_t* status, void* stream) {
     const int asked = (flags & BGTQ_PAGED_FORM_MASK) >> BGTQ_PAGED_FORM_SHIFT;
     if (n_seq < 0 || n_tok < 0 || n_kv < 1 || n_q < 1 || table_cols < 0 || max_q < 1 || max_tokens < 0 ||
-        (flags & ~(BGTQ_PAGED_BF16 | BGTQ_PAGED_CAUSAL | BGTQ_PAGED_FORM_MASK)) || (asked & (asked - 1) && asked != 15))
+        (flags & ~(BGTQ_PAGED_BF16 | BGTQ_PAGED_CAUSAL | BGTQ_PAGED_FORM_MASK)) || (asked & (asked - 1) && asked < 14) || (asked == 14 && !cu_q) || asked == 13)
         return BGTQ_E_BADARG;
     if (!(scale == scale) || n_q % n_kv) return BGTQ_E_BADARG;
     if (n_q / n_kv > 8) return BGTQ_E_UNSUPPORTED;
@@ -882,12 +889,21 @@ extern "C" __attribute__((visibility("default"))) int bgtq_paged_attend(
     if (n_seq == 0 || n_tok == 0) return BGTQ_OK;
     if (!pages || n_pages < 1 || page_tokens < kUnitTok || page_tokens % kUnitTok || !q || !out || !seq_lens || (!table && table_cols > 0))
         return BGTQ_E_BADARG;
-    const int64_t cap = (int64_t)table_cols * page_tokens;
+    int64_t cap = (int64_t)table_cols * page_tokens;
+    if (cap > max_tokens) cap = max_tokens;
     if (cap > INT32_MAX - 512) return BGTQ_E_TOOBIG;
     if (!aligned(pages, 16) || page_stride % 16 || head_stride % 16 || !aligned(q, 16) || q_st % 8 || q_sh % 8 || !aligned(out, 8) || o_st % 4 ||
         o_sh % 4 || !aligned(workspace, 16))
         return BGTQ_E_ALIGN;
     PdForm f = pd_form(n_seq, n_tok, n_q, n_kv, max_q, max_tokens, flags);
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (f.prefill) {
+        if (!workspace || workspace_bytes < paged_prefill_workspace(n_seq, n_kv, max_tokens)) return BGTQ_E_BADARG;
+        return paged_prefill({{pages, page_stride, head_stride, n_pages, page_tokens / kUnitTok}, table, table_stride, seq_lens, cu_q, n_seq, n_tok, n_q,
+                              n_kv, n_q / n_kv, (flags & BGTQ_PAGED_CAUSAL) ? 1 : 0, (flags & BGTQ_PAGED_BF16) ? 1 : 0, max_tokens,
+                              reinterpret_cast<uint8_t*>(workspace), q, q_st, q_sh, scale * 1.44269504088896340736f, out, o_st, o_sh, lse, status},
+                             st);
+    }
     f.merge = cap > kPdWarps * kBatchTok && f.n_cta > 1;
     const int64_t cols = 8 * f.nt, blocks = n_tok <= n_seq ? n_seq : (int64_t)n_tok * (n_q / n_kv) / cols + n_seq;
     // the list's positions are 32 bits, and the grid's
@@ -895,10 +911,9 @@ extern "C" __attribute__((visibility("default"))) int bgtq_paged_attend(
     const int64_t need = f.n_rank ? 0 : (int64_t)f.n_cta * 2 * cols * (kHD * 4 + 8);
     if (need && (!workspace || workspace_bytes < need)) return BGTQ_E_BADARG;
     PdParams P{{pages, page_stride, head_stride, n_pages, page_tokens / kUnitTok}, q, q_st, q_sh, table, table_stride, seq_lens, cu_q,
-               table_cols, n_seq, n_tok, n_q, n_kv, n_q / n_kv, !cu_q || (flags & BGTQ_PAGED_CAUSAL) ? 1 : 0, f.n_rank ? f.blocks_of_seq : f.n_cta,
+               (int32_t)cap, n_seq, n_tok, n_q, n_kv, n_q / n_kv, !cu_q || (flags & BGTQ_PAGED_CAUSAL) ? 1 : 0, f.n_rank ? f.blocks_of_seq : f.n_cta,
                scale * 1.44269504088896340736f, out, o_st, o_sh, lse, reinterpret_cast<float*>(workspace),
                reinterpret_cast<float2*>(reinterpret_cast<float*>(workspace) + (int64_t)f.n_cta * 2 * cols * kHD), status};
-    const cudaStream_t st = (cudaStream_t)stream;
     const bool bf16 = flags & BGTQ_PAGED_BF16;
     if (f.nt == 1) return bf16 ? pd_launch<1, __nv_bfloat16>(P, f, st) : pd_launch<1, __half>(P, f, st);
     return bf16 ? pd_launch<2, __nv_bfloat16>(P, f, st) : pd_launch<2, __half>(P, f, st);

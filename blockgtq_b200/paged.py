@@ -227,8 +227,8 @@ def paged_kv4_decode_attention(q, pages, block_table, seq_lens, scale=None, retu
 
     ``block_table`` (B, pages per sequence) int32 and ``seq_lens`` (B,) int32: token t of sequence b lies in page ``block_table[b, t // page
     size]``; entries behind the sequence's end are not read.  A sequence without tokens gives zeros and -inf.  Query heads
-    h * n_q / n_kv .. share KV head h, at most 8 of them.  ``max_seq_len``: no sequence is longer (default: what the table holds); it
-    chooses and sizes the launch, not the result."""
+    h * n_q / n_kv .. share KV head h, at most 8 of them.  ``max_seq_len``: sequences are held to it (default: what the table holds);
+    a small one spares the launch what only long sequences need."""
     return _attend(q, pages, block_table, seq_lens, None, 1, _most(max_seq_len), True, scale, return_lse, status, out)
 
 
@@ -237,8 +237,10 @@ def paged_kv4_prefill_attention(q, pages, block_table, seq_lens, cu_q, max_q_len
     """Several query tokens of every sequence over its cached tokens, their own among them: q (n, n_q, 128), rows ``cu_q[b]`` ..
     ``cu_q[b + 1] - 1`` (``cu_q`` (B + 1,) int32) are the last positions of sequence b, and when ``causal`` each sees the tokens up to itself.
 
-    ``max_q_len`` / ``max_seq_len``: no sequence has more query rows / tokens (default: what the shapes allow); they choose and size
-    the launch, not the result.  Rows behind ``cu_q[B]`` are not written.  Otherwise as :func:`paged_kv4_decode_attention`."""
+    ``max_q_len``: no sequence has more query rows (default: all of them; it chooses the launch, and one that has more is attended all the
+    same).  ``max_seq_len``: sequences are held to it (default: what the table holds).  With more than 48 rows per sequence and KV head the
+    tokens are unpacked into a workspace from torch's allocator, 512 bytes per token of ``max_seq_len`` and KV head for every sequence, at
+    most 2 GiB at a time.  Rows behind ``cu_q[B]`` are not written.  Otherwise as :func:`paged_kv4_decode_attention`."""
     if cu_q is None:
         raise ValueError("cu_q says which rows are whose")
     rows = q.shape[0]

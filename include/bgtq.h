@@ -626,7 +626,8 @@ int bgtq_decode_combined_noalloc(const BgtqDecodePlan* plan_host, const BgtqHead
 #define BGTQ_PAGED_F32 2          /* bgtq_paged_read: fp32 outputs */
 #define BGTQ_PAGED_CAUSAL 4       /* bgtq_paged_attend with cu_q: query i sees the tokens up to its own position */
 #define BGTQ_PAGED_FORM_SHIFT 8   /* bgtq_paged_attend: 0 the library chooses; 1, 2, 4 or 8 << 8: clusters of so many CTAs per (sequence, KV */
-#define BGTQ_PAGED_FORM_MASK 0xF00  /* head, block of query rows); 15 << 8: one list of work over all CTAs and a launch that merges */
+#define BGTQ_PAGED_FORM_MASK 0xF00 /* head, block of query rows); 15 << 8: one list of work over all CTAs and a launch that
+                                   * merges; 14 << 8: with cu_q, tcgen05 over a workspace of unpacked tiles (many rows) */
 
 /* Quantise and store n_tok tokens.  k / v element (i, h, d) at k + i * k_st + h * k_sh + d (strides multiples of 4 elements, 8-byte
  * aligned); token i goes to slot slots[i], nowhere when that is negative; the slots of a call are distinct.  rope_cos / rope_sin (may both
@@ -650,9 +651,11 @@ int bgtq_paged_read(const uint8_t* pages, int64_t page_stride, int64_t head_stri
  * one query, n_tok = n_seq.  Otherwise rows cu_q[b] .. cu_q[b + 1] - 1 of q (n_tok, n_q, 128) are its last positions, and with
  * BGTQ_PAGED_CAUSAL row i of n sees the first seq_lens[b] - n + 1 + i tokens.  A row that sees none is zeros, its lse -inf; rows
  * behind cu_q[n_seq] are left as they were.  lse (optional, (n_tok, n_q) fp32): natural logarithm of the sum of exponentials.
- * n_q / n_kv <= 8.  max_q, max_tokens: no sequence has more rows, more tokens (they size the launch; one that has is still attended
- * whole).  workspace:
- * bgtq_paged_workspace_bytes(...) of the same arguments, 16-byte aligned, of no other call that may run at the same time. */
+ * n_q / n_kv <= 8.  max_tokens: sequences are held to it as to the table's capacity.  max_q: no sequence has more rows (it chooses the
+ * launch; one that has is still attended whole).  Both decide how the work is cut, and so the order of sums.  workspace:
+ * bgtq_paged_workspace_bytes(...) of the same arguments, 16-byte aligned, of no other call that may run at the same time; for many
+ * rows it holds the sequences' tokens in fp16, 512 bytes per token of max_tokens and KV head, at most 2 GiB (or one sequence's and
+ * head's) at a time. */
 int64_t bgtq_paged_workspace_bytes(int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv, int32_t max_q,
                 int64_t max_tokens, int32_t flags);
 int bgtq_paged_attend(const void* q, int64_t q_st, int64_t q_sh, const uint8_t* pages, int64_t page_stride, int64_t head_stride,

@@ -105,7 +105,7 @@ def test_library_refuses_before_it_touches_the_device():
                  max_q=1, most=16, scale=1.0, flags=0, ws=p, wsb=1 << 40, out=p, ost=512, osh=128, lse=0, status=0, stream=0) | kw
         return lib.bgtq_paged_attend(*a.values())
     assert attend(n_seq=0, n=0) == _lib.OK
-    for kw, code in ((dict(nq=3), -1), (dict(nq=18), -2), (dict(n=2), -1), (dict(max_q=2), -1), (dict(max_q=0), -1), (dict(cols=1 << 28), -5),
+    for kw, code in ((dict(nq=3), -1), (dict(nq=18), -2), (dict(n=2), -1), (dict(max_q=2), -1), (dict(max_q=0), -1), (dict(cols=1 << 28, most=1 << 40), -5), (dict(flags=14 << 8), -1), (dict(flags=13 << 8), -1),
                      (dict(q=p + 8), -3), (dict(qst=4), -3), (dict(out=p + 4), -3), (dict(ws=0, flags=15 << 8), -1), (dict(wsb=16, flags=15 << 8), -1), (dict(flags=3 << 8), -1), (dict(lens=0), -1),
                      (dict(table=0), -1), (dict(scale=float("nan")), -1), (dict(flags=2), -1), (dict(pages=p + 1), -3)):
         assert attend(**kw) == code, kw

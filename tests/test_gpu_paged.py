@@ -128,11 +128,20 @@ def test_slots_and_positions_out_of_range_are_reported_and_store_nothing():
     assert status.item() == 2 and not k[0].any() and k[1].any()
 
 
-@pytest.fixture(params=["auto", "split", 1, 2, 8])
+FORMS = {"auto": 0, "split": 15, "cluster1": 1, "cluster2": 2, "cluster8": 8}
+
+
+@pytest.fixture(params=list(FORMS))
 def form(request, monkeypatch):
     """The forms that the attention's launch has; the library chooses one by the call's shape."""
     from blockgtq_b200 import paged
-    monkeypatch.setattr(paged, "_FORM", {"auto": 0, "split": 15}.get(request.param, request.param))
+    monkeypatch.setattr(paged, "_FORM", FORMS[request.param])
+
+
+@pytest.fixture(params=[*FORMS, "tcgen05"])
+def rows_form(request, monkeypatch):
+    from blockgtq_b200 import paged
+    monkeypatch.setattr(paged, "_FORM", (FORMS | {"tcgen05": 14})[request.param])
 
 
 def _check(got, lse, ref, rows):
@@ -192,13 +201,13 @@ def test_decode_of_many_sequences_and_of_one_long_one_cut_between_ctas(form):
 PREFILLS = [
     # n_kv, gqa, page, (tokens, queries) per sequence
     (1, 1, 16, [(1, 1)]), (2, 4, 64, [(5, 5), (70, 3), (16, 16)]), (1, 7, 32, [(40, 9), (0, 0), (33, 33)]), (2, 8, 16, [(130, 1), (131, 40)]),
-    (1, 2, 128, [(300, 300)]), (1, 3, 16, [(5, 9), (0, 4), (20, 2)])]
+    (1, 2, 128, [(300, 300)]), (2, 4, 32, [(900, 129), (257, 64)]), (1, 3, 16, [(5, 9), (0, 4), (20, 2)])]
 
 
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n_kv,gqa,page,seqs", PREFILLS)
-def test_prefill_against_64_bits(dtype, n_kv, gqa, page, seqs, causal, form):
+def test_prefill_against_64_bits(dtype, n_kv, gqa, page, seqs, causal, rows_form):
     from blockgtq_b200 import paged_kv4_prefill_attention
     lens, counts = [t for t, _ in seqs], [n for _, n in seqs]
     gen = torch.Generator().manual_seed(sum(lens) + gqa)
@@ -217,23 +226,38 @@ def test_prefill_against_64_bits(dtype, n_kv, gqa, page, seqs, causal, form):
         _check(out, lse, R.attention(q[ends[b]:ends[b + 1]], host, slots[b], seen, 1 / math.sqrt(128)), slice(ends[b], ends[b + 1]))
 
 
-def test_a_page_number_outside_the_pool_leaves_its_tokens_out(form):
+@pytest.mark.parametrize("bad", ["-1", "n", "1 << 30"])
+def test_a_page_number_outside_the_pool_leaves_its_tokens_out(form, bad):
     from blockgtq_b200 import paged_kv4_decode_attention
     gen = torch.Generator().manual_seed(2)
     pages, table, slots = _case(gen, 1, 16, [40, 40])
     q = _noise(gen, 2, 2, 128).half()
-    for bad in (-1, pages.shape[0], 1 << 30):
-        t = table.clone()
-        t[0, 1] = bad
-        status = torch.zeros(1, dtype=torch.int32, device=DEV)
-        out, lse = paged_kv4_decode_attention(q.to(DEV), pages, t.to(DEV), torch.tensor([40, 40], dtype=torch.int32, device=DEV), return_lse=True, status=status)
-        assert status.item() == 4
-        left = torch.cat([slots[0][:16], slots[0][32:]])
-        _check(out, lse, R.attention(q[:1], pages.cpu(), left, [24], 1 / math.sqrt(128)), slice(0, 1))
-        _check(out, lse, R.attention(q[1:], pages.cpu(), slots[1], [40], 1 / math.sqrt(128)), slice(1, 2))
+    table[0, 1] = eval(bad, {"n": pages.shape[0]})
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    out, lse = paged_kv4_decode_attention(q.to(DEV), pages, table.to(DEV), torch.tensor([40, 40], dtype=torch.int32, device=DEV), return_lse=True, status=status)
+    assert status.item() == 4
+    left = torch.cat([slots[0][:16], slots[0][32:]])
+    _check(out, lse, R.attention(q[:1], pages.cpu(), left, [24], 1 / math.sqrt(128)), slice(0, 1))
+    _check(out, lse, R.attention(q[1:], pages.cpu(), slots[1], [40], 1 / math.sqrt(128)), slice(1, 2))
 
 
-def test_more_rows_and_tokens_than_the_caller_said_are_attended_all_the_same(form):
+def test_a_page_number_outside_the_pool_in_a_prefill(rows_form):
+    from blockgtq_b200 import paged_kv4_prefill_attention
+    gen = torch.Generator().manual_seed(2)
+    pages, table, slots = _case(gen, 2, 16, [200, 150])
+    q = _noise(gen, 100, 4, 128).half()
+    table[0, 1], table[0, 9], table[0, 12] = -1, pages.shape[0], 1 << 30
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    out, lse = paged_kv4_prefill_attention(q.to(DEV), pages, table.to(DEV), torch.tensor([200, 150], dtype=torch.int32, device=DEV),
+                                           torch.tensor([0, 60, 100], dtype=torch.int32, device=DEV), return_lse=True, status=status)
+    assert status.item() == 4
+    keep = torch.tensor([i for i in range(200) if i // 16 not in (1, 9, 12)])
+    seen = [int((keep < 141 + i).sum()) for i in range(60)]
+    _check(out, lse, R.attention(q[:60], pages.cpu(), slots[0][keep], seen, 1 / math.sqrt(128)), slice(0, 60))
+    _check(out, lse, R.attention(q[60:], pages.cpu(), slots[1], [111 + i for i in range(40)], 1 / math.sqrt(128)), slice(60, 100))
+
+
+def test_more_rows_than_the_caller_said_are_attended_all_the_same(rows_form):
     from blockgtq_b200 import paged_kv4_prefill_attention
     gen = torch.Generator().manual_seed(17)
     lens, counts = [700, 90, 300], [40, 7, 1]
@@ -241,7 +265,7 @@ def test_more_rows_and_tokens_than_the_caller_said_are_attended_all_the_same(for
     q = _noise(gen, sum(counts), 8, 128).half()
     ends = [0, 40, 47, 48]
     out, lse = paged_kv4_prefill_attention(q.to(DEV), pages, table.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV),
-                                           torch.tensor(ends, dtype=torch.int32, device=DEV), max_q_len=2, max_seq_len=16, return_lse=True)
+                                           torch.tensor(ends, dtype=torch.int32, device=DEV), max_q_len=2, return_lse=True)
     host = pages.cpu()
     for b, (t, m) in enumerate(zip(lens, counts)):
         _check(out, lse, R.attention(q[ends[b]:ends[b + 1]], host, slots[b], [t - m + 1 + i for i in range(m)], 1 / math.sqrt(128)), slice(ends[b], ends[b + 1]))
@@ -253,8 +277,11 @@ def test_a_length_beyond_the_table_is_held_to_it():
     pages, table, slots = _case(gen, 1, 16, [32])
     q = _noise(gen, 1, 2, 128).half()
     for t in (33, 1 << 30, -5):
-        out, lse = paged_kv4_decode_attention(q.to(DEV), pages, table[:, :2].to(DEV), torch.tensor([t], dtype=torch.int32, device=DEV), return_lse=True)
+        n = torch.tensor([t], dtype=torch.int32, device=DEV)
+        out, lse = paged_kv4_decode_attention(q.to(DEV), pages, table[:, :2].to(DEV), n, return_lse=True)
         _check(out, lse, R.attention(q, pages.cpu(), slots[0], [min(32, t)], 1 / math.sqrt(128)), slice(0, 1))
+        out, lse = paged_kv4_decode_attention(q.to(DEV), pages, table.to(DEV), n, return_lse=True, max_seq_len=20)
+        _check(out, lse, R.attention(q, pages.cpu(), slots[0], [min(20, t)], 1 / math.sqrt(128)), slice(0, 1))
 
 
 def test_no_number_in_a_row_shows_and_in_a_hidden_place_does_not(form):
@@ -270,11 +297,38 @@ def test_no_number_in_a_row_shows_and_in_a_hidden_place_does_not(form):
     assert torch.isfinite(run(39)).all()
     nan = run(40).isnan()[0]
     assert nan[:, 32:64].all() and not nan[:, :32].any() and not nan[:, 64:].any()
-    out = paged_kv4_prefill_attention(q, pages, table.to(DEV), torch.tensor([40], dtype=torch.int32, device=DEV), torch.tensor([0, 4], dtype=torch.int32, device=DEV))
-    assert torch.isfinite(out[:3]).all() and out[3, :, 32:64].isnan().all()
     k[0, 0, 0] = math.nan
     paged_kv4_append(pages, slots[0][39:].to(DEV), k.to(DEV), torch.zeros_like(v).to(DEV))
     assert run(40).isnan().all() and torch.isfinite(run(39)).all()
+
+
+def test_no_number_in_a_prefill_shows_in_the_rows_that_see_it(rows_form):
+    from blockgtq_b200 import paged_kv4_append, paged_kv4_prefill_attention
+    gen = torch.Generator().manual_seed(9)
+    pages, table, slots = _case(gen, 1, 16, [300])
+    k, v = (_noise(gen, 2, 1, 128).half() for _ in range(2))
+    v[0, 0, 33] = math.nan                                     # group 1 of V of token 251
+    k[1, 0, 100] = math.nan                                    # K of token 280
+    paged_kv4_append(pages, slots[0][[251, 280]].to(DEV), k.to(DEV), v.to(DEV))
+    q = _noise(gen, 70, 2, 128).half().to(DEV)
+    out, lse = paged_kv4_prefill_attention(q, pages, table.to(DEV), torch.tensor([300], dtype=torch.int32, device=DEV),
+                                           torch.tensor([0, 70], dtype=torch.int32, device=DEV), return_lse=True)
+    first = 300 - 70                                           # position of row 0
+    nan = out.isnan()
+    assert not nan[:251 - first].any() and nan[280 - first:].all() and nan[251 - first:, :, 32:64].all()
+    assert not nan[251 - first:280 - first, :, :32].any() and not nan[251 - first:280 - first, :, 64:].any()
+    assert torch.isfinite(lse[:280 - first]).all() and lse[280 - first:].isnan().all()
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 2.0])
+def test_scales_of_any_sign(scale, rows_form):
+    from blockgtq_b200 import paged_kv4_prefill_attention
+    gen = torch.Generator().manual_seed(19)
+    pages, table, slots = _case(gen, 1, 16, [150])
+    q = _noise(gen, 60, 3, 128).half()
+    out, lse = paged_kv4_prefill_attention(q.to(DEV), pages, table.to(DEV), torch.tensor([150], dtype=torch.int32, device=DEV),
+                                           torch.tensor([0, 60], dtype=torch.int32, device=DEV), return_lse=True, scale=scale)
+    _check(out, lse, R.attention(q, pages.cpu(), slots[0], [91 + i for i in range(60)], scale), slice(0, 60))
 
 
 def test_steps_of_the_cache_from_prompt_to_decode_on_another_stream():
