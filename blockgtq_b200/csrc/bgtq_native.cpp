@@ -336,7 +336,7 @@ PyObject* paged_append(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     bool bad = false;
     const at::Tensor *pages = A.tensor(0, bad), *slots = A.tensor(1, bad), *k = A.tensor(2, bad), *v = A.tensor(3, bad), *q = A.tensor(4, bad),
                      *cs = A.tensor(5, bad), *sn = A.tensor(6, bad), *pos = A.tensor(7, bad), *status = A.tensor(8, bad);
-    if (bad || !pool_ok(pages) || !half_type(k) || !rows_ok(k, k->scalar_type(), 8) || !rows_ok(v, k->scalar_type(), 8) || !status_ok(status))
+    if (bad || !pool_ok(pages) || !half_type(k) || !rows_ok(k, k->scalar_type(), 16) || !rows_ok(v, k->scalar_type(), 16) || !status_ok(status))
         return none();
     const int64_t m = k->size(0), n_kv = pages->size(1);
     if (k->size(1) != n_kv || v->size(0) != m || v->size(1) != n_kv || !vec_ok(slots, at::kLong, m)) return none();
@@ -348,7 +348,7 @@ PyObject* paged_append(PyObject*, PyObject* const* argv, Py_ssize_t n) {
                 return none();
         if (!vec_ok(pos, at::kLong, m)) return none();
     }
-    if (q && (!rows_ok(q, k->scalar_type(), 8) || q->size(0) != m || q->size(1) < 1)) return none();
+    if (q && (!rows_ok(q, k->scalar_type(), 16) || q->size(0) != m || q->size(1) < 1)) return none();
     at::Tensor out;
     if (q) out = empty(q->sizes(), q->scalar_type(), *q);
     const int n_q = q ? (int)q->size(1) : 0, flags = k->scalar_type() == at::kBFloat16 ? BGTQ_PAGED_BF16 : 0;

@@ -9,7 +9,9 @@
 namespace bgtq {
 namespace {
 
-constexpr int kApThreads = 256;
+constexpr int kApThreads = 256, kApBlocks = 4;         // four blocks on an SM: 64 registers a thread
+// 1.5 * 2^23 + 8: a sum with it has the nearest whole number, ties to even, plus 8 in its lower sixteen bits
+constexpr float kRound = 12582920.0f;
 
 struct ApParams {
     uint8_t* pages;
@@ -23,125 +25,190 @@ struct ApParams {
     int64_t cs_st;
     const int64_t* positions;
     int32_t n_positions, n_tok, n_kv, n_q;
+    int32_t kv_chunks, q_chunks, per;                  // chunks of two K (or V) rows, of two queries; chunks of a warp's task
     int32_t* status;
 };
 
-// Eight lanes hold a row: lane j its dims 32 g + 4 j .. + 3 of every group g, so that a group's largest magnitude is three
-// exchanges away and both dims of every rotated pair (d, d + 64) lie in one lane.
+// Eight lanes hold a row: lane j its dims 32 g + 4 j .. + 3 of every group g, so that a group's largest magnitude is three exchanges away, both
+// dims of every rotated pair (d, d + 64) lie in one lane, and a lane's codes are eight bytes of a K row.
+struct Row {
+    uint2 w[4];
+};
 template <typename T>
-__device__ __forceinline__ void ap_load(const T* row, int j, float (&x)[4][4]) {
+__device__ __forceinline__ Row ap_load(const T* row, int j) {
+    Row r;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-        const uint2 w = *reinterpret_cast<const uint2*>(row + 32 * g + 4 * j);
-        const float2 a = PgType<T>::up(w.x), b = PgType<T>::up(w.y);
-        x[g][0] = a.x; x[g][1] = a.y; x[g][2] = b.x; x[g][3] = b.y;
-    }
+    for (int g = 0; g < 4; ++g) r.w[g] = *reinterpret_cast<const uint2*>(row + 32 * g + 4 * j);
+    return r;
 }
-
-__device__ __forceinline__ void ap_rotate(float (&x)[4][4], const float4 (&c)[2], const float4 (&s)[2]) {
+__device__ __forceinline__ float max_nan(float a, float b) {             // NaN when either is
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+// bf16(a / 7) within the scales' range; the quotient by its remainder, as a division rounds it (an infinity ends up as the largest scale).
+__device__ __forceinline__ float ap_scale(float a) {
+    const float c = 1.0f / 7.0f, q0 = __fmul_rn(a, c), q = __fmaf_rn(__fmaf_rn(-7.0f, q0, a), c, q0);
+    return __bfloat162float(__float2bfloat16_rn(fmaxf(fminf(q, kPgScaleMax), kPgScaleMin)));
+}
+// A group's four values -> k = code + 8 + 1.5 * 2^23 each.  x / scale is not divided out: k = round(x * (1 / scale)) is the whole number next to
+// the quotient unless that is within 2^-20 of a tie, and the remainder x - code * scale, exact (11 bits of code * scale, and no more than
+// scale / 2 left), says so: only then is it decided by it.
+__device__ __forceinline__ void ap_codes(const float (&in)[4], float largest, float scale, float (&k)[4]) {
+    float x[4] = {in[0], in[1], in[2], in[3]}, r, far = 0.f;
+    if (largest > 7.45f * scale) {           // (only at the largest scale: beyond it values saturate)
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-        const float cc[4] = {c[g].x, c[g].y, c[g].z, c[g].w}, ss[4] = {s[g].x, s[g].y, s[g].z, s[g].w};
+        for (int e = 0; e < 4; ++e) x[e] = fminf(fmaxf(x[e], -7.45f * scale), 7.45f * scale);
+    }
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(scale));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        k[e] = __fmaf_rn(x[e], r, kRound);
+        far = fmaxf(far, fabsf(__fmaf_rn(-__fsub_rn(k[e], kRound), scale, x[e])));
+    }
+    if (2.f * far >= scale) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float a = x[g][e], b = x[g + 2][e];
-            x[g][e] = __fsub_rn(__fmul_rn(a, cc[e]), __fmul_rn(b, ss[e]));
-            x[g + 2][e] = __fadd_rn(__fmul_rn(b, cc[e]), __fmul_rn(a, ss[e]));
+            const float left = __fmaf_rn(-__fsub_rn(k[e], kRound), scale, x[e]), twice = 2.f * fabsf(left);
+            if (twice > scale || (twice == scale && (__float_as_uint(k[e]) & 1u))) k[e] = __fadd_rn(k[e], copysignf(1.f, left));
         }
     }
 }
 
-// A warp takes two tokens and two rows of each: octet o = lane / 8 is row 2 * chunk + o / 2 of token 2 * pair + o % 2, rows
-// counted over the K heads, the V heads and the query heads.
+// A warp's task: two tokens and a run of chunks of two rows (KV heads' K, then V, then queries); octet o = lane / 8 takes row o / 2 of a chunk for
+// token o % 2.  The tables' rows are read once for all of a task's chunks, and a chunk's rows are requested while the one before is worked on.
+// Bound: memory, 512 bytes in and 144 out per token and KV head, 512 per query row.
 template <typename T>
-__global__ void __launch_bounds__(kApThreads) pg_append_kernel(const ApParams P) {
+__global__ void __launch_bounds__(kApThreads, kApBlocks) pg_append_kernel(const ApParams P) {
     const int lane = threadIdx.x & 31, o = lane >> 3, j = lane & 7;
-    const int n_rows = 2 * P.n_kv + P.n_q, n_chunks = (n_rows + 1) >> 1;
-    const int64_t task = (int64_t)blockIdx.x * (kApThreads / 32) + (threadIdx.x >> 5);
+    const uint32_t n_chunks = 2 * P.kv_chunks + P.q_chunks, n_tasks = (n_chunks + P.per - 1) / P.per;
+    const uint32_t task = blockIdx.x * (kApThreads / 32) + (threadIdx.x >> 5), pair = task / n_tasks;
+    const int64_t tok = 2 * (int64_t)pair + (o & 1);
     grid_launch_dependents();
     grid_dependency_wait();
-    const int64_t pair = task / n_chunks;
-    const int row = 2 * (int)(task - pair * n_chunks) + (o >> 1);
-    const int64_t tok = 2 * pair + (o & 1);
-    const bool there = tok < P.n_tok && row < n_rows;
-    const bool is_k = row < P.n_kv, is_q = row >= 2 * P.n_kv;
-    const int head = is_k ? row : is_q ? row - 2 * P.n_kv : row - P.n_kv;
-    float x[4][4] = {};
-    int64_t slot = -1;
-    if (there) {
-        const T* src = is_k ? reinterpret_cast<const T*>(P.k) + tok * P.k_st + head * P.k_sh
-                     : is_q ? reinterpret_cast<const T*>(P.q) + tok * P.q_st + head * P.q_sh
-                            : reinterpret_cast<const T*>(P.v) + tok * P.v_st + head * P.v_sh;
-        slot = P.slots[tok];
-        ap_load(src, j, x);
-        if (P.cos && (is_k || is_q)) {
-            int64_t p = P.positions[tok];
-            if (p < 0 || p >= P.n_positions) {         // no angle for it: the row is not written, and the caller learns of it
-                if (P.status && (slot >= 0)) *P.status = kStatusOverflow;
-                p = 0;
-                if (is_k) slot = -1;
-            }
-            float4 c[2], s[2];
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                c[g] = *reinterpret_cast<const float4*>(P.cos + p * P.cs_st + 32 * g + 4 * j);
-                s[g] = *reinterpret_cast<const float4*>(P.sin + p * P.cs_st + 32 * g + 4 * j);
-            }
-            ap_rotate(x, c, s);
-        }
-        if (is_q) {
-            T* dst = reinterpret_cast<T*>(P.q_out) + (tok * P.n_q + head) * kHD;
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-                *reinterpret_cast<uint2*>(dst + 32 * g + 4 * j) = make_uint2(PgType<T>::down(x[g][0], x[g][1]), PgType<T>::down(x[g][2], x[g][3]));
-        }
-    }
-    if (is_q) slot = -1;
+    const bool there = tok < P.n_tok;
+    const uint32_t first = (task - pair * n_tasks) * P.per, last = min(n_chunks, first + P.per);
+    if (2 * (int64_t)pair >= P.n_tok) return;
+    // kind (0 K, 1 V, 2 query) and head of this octet's row of a chunk; a row past the end is none
+    auto place = [&](uint32_t chunk, int& kind, int& head) {
+        kind = chunk < (uint32_t)P.kv_chunks ? 0 : chunk < 2u * P.kv_chunks ? 1 : 2;
+        head = 2 * (int)(chunk - kind * (uint32_t)P.kv_chunks) + (o >> 1);
+        return there && head < (kind == 2 ? P.n_q : P.n_kv);
+    };
+    auto fetch = [&](uint32_t chunk) {
+        int kind, head;
+        Row r = {};
+        if (place(chunk, kind, head))
+            r = ap_load(kind == 0 ? reinterpret_cast<const T*>(P.k) + tok * P.k_st + head * P.k_sh
+                        : kind == 1 ? reinterpret_cast<const T*>(P.v) + tok * P.v_st + head * P.v_sh
+                                    : reinterpret_cast<const T*>(P.q) + tok * P.q_st + head * P.q_sh, j);
+        return r;
+    };
+    Row next = fetch(first);
+    int64_t slot = there ? P.slots[tok] : -1;
     const int page_tok = P.units * kUnitTok;
     if (slot >= (int64_t)P.n_pages * page_tok) {
         if (P.status) *P.status = kStatusOverflow;
         slot = -1;
     }
-    uint32_t word[4] = {0x8888u, 0x8888u, 0x8888u, 0x8888u};         // half-words 4 j .. 4 j + 3
-    float scale[4];
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-        float a = 0.f;
-        bool nan = false;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            a = fmaxf(a, fabsf(x[g][e]));
-            nan |= x[g][e] != x[g][e];
+    float cs[2][4] = {}, sn[2][4] = {};
+    bool angle = true;
+    if (P.cos && there && !(first >= (uint32_t)P.kv_chunks && last <= 2u * P.kv_chunks)) {
+        int64_t p = P.positions[tok];
+        if (p < 0 || p >= P.n_positions) { // no angle for it: its key is not stored, and the caller learns of it
+            if (P.status && slot >= 0) *P.status = kStatusOverflow;
+            angle = false;
+            p = 0;
         }
-        if (nan) a = __uint_as_float(0x7fffffffu);
 #pragma unroll
-        for (int d = 1; d < 8; d <<= 1) {
-            const float b = __shfl_xor_sync(0xffffffffu, a, d);
-            a = (a != a || b != b) ? __uint_as_float(0x7fffffffu) : fmaxf(a, b);
-        }
-        const float s = __bfloat162float(__float2bfloat16_rn(__fdiv_rn(a, 7.0f)));
-        scale[g] = s != s ? s : fminf(fmaxf(s, kPgScaleMin), kPgScaleMax);
-        if (s == s) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float c = fminf(fmaxf(rintf(__fdiv_rn(x[g][e], scale[g])), -7.f), 7.f);
-                word[e] = (word[e] & ~(0xfu << (4 * g))) | (uint32_t)((int)c + 8) << (4 * g);
-            }
+        for (int g = 0; g < 2; ++g) {
+            const float4 c = *reinterpret_cast<const float4*>(P.cos + p * P.cs_st + 32 * g + 4 * j);
+            const float4 n = *reinterpret_cast<const float4*>(P.sin + p * P.cs_st + 32 * g + 4 * j);
+            cs[g][0] = c.x; cs[g][1] = c.y; cs[g][2] = c.z; cs[g][3] = c.w;
+            sn[g][0] = n.x; sn[g][1] = n.y; sn[g][2] = n.z; sn[g][3] = n.w;
         }
     }
-    if (slot < 0) return;
-    const int64_t page = slot / page_tok;
-    const int in_page = (int)(slot - page * page_tok), t = in_page & 15;
-    uint8_t* u = P.pages + page * P.page_stride + head * P.head_stride + (in_page >> 4) * kUnitBytes;
-    const uint32_t s01 = PgType<__nv_bfloat16>::down(scale[0], scale[1]), s23 = PgType<__nv_bfloat16>::down(scale[2], scale[3]);
-    if (is_k) {
-        *reinterpret_cast<uint2*>(u + 64 * t + 8 * j) = make_uint2(word[0] | word[1] << 16, word[2] | word[3] << 16);
-        if (j == 0) *reinterpret_cast<uint2*>(u + kUnitKs + 8 * t) = make_uint2(s01, s23);
-    } else {
-        uint8_t* dst = u + kUnitV + 128 * (t >> 1) + 2 * (t & 1) + 16 * j;
+    uint8_t* unit = nullptr;
+    int t = 0;
+    if (slot >= 0) {
+        const int64_t page = (uint64_t)slot < 0x100000000ull ? (int64_t)((uint32_t)slot / (uint32_t)page_tok) : slot / page_tok;
+        const int in_page = (int)(slot - page * page_tok);
+        t = in_page & 15;
+        unit = P.pages + page * P.page_stride + (in_page >> 4) * kUnitBytes;
+    }
+    // the two tokens are neighbours of one pair: their V half-words leave as words
+    const int64_t other = __shfl_xor_sync(0xffffffffu, slot, 8);
+    const bool paired = slot >= 0 && other >= 0 && (slot ^ other) == 1 && ((slot & 1) == (o & 1));
+    for (uint32_t chunk = first; chunk < last; ++chunk) {
+        const Row row = next;
+        if (chunk + 1 < last) next = fetch(chunk + 1);
+        int kind, head;
+        const bool live = place(chunk, kind, head);
+        float x[4][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) *reinterpret_cast<uint16_t*>(dst + 4 * e) = (uint16_t)word[e];
-        if (j == 0) *reinterpret_cast<uint2*>(u + kUnitVs + 8 * t) = make_uint2(s01, s23);
+        for (int g = 0; g < 4; ++g) {
+            const float2 a = PgType<T>::up(row.w[g].x), b = PgType<T>::up(row.w[g].y);
+            x[g][0] = a.x; x[g][1] = a.y; x[g][2] = b.x; x[g][3] = b.y;
+        }
+        if (kind != 1 && P.cos) {
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float a = x[g][e], b = x[g + 2][e];
+                    x[g][e] = __fsub_rn(__fmul_rn(a, cs[g][e]), __fmul_rn(b, sn[g][e]));
+                    x[g + 2][e] = __fadd_rn(__fmul_rn(b, cs[g][e]), __fmul_rn(a, sn[g][e]));
+                }
+        }
+        if (kind == 2) {
+            if (live) {
+                T* dst = reinterpret_cast<T*>(P.q_out) + (tok * P.n_q + head) * kHD + 4 * j;
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    *reinterpret_cast<uint2*>(dst + 32 * g) = make_uint2(PgType<T>::down(x[g][0], x[g][1]), PgType<T>::down(x[g][2], x[g][3]));
+            }
+            continue;
+        }
+        uint32_t half[4] = {};             // half-words 4 j + e (k's other bits are multiples of 2^16)
+        float scale[4];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            float a = max_nan(max_nan(fabsf(x[g][0]), fabsf(x[g][1])), max_nan(fabsf(x[g][2]), fabsf(x[g][3]))), k[4];
+#pragma unroll
+            for (int d = 1; d < 8; d <<= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, d));
+            scale[g] = ap_scale(a);
+            if (a != a) {
+                scale[g] = __uint_as_float(0x7fffffffu);
+                k[0] = k[1] = k[2] = k[3] = kRound;
+            } else {
+                ap_codes(x[g], a, scale[g], k);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) half[e] += __float_as_uint(k[e]) << (4 * g);
+        }
+        const uint2 s4 = make_uint2(PgType<__nv_bfloat16>::down(scale[0], scale[1]), PgType<__nv_bfloat16>::down(scale[2], scale[3]));
+        uint32_t w0 = __byte_perm(half[0], half[1], 0x5410), w1 = __byte_perm(half[2], half[3], 0x5410);
+        uint8_t* const u = unit + head * P.head_stride;
+        if (kind == 0) {
+            if (live && unit && angle) {
+                *reinterpret_cast<uint2*>(u + 64 * t + 8 * j) = make_uint2(w0, w1);
+                if (j == 0) *reinterpret_cast<uint2*>(u + kUnitKs + 8 * t) = s4;
+            }
+            continue;
+        }
+        // V, words of two tokens: the even one's lane takes half-words 4 j, + 1 of both, the odd one's + 2, + 3
+        const uint32_t theirs = __shfl_xor_sync(0xffffffffu, o & 1 ? w0 : w1, 8);
+        if (live && unit) {
+            uint8_t* const dst = u + kUnitV + 128 * (t >> 1) + 16 * j;
+            if (paired) {
+                const uint32_t even = o & 1 ? theirs : w0, odd = o & 1 ? w1 : theirs;
+                *reinterpret_cast<uint2*>(dst + 8 * (o & 1)) = make_uint2(__byte_perm(even, odd, 0x5410), __byte_perm(even, odd, 0x7632));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) *reinterpret_cast<uint16_t*>(dst + 4 * e + 2 * (t & 1)) = (uint16_t)half[e];
+            }
+            if (j == 0) *reinterpret_cast<uint2*>(u + kUnitVs + 8 * t) = s4;
+        }
     }
 }
 
@@ -153,50 +220,56 @@ struct RdParams {
     int32_t* status;
 };
 
-// Eight lanes per row as above; the values are exact in fp16 and fp32, and rounded once to bf16.
+// Four lanes per row, lane j its dims 32 g + 8 j .. + 7; the values are exact in fp16 and fp32, and rounded once to bf16.
 template <typename T>
 __global__ void __launch_bounds__(256) pg_read_kernel(const RdParams P) {
     grid_launch_dependents();
     grid_dependency_wait();
-    const int64_t r = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 3;
-    const int j = threadIdx.x & 7;
-    const int64_t tok = r / (2 * P.n_kv);
-    if (tok >= P.n_tok) return;
-    const int row = (int)(r - tok * 2 * P.n_kv), head = row >> 1;
-    const bool is_v = row & 1;
+    const uint32_t r = (blockIdx.x * 256 + threadIdx.x) >> 2, rows = 2 * (uint32_t)P.n_kv;
+    const int j = threadIdx.x & 3;
+    const uint32_t tok = r / rows;
+    if (tok >= (uint32_t)P.n_tok) return;
+    const int row = (int)(r - tok * rows);
+    const bool is_v = row >= P.n_kv;
+    const int head = is_v ? row - P.n_kv : row;
     int64_t slot = P.slots[tok];
     const int page_tok = P.pool.units * kUnitTok;
     if (slot >= (int64_t)P.pool.n_pages * page_tok) {
         if (P.status) *P.status = kStatusOverflow;
         slot = -1;
     }
-    uint32_t w[4] = {0x8888u, 0x8888u, 0x8888u, 0x8888u};
-    float scale[4] = {0.f, 0.f, 0.f, 0.f};
+    uint32_t w[4] = {};                    // half-words 8 j .. 8 j + 7
+    float scale[4] = {};
     if (slot >= 0) {
-        const int64_t page = slot / page_tok;
+        const int64_t page = (uint64_t)slot < 0x100000000ull ? (int64_t)((uint32_t)slot / (uint32_t)page_tok) : slot / page_tok;
         const int in_page = (int)(slot - page * page_tok), t = in_page & 15;
         const uint8_t* u = P.pool.pages + page * P.pool.page_stride + head * P.pool.head_stride + (in_page >> 4) * kUnitBytes;
         if (is_v) {
-            const uint4 x = *reinterpret_cast<const uint4*>(u + kUnitV + 128 * (t >> 1) + 16 * j);
-            const uint32_t sh = 16u * (t & 1);
-            w[0] = x.x >> sh; w[1] = x.y >> sh; w[2] = x.z >> sh; w[3] = x.w >> sh;
+            const uint4* at = reinterpret_cast<const uint4*>(u + kUnitV + 128 * (t >> 1) + 32 * j);
+            const uint4 x = at[0], y = at[1];
+            const uint32_t pick = t & 1 ? 0x7632u : 0x5410u;
+            w[0] = __byte_perm(x.x, x.y, pick); w[1] = __byte_perm(x.z, x.w, pick);
+            w[2] = __byte_perm(y.x, y.y, pick); w[3] = __byte_perm(y.z, y.w, pick);
         } else {
-            const uint2 x = *reinterpret_cast<const uint2*>(u + 64 * t + 8 * j);
-            w[0] = x.x; w[1] = x.x >> 16; w[2] = x.y; w[3] = x.y >> 16;
+            const uint4 x = *reinterpret_cast<const uint4*>(u + 64 * t + 16 * j);
+            w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
         }
         const uint2 s = *reinterpret_cast<const uint2*>(u + (is_v ? kUnitVs : kUnitKs) + 8 * t);
         scale[0] = pg_lo(s.x); scale[1] = pg_hi(s.x); scale[2] = pg_lo(s.y); scale[3] = pg_hi(s.y);
     }
-    T* dst = reinterpret_cast<T*>(is_v ? P.v : P.k) + (tok * P.n_kv + head) * kHD + 4 * j;
+    T* dst = reinterpret_cast<T*>(is_v ? P.v : P.k) + ((int64_t)tok * P.n_kv + head) * kHD + 8 * j;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-        float x[4];
+        float x[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = (float)((int)(w[e] >> (4 * g) & 15u) - 8) * scale[g];
-        if constexpr (sizeof(T) == 4)
-            *reinterpret_cast<float4*>(dst + 32 * g) = make_float4(x[0], x[1], x[2], x[3]);
-        else
-            *reinterpret_cast<uint2*>(dst + 32 * g) = make_uint2(PgType<T>::down(x[0], x[1]), PgType<T>::down(x[2], x[3]));
+        for (int e = 0; e < 8; ++e) x[e] = slot < 0 ? 0.f : (float)((int)(w[e >> 1] >> (16 * (e & 1) + 4 * g) & 15u) - 8) * scale[g];
+        if constexpr (sizeof(T) == 4) {
+            reinterpret_cast<float4*>(dst + 32 * g)[0] = make_float4(x[0], x[1], x[2], x[3]);
+            reinterpret_cast<float4*>(dst + 32 * g)[1] = make_float4(x[4], x[5], x[6], x[7]);
+        } else {
+            *reinterpret_cast<uint4*>(dst + 32 * g) =
+                make_uint4(PgType<T>::down(x[0], x[1]), PgType<T>::down(x[2], x[3]), PgType<T>::down(x[4], x[5]), PgType<T>::down(x[6], x[7]));
+        }
     }
 }
 
@@ -225,13 +298,19 @@ extern "C" __attribute__((visibility("default"))) int bgtq_paged_append(
     if (!slots || !k || !v || (q == nullptr) != (n_q == 0) || (q && !q_out) || !rope_cos != !rope_sin) return BGTQ_E_BADARG;
     if (rope_cos && (!positions || n_positions < 1)) return BGTQ_E_BADARG;
     if (q && !rope_cos) return BGTQ_E_BADARG;
-    if (!aligned(k, 8) || !aligned(v, 8) || !aligned(q, 8) || !aligned(q_out, 8) || k_st % 4 || k_sh % 4 || v_st % 4 || v_sh % 4 ||
-        q_st % 4 || q_sh % 4 || !aligned(rope_cos, 16) || !aligned(rope_sin, 16) || rope_st % 4)
+    if (!aligned(k, 16) || !aligned(v, 16) || !aligned(q, 16) || !aligned(q_out, 16) || k_st % 8 || k_sh % 8 || v_st % 8 || v_sh % 8 ||
+        q_st % 8 || q_sh % 8 || !aligned(rope_cos, 16) || !aligned(rope_sin, 16) || rope_st % 4)
         return BGTQ_E_ALIGN;
     ApParams P{pages, page_stride, head_stride, n_pages, page_tokens / kUnitTok, slots, k, v, q, k_st, k_sh, v_st, v_sh, q_st, q_sh, q_out,
-               rope_cos, rope_sin, rope_st, positions, n_positions, n_tok, n_kv, n_q, status};
-    const int64_t tasks = (int64_t)((n_tok + 1) / 2) * ((2 * n_kv + n_q + 1) / 2), blocks = (tasks + kApThreads / 32 - 1) / (kApThreads / 32);
-    if (blocks > INT32_MAX) return BGTQ_E_TOOBIG;
+               rope_cos, rope_sin, rope_st, positions, n_positions, n_tok, n_kv, n_q, (n_kv + 1) / 2, (n_q + 1) / 2, 1, status};
+    // Few tokens: a warp per chunk.  Many: as many chunks per warp as leave eight warps for each of a SM's four schedulers.
+    const int64_t pairs = ((int64_t)n_tok + 1) / 2, chunks = 2 * P.kv_chunks + P.q_chunks;
+    int dev = 0, sms = 148;
+    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    const int64_t per = pairs * chunks / (32ll * sms);
+    P.per = (int32_t)(per < 1 ? 1 : per < chunks ? per : chunks);
+    const int64_t tasks = pairs * ((chunks + P.per - 1) / P.per), blocks = (tasks + kApThreads / 32 - 1) / (kApThreads / 32);
+    if (tasks + kApThreads / 32 > INT32_MAX) return BGTQ_E_TOOBIG;
     const auto kernel = (flags & BGTQ_PAGED_BF16) ? pg_append_kernel<__nv_bfloat16> : pg_append_kernel<__half>;
     return launch_kernel(kernel, dim3((unsigned)blocks), dim3(kApThreads), 0, (cudaStream_t)stream, true, P) == cudaSuccess ? BGTQ_OK
                                                                                                                             : BGTQ_E_LAUNCH;
@@ -246,8 +325,8 @@ extern "C" __attribute__((visibility("default"))) int bgtq_paged_read(
     if (!slots || !k || !v) return BGTQ_E_BADARG;
     if (!aligned(k, 16) || !aligned(v, 16)) return BGTQ_E_ALIGN;
     RdParams P{{pages, page_stride, head_stride, n_pages, page_tokens / kUnitTok}, slots, k, v, n_tok, n_kv, status};
-    const int64_t blocks = ((int64_t)n_tok * 2 * n_kv * 8 + 255) / 256;
-    if (blocks > INT32_MAX) return BGTQ_E_TOOBIG;
+    const int64_t blocks = ((int64_t)n_tok * 2 * n_kv * 4 + 255) / 256;
+    if (blocks * 64 > INT32_MAX) return BGTQ_E_TOOBIG;
     const auto kernel = (flags & BGTQ_PAGED_F32) ? pg_read_kernel<float> : (flags & BGTQ_PAGED_BF16) ? pg_read_kernel<__nv_bfloat16> : pg_read_kernel<__half>;
     return launch_kernel(kernel, dim3((unsigned)blocks), dim3(256), 0, (cudaStream_t)stream, true, P) == cudaSuccess ? BGTQ_OK : BGTQ_E_LAUNCH;
 }

@@ -99,9 +99,9 @@ def _append(pages, slots, k, v, q, cos, sin, positions, status):
     page = _pool(pages)
     dev, n_kv = pages.device, pages.shape[1]
     flags = _type_flag(k.dtype, "k")
-    k = _rows(k, "k", None, n_kv, k.dtype, dev, 8)
+    k = _rows(k, "k", None, n_kv, k.dtype, dev, 16)
     n = k.shape[0]
-    v = _rows(v, "v", n, n_kv, k.dtype, dev, 8)
+    v = _rows(v, "v", n, n_kv, k.dtype, dev, 16)
     slots = _ints(slots, "slots", torch.int64, (n,), dev)
     if (cos is None) != (sin is None) or (cos is None) != (positions is None):
         raise ValueError("cos, sin and positions belong together")
@@ -120,7 +120,7 @@ def _append(pages, slots, k, v, q, cos, sin, positions, status):
     if q is not None:
         if cos is None:
             raise ValueError("q is only taken to be rotated: pass cos, sin and positions")
-        q = _rows(q, "q", n, None, k.dtype, dev, 8)
+        q = _rows(q, "q", n, None, k.dtype, dev, 16)
         n_q, qs = q.shape[1], q.stride()[:2]
         q_out = torch.empty(n, n_q, HD, dtype=q.dtype, device=dev)
         if n_q == 0:

@@ -96,7 +96,7 @@ def test_library_refuses_before_it_touches_the_device():
         return lib.bgtq_paged_append(*a.values())
     assert append(n=0) == _lib.OK
     for kw, code in ((dict(page=24), -1), (dict(page=0), -1), (dict(n_pages=0), -1), (dict(pages=0), -1), (dict(slots=0), -1), (dict(n=-1), -1),
-                     (dict(pages=p + 8), -3), (dict(hs=2300), -3), (dict(k=p + 2), -3), (dict(kst=130), -3), (dict(cos=p), -1),
+                     (dict(pages=p + 8), -3), (dict(hs=2300), -3), (dict(k=p + 2), -3), (dict(kst=132), -3), (dict(cos=p), -1),
                      (dict(cos=p, sin=p, rst=64), -1), (dict(cos=p, sin=p, rst=66, pos=p, npos=1), -3), (dict(q=p, nq=1, qo=p), -1),
                      (dict(nq=1), -1), (dict(flags=2), -1), (dict(flags=64), -1)):
         assert append(**kw) == code, kw
