@@ -300,44 +300,49 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
             atomicMin(&S.nan[3], f.w);
         }
     }
-    // ---- the queries as A operands: sixteen lanes per row, 16 bytes each ----
-    {
+    // ---- the queries as A operands: a warp takes eight rows at a time, four lanes to a row, so that its stores are contiguous (with a row's
+    // pieces side by side every one of them fell into the same banks: 10000 cycles for the CTA's rows) ----
+    if (warp < 16) {
         const bool neg = P.scale_log2 < 0.f, zero = P.scale_log2 == 0.f;
-        constexpr int kStep = kThreads / 16, kIter = (kBlockRows + kStep - 1) / kStep;
-        uint4 w[kIter];
+        uint4 w[2][4];
 #pragma unroll
-        for (int i = 0; i < kIter; ++i) {
-            const int row = i * kStep + (tid >> 4), g = row0 + row;
-            w[i] = make_uint4(0, 0, 0, 0);
-            if (row < kBlockRows && g < n_rows && !zero) {
-                const int pos = g / P.gqa, hq = h * P.gqa + g - pos * P.gqa;
-                w[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(P.q) + (int64_t)(s.q0 + pos) * P.q_st + hq * P.q_sh + 8 * (tid & 15));
+        for (int i = 0; i < 2; ++i) {
+            const int g = row0 + 16 * warp + 8 * i + (lane & 7), pos = g / P.gqa, hq = h * P.gqa + g - pos * P.gqa;
+            const T* src = reinterpret_cast<const T*>(P.q) + (int64_t)(s.q0 + pos) * P.q_st + (int64_t)hq * P.q_sh + 8 * (lane >> 3);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                w[i][k] = make_uint4(0, 0, 0, 0);
+                if (g < n_rows && !zero) w[i][k] = *reinterpret_cast<const uint4*>(src + 32 * k);
             }
         }
 #pragma unroll
-        for (int i = 0; i < kIter; ++i) {
-            const int row = i * kStep + (tid >> 4), kc = tid & 15;
-            const uint32_t ww[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-            float x[8], top = 0.f;
+        for (int i = 0; i < 2; ++i) {
+            const int row = 16 * warp + 8 * i + (lane & 7);
+            float x[4][8], top = 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 v = PgType<T>::up(ww[e]);
-                x[2 * e] = v.x;
-                x[2 * e + 1] = v.y;
-                top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t ww[4] = {w[i][k].x, w[i][k].y, w[i][k].z, w[i][k].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 v = PgType<T>::up(ww[e]);
+                    x[k][2 * e] = v.x;
+                    x[k][2 * e + 1] = v.y;
+                    top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
+                }
             }
-#pragma unroll
-            for (int d = 1; d < 16; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
             float up0, up1;
             const float fac = pg_row_scale(top, up0, up1);
             if (neg) up0 = -up0;
-            uint32_t o[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = pack_half2(x[2 * e] * up0 * up1, x[2 * e + 1] * up0 * up1);
-            if (row < kBlockRows) {
-                *reinterpret_cast<uint4*>(S.q[row >> 7] + ((row & 127) >> 3) * 2048 + kc * 128 + (row & 7) * 16) = make_uint4(o[0], o[1], o[2], o[3]);
-                if (kc == 0) S.xch[row >> 7][0][row & 127] = fac;
+            for (int k = 0; k < 4; ++k) {
+                uint32_t o[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = pack_half2(x[k][2 * e] * up0 * up1, x[k][2 * e + 1] * up0 * up1);
+                *reinterpret_cast<uint4*>(S.q[row >> 7] + ((row & 127) >> 3) * 2048 + (4 * k + (lane >> 3)) * 128 + (row & 7) * 16) = make_uint4(o[0], o[1], o[2], o[3]);
             }
+            if (lane < 8) S.xch[row >> 7][0][row & 127] = fac;
         }
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // Q: generic-proxy stores -> tensor-core reads
@@ -512,9 +517,11 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
         if (!bar_and(3 + mb, 256, ok)) ok = false;
         lsum += S.xch[mb][hf ^ 1][r128];
         const float inv = lsum > 0.f ? 1.0f / lsum : lsum == 0.f ? 0.f : lsum;
+        const bool wide = ((reinterpret_cast<uintptr_t>(P.out) | (uint64_t)(2 * P.o_st) | (uint64_t)(2 * P.o_sh)) & 15u) == 0;
         if (ok) {
-            const int hq = h * P.gqa + g - pos * P.gqa;
-            T* const dst0 = reinterpret_cast<T*>(P.out) + (int64_t)(s.q0 + pos) * P.o_st + (int64_t)hq * P.o_sh + 64 * hf;
+            // through the warp's own piece of the block's query tile, which no product reads any more: 32 rows of 128 bytes, 16-byte pieces
+            // exchanged by row, so that the stores are whole lines
+            uint8_t* const mine = S.q[mb] + (warp & 7) * 4096;
 #pragma unroll 1
             for (int ch = 0; ch < 2; ++ch) {
                 float o[32];
@@ -525,14 +532,30 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
 #pragma unroll
                     for (int c = 0; c < 32; ++c) o[c] = 0.f;
                 }
-                if (rok) {
-                    const float f = S.nan[2 * hf + ch] < lim ? __uint_as_float(0x7fffffffu) : inv;
-                    uint2* dst = reinterpret_cast<uint2*>(dst0 + 32 * ch);
+                const float f = S.nan[2 * hf + ch] < lim ? __uint_as_float(0x7fffffffu) : inv;
 #pragma unroll
-                    for (int c = 0; c < 8; ++c)
-                        dst[c] = make_uint2(PgType<T>::down(o[4 * c] * f, o[4 * c + 1] * f), PgType<T>::down(o[4 * c + 2] * f, o[4 * c + 3] * f));
+                for (int c = 0; c < 4; ++c)
+                    *reinterpret_cast<uint4*>(mine + lane * 128 + (((4 * ch + c) ^ (lane & 7)) << 4)) =
+                        make_uint4(PgType<T>::down(o[8 * c] * f, o[8 * c + 1] * f), PgType<T>::down(o[8 * c + 2] * f, o[8 * c + 3] * f),
+                                   PgType<T>::down(o[8 * c + 4] * f, o[8 * c + 5] * f), PgType<T>::down(o[8 * c + 6] * f, o[8 * c + 7] * f));
+            }
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int r32 = 4 * k + (lane >> 3), gr = row0 + kRows * mb + (warp & 3) * 32 + r32, pr = gr / P.gqa;
+                const uint4 v = *reinterpret_cast<const uint4*>(mine + r32 * 128 + (((lane & 7) ^ (r32 & 7)) << 4));
+                if (gr < n_rows) {
+                    uint2* const dst = reinterpret_cast<uint2*>(reinterpret_cast<T*>(P.out) + (int64_t)(s.q0 + pr) * P.o_st +
+                                                                (int64_t)(h * P.gqa + gr - pr * P.gqa) * P.o_sh + 64 * hf + 8 * (lane & 7));
+                    if (wide) {
+                        *reinterpret_cast<uint4*>(dst) = v;
+                    } else {
+                        dst[0] = make_uint2(v.x, v.y);
+                        dst[1] = make_uint2(v.z, v.w);
+                    }
                 }
             }
+            const int hq = h * P.gqa + g - pos * P.gqa;
             if (rok && hf == 0 && P.lse)
                 P.lse[(int64_t)(s.q0 + pos) * P.n_q + hq] = lsum == 0.f ? -INFINITY : (m_used + log2f(lsum)) * 0.693147180559945309f;
         }
