@@ -40,10 +40,12 @@ __device__ __forceinline__ float pg_hi(uint32_t w) { return __uint_as_float(w & 
 
 template <typename T> struct PgType;
 template <> struct PgType<__half> {
+    static constexpr bool kHalf = true;
     static __device__ __forceinline__ float2 up(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
     static __device__ __forceinline__ uint32_t down(float a, float b) { return pack_half2(a, b); }
 };
 template <> struct PgType<__nv_bfloat16> {
+    static constexpr bool kHalf = false;
     static __device__ __forceinline__ float2 up(uint32_t w) { return make_float2(pg_lo(w), pg_hi(w)); }
     static __device__ __forceinline__ uint32_t down(float a, float b) {
         uint32_t d;
@@ -52,13 +54,15 @@ template <> struct PgType<__nv_bfloat16> {
     }
 };
 
-// A query row of largest magnitude `top`: up0 * up1 = 2^e brings it to [2^13, 2^14); returns 2^-e.  A row of zeros, or with an infinity, stays.
-__device__ __forceinline__ float pg_row_scale(float top, float& up0, float& up1) {
+// A query row of largest magnitude `top` comes to [2^13, 2^14) by 2^e; a row of zeros, or with an infinity, stays.  e: -114 .. 140.
+__device__ __forceinline__ int pg_row_exponent(float top) {
     const int ex = (int)(__float_as_uint(top) >> 23) - 127;
-    const int e = top > 0.f && ex < 128 ? 13 - ex : 0;         // -114 .. 140: in two steps
-    up0 = __uint_as_float((uint32_t)(127 + e / 2) << 23);
-    up1 = __uint_as_float((uint32_t)(127 + e - e / 2) << 23);
-    return __uint_as_float((uint32_t)(127 - e / 2) << 23) * __uint_as_float((uint32_t)(127 - (e - e / 2)) << 23);
+    return top > 0.f && ex < 128 ? 13 - ex : 0;
+}
+// 2^e as a product of two factors
+__device__ __forceinline__ void pg_pow2(int e, float& a, float& b) {
+    a = __uint_as_float((uint32_t)(127 + e / 2) << 23);
+    b = __uint_as_float((uint32_t)(127 + e - e / 2) << 23);
 }
 
 // Lets a kernel use this much dynamic shared memory, once per device.

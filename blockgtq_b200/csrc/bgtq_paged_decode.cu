@@ -268,8 +268,11 @@ __device__ __forceinline__ void pd_query(const PdParams& P, Query<NT>& Q, const 
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        float up0, up1;
-        float fac = pg_row_scale(top, up0, up1) * fabsf(P.scale_log2);
+        float up0, up1, down0, down1;
+        const int ex = pg_row_exponent(top);
+        pg_pow2(ex, up0, up1);
+        pg_pow2(-ex, down0, down1);
+        float fac = fabsf(P.scale_log2) * down0 * down1;
         if (P.scale_log2 < 0.f) up0 = -up0;  // (factors are positive: hidden logits are minus infinity before they meet one)
         if (P.scale_log2 == 0.f) {
             up0 = 0.f;
@@ -870,7 +873,7 @@ extern "C" __attribute__((visibility("default"))) int64_t bgtq_paged_workspace_b
     if (n_seq < 0 || n_tok < 0 || n_kv < 1 || n_q < 1 || n_q % n_kv || max_q < 1 || max_tokens < 0) return BGTQ_E_BADARG;
     if (n_q / n_kv > 8) return BGTQ_E_UNSUPPORTED;
     const PdForm f = pd_form(n_seq, n_tok, n_q, n_kv, max_q, max_tokens, flags);
-    if (f.prefill) return paged_prefill_workspace(n_seq, n_kv, max_tokens);
+    if (f.prefill) return paged_prefill_workspace(n_seq, n_tok, n_q / n_kv, n_kv, max_tokens);
     return f.n_rank ? 0 : (int64_t)f.n_cta * 2 * 8 * f.nt * (kHD * 4 + 8);
 }
 
@@ -898,7 +901,7 @@ extern "C" __attribute__((visibility("default"))) int bgtq_paged_attend(
     PdForm f = pd_form(n_seq, n_tok, n_q, n_kv, max_q, max_tokens, flags);
     const cudaStream_t st = (cudaStream_t)stream;
     if (f.prefill) {
-        if (!workspace || workspace_bytes < paged_prefill_workspace(n_seq, n_kv, max_tokens)) return BGTQ_E_BADARG;
+        if (!workspace || workspace_bytes < paged_prefill_workspace(n_seq, n_tok, n_q / n_kv, n_kv, max_tokens)) return BGTQ_E_BADARG;
         return paged_prefill({{pages, page_stride, head_stride, n_pages, page_tokens / kUnitTok}, table, table_stride, seq_lens, cu_q, n_seq, n_tok, n_q,
                               n_kv, n_q / n_kv, (flags & BGTQ_PAGED_CAUSAL) ? 1 : 0, (flags & BGTQ_PAGED_BF16) ? 1 : 0, max_tokens,
                               reinterpret_cast<uint8_t*>(workspace), q, q_st, q_sh, scale * 1.44269504088896340736f, out, o_st, o_sh, lse, status},

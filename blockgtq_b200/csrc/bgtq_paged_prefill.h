@@ -23,7 +23,7 @@ struct PagedPrefill {
     float* lse;
     int32_t* status;
 };
-int64_t paged_prefill_workspace(int n_seq, int n_kv, int64_t max_tokens);
+int64_t paged_prefill_workspace(int n_seq, int n_tok, int gqa, int n_kv, int64_t max_tokens);
 int paged_prefill(const PagedPrefill& A, cudaStream_t stream);
 
 }  // namespace bgtq

@@ -320,6 +320,39 @@ def test_no_number_in_a_prefill_shows_in_the_rows_that_see_it(rows_form):
     assert torch.isfinite(lse[:280 - first]).all() and lse[280 - first:].isnan().all()
 
 
+def test_a_key_that_is_no_number_shows_wherever_it_lies_in_a_tile(rows_form):
+    from blockgtq_b200 import paged_kv4_append, paged_kv4_prefill_attention
+    gen = torch.Generator().manual_seed(23)
+    pages, table, slots = _case(gen, 1, 16, [160] * 40)
+    k, v = _noise(gen, 40, 1, 128).half(), _noise(gen, 40, 1, 128).half()
+    k[:, 0, 5] = math.nan
+    at = [100 + i for i in range(40)]                          # of sequence i
+    paged_kv4_append(pages, torch.stack([slots[i][t] for i, t in enumerate(at)]).to(DEV), k.to(DEV), v.to(DEV))
+    q = _noise(gen, 40 * 80, 1, 128).half().to(DEV)
+    out = paged_kv4_prefill_attention(q, pages, table.to(DEV), torch.full((40,), 160, dtype=torch.int32, device=DEV),
+                                      torch.arange(0, 41 * 80, 80, dtype=torch.int32, device=DEV), max_q_len=80).view(40, 80, 128)
+    for i, t in enumerate(at):
+        assert torch.isfinite(out[i, :t - 80]).all() and out[i, t - 80:].isnan().all(), i
+
+
+def test_a_prefill_whose_blocks_are_cut_between_ctas():
+    """Few blocks with long contexts beside many short ones, rows that see nothing, and a query of a layer's strided projection."""
+    from blockgtq_b200 import paged_kv4_prefill_attention
+    gen = torch.Generator().manual_seed(29)
+    seqs = [(3000, 70), (1, 1), (0, 40), (5, 90), (129, 129)] + [(40 + i, 20) for i in range(30)]
+    lens, counts = [t for t, _ in seqs], [n for _, n in seqs]
+    pages, table, slots = _case(gen, 2, 64, lens)
+    ends = [sum(counts[:i]) for i in range(len(counts) + 1)]
+    q = _noise(gen, ends[-1], 10, 128).half()
+    out, lse = paged_kv4_prefill_attention(q.to(DEV)[:, 1:7], pages, table.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV),
+                                           torch.tensor(ends, dtype=torch.int32, device=DEV), return_lse=True)
+    host = pages.cpu()
+    for b, (t, m) in enumerate(seqs):
+        if b < 8 or b == len(seqs) - 1:
+            _check(out, lse, R.attention(q[ends[b]:ends[b + 1], 1:7], host, slots[b], [t - m + 1 + i for i in range(m)], 1 / math.sqrt(128)),
+                   slice(ends[b], ends[b + 1]))
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 2.0])
 def test_scales_of_any_sign(scale, rows_form):
     from blockgtq_b200 import paged_kv4_prefill_attention
