@@ -270,11 +270,56 @@ constexpr float kLift = 7.0f, kReach = 15.0f;
 #endif
 constexpr uint32_t kPolyPairs = KPOLY;
 
+// A CTA's share, block by block.  Every role walks it for itself.
+struct Walk {
+    Block b;
+    int g, t0, tiles, h, left, n_blocks;         // block, first tile and tiles of it (zero: its rows see nothing), KV head of the launch; tiles from here on
+    bool first;
+
+    Walk() = default;
+    __device__ __forceinline__ explicit Walk(const Pf& P) {
+        const int4 v = P.start[blockIdx.x], e = P.start[blockIdx.x + 1];
+        n_blocks = P.start[P.n_cta + 1].x;
+        g = v.x;
+        t0 = v.y;
+        h = v.z;
+        left = e.w - v.w;
+        first = true;
+        if (left > 0) b = P.blk[g];
+        tiles = left > 0 && b.sees ? run() : 0;
+    }
+    __device__ __forceinline__ int run() const { return min(b.tiles - t0, left); }
+    __device__ __forceinline__ bool whole() const { return t0 == 0 && left >= b.tiles; }
+    __device__ __forceinline__ bool more() const { return left > run(); }
+    __device__ __forceinline__ int next_g() const { return g + 1 == n_blocks ? 0 : g + 1; }
+    __device__ __forceinline__ int next_h() const { return h + (g + 1 == n_blocks); }
+    __device__ __forceinline__ int next_tiles(const Block& n) const { return n.sees ? min(n.tiles, left - run()) : 0; }
+    __device__ __forceinline__ void step(const Block& n) {     // n: the record of next_g()
+        left -= run();
+        first = false;
+        h = next_h();
+        g = next_g();
+        t0 = 0;
+        b = n;
+        tiles = n.sees ? run() : 0;
+    }
+    __device__ __forceinline__ void step_from(const Walk& w) { // the same from the block before, with its own record in place
+        left = w.left - w.run();
+        first = false;
+        h = w.next_h();
+        g = w.next_g();
+        t0 = 0;
+        n_blocks = w.n_blocks;
+        tiles = b.sees ? run() : 0;
+    }
+};
+
 struct PfSmem {
     __align__(128) uint8_t q[kBlocks][kPart];
     __align__(128) uint8_t ring[kSlots][kPart];
     __align__(16) uint8_t stage[16][2048];      // per softmax warp: 64 bytes of each of its rows on their way out
-    __align__(16) Block next[kBlocks];          // the block behind the one that is worked on
+    __align__(16) Walk walk[kBlocks][2];        // the softmax's: the block that is worked on and the one behind it, in turn (not in registers,
+                                                // where the tiles' loop needs them)
     __align__(8) uint64_t full[kSlots], empty[kSlots], q_ready[kBlocks], s_ready[kBlocks], p_ready[kBlocks][2], o_ready[kBlocks];
     float xch[kBlocks][2][kRows];       // the two threads of a row: maxima, at the end denominators
     int16_t ex[kBlocks][kRows];         // the rows' queries are times 2^ex
@@ -351,40 +396,6 @@ __device__ __forceinline__ bool pf_wait(PfSmem& S, uint64_t* bar, uint32_t parit
     S.failed = 1;
     return false;
 }
-
-// A CTA's share, block by block.  Every role walks it for itself.
-struct Walk {
-    Block b;
-    int g, t0, tiles, h, left, n_blocks;         // block, first tile and tiles of it (zero: its rows see nothing), KV head of the launch; tiles from here on
-    bool first;
-
-    __device__ __forceinline__ Walk(const Pf& P) {
-        const int4 v = P.start[blockIdx.x], e = P.start[blockIdx.x + 1];
-        n_blocks = P.start[P.n_cta + 1].x;
-        g = v.x;
-        t0 = v.y;
-        h = v.z;
-        left = e.w - v.w;
-        first = true;
-        if (left > 0) b = P.blk[g];
-        tiles = left > 0 && b.sees ? run() : 0;
-    }
-    __device__ __forceinline__ int run() const { return min(b.tiles - t0, left); }
-    __device__ __forceinline__ bool whole() const { return t0 == 0 && left >= b.tiles; }
-    __device__ __forceinline__ bool more() const { return left > run(); }
-    __device__ __forceinline__ int next_g() const { return g + 1 == n_blocks ? 0 : g + 1; }
-    __device__ __forceinline__ int next_h() const { return h + (g + 1 == n_blocks); }
-    __device__ __forceinline__ int next_tiles(const Block& n) const { return n.sees ? min(n.tiles, left - run()) : 0; }
-    __device__ __forceinline__ void step(const Block& n) {     // n: the record of next_g()
-        left -= run();
-        first = false;
-        h = next_h();
-        g = next_g();
-        t0 = 0;
-        b = n;
-        tiles = n.sees ? run() : 0;
-    }
-};
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
@@ -510,7 +521,6 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
         const int mb = warp >> 3, hf = (warp >> 2) & 1, r128 = (warp & 3) * 32 + lane, w8 = warp & 7;
         const uint32_t tlane = tmem + ((uint32_t)((warp & 3) * 32) << 16);   // this warp's quarter of the lanes
         const uint32_t colS = tlane + kColS + 128u * mb, colO = tlane + kColO + 128u * mb + 64u * hf, sS = colS + 64u * hf;
-        const bool wide = ((reinterpret_cast<uintptr_t>(P.out) | (uint64_t)(2 * P.o_st) | (uint64_t)(2 * P.o_sh)) & 15u) == 0;
         int done = 0;                                     // tiles so far
         // A block's queries go straight to their places in the operand; a warp takes sixteen rows, eight at a time and four lanes to a row, so that
         // its pieces are contiguous there.  They are requested while the last tile before them is worked on, and bf16 ones then made fp16, so that the
@@ -575,22 +585,24 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
             __syncwarp();
             if (lane == 0) mbar_arrive(&S.q_ready[mb]);
         };
-        Walk w(P);
+        if ((tid & 255) == 0) S.walk[mb][0] = Walk(P);
         if (PgType<T>::kHalf && (tid & 255) < kRows) S.ex[mb][tid & 127] = 0;
-        bool go = w.left > 0;
-        if (go && w.tiles > 0) {
-            fetch(w.b, w.h);
+        bar_and(3 + mb, 256, true);
+        bool more = S.walk[mb][0].left > 0;
+        if (more && S.walk[mb][0].tiles > 0) {
+            fetch(S.walk[mb][0].b, S.walk[mb][0].h);
             ready();
         }
-        while (go) {
-            const Block sg = w.b;
-            const int tiles = w.tiles, tile0 = w.t0, h = P.h0 + w.h, n_rows = sg.n * P.gqa, row0 = sg.row0 + kRows * mb;
-            const bool more = w.more();
+        for (int turn = 0; more; turn ^= 1) {
+            const Walk& w = S.walk[mb][turn];
+            Walk& next = S.walk[mb][turn ^ 1];
+            const int tiles = w.tiles, tile0 = w.t0;
+            more = w.more();
             if (more && w8 == 0 && lane < 2)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(&S.next[mb]) + 16 * lane),
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(&next.b) + 16 * lane),
                              "l"(reinterpret_cast<const uint8_t*>(P.blk + w.next_g()) + 16 * lane) : "memory");
             for (int t = tid & 255; t < tiles; t += 256) {
-                const int4 f = P.nan[((int64_t)sg.si * P.n_h + w.h) * P.max_tiles + tile0 + t];
+                const int4 f = P.nan[((int64_t)w.b.si * P.n_h + w.h) * P.max_tiles + tile0 + t];
                 if (min(min(f.x, f.y), min(f.z, f.w)) != INT_MAX) {
                     atomicMin(&S.nan[mb][0], f.x);
                     atomicMin(&S.nan[mb][1], f.y);
@@ -599,13 +611,15 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                 }
             }
             bar_and(3 + mb, 256, true);                // (exponents are there)
-            const int g = row0 + r128, pos = pf_pos(P, g), behind = sg.len - sg.n + 1;
-            const bool rok = g < n_rows;
-            const int lim = !rok ? 0 : (P.causal ? max(0, min(sg.len, behind + pos)) : sg.len);
+            int lim;
+            {
+                const int g = w.b.row0 + kRows * mb + r128, pos = pf_pos(P, g);
+                lim = pos >= w.b.n ? 0 : P.causal ? max(0, min(w.b.len, w.b.len - w.b.n + 1 + pos)) : w.b.len;
+            }
             float down0, down1;
             pg_pow2(-S.ex[mb][r128], down0, down1);
             const float sc = (P.scale_log2 == 0.f ? 1.f : fabsf(P.scale_log2)) * down0 * down1;
-            const uint8_t* const valid = P.valid + (int64_t)sg.si * P.max_tiles + tile0;
+            const uint8_t* const valid = P.valid + (int64_t)w.b.si * P.max_tiles + tile0;
             uint32_t units = tiles > 0 ? valid[0] : 0;
             float m_used = -INFINITY, lsum = 0.f;    // what this row scales by (log2), this half's denominator
             const uint64_t sc2 = pack_f2(sc, sc);
@@ -664,7 +678,7 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                         for (int ch = 0; ch < 8; ++ch) tmem_scale8(colO + 8u * ch, alpha);
                     }
                 }
-                if (last && w.next_tiles(S.next[mb]) > 0) fetch(S.next[mb], w.next_h());        // (the last product with the queries is done)
+                if (last && w.next_tiles(next.b) > 0) fetch(next.b, w.next_h());        // (the last product with the queries is done)
                 const float z = m_used == -INFINITY ? 0.f : m_used;
                 const uint64_t nz2 = pack_f2(-z, -z);
                 uint64_t ps[2] = {0ull, 0ull};
@@ -706,7 +720,6 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
             }
             done += tiles;
             // ---- what comes next, and the rows' results, or their part of them ----
-            Block next = sg;
             if (more) {
                 if (tiles == 0) {                      // (nobody waited for the record, nor fetched)
                     if (w8 == 0) {
@@ -715,9 +728,8 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                     }
                     bar_and(3 + mb, 256, true);
                 }
-                next = S.next[mb];
-                if (ok && w.next_tiles(next) > 0) {
-                    if (tiles == 0) fetch(next, w.next_h());
+                if (ok && w.next_tiles(next.b) > 0) {
+                    if (tiles == 0) fetch(next.b, w.next_h());
                     ready();
                 }
             }
@@ -726,9 +738,10 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                 tc_fence_after_sync();
             }
             const bool bad0 = S.nan[mb][2 * hf] < lim, bad1 = S.nan[mb][2 * hf + 1] < lim;
-            bar_and(3 + mb, 256, true);                // (maxima, the next record, and which numbers are none, are read before their places change)
+            bar_and(3 + mb, 256, true);                // (maxima, and which numbers are none, are read before their places change)
             S.xch[mb][hf][r128] = lsum;
             if ((tid & 255) < 4) S.nan[mb][tid & 3] = INT_MAX;
+            if ((tid & 255) == 0 && more) next.step_from(w);
             if (!bar_and(3 + mb, 256, ok)) {
                 ok = false;
                 break;
@@ -740,12 +753,14 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
             uint8_t* const st = S.stage[warp];         // 64 bytes per row, 16-byte pieces exchanged by row
             auto stage = [&](int c, uint4 v) { *reinterpret_cast<uint4*>(st + lane * 64 + ((c ^ (lane >> 1 & 3)) << 4)) = v; };
             auto staged = [&](int r32) { return *reinterpret_cast<const uint4*>(st + r32 * 64 + (((lane & 3) ^ (r32 >> 1 & 3)) << 4)); };
+            const bool wide = ((reinterpret_cast<uintptr_t>(P.out) | (uint64_t)(2 * P.o_st) | (uint64_t)(2 * P.o_sh)) & 15u) == 0;
             T* to[4];                                  // rows lane / 4 + 8 k, this lane's piece; null: none
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const int gr = row0 + (warp & 3) * 32 + (lane >> 2) + 8 * k, pr = pf_pos(P, gr);
-                to[k] = gr < n_rows ? reinterpret_cast<T*>(P.out) + (int64_t)(sg.q0 + pr) * P.o_st + (int64_t)(h * P.gqa + gr - pr * P.gqa) * P.o_sh + 64 * hf + 8 * (lane & 3)
-                                    : nullptr;
+                const int gr = w.b.row0 + kRows * mb + (warp & 3) * 32 + (lane >> 2) + 8 * k, pr = pf_pos(P, gr);
+                to[k] = pr < w.b.n ? reinterpret_cast<T*>(P.out) + (int64_t)(w.b.q0 + pr) * P.o_st +
+                                         (int64_t)((P.h0 + w.h) * P.gqa + gr - pr * P.gqa) * P.o_sh + 64 * hf + 8 * (lane & 3)
+                                   : nullptr;
             }
 #pragma unroll 1
             for (int ch = 0; ch < 2; ++ch) {
@@ -794,15 +809,15 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                 }
             }
             if (hf == 0) {
+                const int g = w.b.row0 + kRows * mb + r128, pos = pf_pos(P, g);
                 if (!whole)
                     P.part_ml[slot + lane] = make_float2(m_used, lsum);
-                else if (rok && P.lse)
-                    P.lse[(int64_t)(sg.q0 + pos) * P.n_q + h * P.gqa + g - pos * P.gqa] =
+                else if (pos < w.b.n && P.lse)
+                    P.lse[(int64_t)(w.b.q0 + pos) * P.n_q + (P.h0 + w.h) * P.gqa + g - pos * P.gqa] =
                         lsum == 0.f ? -INFINITY : (m_used + log2f(lsum)) * 0.693147180559945309f;
             }
             tc_fence_before_sync();                    // (O is read before the next block's first product into it)
-            if (!more) break;
-            w.step(next);
+            bar_and(3 + mb, 256, true);                // (and this block's record, before the one after the next takes its place)
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
     }
