@@ -11,8 +11,8 @@
 // and accumulators are fp32).  Queries are brought to [2^13, 2^14) by a power of two each, so that bf16 queries of any
 // magnitude are exact in fp16 too.
 //
-// P * vs <= 2^14 holds for every magnitude of V: a column's reference M is the running maximum of S f + log2(max_g vs), minus 6, and moves
-// (O rescaled) only when a value exceeds it by 2^14.
+// P * vs <= 2^14 holds for every magnitude of V: a warp keeps the largest V scale R that it has met, a column's reference M is 6 below its largest
+// S f + log2 R, and both move (O rescaled) only when a logit or a scale passes what they allow.
 //
 // Work, in one of two forms:
 //   split    the 32-token batches of all (sequence, block of columns, KV head) triples form one list, each triple padded to whole rounds
@@ -29,7 +29,7 @@ namespace {
 constexpr int kPdWarps = 8, kPdThreads = 32 * kPdWarps;
 constexpr int kBatchTok = 32;
 constexpr int kBatchBytes = kBatchTok / kUnitTok * kUnitBytes;
-constexpr float kLift = 6.f, kReach = 14.f;       // log2 of P * vs at a reference's setting, and where it moves
+constexpr float kLift = 6.f, kReach = 14.f;       // log2 of P * R at a reference's setting, and where it moves
 constexpr int kOutRow = 132;                      // floats between columns of a warp's state in shared memory
 
 struct PdParams {
@@ -290,20 +290,36 @@ __device__ __forceinline__ void pd_query(const PdParams& P, Query<NT>& Q, const 
 template <int NT>
 struct State {
     float o[NT][2][4][4];            // [i][n]: rows 32 n + 4 r + 2 i (+ 1), columns 2 c (+ 1)
-    float m[NT][2], l[NT][2];
+    float m[NT][2], l[NT][2];        // reference, denominator
+    float top[NT][2];                // the largest logit that the reference allows
+    uint32_t r;                      // the largest V scale so far, as a pair of bf16
 };
 
 template <typename V> __device__ __forceinline__ V at(const uint8_t* p) { return *reinterpret_cast<const V*>(p); }
 template <int N> struct Int { static constexpr int value = N; };
 template <typename F> __device__ __forceinline__ void each_group(F f) { f(Int<0>{}); f(Int<1>{}); f(Int<2>{}); f(Int<3>{}); }
 
-// 16 tokens at u in shared memory.  kEdge: some of them (tokens from len on of the sequence, from lim[] on of a column) are hidden.
-template <int NT, bool kEdge>
-__device__ __forceinline__ void pd_unit(const uint8_t* u, const Magic& mg, const Query<NT>& Q, State<NT>& st, int r, int c, int t0, int len, const int (&lim)[NT][2]) {
-    float s[NT][4];
-    {
-        const uint4 x = at<uint4>(u + r * 64 + c * 16), y = at<uint4>(u + 512 + r * 64 + c * 16);
-        const uint2 ka = at<uint2>(u + kUnitKs + r * 8), kc = at<uint2>(u + kUnitKs + 64 + r * 8);
+__device__ __forceinline__ uint32_t max_bf2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+// U units of 16 tokens at u in shared memory.  kEdge: some of them (tokens from len on of the sequence, from lim[] on of a column) are hidden.
+template <int NT, int U, bool kEdge>
+__device__ __forceinline__ void pd_units(const uint8_t* u, const Magic& mg, const Query<NT>& Q, State<NT>& st, int r, int c, int t0, int len, const int (&lim)[NT][2]) {
+    float s[U][NT][4];
+    uint2 va[U], vc[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const uint8_t* const k = u + i * kUnitBytes;
+        const uint4 x = at<uint4>(k + r * 64 + c * 16), y = at<uint4>(k + 512 + r * 64 + c * 16);
+        const uint2 ka = at<uint2>(k + kUnitKs + r * 8), kc = at<uint2>(k + kUnitKs + 64 + r * 8);
+        va[i] = at<uint2>(k + kUnitVs + r * 8);
+        vc[i] = at<uint2>(k + kUnitVs + 64 + r * 8);
+        if (kEdge) {
+            if (t0 + 16 * i + r >= len) va[i] = make_uint2(0, 0);               // what lies behind the sequence may be anything
+            if (t0 + 16 * i + 8 + r >= len) vc[i] = make_uint2(0, 0);
+        }
         const float sa[4] = {pg_lo(ka.x), pg_hi(ka.x), pg_lo(ka.y), pg_hi(ka.y)};
         const float sc[4] = {pg_lo(kc.x), pg_hi(kc.x), pg_lo(kc.y), pg_hi(kc.y)};
         const uint4 x8 = make_uint4(x.x >> 8, x.y >> 8, x.z >> 8, x.w >> 8), y8 = make_uint4(y.x >> 8, y.y >> 8, y.z >> 8, y.w >> 8);
@@ -314,53 +330,63 @@ __device__ __forceinline__ void pd_unit(const uint8_t* u, const Magic& mg, const
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float acc[4];
+                float(&d)[4] = s[i][nt];
                 const uint32_t b0[2] = {Q.b[nt][g][0], Q.b[nt][g][1]}, b1[2] = {Q.b[nt][g][2], Q.b[nt][g][3]};
                 mma_new(acc, a0, b0);
                 mma_acc(acc, a1, b1);
                 if (g == 0) {
-                    s[nt][0] = acc[0] * sa[g]; s[nt][1] = acc[1] * sa[g];
-                    s[nt][2] = acc[2] * sc[g]; s[nt][3] = acc[3] * sc[g];
+                    d[0] = acc[0] * sa[g]; d[1] = acc[1] * sa[g];
+                    d[2] = acc[2] * sc[g]; d[3] = acc[3] * sc[g];
                 } else {
-                    s[nt][0] = fmaf(acc[0], sa[g], s[nt][0]); s[nt][1] = fmaf(acc[1], sa[g], s[nt][1]);
-                    s[nt][2] = fmaf(acc[2], sc[g], s[nt][2]); s[nt][3] = fmaf(acc[3], sc[g], s[nt][3]);
+                    d[0] = fmaf(acc[0], sa[g], d[0]); d[1] = fmaf(acc[1], sa[g], d[1]);
+                    d[2] = fmaf(acc[2], sc[g], d[2]); d[3] = fmaf(acc[3], sc[g], d[3]);
                 }
             }
         });
     }
-    uint2 va = at<uint2>(u + kUnitVs + r * 8), vc = at<uint2>(u + kUnitVs + 64 + r * 8);
-    if (kEdge) {
-        if (t0 + r >= len) va = make_uint2(0, 0);               // what lies behind the sequence may be anything
-        if (t0 + 8 + r >= len) vc = make_uint2(0, 0);
-    }
-    const float ha[4] = {pg_lo(va.x), pg_hi(va.x), pg_lo(va.y), pg_hi(va.y)};
-    const float hc[4] = {pg_lo(vc.x), pg_hi(vc.x), pg_lo(vc.y), pg_hi(vc.y)};
-    const float la = lg2(fmaxf(fmaxf(fmaxf(ha[0], ha[1]), fmaxf(ha[2], ha[3])), kPgScaleMin));
-    const float lc = lg2(fmaxf(fmaxf(fmaxf(hc[0], hc[1]), fmaxf(hc[2], hc[3])), kPgScaleMin));
+    uint32_t r2 = st.r;
     float top[NT][2];
-    bool move = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) top[nt][0] = top[nt][1] = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        r2 = max_bf2(r2, max_bf2(max_bf2(va[i].x, va[i].y), max_bf2(vc[i].x, vc[i].y)));
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                if (kEdge) {
+                    if (t0 + 16 * i + r >= lim[nt][e]) s[i][nt][e] = -INFINITY;
+                    if (t0 + 16 * i + 8 + r >= lim[nt][e]) s[i][nt][2 + e] = -INFINITY;
+                }
+                top[nt][e] = fmaxf(top[nt][e], fmaxf(s[i][nt][e], s[i][nt][2 + e]));
+            }
+    }
+    bool move = r2 != st.r;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            if (kEdge) {
-                if (t0 + r >= lim[nt][e]) s[nt][e] = -INFINITY;
-                if (t0 + 8 + r >= lim[nt][e]) s[nt][2 + e] = -INFINITY;
-            }
-            top[nt][e] = fmaxf(fmaf(s[nt][e], Q.f[nt][e], la), fmaf(s[nt][2 + e], Q.f[nt][e], lc));
-            move |= top[nt][e] > st.m[nt][e] + kReach;
+            top[nt][e] *= Q.f[nt][e];
+            move |= top[nt][e] > st.top[nt][e];
         }
     if (__any_sync(0xffffffffu, move)) {
+        r2 = max_bf2(r2, __byte_perm(r2, r2, 0x1032));
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) r2 = max_bf2(r2, __shfl_xor_sync(0xffffffffu, r2, d));
+        st.r = r2;
+        const float lr = lg2(fmaxf(pg_hi(r2), kPgScaleMin));
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 float t = top[nt][e];
-                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
-                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
-                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
-                const float m = fmaxf(st.m[nt][e], t - kLift);
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, d));
+                const float m = fmaxf(st.m[nt][e], t + lr - kLift);
                 const float alpha = m == -INFINITY ? 1.f : ex2(st.m[nt][e] - m);
                 st.m[nt][e] = m;
+                st.top[nt][e] = m + (kReach - lr);
                 st.l[nt][e] *= alpha;
 #pragma unroll
                 for (int n = 0; n < 4; ++n)
@@ -371,34 +397,40 @@ __device__ __forceinline__ void pd_unit(const uint8_t* u, const Magic& mg, const
                     }
             }
     }
-    float p[NT][4];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int i = 0; i < U; ++i) {
+        float p[NT][4];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const float z = kEdge && st.m[nt][e] == -INFINITY ? 0.f : st.m[nt][e];
-            p[nt][e] = ex2(fmaf(s[nt][e], Q.f[nt][e], -z));
-            p[nt][2 + e] = ex2(fmaf(s[nt][2 + e], Q.f[nt][e], -z));
-            st.l[nt][e] += p[nt][e] + p[nt][2 + e];
-        }
-    const uint4 x = at<uint4>(u + kUnitV + c * 128 + r * 16), y = at<uint4>(u + kUnitV + 512 + c * 128 + r * 16);
-    const uint4 x8 = make_uint4(x.x >> 8, x.y >> 8, x.z >> 8, x.w >> 8), y8 = make_uint4(y.x >> 8, y.y >> 8, y.z >> 8, y.w >> 8);
-    each_group([&](auto gi) {
-        constexpr int g = decltype(gi)::value;
-        const uint32_t a0[4] = {codes<g>(mg, x.x, x8.x), codes<g>(mg, x.y, x8.y), codes<g>(mg, y.x, y8.x), codes<g>(mg, y.y, y8.y)};
-        const uint32_t a1[4] = {codes<g>(mg, x.z, x8.z), codes<g>(mg, x.w, x8.w), codes<g>(mg, y.z, y8.z), codes<g>(mg, y.w, y8.w)};
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            float w[4] = {p[nt][0] * ha[g], p[nt][1] * ha[g], p[nt][2] * hc[g], p[nt][3] * hc[g]};
-            if (kEdge) {                                        // (a hidden token's scale may be no number)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = s[nt][e] == -INFINITY ? 0.f : w[e];
+            for (int e = 0; e < 2; ++e) {
+                const float z = kEdge && st.m[nt][e] == -INFINITY ? 0.f : st.m[nt][e];
+                p[nt][e] = ex2(fmaf(s[i][nt][e], Q.f[nt][e], -z));
+                p[nt][2 + e] = ex2(fmaf(s[i][nt][2 + e], Q.f[nt][e], -z));
+                st.l[nt][e] += p[nt][e] + p[nt][2 + e];
             }
-            const uint32_t b[2] = {transposed(pack_half2(w[0], w[1])), transposed(pack_half2(w[2], w[3]))};
-            mma_acc(st.o[nt][0][g], a0, b);
-            mma_acc(st.o[nt][1][g], a1, b);
-        }
-    });
+        const uint8_t* const v = u + i * kUnitBytes + kUnitV + c * 128 + r * 16;
+        const uint4 x = at<uint4>(v), y = at<uint4>(v + 512);
+        const float ha[4] = {pg_lo(va[i].x), pg_hi(va[i].x), pg_lo(va[i].y), pg_hi(va[i].y)};
+        const float hc[4] = {pg_lo(vc[i].x), pg_hi(vc[i].x), pg_lo(vc[i].y), pg_hi(vc[i].y)};
+        const uint4 x8 = make_uint4(x.x >> 8, x.y >> 8, x.z >> 8, x.w >> 8), y8 = make_uint4(y.x >> 8, y.y >> 8, y.z >> 8, y.w >> 8);
+        each_group([&](auto gi) {
+            constexpr int g = decltype(gi)::value;
+            const uint32_t a0[4] = {codes<g>(mg, x.x, x8.x), codes<g>(mg, x.y, x8.y), codes<g>(mg, y.x, y8.x), codes<g>(mg, y.y, y8.y)};
+            const uint32_t a1[4] = {codes<g>(mg, x.z, x8.z), codes<g>(mg, x.w, x8.w), codes<g>(mg, y.z, y8.z), codes<g>(mg, y.w, y8.w)};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float w[4] = {p[nt][0] * ha[g], p[nt][1] * ha[g], p[nt][2] * hc[g], p[nt][3] * hc[g]};
+                if (kEdge) {                                        // (a hidden token's scale may be no number)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = s[i][nt][e] == -INFINITY ? 0.f : w[e];
+                }
+                const uint32_t b[2] = {transposed(pack_half2(w[0], w[1])), transposed(pack_half2(w[2], w[3]))};
+                mma_acc(st.o[nt][0][g], a0, b);
+                mma_acc(st.o[nt][1][g], a1, b);
+            }
+        });
+    }
 }
 
 // Writes a column's row: four dims per lane.
@@ -424,6 +456,7 @@ struct Copies {
     const uint8_t* from;             // lane i: unit i % 2 of batch 16 * block + i / 2, null: not there
     int issued, n;
     uint32_t have;                   // two bits per stage: which of its units are there
+    bool all;                        // the sixteen batches that `from` is about lack none
 };
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
@@ -453,8 +486,8 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
         asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(n_rank));
         if (n_rank > 1) cluster_arrive();            // a CTA's shared memory may be written once that CTA runs
     }
-    grid_launch_dependents();
     grid_dependency_wait();
+    grid_launch_dependents();              // (behind the wait: what the merging launch reads ahead of its own is complete)
 
     Segment g;
     uint32_t pos = 0, end = 0, begin = 0, seq_start = 0;
@@ -529,17 +562,19 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
                 else if (P.status)
                     *P.status = kStatusBadPage;
             }
+            w.all = __all_sync(0xffffffffu, kk >= w.n || w.from);
         }
         const uint8_t* src = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(w.from), 2 * (k & 15) + (lane & 1)));
-        const uint32_t there = __ballot_sync(0xffffffffu, src != nullptr) & 3u;
         uint64_t* bar = &S.full[warp][stage];
-        if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)__popc(there) * kUnitBytes);
+        uint32_t there = 3u;
+        if (!w.all) there = __ballot_sync(0xffffffffu, src != nullptr) & 3u;
+        if (lane == 0) mbar_arrive_expect_tx(bar, w.all ? kBatchBytes : (uint32_t)__popc(there) * kUnitBytes);
         __syncwarp();
         if (lane < 2 && src) bulk_g2s_hint(S.ring[warp][stage] + lane * kUnitBytes, src, kUnitBytes, bar, policy);
         w.have = (w.have & ~(3u << (2 * stage))) | there << (2 * stage);
     };
     auto begin_copies = [&](const Segment& sg) {
-        Copies w{nullptr, 0, 0, 0};
+        Copies w{nullptr, 0, 0, 0, false};
         // batches that no row of the block sees are left out
         const int last_row = min((sg.cb + 1) * kCols, sg.s.n * P.gqa) - 1;
         const int lim_max = P.causal ? max(0, sg.s.len - sg.s.n + 1 + last_row / P.gqa) : sg.s.len;
@@ -566,7 +601,7 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
         const int lim_min = P.causal ? max(0, behind + row0 / P.gqa) : g.s.len;
         State<NT> st = {};
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) st.m[nt][0] = st.m[nt][1] = -INFINITY;
+        for (int nt = 0; nt < NT; ++nt) st.m[nt][0] = st.m[nt][1] = st.top[nt][0] = st.top[nt][1] = -INFINITY;
         int t0 = (g.first + warp) * kBatchTok, stage = 0;
         for (int k = 0; k < w.n && ok; ++k) {
             if (!__all_sync(0xffffffffu, mbar_wait_bounded(&S.full[warp][stage], phases >> stage & 1u))) {
@@ -577,12 +612,16 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
             const uint8_t* const tile = S.ring[warp][stage];
             const uint32_t there = w.have >> (2 * stage) & 3u;
             if (there == 3u && t0 + kBatchTok <= lim_min) {
-                pd_unit<NT, false>(tile, mg, Q, st, r, c, t0, g.s.len, lim);
-                pd_unit<NT, false>(tile + kUnitBytes, mg, Q, st, r, c, t0 + kUnitTok, g.s.len, lim);
+                if (NT == 1) {
+                    pd_units<NT, 2, false>(tile, mg, Q, st, r, c, t0, g.s.len, lim);
+                } else {
+                    pd_units<NT, 1, false>(tile, mg, Q, st, r, c, t0, g.s.len, lim);
+                    pd_units<NT, 1, false>(tile + kUnitBytes, mg, Q, st, r, c, t0 + kUnitTok, g.s.len, lim);
+                }
             } else {
 #pragma unroll 1
                 for (int i = 0; i < 2; ++i)
-                    if (there >> i & 1u) pd_unit<NT, true>(tile + i * kUnitBytes, mg, Q, st, r, c, t0 + i * kUnitTok, g.s.len, lim);
+                    if (there >> i & 1u) pd_units<NT, 1, true>(tile + i * kUnitBytes, mg, Q, st, r, c, t0 + i * kUnitTok, g.s.len, lim);
             }
             __syncwarp();
             if (w.issued < w.n) issue(g, w, stage);
@@ -704,9 +743,10 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
     if (!ok && lane == 0 && P.status) *P.status = kStatusWaitTimeout;
 }
 
-// Block (i, col): column col of the triple that the end of CTA i's share cuts, if that is its first cut.  Eight warps share the
-// partials, four of them requested at a time.
-template <int NT, typename T>
+// Block (i, col): column col of a triple that is cut.  kByTriple (one query row per sequence, no more triples than CTAs): of triple i.  Otherwise of
+// the one that the end of CTA i's share cuts, if that is its first cut.  Eight warps share the partials, four of them requested at a
+// time.  Where the triples lie is looked up before the partials are there: the lengths were complete before the attention began.
+template <int NT, typename T, bool kByTriple>
 __global__ void __launch_bounds__(256) pg_merge_kernel(const PdParams P) {
     __shared__ ScanSmem scan;
     __shared__ float4 sum_o[8][32];
@@ -714,21 +754,39 @@ __global__ void __launch_bounds__(256) pg_merge_kernel(const PdParams P) {
     constexpr int kCols = 8 * NT;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = blockIdx.y;
     grid_launch_dependents();
-    grid_dependency_wait();
-    uint32_t total, seq_start, share = 0;
+    uint32_t total, seq_start, share = 0, triple;
     int seq;
-    pd_find<NT>(P, scan, total, seq, seq_start, [&](uint32_t t) {
-        share = pd_share(t, P.n_cta);
-        return ((uint32_t)blockIdx.x + 1) * share;
-    });
-    const uint64_t cut = ((uint64_t)blockIdx.x + 1) * share;
-    if (cut >= total || seq < 0) return;
+    if (kByTriple) {
+        const int wanted = blockIdx.x / P.n_kv;
+        uint32_t before = 0;
+        for (int i = 0; i < wanted; i += 32)
+            if (i + lane < wanted) before += pd_work<NT>(P, pd_seq(P, i + lane));
+        uint32_t rest = 0;
+        for (int i = wanted; i < P.n_seq; i += 32)
+            if (i + lane < P.n_seq) rest += pd_work<NT>(P, pd_seq(P, i + lane));
+        seq_start = __reduce_add_sync(0xffffffffu, before);
+        total = seq_start + __reduce_add_sync(0xffffffffu, rest);
+        share = pd_share(total, P.n_cta);
+        seq = wanted;
+        triple = blockIdx.x - (uint32_t)wanted * P.n_kv;
+    } else {
+        pd_find<NT>(P, scan, total, seq, seq_start, [&](uint32_t t) {
+            share = pd_share(t, P.n_cta);
+            return ((uint32_t)blockIdx.x + 1) * share;
+        });
+        if (((uint64_t)blockIdx.x + 1) * share >= total || seq < 0) seq = -1;
+        triple = 0;
+    }
+    grid_dependency_wait();
+    if (seq < 0) return;
     const SeqInfo s = pd_seq(P, seq);
     if (s.len == 0) return;
-    const uint32_t np = pd_padded(s), triple = ((uint32_t)cut - seq_start) / np, a = seq_start + triple * np, b = a + np;
-    if (a == (uint32_t)cut || a + share < (uint32_t)cut) return;              // not cut here, or not for the first time
+    const uint32_t np = pd_padded(s);
+    if (!kByTriple) triple = ((blockIdx.x + 1) * share - seq_start) / np;
+    const uint32_t a = seq_start + triple * np, b = a + np;
+    const int j0 = kByTriple ? (int)(a / share) : (int)blockIdx.x, j1 = min(P.n_cta - 1, (int)((b - 1) / share));      // CTAs that hold a part of it
+    if (kByTriple ? j0 == j1 : a == (blockIdx.x + 1) * share || a + share < (blockIdx.x + 1) * share) return;          // not cut, not here, or not for the first time
     const int cb = (int)(triple / P.n_kv), h = (int)(triple - (uint32_t)cb * P.n_kv);
-    const int j0 = blockIdx.x, j1 = min(P.n_cta - 1, (int)((b - 1) / share));      // CTAs that hold a part of it
     const size_t slot0 = (size_t)(2 * j0 + (a != (uint32_t)j0 * share ? 1 : 0)) * kCols + col;
     auto slot_of = [&](int j) { return j == j0 ? slot0 : (size_t)2 * j * kCols + col; };
     float m = -INFINITY, l = 0.f;
@@ -791,8 +849,11 @@ int pd_launch_split(const PdParams& P, bool merge, cudaStream_t stream) {
     if (!pg_allow_smem(kernel, smem, allowed)) return BGTQ_E_LAUNCH;
     if (launch_kernel(kernel, dim3(P.n_cta), dim3(kPdThreads), smem, stream, true, P) != cudaSuccess) return BGTQ_E_LAUNCH;
     if (!merge) return BGTQ_OK;
-    const dim3 grid(P.n_cta - 1, P.cu_q ? 8 * NT : P.gqa);
-    return launch_kernel(pg_merge_kernel<NT, T>, grid, dim3(256), 0, stream, true, P) == cudaSuccess ? BGTQ_OK : BGTQ_E_LAUNCH;
+    const int64_t triples = (int64_t)P.n_seq * P.n_kv;
+    const bool by_triple = !P.cu_q && triples <= P.n_cta;
+    const dim3 grid(by_triple ? (unsigned)triples : P.n_cta - 1, P.cu_q ? 8 * NT : P.gqa);
+    const auto merging = by_triple ? pg_merge_kernel<NT, T, true> : pg_merge_kernel<NT, T, false>;
+    return launch_kernel(merging, grid, dim3(256), 0, stream, true, P) == cudaSuccess ? BGTQ_OK : BGTQ_E_LAUNCH;
 }
 template <int NT, typename T, int kStages>
 int pd_launch_cluster(const PdParams& P, int64_t triples, int n_rank, cudaStream_t stream) {
