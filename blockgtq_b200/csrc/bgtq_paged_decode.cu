@@ -855,28 +855,51 @@ int pd_launch_split(const PdParams& P, bool merge, cudaStream_t stream) {
     const auto merging = by_triple ? pg_merge_kernel<NT, T, true> : pg_merge_kernel<NT, T, false>;
     return launch_kernel(merging, grid, dim3(256), 0, stream, true, P) == cudaSuccess ? BGTQ_OK : BGTQ_E_LAUNCH;
 }
+template <int NT, int kStages>
+struct ClusterLaunch {
+    static constexpr int kBase = (int)sizeof(PdSmem<NT, kStages>), kRow = 8 * NT * (kHD * 4 + 8);
+    static_assert(kBase + 8 * kRow <= 227 * 1024, "a cluster of eight fits");
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    ClusterLaunch(int64_t triples, int n_rank, cudaStream_t stream) {
+        cfg.gridDim = dim3((unsigned)(triples * n_rank));
+        cfg.blockDim = dim3(kPdThreads);
+        cfg.dynamicSmemBytes = kBase + (n_rank > 1 ? n_rank * kRow : 0);
+        cfg.stream = stream;
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = n_rank;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 2;
+    }
+};
 template <int NT, typename T, int kStages>
 int pd_launch_cluster(const PdParams& P, int64_t triples, int n_rank, cudaStream_t stream) {
-    constexpr int base = (int)sizeof(PdSmem<NT, kStages>), row = 8 * NT * (kHD * 4 + 8);
-    static_assert(base + 8 * row <= 227 * 1024, "a cluster of eight fits");
     const auto kernel = pg_attend_kernel<NT, T, true, kStages>;
+    ClusterLaunch<NT, kStages> L(triples, n_rank, stream);
     static std::atomic<uint64_t> allowed{0};
-    if (!pg_allow_smem(kernel, base + 8 * row, allowed)) return BGTQ_E_LAUNCH;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(triples * n_rank));
-    cfg.blockDim = dim3(kPdThreads);
-    cfg.dynamicSmemBytes = base + (n_rank > 1 ? n_rank * row : 0);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = n_rank;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    if (cudaLaunchKernelEx(&cfg, kernel, P) != cudaSuccess || cudaGetLastError() != cudaSuccess) return BGTQ_E_LAUNCH;
-    return BGTQ_OK;
+    if (!pg_allow_smem(kernel, L.kBase + 8 * L.kRow, allowed)) return BGTQ_E_LAUNCH;
+    return cudaLaunchKernelEx(&L.cfg, kernel, P) == cudaSuccess && cudaGetLastError() == cudaSuccess ? BGTQ_OK : BGTQ_E_LAUNCH;
+}
+// Clusters of n_rank CTAs, each with an SM for itself, that the device runs at once (its groups of SMs are no multiples of eight).
+template <int NT, int kStages>
+int pd_clusters(int n_rank, int dev) {
+    static std::atomic<int> known[64][9];
+    if (dev >= 0 && dev < 64)
+        if (const int n = known[dev][n_rank].load(std::memory_order_relaxed)) return n;
+    const auto kernel = pg_attend_kernel<NT, __half, true, kStages>;
+    ClusterLaunch<NT, kStages> L(1, n_rank, nullptr);
+    L.cfg.numAttrs = 1;
+    static std::atomic<uint64_t> allowed{0};
+    int n = 0;
+    if (!pg_allow_smem(kernel, L.kBase + 8 * L.kRow, allowed) || cudaOccupancyMaxActiveClusters(&n, kernel, &L.cfg) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    if (dev >= 0 && dev < 64) known[dev][n_rank].store(n, std::memory_order_relaxed);
+    return n;
 }
 template <int NT, typename T>
 int pd_launch(const PdParams& P, const PdForm& f, cudaStream_t stream) {
@@ -895,9 +918,11 @@ using namespace bgtq;
 // Column tiles of a product: eight query rows are the operand's width; more of them share what is read and unpacked.
 static int pd_tiles(int32_t n_q, int32_t n_kv, int32_t max_q) { return (int64_t)max_q * (n_q / n_kv) <= 8 ? 1 : 2; }
 
-constexpr int kPrefillRows = 48;        // rows of a (sequence, KV head) above which the tcgen05 form is the faster one
-
-// How a call is launched, from its shape.
+// How a call is launched, from its shape: the form that the measured costs make the cheapest (in microseconds, 300 to 131072 tokens over 2 to 64
+// KV heads and sequences; a round is 256 tokens of a CTA).
+//   clusters  4.4 and 1.45 for each round while every CTA has an SM for itself, 2.1 where two share one; with 16 columns 5 and 1.95.
+//   list      5.6, the merging launch among them, and 2.25 for each round of the CTAs that are resident and one more; with 16 columns 9.
+//   tcgen05   20, unpacking at 4.2 MB (of 144 and 512 bytes per token and head) and 1.75 for each tile of a CTA.
 static PdForm pd_form(int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv, int32_t max_q, int64_t max_tokens, int32_t flags) {
     PdForm f{};
     int dev = 0, sms = 148;
@@ -913,18 +938,20 @@ static PdForm pd_form(int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv, i
     const double most = (double)blocks * n_kv * (double)rounds;
     f.n_cta = (int)(most < 1 ? 1 : most < (double)resident ? most : (double)resident);
     const int asked = (flags & BGTQ_PAGED_FORM_MASK) >> BGTQ_PAGED_FORM_SHIFT;
-    f.prefill = asked == 14 || (asked == 0 && max_q * gqa > kPrefillRows);
+    f.prefill = asked == 14;
     if (f.prefill || asked == 15) return f;
-    // Measured, in microseconds (8 KV heads, 100 to 131072 tokens): a cluster takes 4.4 and 1.45 for each round of its CTAs' warps while every CTA
-    // has an SM for itself, 2.1 where two share one (only without the exchange's memory); the list takes 9, the merging launch among
-    // them, and 2.2 for each round of the CTAs that are resident.
     int n = 8;
-    while (n > 1 && f.triples * n > sms) n /= 2;
+    while (n > 1 && (f.triples * n > sms || f.triples > (f.nt == 1 ? pd_clusters<1, 4>(n, dev) : pd_clusters<2, 2>(n, dev)))) n /= 2;
     if (asked) n = asked;
     f.alone = f.triples * n <= sms;
     const int64_t waves = (f.triples * n + resident - 1) / resident;
-    const double cluster = 4.4 + (f.alone ? 1.45 : 2.1) * (double)(waves * ((rounds + n - 1) / n));
-    const double split = 9.0 + 2.2 * (most + (double)resident - 1) / (double)resident;
+    const double cluster = (f.nt == 1 ? 4.4 : 5.0) + (f.nt > 1 ? 1.95 : f.alone ? 1.45 : 2.1) * (double)(waves * ((rounds + n - 1) / n));
+    const double split = (f.nt == 1 ? 5.6 : 9.0) + 2.25 * (most + (double)resident - 1) / (double)resident;
+    if (!asked && f.nt > 1) {
+        const double pairs = (double)n_seq * n_kv, tiles = pairs * (double)((max_q * gqa + 255) / 256) * (double)((max_tokens + 127) / 128);
+        f.prefill = 20.0 + pairs * (double)max_tokens * 656e-6 / 4.2 + 1.75 * (tiles + sms - 1) / sms < (cluster < split ? cluster : split);
+        if (f.prefill) return f;
+    }
     if (asked || cluster < split) f.n_rank = n;
     return f;
 }

@@ -238,7 +238,7 @@ def paged_kv4_prefill_attention(q, pages, block_table, seq_lens, cu_q, max_q_len
     ``cu_q[b + 1] - 1`` (``cu_q`` (B + 1,) int32) are the last positions of sequence b, and when ``causal`` each sees the tokens up to itself.
 
     ``max_q_len``: no sequence has more query rows (default: all of them; it chooses the launch, and one that has more is attended all the
-    same).  ``max_seq_len``: sequences are held to it (default: what the table holds).  With more than 48 rows per sequence and KV head the
+    same).  ``max_seq_len``: sequences are held to it (default: what the table holds).  With many rows per sequence and KV head the
     tokens are unpacked into a workspace from torch's allocator, 512 bytes per token of ``max_seq_len`` and KV head for every sequence, at
     most 2 GiB at a time.  Rows behind ``cu_q[B]`` are not written.  Otherwise as :func:`paged_kv4_decode_attention`."""
     if cu_q is None:
