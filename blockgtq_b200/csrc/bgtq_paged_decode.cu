@@ -16,7 +16,8 @@
 //
 // Work, in one of two forms:
 //   split    the 32-token batches of all (sequence, block of columns, KV head) triples form one list, each triple padded to whole rounds
-//            of eight, and the list is cut evenly over the CTAs.  Triples cut between CTAs are merged by a second launch.
+//            of eight and headed by kTripleCost places for what it costs beside them (a CTA with many short ones would come last), and
+//            the list is cut evenly over the CTAs.  Triples cut between CTAs are merged by a second launch.
 //   cluster  a cluster of 1 to 8 CTAs per triple, which merge their shares in distributed shared memory: no list, no second launch.
 // In a CTA eight warps take batches in turn, each with a ring of bulk copies of its own (the next triple's first ones travel while this
 // one's states are merged in shared memory).
@@ -29,6 +30,9 @@ namespace {
 constexpr int kPdWarps = 8, kPdThreads = 32 * kPdWarps;
 constexpr int kBatchTok = 32;
 constexpr int kBatchBytes = kBatchTok / kUnitTok * kUnitBytes;
+// Places for what a triple costs beside its batches, a multiple of kPdWarps.  64 sequences of up to 9100 tokens x 8 KV heads: 110 us without,
+// 91.4 with 8, 87.5 with 16, 89.4 with 24; 63 short ones beside one of 30000: 26.6, 27.9, 32.0.
+constexpr uint32_t kTripleCost = 16;
 constexpr float kLift = 6.f, kReach = 14.f;       // log2 of P * R at a reference's setting, and where it moves
 constexpr int kOutRow = 132;                      // floats between columns of a warp's state in shared memory
 
@@ -78,9 +82,10 @@ __device__ __forceinline__ SeqInfo pd_seq(const PdParams& P, int i) {
 }
 __device__ __forceinline__ uint32_t pd_batches(const SeqInfo& s) { return (uint32_t)((s.len + kBatchTok - 1) / kBatchTok); }
 __device__ __forceinline__ uint32_t pd_padded(const SeqInfo& s) { return (pd_batches(s) + kPdWarps - 1) / kPdWarps * kPdWarps; }
+__device__ __forceinline__ uint32_t pd_places(const SeqInfo& s) { return s.len > 0 ? pd_padded(s) + kTripleCost : 0u; }
 template <int NT>
 __device__ __forceinline__ uint32_t pd_work(const PdParams& P, const SeqInfo& s) {
-    return pd_padded(s) * (uint32_t)P.n_kv * (uint32_t)((s.n * P.gqa + 8 * NT - 1) / (8 * NT));
+    return pd_places(s) * (uint32_t)P.n_kv * (uint32_t)((s.n * P.gqa + 8 * NT - 1) / (8 * NT));
 }
 
 struct ScanSmem {
@@ -493,13 +498,13 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
     uint32_t pos = 0, end = 0, begin = 0, seq_start = 0;
     // split: the segment that starts at pos
     auto at_pos = [&]() {
-        const uint32_t nb = pd_batches(g.s), np = pd_padded(g.s), triple = (pos - seq_start) / np, first = (pos - seq_start) - triple * np;
-        const uint32_t count = min(np - first, end - pos);
+        const uint32_t nb = pd_batches(g.s), np = pd_places(g.s), triple = (pos - seq_start) / np, at = (pos - seq_start) - triple * np;
+        const uint32_t count = min(np - at, end - pos), to = at + count - min(at + count, kTripleCost);
         g.cb = (int)(triple / P.n_kv);
         g.h = (int)(triple - (uint32_t)g.cb * P.n_kv);
-        g.first = (int)first;
-        g.n = (int)(min(first + count, nb) - first);
-        g.whole = first == 0 && count == np;
+        g.first = (int)(at - min(at, kTripleCost));
+        g.n = (int)min(to, nb) - g.first;
+        g.whole = g.first == 0 && to >= nb;
         return count;
     };
     // cluster: this CTA's share of the triple
@@ -544,6 +549,7 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
         g.s = pd_seq(P, g.seq);
         if (g.s.len == 0) return;                    // (row ranges that do not follow one another: the list is not one then)
         count = at_pos();
+        if (g.n <= 0) return;
     }
 
     uint32_t phases = 0;                   // of this warp's stages
@@ -656,6 +662,7 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
                 next_count = at_pos();
                 next = g;
                 g = keep;
+                more = next.n > 0;           // (the share's end may fall behind a triple's head)
             }
         }
         if (more) w = begin_copies(next);
@@ -781,13 +788,13 @@ __global__ void __launch_bounds__(256) pg_merge_kernel(const PdParams P) {
     if (seq < 0) return;
     const SeqInfo s = pd_seq(P, seq);
     if (s.len == 0) return;
-    const uint32_t np = pd_padded(s);
+    const uint32_t np = pd_places(s);
     if (!kByTriple) triple = ((blockIdx.x + 1) * share - seq_start) / np;
     const uint32_t a = seq_start + triple * np, b = a + np;
-    const int j0 = kByTriple ? (int)(a / share) : (int)blockIdx.x, j1 = min(P.n_cta - 1, (int)((b - 1) / share));      // CTAs that hold a part of it
-    if (kByTriple ? j0 == j1 : a == (blockIdx.x + 1) * share || a + share < (blockIdx.x + 1) * share) return;          // not cut, not here, or not for the first time
+    const int j0 = (int)((a + kTripleCost) / share), j1 = min(P.n_cta - 1, (int)((b - 1) / share));      // the CTAs that hold a part of it
+    if (j0 >= j1 || (!kByTriple && j0 != (int)blockIdx.x)) return;                                       // not cut, or not for the first time
     const int cb = (int)(triple / P.n_kv), h = (int)(triple - (uint32_t)cb * P.n_kv);
-    const size_t slot0 = (size_t)(2 * j0 + (a != (uint32_t)j0 * share ? 1 : 0)) * kCols + col;
+    const size_t slot0 = (size_t)(2 * j0 + (a > (uint32_t)j0 * share ? 1 : 0)) * kCols + col;
     auto slot_of = [&](int j) { return j == j0 ? slot0 : (size_t)2 * j * kCols + col; };
     float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -935,8 +942,8 @@ static PdForm pd_form(int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv, i
     const int64_t resident = (f.nt == 1 ? 2 : 1) * (int64_t)sms;
     // all sequences' column blocks together, at most
     const int64_t blocks = n_tok <= n_seq ? n_seq : n_tok * gqa / cols + n_seq;
-    const double most = (double)blocks * n_kv * (double)rounds;
-    f.n_cta = (int)(most < 1 ? 1 : most < (double)resident ? most : (double)resident);
+    const double most = (double)blocks * n_kv * (double)rounds, places = (double)blocks * n_kv * (double)(rounds + kTripleCost / kPdWarps);
+    f.n_cta = (int)(places < 1 ? 1 : places < (double)resident ? places : (double)resident);
     const int asked = (flags & BGTQ_PAGED_FORM_MASK) >> BGTQ_PAGED_FORM_SHIFT;
     f.prefill = asked == 14;
     if (f.prefill || asked == 15) return f;
@@ -998,7 +1005,7 @@ extern "C" __attribute__((visibility("default"))) int bgtq_paged_attend(
     f.merge = cap > kPdWarps * kBatchTok && f.n_cta > 1;
     const int64_t cols = 8 * f.nt, blocks = n_tok <= n_seq ? n_seq : (int64_t)n_tok * (n_q / n_kv) / cols + n_seq;
     // the list's positions are 32 bits, and the grid's
-    if ((double)blocks * n_kv * (double)(cap / kBatchTok + kPdWarps) > 2.0e9 || (double)f.triples * 8 > 2.0e9) return BGTQ_E_TOOBIG;
+    if ((double)blocks * n_kv * (double)(cap / kBatchTok + 2 * kPdWarps + kTripleCost) > 2.0e9 || (double)f.triples * 8 > 2.0e9) return BGTQ_E_TOOBIG;
     const int64_t need = f.n_rank ? 0 : (int64_t)f.n_cta * 2 * cols * (kHD * 4 + 8);
     if (need && (!workspace || workspace_bytes < need)) return BGTQ_E_BADARG;
     PdParams P{{pages, page_stride, head_stride, n_pages, page_tokens / kUnitTok}, q, q_st, q_sh, table, table_stride, seq_lens, cu_q,
