@@ -11,8 +11,10 @@
 // and accumulators are fp32).  Queries are brought to [2^13, 2^14) by a power of two each, so that bf16 queries of any
 // magnitude are exact in fp16 too.
 //
-// P * vs <= 2^14 holds for every magnitude of V: a warp keeps the largest V scale R that it has met, a column's reference M is 6 below its largest
-// S f + log2 R, and both move (O rescaled) only when a logit or a scale passes what they allow.
+// P * vs <= 2^13 holds for every magnitude of V: a warp keeps a power of two R above every V scale that it has met, a column's reference M is 12
+// below its largest S f + log2 R, and both move (O rescaled) only when a scale passes R or a logit the largest by more than 1.  The weight of
+// the token that set the reference is then a power of two times its scale, which fp16 holds: where one token has nearly all the weight, as
+// in a sequence of one, its values come out as they are.  (With a reference that waited for 2^8 more, such rows were off by fp16's rounding.)
 //
 // Work, in one of two forms:
 //   split    the 32-token batches of all (sequence, block of columns, KV head) triples form one list, each triple padded to whole rounds
@@ -33,7 +35,7 @@ constexpr int kBatchBytes = kBatchTok / kUnitTok * kUnitBytes;
 // Places for what a triple costs beside its batches, a multiple of kPdWarps.  64 sequences of up to 9100 tokens x 8 KV heads: 110 us without,
 // 91.4 with 8, 87.5 with 16, 89.4 with 24; 63 short ones beside one of 30000: 26.6, 27.9, 32.0.
 constexpr uint32_t kTripleCost = 16;
-constexpr float kLift = 6.f, kReach = 14.f;       // log2 of P * R at a reference's setting, and where it moves
+constexpr float kLift = 12.f, kReach = 13.f;      // log2 of P * R at a reference's setting, and where it moves
 constexpr int kOutRow = 132;                      // floats between columns of a warp's state in shared memory
 
 struct PdParams {
@@ -297,7 +299,7 @@ struct State {
     float o[NT][2][4][4];            // [i][n]: rows 32 n + 4 r + 2 i (+ 1), columns 2 c (+ 1)
     float m[NT][2], l[NT][2];        // reference, denominator
     float top[NT][2];                // the largest logit that the reference allows
-    uint32_t r;                      // the largest V scale so far, as a pair of bf16
+    uint32_t r;                      // a power of two above every V scale so far, as a pair of bf16
 };
 
 template <typename V> __device__ __forceinline__ V at(const uint8_t* p) { return *reinterpret_cast<const V*>(p); }
@@ -379,8 +381,11 @@ __device__ __forceinline__ void pd_units(const uint8_t* u, const Magic& mg, cons
         r2 = max_bf2(r2, __byte_perm(r2, r2, 0x1032));
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) r2 = max_bf2(r2, __shfl_xor_sync(0xffffffffu, r2, d));
-        st.r = r2;
-        const float lr = lg2(fmaxf(pg_hi(r2), kPgScaleMin));
+        if (r2 != st.r) {                  // the power of two above it (scales lie between 2^-17 and 2^14; with none it is 2^-17)
+            const uint32_t up = max(((r2 & 0x7f80u) + 0x80u), 0x3700u);
+            st.r = up | up << 16;
+        }
+        const float lr = (float)((int)((st.r & 0x7fffu) >> 7) - 127);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll

@@ -444,3 +444,24 @@ def test_results_do_not_change_from_call_to_call():
     first = paged_kv4_decode_attention(*args)
     for _ in range(5):
         assert torch.equal(first, paged_kv4_decode_attention(*args))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_one_token_with_all_the_weight_gives_its_values_as_they_are(dtype, form):
+    """Its weight times its scale is exact, the sum over its weight is code x scale within a few steps of fp32.  That product has 11 bits: fp16
+    holds it, so fp16 is equal.  bf16 rounds it, from a sum that may lie 2^-22 beside a tie: within half a step and that.
+    In the second sequence the other tokens' logits lie at least 40 (in powers of two) below it."""
+    from blockgtq_b200 import paged_kv4_append, paged_kv4_decode_attention, paged_kv4_read
+    gen = torch.Generator().manual_seed(5)
+    pages, table, slots = _case(gen, 2, 16, [1, 70], dtype=dtype)
+    v = _noise(gen, 70, 2, 128).to(dtype)
+    k = torch.full((70, 2, 128), -7.0).to(dtype)
+    k[37] = 7.0
+    paged_kv4_append(pages, slots[1].to(DEV), k.to(DEV), v.to(DEV))
+    paged_kv4_append(pages, slots[0].to(DEV), k[:1].to(DEV), v[5:6].to(DEV))
+    q = torch.ones(2, 14, 128).to(dtype).to(DEV)
+    out = paged_kv4_decode_attention(q, pages, table.to(DEV), torch.tensor([1, 70], dtype=torch.int32, device=DEV))
+    for b, t in ((0, 0), (1, 37)):
+        want = paged_kv4_read(pages, slots[b][t:t + 1].to(DEV), dtype=torch.float16)[1][0].double().repeat_interleave(7, 0)
+        slack = 0 if dtype == torch.float16 else 2 ** -8 + 2 ** -20
+        assert bool(((out[b].double() - want).abs() <= slack * want.abs()).all())
