@@ -405,7 +405,9 @@ PyObject* paged_attend(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     if (m < 1 || n_seq < 1 || n_seq > INT32_MAX || n_q < 1 || n_q % n_kv || n_q / n_kv > 8 || cap > INT32_MAX || !vec_ok(lens, at::kInt, n_seq) ||
         (cu ? !vec_ok(cu, at::kInt, n_seq + 1) : m != n_seq) || max_q < 1 || max_q > INT32_MAX || scale != scale)
         return none();
-    if (given && (!rows_ok(given, q->scalar_type(), 8) || given->sizes() != q->sizes())) return none();
+    if (given && (!rows_ok(given, q->scalar_type(), 8) || given->sizes() != q->sizes() || given->data_ptr() == q->data_ptr() ||
+                  (m > 1 && given->stride(0) < kHD) || (n_q > 1 && given->stride(1) < kHD)))
+        return none();
     if (most < 0 || most > cap) most = cap;
     if (q->scalar_type() == at::kBFloat16) flags |= BGTQ_PAGED_BF16;
     const int64_t need = G.paged_workspace((int)n_seq, (int)m, (int)n_q, (int)n_kv, (int)max_q, most, flags);

@@ -120,21 +120,21 @@ __global__ void __launch_bounds__(kApThreads, L == 8 ? 4 : 2) pg_append_kernel(c
         slot = -1;
     }
     float cs[2][E] = {}, sn[2][E] = {};
-    bool angle = true;
-    if (P.cos && there && !(first >= (uint32_t)P.kv_chunks && last <= 2u * P.kv_chunks)) {
+    if (P.cos && there) {
         int64_t p = P.positions[tok];
-        if (p < 0 || p >= P.n_positions) { // no angle for it: its key is not stored, and the caller learns of it
+        if (p < 0 || p >= P.n_positions) { // no angle for it: the token is not stored, and the caller learns of it
             if (P.status && slot >= 0) *P.status = kStatusOverflow;
-            angle = false;
+            slot = -1;
             p = 0;
         }
+        if (!(first >= (uint32_t)P.kv_chunks && last <= 2u * P.kv_chunks))         // (V alone needs none)
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
+            for (int g = 0; g < 2; ++g)
 #pragma unroll
-            for (int i = 0; i < E; i += 4) {
-                *reinterpret_cast<float4*>(&cs[g][i]) = *reinterpret_cast<const float4*>(P.cos + p * P.cs_st + 32 * g + E * j + i);
-                *reinterpret_cast<float4*>(&sn[g][i]) = *reinterpret_cast<const float4*>(P.sin + p * P.cs_st + 32 * g + E * j + i);
-            }
+                for (int i = 0; i < E; i += 4) {
+                    *reinterpret_cast<float4*>(&cs[g][i]) = *reinterpret_cast<const float4*>(P.cos + p * P.cs_st + 32 * g + E * j + i);
+                    *reinterpret_cast<float4*>(&sn[g][i]) = *reinterpret_cast<const float4*>(P.sin + p * P.cs_st + 32 * g + E * j + i);
+                }
     }
     uint8_t* unit = nullptr;
     int t = 0;
@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(kApThreads, L == 8 ? 4 : 2) pg_append_kernel(c
         for (int e = 0; e < E; e += 2) word[e / 2] = __byte_perm(half[e], half[e + 1], 0x5410);
         uint8_t* const u = unit + head * P.head_stride;
         if (kind == 0) {
-            if (live && unit && angle) {
+            if (live && unit) {
                 *reinterpret_cast<typename Vec<E>::type*>(u + 64 * t + 2 * E * j) = *reinterpret_cast<typename Vec<E>::type*>(word);
                 if (j == 0) *reinterpret_cast<uint2*>(u + kUnitKs + 8 * t) = s4;
             }

@@ -994,7 +994,7 @@ extern "C" __attribute__((visibility("default"))) int bgtq_paged_attend(
         return BGTQ_E_BADARG;
     int64_t cap = (int64_t)table_cols * page_tokens;
     if (cap > max_tokens) cap = max_tokens;
-    if (cap > INT32_MAX - 512) return BGTQ_E_TOOBIG;
+    if (cap > INT32_MAX - 512 || max_tokens > INT64_MAX / 1024) return BGTQ_E_TOOBIG;
     if (!aligned(pages, 16) || page_stride % 16 || head_stride % 16 || !aligned(q, 16) || q_st % 8 || q_sh % 8 || !aligned(out, 8) || o_st % 4 ||
         o_sh % 4 || !aligned(workspace, 16))
         return BGTQ_E_ALIGN;
@@ -1003,7 +1003,7 @@ extern "C" __attribute__((visibility("default"))) int bgtq_paged_attend(
     if (f.prefill) {
         if (!workspace || workspace_bytes < paged_prefill_workspace(n_seq, n_tok, n_q / n_kv, n_kv, max_tokens)) return BGTQ_E_BADARG;
         return paged_prefill({{pages, page_stride, head_stride, n_pages, page_tokens / kUnitTok}, table, table_stride, seq_lens, cu_q, n_seq, n_tok, n_q,
-                              n_kv, n_q / n_kv, (flags & BGTQ_PAGED_CAUSAL) ? 1 : 0, (flags & BGTQ_PAGED_BF16) ? 1 : 0, max_tokens,
+                              n_kv, n_q / n_kv, (flags & BGTQ_PAGED_CAUSAL) ? 1 : 0, (flags & BGTQ_PAGED_BF16) ? 1 : 0, max_tokens, (int32_t)cap,
                               reinterpret_cast<uint8_t*>(workspace), q, q_st, q_sh, scale * 1.44269504088896340736f, out, o_st, o_sh, lse, status},
                              st);
     }

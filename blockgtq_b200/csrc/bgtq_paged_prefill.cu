@@ -924,7 +924,7 @@ int paged_prefill(const PagedPrefill& A, cudaStream_t stream) {
             Pf P{};
             P.pool = A.pool;
             P.table = A.table; P.tb_st = A.tb_st; P.lens = A.lens; P.cu_q = A.cu_q;
-            P.cap = (int32_t)A.max_tokens; P.n_tok = A.n_tok; P.n_q = A.n_q; P.n_kv = A.n_kv; P.gqa = A.gqa; P.causal = A.causal;
+            P.cap = A.cap; P.n_tok = A.n_tok; P.n_q = A.n_q; P.n_kv = A.n_kv; P.gqa = A.gqa; P.causal = A.causal;
             P.gqa_inv = A.gqa > 1 ? (uint32_t)(0x100000000ull / A.gqa + (0x100000000ull % A.gqa != 0)) : 0;
             P.seq0 = s0; P.n_seq = ns; P.h0 = h0; P.n_h = nh; P.max_tiles = (int32_t)tiles;
             P.tiles = ws;

@@ -13,7 +13,8 @@ struct PagedPrefill {
     int64_t tb_st;
     const int32_t *lens, *cu_q;
     int32_t n_seq, n_tok, n_q, n_kv, gqa, causal, bf16;
-    int64_t max_tokens;
+    int64_t max_tokens;             // the workspace's
+    int32_t cap;                    // sequences are held to it: max_tokens and what the table holds
     uint8_t* workspace;
     const void* q;
     int64_t q_st, q_sh;             // elements; rows on 16-byte boundaries

@@ -85,7 +85,7 @@ def paged_kv4_append(pages, slots, k, v, q=None, cos=None, sin=None, positions=N
     ``slots`` (n,) int64: page * page size + place in the page, distinct; a token with a negative one is not stored.
     ``cos`` / ``sin`` (n_positions, 64) fp32 with ``positions`` (n,) int64: k, and ``q`` (n, n_q, 128), go through the rotary
     embedding first (dims d and d + 64 are a pair; fp32, k quantised from the unrounded result).  Returns the rotated q (n, n_q, 128),
-    or None without one.  ``status``: optional int32 tensor, set to 2 where a slot or position is out of range (nothing stored)."""
+    or None without one.  ``status``: optional int32 tensor, set to 2 where a slot or position is out of range (the token is not stored)."""
     r = _lib.host().paged_append(pages, slots, k, v, q, cos, sin, positions, status)
     if r is None:
         return _append(pages, slots, k, v, q, cos, sin, positions, status)
@@ -199,6 +199,8 @@ def _attend_any(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, flags,
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1 or out.stride(0) % 4 or out.stride(1) % 4 \
             or out.data_ptr() % 8:
         raise ValueError("out must be like q, with rows of 8-byte alignment")
+    elif out.data_ptr() == q.data_ptr() or any(st < HD and k > 1 for st, k in zip(out.stride(), out.shape[:2])):
+        raise ValueError("out must have rows of its own, apart from one another and from q")
     lse = torch.empty(n, n_q, dtype=torch.float32, device=dev) if return_lse else None
     cap = block_table.shape[1] * page
     max_tokens = cap if max_tokens < 0 else min(max_tokens, cap)
@@ -228,7 +230,7 @@ def paged_kv4_decode_attention(q, pages, block_table, seq_lens, scale=None, retu
     ``block_table`` (B, pages per sequence) int32 and ``seq_lens`` (B,) int32: token t of sequence b lies in page ``block_table[b, t // page
     size]``; entries behind the sequence's end are not read.  A sequence without tokens gives zeros and -inf.  Query heads
     h * n_q / n_kv .. share KV head h, at most 8 of them.  ``max_seq_len``: sequences are held to it (default: what the table holds);
-    a small one spares the launch what only long sequences need."""
+    a small one spares the launch what only long sequences need.  ``out``: where the result goes, like q but not q itself."""
     return _attend(q, pages, block_table, seq_lens, None, 1, _most(max_seq_len), True, scale, return_lse, status, out)
 
 
@@ -288,8 +290,10 @@ class PagedKV4Cache:
         return i
 
     def free_sequence(self, seq: int):
-        """Gives the sequence's pages back."""
+        """Gives the sequence's pages back.  A step that it is part of ends with it."""
         self._free.extend(reversed(self._seqs.pop(seq)[1]))
+        if self._step is not None and seq in self._step["seqs"]:
+            self._step = None
 
     def seq_len(self, seq: int) -> int:
         return self._seqs[seq][0]
@@ -335,7 +339,7 @@ class PagedKV4Cache:
         table = torch.tensor([r + [0] * (width - len(r)) for r in rows], dtype=torch.int32).to(self.device)
         small = torch.tensor(lens + ends, dtype=torch.int32).to(self.device)
         self._step = {"slots": wide[0], "positions": wide[1], "table": table, "lens": small[:len(seqs)], "ends": small[len(seqs):],
-                      "most_q": max(counts), "most": max(lens)}
+                      "most_q": max(counts), "most": max(lens), "rows": len(slots), "seqs": frozenset(seqs)}
 
     @torch.no_grad()
     def append_and_attend(self, layer_idx, q, k, v, rope=None):
@@ -344,8 +348,8 @@ class PagedKV4Cache:
         if self._step is None:
             raise RuntimeError("begin_step comes first")
         s, pages = self._step, self.pages[layer_idx]
-        if q.shape[1:] != (self.nq, HD):
-            raise ValueError(f"q must be (tokens, {self.nq}, {HD}), got {tuple(q.shape)}")
+        if q.shape != (s["rows"], self.nq, HD):
+            raise ValueError(f"q must be ({s['rows']}, {self.nq}, {HD}), the step's tokens, got {tuple(q.shape)}")
         if rope is None:
             paged_kv4_append(pages, s["slots"], k, v, status=self.status)
         else:

@@ -150,3 +150,26 @@ def test_pages_are_handed_out_and_given_back():
         c.seq_len(a)
     c.begin_step([b], [1])
     assert c._step["slots"].tolist() == [int(c._step["table"][0, 1]) * 16]
+
+
+def test_a_result_with_rows_of_its_own():
+    q = _rows(h=4)
+    args = (q, _pages(), torch.zeros(4, 1, dtype=torch.int32), torch.ones(4, dtype=torch.int32))
+    for out in (q, torch.zeros(1, 4, 128, dtype=torch.float16).expand(4, 4, 128), torch.zeros(4, 1, 128, dtype=torch.float16).expand(4, 4, 128)):
+        with pytest.raises(ValueError, match="of its own"):
+            paged_kv4_decode_attention(*args, out=out)
+
+
+def test_a_step_takes_its_tokens_and_ends_with_its_sequences():
+    c = PagedKV4Cache(1, 4, 2, n_pages=6, max_seq_len=100, page_size=16, device="cpu")
+    a, b, other = (c.add_sequence() for _ in range(3))
+    c.begin_step([a, b], [3, 2])
+    for n in (4, 6):                                    # rows of other numbers than the step's
+        with pytest.raises(ValueError, match="step"):
+            c.append_and_attend(0, _rows(n, 4), _rows(n), _rows(n))
+    c.free_sequence(other)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        c.append_and_attend(0, _rows(5, 4), _rows(5), _rows(5))
+    c.free_sequence(b)                                  # its pages may be another's from here on
+    with pytest.raises(RuntimeError, match="begin_step"):
+        c.append_and_attend(0, _rows(5, 4), _rows(5), _rows(5))

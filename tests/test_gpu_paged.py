@@ -465,3 +465,109 @@ def test_one_token_with_all_the_weight_gives_its_values_as_they_are(dtype, form)
         want = paged_kv4_read(pages, slots[b][t:t + 1].to(DEV), dtype=torch.float16)[1][0].double().repeat_interleave(7, 0)
         slack = 0 if dtype == torch.float16 else 2 ** -8 + 2 ** -20
         assert bool(((out[b].double() - want).abs() <= slack * want.abs()).all())
+
+
+@pytest.mark.parametrize("n", [6, 5000])
+def test_a_token_without_an_angle_is_not_stored_at_all(n):
+    from blockgtq_b200 import page_bytes, paged_kv4_append
+    gen = torch.Generator().manual_seed(n)
+    n_pages = n // 64 + 1
+    k, v = (_noise(gen, n, 4, 128).half().to(DEV) for _ in range(2))
+    cos, sin = (x.to(DEV) for x in _tables(n))
+    slots, pos = torch.arange(n, device=DEV), torch.arange(n, device=DEV)
+    bad = torch.tensor([1, n - 2], device=DEV)
+    pos[bad] = torch.tensor([n, -1], device=DEV)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    got, want = (torch.zeros(n_pages, 4, page_bytes(64), dtype=torch.uint8, device=DEV) for _ in range(2))
+    paged_kv4_append(got, slots, k, v, cos=cos, sin=sin, positions=pos, status=status)
+    assert status.item() == 2
+    status.zero_()
+    slots[bad] = -1
+    paged_kv4_append(want, slots, k, v, cos=cos, sin=sin, positions=pos, status=status)
+    assert status.item() == 0 and torch.equal(got, want)
+
+
+def test_tables_of_any_stride(rows_form):
+    from blockgtq_b200 import paged_kv4_prefill_attention
+    gen = torch.Generator().manual_seed(8)
+    pages, table, slots = _case(gen, 2, 16, [70, 33])
+    q = _noise(gen, 20, 8, 128).half()
+    i32 = dict(dtype=torch.int32, device=DEV)
+    lens, cu = torch.tensor([70, 9, 33, 9], **i32)[::2], torch.tensor([0, 9, 12, 9, 20, 9], **i32)[::2]
+    wide = torch.zeros(2, table.shape[1] + 3, **i32)
+    wide[:, 2:-1] = table
+    for tab in (wide[:, 2:-1], table.to(DEV).t().contiguous().t()):
+        out, lse = paged_kv4_prefill_attention(q.to(DEV), pages, tab, lens, cu, return_lse=True)
+        for b, (a, z, t) in enumerate([(0, 12, 70), (12, 20, 33)]):
+            _check(out, lse, R.attention(q[a:z], pages.cpu(), slots[b], [t - z + a + 1 + i for i in range(z - a)], 1 / math.sqrt(128)), slice(a, z))
+
+
+def test_pages_behind_four_gigabytes(rows_form):
+    """A pool of 5 GB whose heads are 2.4 GB apart: pages on both sides of 2^32 bytes."""
+    from blockgtq_b200 import page_bytes, paged_kv4_append, paged_kv4_prefill_attention, paged_kv4_read
+    gen = torch.Generator().manual_seed(9)
+    n_pages, t = 1 << 20, 150
+    pages = torch.empty(2, n_pages, page_bytes(16), dtype=torch.uint8, device=DEV).transpose(0, 1)
+    order = [n_pages - 1 - 97 * i for i in range(5)] + [3 * i for i in range(5)]
+    slots = torch.tensor([order[i // 16] * 16 + i % 16 for i in range(t)])
+    k, v, q = (_noise(gen, t, h, 128).half() for h in (2, 2, 4))
+    paged_kv4_append(pages, slots.to(DEV), k.to(DEV), v.to(DEV))
+    small = torch.zeros(10, 2, page_bytes(16), dtype=torch.uint8)
+    for i, p in enumerate(order):
+        small[i] = pages[p].cpu()
+    here = torch.arange(t)
+    ref = R.attention(q[:20], small, here, [t - 19 + i for i in range(20)], 1 / math.sqrt(128))
+    i32 = dict(dtype=torch.int32, device=DEV)
+    out, lse = paged_kv4_prefill_attention(q[:20].to(DEV), pages, torch.tensor([order], **i32), torch.tensor([t], **i32), torch.tensor([0, 20], **i32), return_lse=True)
+    _check(out, lse, ref, slice(0, 20))
+    for far, near in zip(paged_kv4_read(pages, slots.to(DEV)), paged_kv4_read(small.to(DEV), here.to(DEV))):
+        assert torch.equal(far, near)
+
+
+def test_two_graphs_of_one_pool_of_memory(rows_form):
+    """Their workspaces may be the same memory: replayed in turn, each gives its own results."""
+    from blockgtq_b200 import paged_kv4_prefill_attention
+    gen = torch.Generator().manual_seed(12)
+    pages, table, slots = _case(gen, 2, 16, [900, 300])
+    i32 = dict(dtype=torch.int32, device=DEV)
+    cases, graphs, pool = [(0, 900, 40), (1, 300, 290)], [], None
+    for b, t, n in cases:
+        q = _noise(gen, n, 4, 128).half()
+        args = (q.to(DEV), pages, table[b:b + 1].to(DEV), torch.tensor([t], **i32), torch.tensor([0, n], **i32))
+        paged_kv4_prefill_attention(*args)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=pool):
+            out = paged_kv4_prefill_attention(*args)
+        pool = g.pool()
+        want = R.attention(q, pages.cpu(), slots[b], [t - n + 1 + i for i in range(n)], 1 / math.sqrt(128))
+        graphs.append((g, out, args, want, n))
+    for which in (0, 1, 1, 0, 1, 0):
+        g, out, _, want, n = graphs[which]
+        g.replay()
+        torch.cuda.synchronize()
+        _check(out, None, want, slice(0, n))
+
+
+@pytest.mark.parametrize("form", [1, 8, 14, 15])
+def test_the_library_reads_no_further_than_the_table(form):
+    """Lengths and max_tokens beyond the table's width: a row of it is not left."""
+    from blockgtq_b200 import _lib
+    gen = torch.Generator().manual_seed(14)
+    pages, table, slots = _case(gen, 2, 16, [48, 48])
+    i32 = dict(dtype=torch.int32, device=DEV)
+    wide = torch.full((2, 40), -1, **i32)                 # what lies behind a row would be reported
+    wide[:, :3] = table[:, :3].to(DEV)
+    q = _noise(gen, 10, 4, 128).half()
+    qd, out, status = q.to(DEV), torch.zeros(10, 4, 128, dtype=torch.float16, device=DEV), torch.zeros(1, **i32)
+    lens, cu = torch.tensor([400, 48], **i32), torch.tensor([0, 6, 10], **i32)
+    flags, lib = _lib.PAGED_CAUSAL | form << _lib.PAGED_FORM_SHIFT, _lib.lib()
+    need = lib.bgtq_paged_workspace_bytes(2, 10, 4, 2, 6, 500, flags)
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=DEV)
+    rc = lib.bgtq_paged_attend(qd.data_ptr(), 512, 128, pages.data_ptr(), pages.stride(0), pages.stride(1), pages.shape[0], 16, wide.data_ptr(), 40, 3,
+                               lens.data_ptr(), cu.data_ptr(), 2, 10, 4, 2, 6, 500, 1 / math.sqrt(128), flags, ws.data_ptr(), need, out.data_ptr(), 512, 128,
+                               0, status.data_ptr(), _lib.stream_ptr(torch.device(DEV)))
+    torch.cuda.synchronize()
+    assert rc == 0 and status.item() == 0
+    for b, (a, z) in enumerate([(0, 6), (6, 10)]):
+        _check(out, None, R.attention(q[a:z], pages.cpu(), slots[b], [48 - z + a + 1 + i for i in range(z - a)], 1 / math.sqrt(128)), slice(a, z))
