@@ -11,10 +11,11 @@
 // and accumulators are fp32).  Queries are brought to [2^13, 2^14) by a power of two each, so that bf16 queries of any
 // magnitude are exact in fp16 too.
 //
-// P * vs <= 2^13 holds for every magnitude of V: a warp keeps a power of two R above every V scale that it has met, a column's reference M is 12
-// below its largest S f + log2 R, and both move (O rescaled) only when a scale passes R or a logit the largest by more than 1.  The weight of
+// P * vs <= 2^15 holds for every magnitude of V: a warp keeps a power of two R above every V scale that it has met, a column's reference M is 12
+// below its largest S f + log2 R, and both move (O rescaled) only when a scale passes R or a logit the largest by more than 3.  The weight of
 // the token that set the reference is then a power of two times its scale, which fp16 holds: where one token has nearly all the weight, as
-// in a sequence of one, its values come out as they are.  (With a reference that waited for 2^8 more, such rows were off by fp16's rounding.)
+// in a sequence of one, its values come out as they are.  (Moving at 1: 16 sequences of 2047 tokens, 4 rows each, 21.1 us instead of 20.0; at 8,
+// rows of one dominating token lie up to 1.5 times as far from 64 bits.)
 //
 // Work, in one of two forms:
 //   split    the 32-token batches of all (sequence, block of columns, KV head) triples form one list, each triple padded to whole rounds
@@ -35,7 +36,7 @@ constexpr int kBatchBytes = kBatchTok / kUnitTok * kUnitBytes;
 // Places for what a triple costs beside its batches, a multiple of kPdWarps.  64 sequences of up to 9100 tokens x 8 KV heads: 110 us without,
 // 91.4 with 8, 87.5 with 16, 89.4 with 24; 63 short ones beside one of 30000: 26.6, 27.9, 32.0.
 constexpr uint32_t kTripleCost = 16;
-constexpr float kLift = 12.f, kReach = 13.f;      // log2 of P * R at a reference's setting, and where it moves
+constexpr float kLift = 12.f, kReach = 15.f;      // log2 of P * R at a reference's setting, and where it moves
 constexpr int kOutRow = 132;                      // floats between columns of a warp's state in shared memory
 
 struct PdParams {
