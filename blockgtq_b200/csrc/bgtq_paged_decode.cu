@@ -18,9 +18,10 @@
 // rows of one dominating token lie up to 1.5 times as far from 64 bits.)
 //
 // Work, in one of two forms:
-//   split    the 32-token batches of all (sequence, block of columns, KV head) triples form one list, each triple padded to whole rounds
-//            of eight and headed by kTripleCost places for what it costs beside them (a CTA with many short ones would come last), and
-//            the list is cut evenly over the CTAs.  Triples cut between CTAs are merged by a second launch.
+//   split    the 32-token batches of all (sequence, block of columns, KV head) triples form one list, each triple headed by kTripleCost
+//            places for what it costs beside them (a CTA with many short ones would come last), and the list is cut evenly over the
+//            CTAs.  Triples cut between CTAs are merged by a second launch.  (Shares and triples of whole rounds of eight, as the warps
+//            take them: 8 sequences of 32768 tokens x 2 KV heads 27.1 us instead of 26.1, 63 short ones beside one of 30000 tokens 27.8 instead of 25.5.)
 //   cluster  a cluster of 1 to 8 CTAs per triple, which merge their shares in distributed shared memory: no list, no second launch.
 // In a CTA eight warps take batches in turn, each with a ring of bulk copies of its own (the next triple's first ones travel while this
 // one's states are merged in shared memory).
@@ -48,6 +49,7 @@ struct PdParams {
     const int32_t* lens;
     const int32_t* cu_q;             // null: one query row per sequence
     int32_t cap, n_seq, n_tok, n_q, n_kv, gqa, causal;
+    int32_t grain;                   // split: a triple's places and a CTA's share are multiples of it (1, or 8 where no triple may be cut)
     int32_t n_cta;                   // split: CTAs;  cluster: column blocks of a sequence that have a cluster of their own
     float scale_log2;
     void* out;
@@ -84,11 +86,11 @@ __device__ __forceinline__ SeqInfo pd_seq(const PdParams& P, int i) {
     return s;
 }
 __device__ __forceinline__ uint32_t pd_batches(const SeqInfo& s) { return (uint32_t)((s.len + kBatchTok - 1) / kBatchTok); }
-__device__ __forceinline__ uint32_t pd_padded(const SeqInfo& s) { return (pd_batches(s) + kPdWarps - 1) / kPdWarps * kPdWarps; }
-__device__ __forceinline__ uint32_t pd_places(const SeqInfo& s) { return s.len > 0 ? pd_padded(s) + kTripleCost : 0u; }
+__device__ __forceinline__ uint32_t pd_whole(const PdParams& P, uint32_t n) { return (n + P.grain - 1) & ~(uint32_t)(P.grain - 1); }
+__device__ __forceinline__ uint32_t pd_places(const PdParams& P, const SeqInfo& s) { return s.len > 0 ? pd_whole(P, pd_batches(s)) + kTripleCost : 0u; }
 template <int NT>
 __device__ __forceinline__ uint32_t pd_work(const PdParams& P, const SeqInfo& s) {
-    return pd_places(s) * (uint32_t)P.n_kv * (uint32_t)((s.n * P.gqa + 8 * NT - 1) / (8 * NT));
+    return pd_places(P, s) * (uint32_t)P.n_kv * (uint32_t)((s.n * P.gqa + 8 * NT - 1) / (8 * NT));
 }
 
 struct ScanSmem {
@@ -182,8 +184,11 @@ __device__ __forceinline__ void pd_find(const PdParams& P, ScanSmem& S, uint32_t
     start = S.start;
 }
 
-__device__ __forceinline__ uint32_t pd_share(uint32_t total, int n_cta) {
-    return ((total + n_cta - 1) / n_cta + kPdWarps - 1) / kPdWarps * kPdWarps;
+// A CTA's share.  Short ones are whole rounds: the warps' chains are what they take (one sequence of 24000 tokens x 8 KV heads, 24 places instead
+// of 21: 14.6 us instead of 15.2; of 12000, 16 instead of 11: 13.0 instead of 12.2).
+__device__ __forceinline__ uint32_t pd_share(const PdParams& P, uint32_t total) {
+    const uint32_t n = (total + P.n_cta - 1) / P.n_cta;
+    return n <= 4 * kPdWarps ? (n + kPdWarps - 1) / kPdWarps * kPdWarps : pd_whole(P, n);
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -504,7 +509,7 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
     uint32_t pos = 0, end = 0, begin = 0, seq_start = 0;
     // split: the segment that starts at pos
     auto at_pos = [&]() {
-        const uint32_t nb = pd_batches(g.s), np = pd_places(g.s), triple = (pos - seq_start) / np, at = (pos - seq_start) - triple * np;
+        const uint32_t nb = pd_batches(g.s), np = pd_places(P, g.s), triple = (pos - seq_start) / np, at = (pos - seq_start) - triple * np;
         const uint32_t count = min(np - at, end - pos), to = at + count - min(at + count, kTripleCost);
         g.cb = (int)(triple / P.n_kv);
         g.h = (int)(triple - (uint32_t)g.cb * P.n_kv);
@@ -515,7 +520,7 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
     };
     // cluster: this CTA's share of the triple
     auto share_of = [&]() {
-        const uint32_t nb = pd_batches(g.s), per = pd_padded(g.s) / kPdWarps, a = per * rank / n_rank * kPdWarps, b = per * (rank + 1) / n_rank * kPdWarps;
+        const uint32_t nb = pd_batches(g.s), per = (nb + kPdWarps - 1) / kPdWarps, a = per * rank / n_rank * kPdWarps, b = per * (rank + 1) / n_rank * kPdWarps;
         g.first = (int)a;
         g.n = (int)(min(b, nb) - min(a, nb));
         g.whole = true;
@@ -546,7 +551,7 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
         }
         uint32_t total, share = 0;
         pd_find<NT>(P, S.scan, total, g.seq, seq_start, [&](uint32_t t) {
-            share = pd_share(t, P.n_cta);
+            share = pd_share(P, t);
             return (uint32_t)blockIdx.x * share;
         });
         if ((uint64_t)blockIdx.x * share >= total || g.seq < 0) return;
@@ -759,11 +764,11 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
 // Block (i, col): column col of a triple that is cut.  kByTriple (one query row per sequence, no more triples than CTAs): of triple i.  Otherwise of
 // the one that the end of CTA i's share cuts, if that is its first cut.  Eight warps share the partials, four of them requested at a
 // time.  Where the triples lie is looked up before the partials are there: the lengths were complete before the attention began.
-template <int NT, typename T, bool kByTriple>
-__global__ void __launch_bounds__(256) pg_merge_kernel(const PdParams P) {
+template <int NT, typename T, bool kByTriple, int kWarps>
+__global__ void __launch_bounds__(32 * kWarps) pg_merge_kernel(const PdParams P) {
     __shared__ ScanSmem scan;
-    __shared__ float4 sum_o[8][32];
-    __shared__ float sum_l[8];
+    __shared__ float4 sum_o[kWarps][32];
+    __shared__ float sum_l[kWarps];
     constexpr int kCols = 8 * NT;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = blockIdx.y;
     grid_launch_dependents();
@@ -779,12 +784,12 @@ __global__ void __launch_bounds__(256) pg_merge_kernel(const PdParams P) {
             if (i + lane < P.n_seq) rest += pd_work<NT>(P, pd_seq(P, i + lane));
         seq_start = __reduce_add_sync(0xffffffffu, before);
         total = seq_start + __reduce_add_sync(0xffffffffu, rest);
-        share = pd_share(total, P.n_cta);
+        share = pd_share(P, total);
         seq = wanted;
         triple = blockIdx.x - (uint32_t)wanted * P.n_kv;
     } else {
         pd_find<NT>(P, scan, total, seq, seq_start, [&](uint32_t t) {
-            share = pd_share(t, P.n_cta);
+            share = pd_share(P, t);
             return ((uint32_t)blockIdx.x + 1) * share;
         });
         if (((uint64_t)blockIdx.x + 1) * share >= total || seq < 0) seq = -1;
@@ -794,7 +799,7 @@ __global__ void __launch_bounds__(256) pg_merge_kernel(const PdParams P) {
     if (seq < 0) return;
     const SeqInfo s = pd_seq(P, seq);
     if (s.len == 0) return;
-    const uint32_t np = pd_places(s);
+    const uint32_t np = pd_places(P, s);
     if (!kByTriple) triple = ((blockIdx.x + 1) * share - seq_start) / np;
     const uint32_t a = seq_start + triple * np, b = a + np;
     const int j0 = (int)((a + kTripleCost) / share), j1 = min(P.n_cta - 1, (int)((b - 1) / share));      // the CTAs that hold a part of it
@@ -804,13 +809,13 @@ __global__ void __launch_bounds__(256) pg_merge_kernel(const PdParams P) {
     auto slot_of = [&](int j) { return j == j0 ? slot0 : (size_t)2 * j * kCols + col; };
     float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int j = j0 + warp; j <= j1; j += 32) {
+    for (int j = j0 + warp; j <= j1; j += 4 * kWarps) {
         float2 ml[4];
         float4 v[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const bool there = j + 8 * i <= j1;
-            const size_t slot = there ? slot_of(j + 8 * i) : slot0;
+            const bool there = j + kWarps * i <= j1;
+            const size_t slot = there ? slot_of(j + kWarps * i) : slot0;
             ml[i] = P.part_ml[slot];
             v[i] = *reinterpret_cast<const float4*>(P.part_o + slot * kHD + 4 * lane);
             if (!there) {
@@ -830,7 +835,7 @@ __global__ void __launch_bounds__(256) pg_merge_kernel(const PdParams P) {
             o.x = fmaf(f, v[i].x, o.x); o.y = fmaf(f, v[i].y, o.y); o.z = fmaf(f, v[i].z, o.z); o.w = fmaf(f, v[i].w, o.w);
         }
     }
-    __shared__ float sum_m[8];
+    __shared__ float sum_m[kWarps];
     sum_o[warp][lane] = o;
     if (lane == 0) {
         sum_l[warp] = l;
@@ -842,10 +847,10 @@ __global__ void __launch_bounds__(256) pg_merge_kernel(const PdParams P) {
     l = 0.f;
     o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, sum_m[i]);
+    for (int i = 0; i < kWarps; ++i) m = fmaxf(m, sum_m[i]);
     const float z = m == -INFINITY ? 0.f : m;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < kWarps; ++i) {
         const float f = ex2(sum_m[i] - z);
         const float4 v = sum_o[i][lane];
         l = fmaf(f, sum_l[i], l);
@@ -865,8 +870,12 @@ int pd_launch_split(const PdParams& P, bool merge, cudaStream_t stream) {
     const int64_t triples = (int64_t)P.n_seq * P.n_kv;
     const bool by_triple = !P.cu_q && triples <= P.n_cta;
     const dim3 grid(by_triple ? (unsigned)triples : P.n_cta - 1, P.cu_q ? 8 * NT : P.gqa);
-    const auto merging = by_triple ? pg_merge_kernel<NT, T, true> : pg_merge_kernel<NT, T, false>;
-    return launch_kernel(merging, grid, dim3(256), 0, stream, true, P) == cudaSuccess ? BGTQ_OK : BGTQ_E_LAUNCH;
+    // As many warps as take a triple's partials in one pass, but not more: 8 triples of 37 partials 15.3 us with 8, 14.6 with 16 (20000
+    // tokens); 160 of two or three 15.5 with 8 and 19.7 with 16.
+    const int warps = !by_triple || P.n_cta <= 4 * triples ? 2 : P.n_cta <= 16 * triples ? 8 : 16;
+    const auto merging = !by_triple ? pg_merge_kernel<NT, T, false, 2>
+                         : warps == 2 ? pg_merge_kernel<NT, T, true, 2> : warps == 8 ? pg_merge_kernel<NT, T, true, 8> : pg_merge_kernel<NT, T, true, 16>;
+    return launch_kernel(merging, grid, dim3(32 * warps), 0, stream, true, P) == cudaSuccess ? BGTQ_OK : BGTQ_E_LAUNCH;
 }
 template <int NT, int kStages>
 struct ClusterLaunch {
@@ -1015,7 +1024,7 @@ extern "C" __attribute__((visibility("default"))) int bgtq_paged_attend(
     const int64_t need = f.n_rank ? 0 : (int64_t)f.n_cta * 2 * cols * (kHD * 4 + 8);
     if (need && (!workspace || workspace_bytes < need)) return BGTQ_E_BADARG;
     PdParams P{{pages, page_stride, head_stride, n_pages, page_tokens / kUnitTok}, q, q_st, q_sh, table, table_stride, seq_lens, cu_q,
-               (int32_t)cap, n_seq, n_tok, n_q, n_kv, n_q / n_kv, !cu_q || (flags & BGTQ_PAGED_CAUSAL) ? 1 : 0, f.n_rank ? f.blocks_of_seq : f.n_cta,
+               (int32_t)cap, n_seq, n_tok, n_q, n_kv, n_q / n_kv, !cu_q || (flags & BGTQ_PAGED_CAUSAL) ? 1 : 0, f.merge ? 1 : kPdWarps, f.n_rank ? f.blocks_of_seq : f.n_cta,
                scale * 1.44269504088896340736f, out, o_st, o_sh, lse, reinterpret_cast<float*>(workspace),
                reinterpret_cast<float2*>(reinterpret_cast<float*>(workspace) + (int64_t)f.n_cta * 2 * cols * kHD), status};
     const bool bf16 = flags & BGTQ_PAGED_BF16;
