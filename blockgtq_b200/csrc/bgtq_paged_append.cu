@@ -31,6 +31,11 @@ struct ApParams {
 
 // L lanes hold a row: lane j its dims 32 g + E j .. + E - 1 of every group g, E = 32 / L, so that a group's largest magnitude is two or three
 // exchanges away, both dims of every rotated pair (d, d + 64) lie in one lane, and a lane's codes are 2 E bytes of a K row.
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
 template <int E>
 struct Row {
     uint32_t w[4][E / 2];
@@ -83,11 +88,16 @@ __device__ __forceinline__ void ap_codes(const float (&in)[E], float largest, fl
 }
 
 // A warp's task: two tokens and a run of chunks of 16 / L rows (KV heads' K, then V, then queries); the L lanes o take row o / 2 of a chunk for
-// token o % 2.  The tables' rows are read once for all of a task's chunks, and a chunk's rows are requested while the one before is worked on.
-// Bound: memory, 512 bytes in and 144 out per token and KV head, 512 per query row.
+// token o % 2.  The tables' rows are read once for all of a task's chunks.
+// Bound: memory, 512 bytes in and 144 out per token and KV head, 512 per query row, where there are queries: 65536 tokens of 32 query and 8 KV
+// heads 223 us, 6.5 TB/s, and 16384 63.8 us, 5.7 TB/s, with three chunks of a warp on their way to shared memory (in registers there was room
+// for one: 289 and 82 us; three CTAs on an SM instead of two, with spills: 267 and 78).  Without queries the quantisation's
+// instructions: 16384 tokens 30.7 us, 2.8 TB/s.  32 tokens: 2.9 us, a chain of latencies.
 template <typename T, int L>
 __global__ void __launch_bounds__(kApThreads, L == 8 ? 4 : 2) pg_append_kernel(const ApParams P) {
     constexpr int E = 32 / L, kHeads = 16 / L;
+    constexpr uint32_t kAhead = L == 4 ? 3 : 0;            // chunks of a warp on their way
+    __shared__ __align__(16) uint4 ring[kAhead ? kApThreads / 32 * kAhead * 4 * 32 : 1];
     const int lane = threadIdx.x & 31, o = lane / L, j = lane % L;
     const uint32_t n_chunks = 2 * P.kv_chunks + P.q_chunks, n_tasks = (n_chunks + P.per - 1) / P.per;
     const uint32_t task = blockIdx.x * (kApThreads / 32) + (threadIdx.x >> 5), pair = task / n_tasks;
@@ -103,16 +113,38 @@ __global__ void __launch_bounds__(kApThreads, L == 8 ? 4 : 2) pg_append_kernel(c
         head = kHeads * (int)(chunk - kind * (uint32_t)P.kv_chunks) + (o >> 1);
         return there && head < (kind == 2 ? P.n_q : P.n_kv);
     };
+    auto row_of = [&](int kind, int head) {
+        return kind == 0 ? reinterpret_cast<const T*>(P.k) + tok * P.k_st + head * P.k_sh
+               : kind == 1 ? reinterpret_cast<const T*>(P.v) + tok * P.v_st + head * P.v_sh
+                           : reinterpret_cast<const T*>(P.q) + tok * P.q_st + head * P.q_sh;
+    };
     auto fetch = [&](uint32_t chunk) {
         int kind, head;
         Row<E> r = {};
-        if (place(chunk, kind, head))
-            r = ap_load<E>(kind == 0 ? reinterpret_cast<const T*>(P.k) + tok * P.k_st + head * P.k_sh
-                        : kind == 1 ? reinterpret_cast<const T*>(P.v) + tok * P.v_st + head * P.v_sh
-                                    : reinterpret_cast<const T*>(P.q) + tok * P.q_st + head * P.q_sh, j);
+        if (place(chunk, kind, head)) r = ap_load<E>(row_of(kind, head), j);
         return r;
     };
-    Row<E> next = fetch(first);
+    // Bulk: the next chunks are on their way to shared memory, each lane's pieces to places of its own.
+    const uint32_t mine = kAhead ? smem_u32(ring) + ((threadIdx.x >> 5) * kAhead * 4 * 32 + lane) * 16 : 0u;
+    auto request = [&](uint32_t chunk, uint32_t slot) {
+        if (chunk < last) {
+            int kind, head;
+            const bool live = place(chunk, kind, head);
+            const T* const src = live ? row_of(kind, head) + E * j : reinterpret_cast<const T*>(P.k);
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(mine + (slot * 4 + g) * 512), "l"(live ? src + 32 * g : src), "r"(live ? 16 : 0)
+                             : "memory");
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    Row<E> next;
+    if constexpr (kAhead) {
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) request(first + i, i);
+    } else {
+        next = fetch(first);
+    }
     int64_t slot = there ? P.slots[tok] : -1;
     const int page_tok = P.units * kUnitTok;
     if (slot >= (int64_t)P.n_pages * page_tok) {
@@ -147,9 +179,17 @@ __global__ void __launch_bounds__(kApThreads, L == 8 ? 4 : 2) pg_append_kernel(c
     // the two tokens are neighbours of one pair: their V half-words leave as words
     const int64_t other = __shfl_xor_sync(0xffffffffu, slot, L);
     const bool paired = slot >= 0 && other >= 0 && (slot ^ other) == 1 && ((slot & 1) == (o & 1));
+    uint32_t slot_of = 0;
     for (uint32_t chunk = first; chunk < last; ++chunk) {
-        const Row<E> row = next;
-        if (chunk + 1 < last) next = fetch(chunk + 1);
+        Row<E> row;
+        if constexpr (kAhead) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+#pragma unroll
+            for (int g = 0; g < 4; ++g) *reinterpret_cast<uint4*>(row.w[g]) = lds128(mine + (slot_of * 4 + g) * 512);
+        } else {
+            row = next;
+            if (chunk + 1 < last) next = fetch(chunk + 1);
+        }
         int kind, head;
         const bool live = place(chunk, kind, head);
         float x[4][E];
@@ -161,6 +201,10 @@ __global__ void __launch_bounds__(kApThreads, L == 8 ? 4 : 2) pg_append_kernel(c
                 x[g][e] = a.x;
                 x[g][e + 1] = a.y;
             }
+        if constexpr (kAhead) {
+            request(chunk + kAhead, slot_of);
+            slot_of = slot_of == kAhead - 1 ? 0 : slot_of + 1;
+        }
         if (kind != 1 && P.cos) {
 #pragma unroll
             for (int g = 0; g < 2; ++g)
@@ -247,6 +291,7 @@ struct RdParams {
 };
 
 // Four lanes per row, lane j its dims 32 g + 8 j .. + 7; the values are exact in fp16 and fp32, and rounded once to bf16.
+// Bound: memory, 144 bytes in and 512 out per token and KV head: 16384 tokens of 8 KV heads 15.9 us, 5.4 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(256) pg_read_kernel(const RdParams P) {
     grid_launch_dependents();
@@ -328,8 +373,8 @@ extern "C" __attribute__((visibility("default"))) int bgtq_paged_append(
         q_st % 8 || q_sh % 8 || !aligned(rope_cos, 16) || !aligned(rope_sin, 16) || rope_st % 4)
         return BGTQ_E_ALIGN;
     // Few rows: as many warps as there are, two rows each and eight lanes to a row (32 tokens of 32 query and 8 KV heads 2.8 us, 3.0 with four).
-    // Otherwise four rows and four lanes to a row (4096 tokens 18.8 us, 21.8), as many chunks one behind the other as leave the SMs
-    // one round of resident warps (6 of 12 per warp 20.9).
+    // Otherwise four rows and four lanes to a row (4096 tokens 3 us less, measured before the ring), as many chunks one behind the other as leave the SMs
+    // one round of resident warps (6 of 12 per warp: 2 us more).
     int dev = 0, sms = 148;
     if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     const int64_t pairs = ((int64_t)n_tok + 1) / 2;
