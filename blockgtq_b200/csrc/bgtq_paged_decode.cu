@@ -581,13 +581,12 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
             }
             w.all = __all_sync(0xffffffffu, kk >= w.n || w.from);
         }
-        const uint8_t* src = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(w.from), 2 * (k & 15) + (lane & 1)));
         uint64_t* bar = &S.full[warp][stage];
         uint32_t there = 3u;
-        if (!w.all) there = __ballot_sync(0xffffffffu, src != nullptr) & 3u;
+        if (!w.all) there = __ballot_sync(0xffffffffu, w.from != nullptr) >> (2 * (k & 15)) & 3u;
         if (lane == 0) mbar_arrive_expect_tx(bar, w.all ? kBatchBytes : (uint32_t)__popc(there) * kUnitBytes);
-        __syncwarp();
-        if (lane < 2 && src) bulk_g2s_hint(S.ring[warp][stage] + lane * kUnitBytes, src, kUnitBytes, bar, policy);
+        // (the lanes that hold the addresses; a copy that ends before the arrival finds the phase open all the same)
+        if (lane >> 1 == (k & 15) && w.from) bulk_g2s_hint(S.ring[warp][stage] + (lane & 1) * kUnitBytes, w.from, kUnitBytes, bar, policy);
         w.have = (w.have & ~(3u << (2 * stage))) | there << (2 * stage);
     };
     auto begin_copies = [&](const Segment& sg) {
