@@ -612,8 +612,10 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
             bar_and(3 + mb, 256, true);                // (exponents are there)
             int lim;
             {
-                const int g = w.b.row0 + kRows * mb + r128, pos = pf_pos(P, g);
-                lim = pos >= w.b.n ? 0 : P.causal ? max(0, min(w.b.len, w.b.len - w.b.n + 1 + pos)) : w.b.len;
+                // (rows behind the last one, zeros, compute what that one's limit lets them: with none of the tokens each of their tiles
+                // would be one that is cut, and these blocks, 1.6 times as long as the others, the launch's end)
+                const int g = w.b.row0 + kRows * mb + r128, pos = min(pf_pos(P, g), w.b.n - 1);
+                lim = P.causal ? max(0, min(w.b.len, w.b.len - w.b.n + 1 + pos)) : w.b.len;
             }
             float down0, down1;
             pg_pow2(-S.ex[mb][r128], down0, down1);
