@@ -23,6 +23,11 @@
 //            CTAs.  Triples cut between CTAs are merged by a second launch.  (Shares and triples of whole rounds of eight, as the warps
 //            take them: 8 sequences of 32768 tokens x 2 KV heads 27.1 us instead of 26.1, 63 short ones beside one of 30000 tokens 27.8 instead of 25.5.)
 //   cluster  a cluster of 1 to 8 CTAs per triple, which merge their shares in distributed shared memory: no list, no second launch.
+// What bounds it: with long caches the warps' instructions, 320 for a unit of 16 tokens and one column tile (128 of them make codes of 144
+// bytes' nibbles, 46 are the loop's), issued in 63 % of the cycles with the ALU half busy, 16 warps on an SM by their registers.  One sequence
+// of 131072 tokens x 8 KV heads 39.3 us, 3.8 TB/s; 64 of 4500 81.4 us, 4.1 TB/s (loads alone, nothing computed: 27.8 and 57.4).  With short ones
+// a launch and the chain length - page number - page - merging: 500 tokens 5.9 us, 4 sequences of 4099 8.4.
+//
 // In a CTA eight warps take batches in turn, each with a ring of bulk copies of its own (the next triple's first ones travel while this
 // one's states are merged in shared memory).
 #include "bgtq_paged_common.cuh"

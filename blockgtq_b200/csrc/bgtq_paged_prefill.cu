@@ -15,7 +15,10 @@
 //           Queries are brought to [2^13, 2^14) by a power of two per row, which makes bf16 queries exact in fp16.
 //   merge   rows of the blocks that the shares cut.
 //
-// What bounds attend: per tile 32 products of 64 cycles and 32768 exponentials at 16 a cycle, 2048 cycles each.
+// What bounds attend: per tile 32 products of 64 cycles and 32768 exponentials at 16 a cycle, 2048 cycles each; a tile takes about 3200, the chain
+// of a block's S, its softmax (1900 cycles) and its P . vhat beside the other block's.  8192 positions x 32 query and 8 KV heads, causal: 506 us
+// in short runs, 1.09 PFLOP/s, and 562 in long ones, 0.98 PFLOP/s, where the power limit lowers the clock.  Chunks of 195 to 700 rows behind 700
+// to 9100 tokens of 2 KV heads x 8: 114 us for the three launches, every CTA's share done between 77 and 95 us.
 // Every wait is bounded: one that gives up is recorded in shared memory, where the others see it, and in the caller's status word; the CTA then
 // drains its copies and products, releases its tensor memory and returns.
 #include "bgtq_paged_common.cuh"
@@ -80,7 +83,8 @@ __device__ __forceinline__ Seq pf_seq(const Pf& P, int i) {
 // ------------------------------------------------------------------------------------------------------------------
 // unpack: a warp per unit of 16 tokens.  Operand layout (no swizzle, K-major): element (row, k) at
 //     (row / 8) * 2048 + (k / 8) * 128 + (row % 8) * 16 + (k % 8) * 2.
-// Bound: memory, 144 bytes in and 512 out per token and head.  Every store is 16 bytes, a warp's are whole 128-byte lines.
+// Bound: memory, 144 bytes in and 512 out per token and head, at 4.2 TB/s (8192 tokens x 8 heads: 43 MB in 10 us).  Every store is 16 bytes, a
+// warp's are whole 128-byte lines.
 // ------------------------------------------------------------------------------------------------------------------
 template <int G>
 __device__ __forceinline__ uint32_t value2(uint32_t w, uint32_t scale) {        // the pair of codes of group G, times the scales
@@ -830,6 +834,7 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
 
 // ------------------------------------------------------------------------------------------------------------------
 // merge: block (i, y) eight rows of the block that the end of CTA i's share cuts, if that is its first cut; a warp per row.
+// Bound: memory, at most 148 cuts x 256 rows x two parts of 520 bytes, 39 MB that are still in L2.
 // ------------------------------------------------------------------------------------------------------------------
 template <typename T>
 __global__ void __launch_bounds__(256) pg_prefill_merge_kernel(const Pf P) {
