@@ -833,40 +833,65 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// merge: block (i, y) eight rows of the block that the end of CTA i's share cuts, if that is its first cut; a warp per row.
+// merge: block (i, y) 32 rows of the block that the end of CTA i's share cuts, if that is its first cut; a warp four of them at a time, so that what
+// is looked up first, three loads one behind the other, is looked up for 32 rows together.
 // Bound: memory, at most 148 cuts x 256 rows x two parts of 520 bytes, 39 MB that are still in L2.
 // ------------------------------------------------------------------------------------------------------------------
+constexpr int kMergeRows = 4;
 template <typename T>
 __global__ void __launch_bounds__(256) pg_prefill_merge_kernel(const Pf P) {
-    const int lane = threadIdx.x & 31, row = blockIdx.y * 8 + (threadIdx.x >> 5), j0 = blockIdx.x;
+    const int lane = threadIdx.x & 31, row0 = (blockIdx.y * 8 + (threadIdx.x >> 5)) * kMergeRows, j0 = blockIdx.x;
     grid_launch_dependents();
     grid_dependency_wait();
     const int4 a = P.start[j0], b = P.start[j0 + 1];
-    if (b.w == P.start[P.n_cta].w || b.y == 0) return;          // nothing behind, or cut between blocks
+    const int all = P.start[P.n_cta].w, behind = P.start[min(j0 + 2 + lane, P.n_cta)].w;
+    if (b.w == all || b.y == 0) return;                         // nothing behind, or cut between blocks
     const bool same = a.x == b.x && a.z == b.z;                 // the CTA's only block
     if (same && a.y > 0) return;                                // (cut before)
     const Block bk = P.blk[b.x];
-    const int g = bk.row0 + row, pos = pf_pos(P, g);
-    if (pos >= bk.n) return;
-    int j1 = j0 + 1;                                            // the last CTA that holds a part of it
     const int end = b.w - b.y + bk.tiles;
-    while (j1 + 1 < P.n_cta && P.start[j1 + 1].w < end) ++j1;
-    float m = -INFINITY, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int j = j0; j <= j1; ++j) {
-        const size_t slot = (size_t)(2 * j + (j == j0 && !same ? 1 : 0)) * kBlockRows + row;
-        const float2 ml = P.part_ml[slot];
-        const float4 v = *reinterpret_cast<const float4*>(P.part_o + slot * kHD + 4 * lane);
-        const float top = fmaxf(m, ml.x), z = top == -INFINITY ? 0.f : top, f = pf_exp2(m - z), f1 = pf_exp2(ml.x - z);
-        l = fmaf(f1, ml.y, l * f);
-        o.x = fmaf(f1, v.x, o.x * f); o.y = fmaf(f1, v.y, o.y * f); o.z = fmaf(f1, v.z, o.z * f); o.w = fmaf(f1, v.w, o.w * f);
-        m = top;
+    int j1 = j0 + 1;                                            // the last CTA that holds a part of it
+    for (int w = behind;; w = P.start[min(j1 + 1 + lane, P.n_cta)].w) {
+        const uint32_t more = __ballot_sync(0xffffffffu, j1 + 1 + lane < P.n_cta && w < end);
+        j1 += __popc(more);
+        if (more != 0xffffffffu) break;
     }
-    const int hq = (P.h0 + b.z) * P.gqa + g - pos * P.gqa;
-    const float inv = l > 0.f ? 1.0f / l : l == 0.f ? 0.f : l;
-    *reinterpret_cast<uint2*>(reinterpret_cast<T*>(P.out) + (int64_t)(bk.q0 + pos) * P.o_st + (int64_t)hq * P.o_sh + 4 * lane) =
-        make_uint2(PgType<T>::down(o.x * inv, o.y * inv), PgType<T>::down(o.z * inv, o.w * inv));
-    if (P.lse && lane == 0) P.lse[(int64_t)(bk.q0 + pos) * P.n_q + hq] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945309f;
+    float m[kMergeRows], l[kMergeRows];
+    float4 o[kMergeRows];
+#pragma unroll
+    for (int i = 0; i < kMergeRows; ++i) {
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+        o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    for (int j = j0; j <= j1; ++j) {
+        const size_t slot = (size_t)(2 * j + (j == j0 && !same ? 1 : 0)) * kBlockRows + row0;
+        float2 ml[kMergeRows];
+        float4 v[kMergeRows];
+#pragma unroll
+        for (int i = 0; i < kMergeRows; ++i) {
+            ml[i] = P.part_ml[slot + i];
+            v[i] = *reinterpret_cast<const float4*>(P.part_o + (slot + i) * kHD + 4 * lane);
+        }
+#pragma unroll
+        for (int i = 0; i < kMergeRows; ++i) {
+            const float top = fmaxf(m[i], ml[i].x), z = top == -INFINITY ? 0.f : top, f = pf_exp2(m[i] - z), f1 = pf_exp2(ml[i].x - z);
+            l[i] = fmaf(f1, ml[i].y, l[i] * f);
+            o[i].x = fmaf(f1, v[i].x, o[i].x * f); o[i].y = fmaf(f1, v[i].y, o[i].y * f);
+            o[i].z = fmaf(f1, v[i].z, o[i].z * f); o[i].w = fmaf(f1, v[i].w, o[i].w * f);
+            m[i] = top;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kMergeRows; ++i) {
+        const int g = bk.row0 + row0 + i, pos = pf_pos(P, g);
+        if (pos >= bk.n) return;
+        const int hq = (P.h0 + b.z) * P.gqa + g - pos * P.gqa;
+        const float inv = l[i] > 0.f ? 1.0f / l[i] : l[i] == 0.f ? 0.f : l[i];
+        *reinterpret_cast<uint2*>(reinterpret_cast<T*>(P.out) + (int64_t)(bk.q0 + pos) * P.o_st + (int64_t)hq * P.o_sh + 4 * lane) =
+            make_uint2(PgType<T>::down(o[i].x * inv, o[i].y * inv), PgType<T>::down(o[i].z * inv, o[i].w * inv));
+        if (P.lse && lane == 0) P.lse[(int64_t)(bk.q0 + pos) * P.n_q + hq] = l[i] == 0.f ? -INFINITY : (m[i] + log2f(l[i])) * 0.693147180559945309f;
+    }
 }
 
 }  // namespace
@@ -947,7 +972,7 @@ int paged_prefill(const PagedPrefill& A, cudaStream_t stream) {
             P.out = A.out; P.o_st = A.o_st; P.o_sh = A.o_sh; P.lse = A.lse; P.status = A.status;
             if (launch_kernel(pg_unpack_kernel, dim3((unsigned)tiles + 1, nh, ns), dim3(256), 0, stream, true, P) != cudaSuccess) return BGTQ_E_LAUNCH;
             if (launch_kernel(kernel, dim3(n_cta), dim3(kThreads), sizeof(PfSmem), stream, true, P) != cudaSuccess) return BGTQ_E_LAUNCH;
-            if (launch_kernel(merge, dim3(n_cta - 1, kBlockRows / 8), dim3(256), 0, stream, true, P) != cudaSuccess) return BGTQ_E_LAUNCH;
+            if (launch_kernel(merge, dim3(n_cta - 1, kBlockRows / (8 * kMergeRows)), dim3(256), 0, stream, true, P) != cudaSuccess) return BGTQ_E_LAUNCH;
         }
     return BGTQ_OK;
 }
