@@ -571,3 +571,39 @@ def test_the_library_reads_no_further_than_the_table(form):
     assert rc == 0 and status.item() == 0
     for b, (a, z) in enumerate([(0, 6), (6, 10)]):
         _check(out, None, R.attention(q[a:z], pages.cpu(), slots[b], [48 - z + a + 1 + i for i in range(z - a)], 1 / math.sqrt(128)), slice(a, z))
+
+
+@pytest.mark.parametrize("n_kv,lens", [(3, [70001, 41, 33000, 0, 12345]), (1, [120000])])
+def test_long_sequences_whose_shares_end_inside_a_round(n_kv, lens, monkeypatch):
+    """Shares of odd numbers of batches, and more partials of a triple than are merged in one pass."""
+    from blockgtq_b200 import paged, paged_kv4_decode_attention
+    monkeypatch.setattr(paged, "_FORM", FORMS["split"])
+    gen = torch.Generator().manual_seed(len(lens))
+    pages, table, slots = _case(gen, n_kv, 64, lens)
+    q = (_noise(gen, len(lens), n_kv, 128) * 3).half()
+    out, lse = paged_kv4_decode_attention(q.to(DEV), pages, table.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV), return_lse=True)
+    host = pages.cpu()
+    for b, t in enumerate(lens):
+        _check(out, lse, R.attention(q[b:b + 1], host, slots[b], [t], 1 / math.sqrt(128)), slice(b, b + 1))
+
+
+def test_calls_on_two_streams_at_once():
+    from blockgtq_b200 import paged_kv4_decode_attention, paged_kv4_prefill_attention
+    gen = torch.Generator().manual_seed(51)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    lens = [5000, 17, 2600]
+    pages, table, _ = _case(gen, 2, 16, lens)
+    q, rows = (_noise(gen, n, 8, 128).half().to(DEV) for n in (3, 900))
+    args = pages, table.to(DEV), torch.tensor(lens, **i32)
+    cu = torch.tensor([0, 400, 417, 900], **i32)
+    want = paged_kv4_decode_attention(q, *args), paged_kv4_prefill_attention(rows, *args, cu)
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(DEV) for _ in range(2)], ([], [])
+    for _ in range(10):
+        with torch.cuda.stream(streams[0]):
+            got[0].append(paged_kv4_decode_attention(q, *args))
+        with torch.cuda.stream(streams[1]):
+            got[1].append(paged_kv4_prefill_attention(rows, *args, cu))
+    torch.cuda.synchronize()
+    for results, w in zip(got, want):
+        assert all(torch.equal(r, w) for r in results)
