@@ -1,21 +1,22 @@
 // Attention of few query rows per (sequence, KV head) over the paged 4-bit cache, on mma.sync, straight from the packed codes.
 //
 //     S[t, col] = sum_g ks[t, g] * (sum_{d in g} q[col, d] (u[t, d] - 8)),   P = 2^(S f - M),
-//     O[d, col] = sum_t P[t, col] vs[t, g(d)] (u[t, d] - 8),   out = O / sum_t P
+//     O[d, col] = sum_t P[t, col] * (vs[t, g(d)] (u[t, d] - 8)),   out = O / sum_t P
 //
 // A column is one query row: a query head of the KV head's group in a decode step, (position, head) pairs of a chunk.  Codes become
 // u - 8 in fp16: a mask makes 1024 + u or 1024 + 16 u of two of them at once, one exact operation the rest.  (As subnormal numbers, u * 2^-24
 // without that operation, with the eights in the accumulators' start or in a product of their own: operands are aligned by their exponent
 // field, not by their leading bit, which cost ten bits of the sums; and over tokens the eights take theirs of the accumulators.)  The K scales
-// multiply the groups' sums, the V scales the weights.  Nothing is rounded but P * vs (fp16, as the product's operand; sums, maxima, scales
-// and accumulators are fp32).  Queries are brought to [2^13, 2^14) by a power of two each, so that bf16 queries of any
+// multiply the groups' sums; V's operand is code * scale, exactly an fp16 number.  Nothing is rounded but P (fp16, as the product's operand; sums,
+// maxima, scales and accumulators are fp32).  Queries are brought to [2^13, 2^14) by a power of two each, so that bf16 queries of any
 // magnitude are exact in fp16 too.
 //
-// P * vs <= 2^15 holds for every magnitude of V: a warp keeps a power of two R above every V scale that it has met, a column's reference M is 12
-// below its largest S f + log2 R, and both move (O rescaled) only when a scale passes R or a logit the largest by more than 3.  The weight of
-// the token that set the reference is then a power of two times its scale, which fp16 holds: where one token has nearly all the weight, as
-// in a sequence of one, its values come out as they are.  (Moving at 1: 16 sequences of 2047 tokens, 4 rows each, 21.1 us instead of 20.0; at 8,
-// rows of one dominating token lie up to 1.5 times as far from 64 bits.)
+// P <= 2^15: a column's reference M is 12 below its largest S f, and moves (O rescaled) only when a logit passes the largest by more than 3.  The
+// weight of the token that set the reference is then a power of two: where one token has nearly all the weight, as in a sequence of one, its values
+// come out as they are.  Weights below 2^-26 of the largest are subnormal in fp16, and cut at 2^-37 of it.  V's scales are not taken into the weights,
+// although that saves a product per pair of codes: one token of large V, even one of hardly any weight, then pushes the others' weights out of
+// fp16's range (values of 0.01 beside one of 65000, a token of zeros at 2^14 of their weight: their sum off by half).  (Moving at 1: 16 sequences of 2047
+// tokens, 4 rows each, 21.1 us instead of 20.0; at 8, rows of one dominating token lie up to 1.5 times as far from 64 bits.)
 //
 // Work, in one of two forms:
 //   split    the 32-token batches of all (sequence, block of columns, KV head) triples form one list, each triple headed by kTripleCost
@@ -33,6 +34,8 @@
 #include "bgtq_paged_common.cuh"
 #include "bgtq_paged_prefill.h"
 
+#include <limits.h>
+
 namespace bgtq {
 namespace {
 
@@ -42,7 +45,7 @@ constexpr int kBatchBytes = kBatchTok / kUnitTok * kUnitBytes;
 // Places for what a triple costs beside its batches, a multiple of kPdWarps.  64 sequences of up to 9100 tokens x 8 KV heads: 110 us without,
 // 91.4 with 8, 87.5 with 16, 89.4 with 24; 63 short ones beside one of 30000: 26.6, 27.9, 32.0.
 constexpr uint32_t kTripleCost = 16;
-constexpr float kLift = 12.f, kReach = 15.f;      // log2 of P * R at a reference's setting, and where it moves
+constexpr float kLift = 12.f, kReach = 15.f;      // log2 of P at a reference's setting, and where it moves
 constexpr int kOutRow = 132;                      // floats between columns of a warp's state in shared memory
 
 struct PdParams {
@@ -310,34 +313,41 @@ struct State {
     float o[NT][2][4][4];            // [i][n]: rows 32 n + 4 r + 2 i (+ 1), columns 2 c (+ 1)
     float m[NT][2], l[NT][2];        // reference, denominator
     float top[NT][2];                // the largest logit that the reference allows
-    uint32_t r;                      // a power of two above every V scale so far, as a pair of bf16
 };
 
 template <typename V> __device__ __forceinline__ V at(const uint8_t* p) { return *reinterpret_cast<const V*>(p); }
 template <int N> struct Int { static constexpr int value = N; };
 template <typename F> __device__ __forceinline__ void each_group(F f) { f(Int<0>{}); f(Int<1>{}); f(Int<2>{}); f(Int<3>{}); }
 
-__device__ __forceinline__ uint32_t max_bf2(uint32_t a, uint32_t b) {
-    uint32_t d;
-    asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-    return d;
+// A value of V that is no number, in a unit that some columns see only in part: as an operand it would reach all of them.  Its scale becomes zero,
+// and the columns that see it become none.  s0, s1: scales of tokens t, t + 1, group c.
+template <int NT>
+__device__ __forceinline__ void pd_no_number(State<NT>& st, float& s0, float& s1, int t, int c, const int (&lim)[NT][2]) {
+    const int first = s0 != s0 ? t : s1 != s1 ? t + 1 : INT_MAX;
+    if (s0 != s0) s0 = 0.f;
+    if (s1 != s1) s1 = 0.f;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const int first_g = __reduce_min_sync(0xffffffffu, c == g ? first : INT_MAX);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (first_g < lim[nt][e])
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) st.o[nt][i][g][e] = st.o[nt][i][g][2 + e] = __uint_as_float(0x7fffffffu);
+    }
 }
+
 // U units of 16 tokens at u in shared memory.  kEdge: some of them (tokens from len on of the sequence, from lim[] on of a column) are hidden.
 template <int NT, int U, bool kEdge>
 __device__ __forceinline__ void pd_units(const uint8_t* u, const Magic& mg, const Query<NT>& Q, State<NT>& st, int r, int c, int t0, int len, const int (&lim)[NT][2]) {
     float s[U][NT][4];
-    uint2 va[U], vc[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
         const uint8_t* const k = u + i * kUnitBytes;
         const uint4 x = at<uint4>(k + r * 64 + c * 16), y = at<uint4>(k + 512 + r * 64 + c * 16);
         const uint2 ka = at<uint2>(k + kUnitKs + r * 8), kc = at<uint2>(k + kUnitKs + 64 + r * 8);
-        va[i] = at<uint2>(k + kUnitVs + r * 8);
-        vc[i] = at<uint2>(k + kUnitVs + 64 + r * 8);
-        if (kEdge) {
-            if (t0 + 16 * i + r >= len) va[i] = make_uint2(0, 0);               // what lies behind the sequence may be anything
-            if (t0 + 16 * i + 8 + r >= len) vc[i] = make_uint2(0, 0);
-        }
         const float sa[4] = {pg_lo(ka.x), pg_hi(ka.x), pg_lo(ka.y), pg_hi(ka.y)};
         const float sc[4] = {pg_lo(kc.x), pg_hi(kc.x), pg_lo(kc.y), pg_hi(kc.y)};
         const uint4 x8 = make_uint4(x.x >> 8, x.y >> 8, x.z >> 8, x.w >> 8), y8 = make_uint4(y.x >> 8, y.y >> 8, y.z >> 8, y.w >> 8);
@@ -362,13 +372,11 @@ __device__ __forceinline__ void pd_units(const uint8_t* u, const Magic& mg, cons
             }
         });
     }
-    uint32_t r2 = st.r;
     float top[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) top[nt][0] = top[nt][1] = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-        r2 = max_bf2(r2, max_bf2(max_bf2(va[i].x, va[i].y), max_bf2(vc[i].x, vc[i].y)));
+    for (int i = 0; i < U; ++i)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -379,8 +387,7 @@ __device__ __forceinline__ void pd_units(const uint8_t* u, const Magic& mg, cons
                 }
                 top[nt][e] = fmaxf(top[nt][e], fmaxf(s[i][nt][e], s[i][nt][2 + e]));
             }
-    }
-    bool move = r2 != st.r;
+    bool move = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -389,14 +396,6 @@ __device__ __forceinline__ void pd_units(const uint8_t* u, const Magic& mg, cons
             move |= top[nt][e] > st.top[nt][e];
         }
     if (__any_sync(0xffffffffu, move)) {
-        r2 = max_bf2(r2, __byte_perm(r2, r2, 0x1032));
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) r2 = max_bf2(r2, __shfl_xor_sync(0xffffffffu, r2, d));
-        if (r2 != st.r) {                  // the power of two above it (scales lie between 2^-17 and 2^14; with none it is 2^-17)
-            const uint32_t up = max(((r2 & 0x7f80u) + 0x80u), 0x3700u);
-            st.r = up | up << 16;
-        }
-        const float lr = (float)((int)((st.r & 0x7fffu) >> 7) - 127);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -404,10 +403,10 @@ __device__ __forceinline__ void pd_units(const uint8_t* u, const Magic& mg, cons
                 float t = top[nt][e];
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, d));
-                const float m = fmaxf(st.m[nt][e], t + lr - kLift);
+                const float m = fmaxf(st.m[nt][e], t - kLift);
                 const float alpha = m == -INFINITY ? 1.f : ex2(st.m[nt][e] - m);
                 st.m[nt][e] = m;
-                st.top[nt][e] = m + (kReach - lr);
+                st.top[nt][e] = m + kReach;
                 st.l[nt][e] *= alpha;
 #pragma unroll
                 for (int n = 0; n < 4; ++n)
@@ -420,35 +419,44 @@ __device__ __forceinline__ void pd_units(const uint8_t* u, const Magic& mg, cons
     }
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-        float p[NT][4];
+        uint32_t b[NT][2];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
+            float p[4];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const float z = kEdge && st.m[nt][e] == -INFINITY ? 0.f : st.m[nt][e];
-                p[nt][e] = ex2(fmaf(s[i][nt][e], Q.f[nt][e], -z));
-                p[nt][2 + e] = ex2(fmaf(s[i][nt][2 + e], Q.f[nt][e], -z));
-                st.l[nt][e] += p[nt][e] + p[nt][2 + e];
+                p[e] = ex2(fmaf(s[i][nt][e], Q.f[nt][e], -z));
+                p[2 + e] = ex2(fmaf(s[i][nt][2 + e], Q.f[nt][e], -z));
+                st.l[nt][e] += p[e] + p[2 + e];
             }
-        const uint8_t* const v = u + i * kUnitBytes + kUnitV + c * 128 + r * 16;
-        const uint4 x = at<uint4>(v), y = at<uint4>(v + 512);
-        const float ha[4] = {pg_lo(va[i].x), pg_hi(va[i].x), pg_lo(va[i].y), pg_hi(va[i].y)};
-        const float hc[4] = {pg_lo(vc[i].x), pg_hi(vc[i].x), pg_lo(vc[i].y), pg_hi(vc[i].y)};
+            b[nt][0] = transposed(pack_half2(p[0], p[1]));
+            b[nt][1] = transposed(pack_half2(p[2], p[3]));
+        }
+        const uint8_t* const unit = u + i * kUnitBytes;
+        const uint4 x = at<uint4>(unit + kUnitV + c * 128 + r * 16), y = at<uint4>(unit + kUnitV + 512 + c * 128 + r * 16);
+        // scales of the unit's tokens 2 r, 2 r + 1, group c, exact in fp16; the lanes get theirs from one another (11 instructions; 24 if
+        // each lane converted its eight pairs for itself)
+        float s0 = pg_lo(at<uint16_t>(unit + kUnitVs + 16 * r + 2 * c)), s1 = pg_lo(at<uint16_t>(unit + kUnitVs + 16 * r + 8 + 2 * c));
+        if (kEdge) {
+            const int t = t0 + 16 * i + 2 * r;
+            if (t >= len) s0 = 0.f;                                             // what lies behind the sequence may be anything
+            if (t + 1 >= len) s1 = 0.f;
+            if (__any_sync(0xffffffffu, s0 != s0 || s1 != s1)) pd_no_number<NT>(st, s0, s1, t, c, lim);
+        }
+        const uint32_t mine = pack_half2(s0, s1);
         const uint4 x8 = make_uint4(x.x >> 8, x.y >> 8, x.z >> 8, x.w >> 8), y8 = make_uint4(y.x >> 8, y.y >> 8, y.z >> 8, y.w >> 8);
         each_group([&](auto gi) {
             constexpr int g = decltype(gi)::value;
-            const uint32_t a0[4] = {codes<g>(mg, x.x, x8.x), codes<g>(mg, x.y, x8.y), codes<g>(mg, y.x, y8.x), codes<g>(mg, y.y, y8.y)};
-            const uint32_t a1[4] = {codes<g>(mg, x.z, x8.z), codes<g>(mg, x.w, x8.w), codes<g>(mg, y.z, y8.z), codes<g>(mg, y.w, y8.w)};
+            const uint32_t sx = __shfl_sync(0xffffffffu, mine, 4 * c + g), sy = __shfl_sync(0xffffffffu, mine, 4 * c + 16 + g);
+            const uint32_t a0[4] = {hmul2_u32(codes<g>(mg, x.x, x8.x), sx), hmul2_u32(codes<g>(mg, x.y, x8.y), sx),
+                                    hmul2_u32(codes<g>(mg, y.x, y8.x), sy), hmul2_u32(codes<g>(mg, y.y, y8.y), sy)};
+            const uint32_t a1[4] = {hmul2_u32(codes<g>(mg, x.z, x8.z), sx), hmul2_u32(codes<g>(mg, x.w, x8.w), sx),
+                                    hmul2_u32(codes<g>(mg, y.z, y8.z), sy), hmul2_u32(codes<g>(mg, y.w, y8.w), sy)};
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                float w[4] = {p[nt][0] * ha[g], p[nt][1] * ha[g], p[nt][2] * hc[g], p[nt][3] * hc[g]};
-                if (kEdge) {                                        // (a hidden token's scale may be no number)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) w[e] = s[i][nt][e] == -INFINITY ? 0.f : w[e];
-                }
-                const uint32_t b[2] = {transposed(pack_half2(w[0], w[1])), transposed(pack_half2(w[2], w[3]))};
-                mma_acc(st.o[nt][0][g], a0, b);
-                mma_acc(st.o[nt][1][g], a1, b);
+                mma_acc(st.o[nt][0][g], a0, b[nt]);
+                mma_acc(st.o[nt][1][g], a1, b[nt]);
             }
         });
     }
