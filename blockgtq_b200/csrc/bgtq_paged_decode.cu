@@ -403,10 +403,11 @@ __device__ __forceinline__ void pd_units(const uint8_t* u, const Magic& mg, cons
                 float t = top[nt][e];
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, d));
-                const float m = fmaxf(st.m[nt][e], t - kLift);
+                // (where fp32's steps are wider than these distances, they become none)
+                const float m = fmaxf(st.m[nt][e], t - (t - kLift) > kReach ? t : t - kLift);
                 const float alpha = m == -INFINITY ? 1.f : ex2(st.m[nt][e] - m);
                 st.m[nt][e] = m;
-                st.top[nt][e] = m + kReach;
+                st.top[nt][e] = m + kReach - m > kReach ? m : m + kReach;
                 st.l[nt][e] *= alpha;
 #pragma unroll
                 for (int n = 0; n < 4; ++n)
@@ -426,8 +427,9 @@ __device__ __forceinline__ void pd_units(const uint8_t* u, const Magic& mg, cons
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const float z = kEdge && st.m[nt][e] == -INFINITY ? 0.f : st.m[nt][e];
-                p[e] = ex2(fmaf(s[i][nt][e], Q.f[nt][e], -z));
-                p[2 + e] = ex2(fmaf(s[i][nt][2 + e], Q.f[nt][e], -z));
+                // (product and difference rounded apart, as the references were: fused, logits beyond 2^26 differ from theirs by more than a weight's range)
+                p[e] = ex2(__fmul_rn(s[i][nt][e], Q.f[nt][e]) - z);
+                p[2 + e] = ex2(__fmul_rn(s[i][nt][2 + e], Q.f[nt][e]) - z);
                 st.l[nt][e] += p[e] + p[2 + e];
             }
             b[nt][0] = transposed(pack_half2(p[0], p[1]));

@@ -269,6 +269,7 @@ constexpr int kSlots = 4;
 constexpr uint32_t kTmemCols = 512;     // S (and P) of block m: columns [128 m, 128 m + 128); O of block m: [256 + 128 m, 384 + 128 m)
 constexpr uint32_t kColS = 0, kColO = 256;
 constexpr float kLift = 7.0f, kReach = 15.0f;
+constexpr float kHuge = 1048576.0f;     // 2^20: a fused product's rounding is 2^-4 of a power of two here
 // Of 16 pairs of exponentials, those that go to the FMA pipe: 8192 positions x 32 heads 506 us with two of them, 509 with none, 510 with three,
 // 517 with four.
 constexpr uint32_t kPolyPairs = 0x8080;
@@ -627,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
             const uint8_t* const valid = P.valid + (int64_t)w.b.si * P.max_tiles + tile0;
             uint32_t units = tiles > 0 ? valid[0] : 0;
             float m_used = -INFINITY, lsum = 0.f;    // what this row scales by (log2), this half's denominator
-            const uint64_t sc2 = pack_f2(sc, sc);
+            bool huge = false;                       // logits whose steps in fp32 are no longer small beside a weight's range
             for (int i = 0; i < tiles; ++i) {
                 if (!__all_sync(0xffffffffu, pf_wait(S, &S.s_ready[mb], (uint32_t)(done + i) & 1u))) ok = false;
                 tc_fence_after_sync();
@@ -662,18 +663,21 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                     asm volatile("cp.async.wait_all;" ::: "memory");
                     __syncwarp();
                 }
-                const bool move = bar_or(1 + mb, m_half > m_used + kReach || (m_used == -INFINITY && m_half > -INFINITY) || !ok);
+                const bool move = bar_or(1 + mb, m_half - m_used > kReach || !ok);
                 if (move) {
                     S.xch[mb][hf][r128] = m_half;
                     const bool all_ok = bar_and(3 + mb, 256, ok);
                     if (!all_ok) { ok = false; break; }              // (the same verdict for the whole block)
-                    const float m_new = fmaxf(m_half, S.xch[mb][hf ^ 1][r128]) - kLift;
+                    const float top_m = fmaxf(m_half, S.xch[mb][hf ^ 1][r128]);
+                    // (where fp32's steps are wider than the distance, it becomes none)
+                    const float m_new = top_m - (top_m - kLift) > kReach ? top_m : top_m - kLift;
                     float alpha = 1.f;
                     if (m_used == -INFINITY) m_used = m_new;         // nothing accumulated for this row yet
-                    else if (m_new > m_used + (kReach - kLift)) {
+                    else if (top_m - m_used > kReach) {
                         alpha = pf_exp2(m_used - m_new);
                         m_used = m_new;
                     }
+                    huge = __any_sync(0xffffffffu, fabsf(m_used) >= kHuge && m_used > -INFINITY);
                     lsum *= alpha;
                     if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
                         // O is at rest between the previous tile's product and this tile's
@@ -685,10 +689,14 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                 }
                 if (last && w.next_tiles(next.b) > 0) fetch(next.b, w.next_h());        // (the last product with the queries is done)
                 const float z = m_used == -INFINITY ? 0.f : m_used;
-                const uint64_t nz2 = pack_f2(-z, -z);
+                const uint64_t nz2 = pack_f2(-z, -z), sc2 = huge ? pack_f2(1.f, 1.f) : pack_f2(sc, sc);
                 uint64_t ps[2] = {0ull, 0ull};
                 auto put = [&](uint32_t c0) {       // P of the columns in sv -> 16 columns of the half's own part of S
                     uint32_t pk[16];
+                    if (huge) {                     // product and difference rounded apart, as the reference was
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) sv[c] = __fmul_rn(sv[c], sc);
+                    }
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         float x0, x1, p0, p1;

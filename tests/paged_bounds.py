@@ -45,8 +45,9 @@ def logit_cut(q, k):
     return torch.maximum(group, one)
 
 
-def attention(q, pages, slots, seen, scale):
-    """q (n, n_q, 128) over the tokens at ``slots``, row i the first seen[i] of them -> out, lse in 64 bits and the bound of each."""
+def attention(q, pages, slots, seen, scale, apart=False):
+    """q (n, n_q, 128) over the tokens at ``slots``, row i the first seen[i] of them -> out, lse in 64 bits and the bound of each.  ``apart``: keys
+    are equal, and then their logits are too, or so far apart that one has no weight beside the other: what logits lose changes no weight."""
     k, v, _, _ = R.read(pages, slots)
     n, n_q = q.shape[:2]
     gqa = n_q // pages.shape[1]
@@ -68,7 +69,8 @@ def attention(q, pages, slots, seen, scale):
             d = d + abs(scale) * 2.0 ** -23 * qd[i].abs().amax(-1) * k[:m].abs().sum(-1).amax(0)
         mean = torch.einsum("ht,thd->hd", p, v[:m].abs())
         cuts = (m / 16 + 16) * 18 * 2.0 ** -24
-        tol[i] = (2.0 ** -11 + 2 * d[:, None] + 2.0 ** -20 + cuts) * mean + cuts * 2.0 ** -14 + 2.0 ** -32 * v[:m].abs().sum(0) \
+        between = torch.full_like(d, 3e-6) if apart else d
+        tol[i] = (2.0 ** -11 + 2 * between[:, None] + 2.0 ** -20 + cuts) * mean + cuts * 2.0 ** -14 + 2.0 ** -32 * v[:m].abs().sum(0) \
             + R.HALF[q.dtype] * out[i].abs() * 1.01 + 2.0 ** -25
         tol_lse[i] = d + lse[i].abs() * 2.0 ** -22 + (m / 16 + 32) * 2.0 ** -23 + 2.0 ** -20
     return out, lse, tol, tol_lse

@@ -90,3 +90,19 @@ def test_values_of_every_magnitude(form):
     q = torch.randn(rows, 8, 128, generator=gen).half()
     out, lse = _attend(q, pages, table, t, form, rows)
     W.check(out, lse, W.attention(q, pages.cpu(), slots, [t - rows + 1 + i for i in range(rows)], SCALE), slice(0, rows))
+
+
+@pytest.mark.parametrize("rows", [1, 5])
+@pytest.mark.parametrize("dtype,size", [(torch.float16, 1.0), (torch.float16, 2.0 ** 6), (torch.float16, 15000.0), (torch.bfloat16, 1e12), (torch.bfloat16, 1e28)])
+def test_logits_of_any_magnitude(dtype, size, rows, form):
+    """Keys of 9000 in size under queries of `size`: logits up to what fp32 holds.  Their steps are then larger than a weight's whole range."""
+    gen = torch.Generator().manual_seed(77)
+    t = 500
+    one = 3000 * torch.randn(1, 2, 128, generator=gen)
+    k = one.repeat(t, 1, 1)
+    k[5:9], k[300] = -k[5:9], -k[300]                           # each head has its largest logit in many tokens, or in these
+    v = torch.randn(t, 2, 128, generator=gen).to(dtype)
+    pages, table, slots = _pages(k.to(dtype), v)
+    q = (size * torch.randn(rows, 8, 128, generator=gen)).to(dtype)
+    out, lse = _attend(q, pages, table, t, form, rows)
+    W.check(out, lse, W.attention(q, pages.cpu(), slots, [t - rows + 1 + i for i in range(rows)], SCALE, apart=True), slice(0, rows))
