@@ -65,6 +65,10 @@ __device__ __forceinline__ void pg_pow2(int e, float& a, float& b) {
     b = __uint_as_float((uint32_t)(127 + e - e / 2) << 23);
 }
 
+// The factor from products to logits is held above zero: hidden ones are minus infinity before it.  (Products are below 2^38: nothing is left of
+// them at the smallest normal number either.)
+constexpr float kPgFactorMin = 1.17549435e-38f;
+
 // Lets a kernel use this much dynamic shared memory, once per device.
 template <typename K>
 inline bool pg_allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {

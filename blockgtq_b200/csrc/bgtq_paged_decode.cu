@@ -293,7 +293,7 @@ __device__ __forceinline__ void pd_query(const PdParams& P, Query<NT>& Q, const 
         const int ex = pg_row_exponent(top);
         pg_pow2(ex, up0, up1);
         pg_pow2(-ex, down0, down1);
-        float fac = fabsf(P.scale_log2) * down0 * down1;
+        float fac = fmaxf(fabsf(P.scale_log2) * down0 * down1, kPgFactorMin);
         if (P.scale_log2 < 0.f) up0 = -up0;  // (factors are positive: hidden logits are minus infinity before they meet one)
         if (P.scale_log2 == 0.f) {
             up0 = 0.f;

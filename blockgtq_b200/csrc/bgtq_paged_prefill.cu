@@ -624,7 +624,7 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
             }
             float down0, down1;
             pg_pow2(-S.ex[mb][r128], down0, down1);
-            const float sc = (P.scale_log2 == 0.f ? 1.f : fabsf(P.scale_log2)) * down0 * down1;
+            const float sc = fmaxf((P.scale_log2 == 0.f ? 1.f : fabsf(P.scale_log2)) * down0 * down1, kPgFactorMin);
             const uint8_t* const valid = P.valid + (int64_t)w.b.si * P.max_tiles + tile0;
             uint32_t units = tiles > 0 ? valid[0] : 0;
             float m_used = -INFINITY, lsum = 0.f;    // what this row scales by (log2), this half's denominator

@@ -106,3 +106,14 @@ def test_logits_of_any_magnitude(dtype, size, rows, form):
     q = (size * torch.randn(rows, 8, 128, generator=gen)).to(dtype)
     out, lse = _attend(q, pages, table, t, form, rows)
     W.check(out, lse, W.attention(q, pages.cpu(), slots, [t - rows + 1 + i for i in range(rows)], SCALE, apart=True), slice(0, rows))
+
+
+def test_a_scale_whose_product_with_a_power_of_two_vanishes(form):
+    """bf16 queries of 2^-130 are brought up by 2^140, which goes out of the scale again: of 1e-30 nothing is left, and every token weighs the same."""
+    gen = torch.Generator().manual_seed(78)
+    t, rows = 300, 5
+    k, v = (torch.randn(t, 2, 128, generator=gen).bfloat16() for _ in range(2))
+    pages, table, slots = _pages(k, v)
+    q = (2.0 ** -130 * torch.randn(rows, 8, 128, generator=gen)).bfloat16()
+    out, lse = _attend(q, pages, table, t, form, rows, scale=1e-30)
+    W.check(out, lse, W.attention(q, pages.cpu(), slots, [t - rows + 1 + i for i in range(rows)], 1e-30), slice(0, rows))
