@@ -18,6 +18,7 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.environ.get("BGTQ_LIB") or os.path.join(PKG, "libbgtq.so")
 NATIVE_SRC = os.path.join(CSRC, "bgtq_native.cpp")
+NATIVE_ROWS = os.path.join(CSRC, "bgtq_paged_rows.h")
 NATIVE = os.path.join(PKG, "_native.so")
 NATIVE_STAMP = os.path.join(PKG, "build", "native.abi")         # the versions it was built for
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -53,7 +54,7 @@ def needs_build() -> bool:
     except OSError:
         pass            # (the module says it itself when it is loaded)
     header = os.path.join(os.path.dirname(PKG), "include", "bgtq.h")
-    if os.path.getmtime(NATIVE) < max(os.path.getmtime(NATIVE_SRC), os.path.getmtime(header)):
+    if os.path.getmtime(NATIVE) < max(os.path.getmtime(f) for f in (NATIVE_SRC, NATIVE_ROWS, header)):
         return True
     t = os.path.getmtime(LIB)
     deps = sources() + glob.glob(os.path.join(CSRC, "*.h")) + glob.glob(os.path.join(CSRC, "*.cuh")) + \

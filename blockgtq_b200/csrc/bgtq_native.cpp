@@ -16,6 +16,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/bgtq.h"
+#include "bgtq_paged_rows.h"
 
 namespace {
 
@@ -405,8 +406,9 @@ PyObject* paged_attend(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     if (m < 1 || n_seq < 1 || n_seq > INT32_MAX || n_q < 1 || n_q % n_kv || n_q / n_kv > 8 || cap > INT32_MAX || !vec_ok(lens, at::kInt, n_seq) ||
         (cu ? !vec_ok(cu, at::kInt, n_seq + 1) : m != n_seq) || max_q < 1 || max_q > INT32_MAX || scale != scale)
         return none();
-    if (given && (!rows_ok(given, q->scalar_type(), 8) || given->sizes() != q->sizes() || given->data_ptr() == q->data_ptr() ||
-                  (m > 1 && given->stride(0) < kHD) || (n_q > 1 && given->stride(1) < kHD)))
+    auto rows = [&](const at::Tensor& x) { return bgtq::PagedRows{reinterpret_cast<uintptr_t>(x.data_ptr()), m, n_q, x.stride(0), x.stride(1)}; };
+    if (given && (!rows_ok(given, q->scalar_type(), 8) || given->sizes() != q->sizes() || !bgtq::paged_rows_apart(rows(*given)) ||
+                  !bgtq::paged_rows_apart(rows(*q), rows(*given))))
         return none();
     if (most < 0 || most > cap) most = cap;
     if (q->scalar_type() == at::kBFloat16) flags |= BGTQ_PAGED_BF16;

@@ -33,6 +33,7 @@
 // one's states are merged in shared memory).
 #include "bgtq_paged_common.cuh"
 #include "bgtq_paged_prefill.h"
+#include "bgtq_paged_rows.h"
 
 #include <limits.h>
 
@@ -1022,6 +1023,9 @@ extern "C" __attribute__((visibility("default"))) int bgtq_paged_attend(
     if (!aligned(pages, 16) || page_stride % 16 || head_stride % 16 || !aligned(q, 16) || q_st % 8 || q_sh % 8 || !aligned(out, 8) || o_st % 4 ||
         o_sh % 4 || !aligned(workspace, 16))
         return BGTQ_E_ALIGN;
+    // CTAs write rows while others read their queries
+    const PagedRows q_rows{reinterpret_cast<uintptr_t>(q), n_tok, n_q, q_st, q_sh}, o_rows{reinterpret_cast<uintptr_t>(out), n_tok, n_q, o_st, o_sh};
+    if (!paged_rows_apart(o_rows) || !paged_rows_apart(q_rows, o_rows)) return BGTQ_E_BADARG;
     PdForm f = pd_form(n_seq, n_tok, n_q, n_kv, max_q, max_tokens, flags);
     const cudaStream_t st = (cudaStream_t)stream;
     if (f.prefill) {

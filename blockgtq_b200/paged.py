@@ -67,6 +67,25 @@ def _ints(x, name, dtype, shape, device):
     return x.contiguous()
 
 
+def _spans(x):
+    """(rows, bytes from one to the next, bytes of all of them) along the two outer dimensions of rows (n, heads, 128) of 16 bits."""
+    return [(n, 2 * st, (max(n, 1) - 1) * 2 * st + 2 * HD) for n, st in zip(x.shape, x.stride()[:2])]
+
+
+def _rows_apart(x):
+    """The rows of x do not overlap one another: those along the smaller stride fit into a step of the larger."""
+    near, far = sorted(_spans(x), key=lambda d: (d[0] > 1, d[1]))
+    return (near[0] <= 1 or near[1] >= 2 * HD) and (far[0] <= 1 or far[1] >= near[2])
+
+
+def _rows_clear(x, y):
+    """The rows of y, of x's shape, are elsewhere, or between those of x with the same stride."""
+    a, b, at = _spans(x), _spans(y), y.data_ptr() - x.data_ptr()
+    if at >= a[0][2] + a[1][2] - 2 * HD or -at >= b[0][2] + b[1][2] - 2 * HD:
+        return True
+    return any(n > 1 and step > 0 and step == b[i][1] and a[1 - i][2] <= at % step <= step - b[1 - i][2] for i, (n, step, _) in enumerate(a))
+
+
 def _status(status, device):
     if status is not None and (status.dtype != torch.int32 or status.numel() < 1 or status.device != device):
         raise ValueError("status must be an int32 tensor on the pages' device")
@@ -179,7 +198,7 @@ def _attend_any(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, flags,
     page = _pool(pages)
     dev, n_kv = pages.device, pages.shape[1]
     flags |= _type_flag(q.dtype, "q")
-    q = _rows(q, "q", None, None, q.dtype, dev, 16)
+    given, q = q, _rows(q, "q", None, None, q.dtype, dev, 16)
     n, n_q = q.shape[:2]
     if n_q < 1 or n_q % n_kv or n_q // n_kv > 8:
         raise ValueError(f"{n_q} query heads over {n_kv} KV heads: a KV head takes 1 to 8 of them")
@@ -199,7 +218,7 @@ def _attend_any(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, flags,
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1 or out.stride(0) % 4 or out.stride(1) % 4 \
             or out.data_ptr() % 8:
         raise ValueError("out must be like q, with rows of 8-byte alignment")
-    elif out.data_ptr() == q.data_ptr() or any(st < HD and k > 1 for st, k in zip(out.stride(), out.shape[:2])):
+    elif not _rows_apart(out) or not _rows_clear(given, out):
         raise ValueError("out must have rows of its own, apart from one another and from q")
     lse = torch.empty(n, n_q, dtype=torch.float32, device=dev) if return_lse else None
     cap = block_table.shape[1] * page
@@ -230,7 +249,8 @@ def paged_kv4_decode_attention(q, pages, block_table, seq_lens, scale=None, retu
     ``block_table`` (B, pages per sequence) int32 and ``seq_lens`` (B,) int32: token t of sequence b lies in page ``block_table[b, t // page
     size]``; entries behind the sequence's end are not read.  A sequence without tokens gives zeros and -inf.  Query heads
     h * n_q / n_kv .. share KV head h, at most 8 of them.  ``max_seq_len``: sequences are held to it (default: what the table holds);
-    a small one spares the launch what only long sequences need.  ``out``: where the result goes, like q but not q itself."""
+    a small one spares the launch what only long sequences need.  ``out``: where the result goes, like q, its rows apart from one
+    another and from q's (other columns of one buffer will do)."""
     return _attend(q, pages, block_table, seq_lens, None, 1, _most(max_seq_len), True, scale, return_lse, status, out)
 
 

@@ -650,8 +650,8 @@ int bgtq_paged_read(const uint8_t* pages, int64_t page_stride, int64_t head_stri
  * token t of sequence b lies in page table[b * table_stride + t / page_tokens].  cu_q NULL: row b of q (n_seq, n_q, 128) is sequence b's
  * one query, n_tok = n_seq.  Otherwise rows cu_q[b] .. cu_q[b + 1] - 1 of q (n_tok, n_q, 128) are its last positions, and with
  * BGTQ_PAGED_CAUSAL row i of n sees the first seq_lens[b] - n + 1 + i tokens.  A row that sees none is zeros, its lse -inf; rows
- * behind cu_q[n_seq] are left as they were.  lse (optional, (n_tok, n_q) fp32): natural logarithm of the sum of exponentials.
- * n_q / n_kv <= 8.  max_tokens: sequences are held to it as to the table's capacity.  max_q: no sequence has more rows (it chooses the
+ * behind cu_q[n_seq] are left as they were.  out's rows do not overlap one another nor q's: elsewhere, or columns of one buffer with q's
+ * stride.  lse (optional, (n_tok, n_q) fp32): natural logarithm of the sum of exponentials.  n_q / n_kv <= 8.  max_tokens: sequences are held to it as to the table's capacity.  max_q: no sequence has more rows (it chooses the
  * launch; one that has is still attended whole).  Both decide how the work is cut, and so the order of sums.  workspace:
  * bgtq_paged_workspace_bytes(...) of the same arguments, 16-byte aligned, of no other call that may run at the same time; for many
  * rows it holds the sequences' tokens in fp16, 512 bytes per token of max_tokens and KV head, at most 2 GiB (or one sequence's and

@@ -1,0 +1,43 @@
+"""GPU: calls of the paged cache's operators as a program makes them: results in buffers of its own, other streams, counted launches."""
+import math
+
+import pytest
+import torch
+
+import paged_bounds as W
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+I32 = dict(dtype=torch.int32, device=DEV)
+
+
+def _sequence(gen, t, n_kv=2, page=16):
+    """Pages in order that hold t random tokens, their table and slots."""
+    from blockgtq_b200 import page_bytes, paged_kv4_append
+    width = -(-t // page)
+    pages = torch.zeros(width, n_kv, page_bytes(page), dtype=torch.uint8, device=DEV)
+    k, v = (torch.randn(t, n_kv, 128, generator=gen).half().to(DEV) for _ in range(2))
+    slots = torch.arange(t)
+    paged_kv4_append(pages, slots.to(DEV), k, v)
+    return pages, torch.arange(width, **I32)[None], slots
+
+
+@pytest.mark.parametrize("rows", [6, 100])
+def test_a_result_in_other_columns_of_the_queries_buffer(rows):
+    from blockgtq_b200 import paged_kv4_prefill_attention
+    gen = torch.Generator().manual_seed(rows)
+    pages, table, _ = _sequence(gen, 300)
+    buffer = torch.randn(rows, 12, 128, generator=gen).half().to(DEV)
+    q, out, rest = buffer[:, 4:8], buffer[:, 8:], buffer[:, :4].clone()
+    args = (pages, table, torch.tensor([300], **I32), torch.tensor([0, rows], **I32))
+    want, before = paged_kv4_prefill_attention(q, *args), q.clone()
+    assert paged_kv4_prefill_attention(q, *args, out=out) is out
+    assert torch.equal(out, want) and torch.equal(q, before) and torch.equal(buffer[:, :4], rest)
+    outer = torch.empty(4, rows, 128, dtype=torch.float16, device=DEV).transpose(0, 1)
+    assert torch.equal(paged_kv4_prefill_attention(q, *args, out=outer), want)
+    wide = torch.zeros(rows + 1, 4, 128, dtype=torch.float16, device=DEV)
+    for bad in (buffer[:, 6:10], buffer[:, 4:8], wide.as_strided((rows, 4, 128), (128, 128, 1))):
+        with pytest.raises(ValueError, match="of its own"):
+            paged_kv4_prefill_attention(q, *args, out=bad)
+    with pytest.raises(ValueError, match="of its own"):
+        paged_kv4_prefill_attention(wide[1:], *args, out=wide[:-1])
