@@ -359,7 +359,11 @@ class PagedKV4Cache:
         table = torch.tensor([r + [0] * (width - len(r)) for r in rows], dtype=torch.int32).to(self.device)
         small = torch.tensor(lens + ends, dtype=torch.int32).to(self.device)
         self._step = {"slots": wide[0], "positions": wide[1], "table": table, "lens": small[:len(seqs)], "ends": small[len(seqs):],
-                      "most_q": max(counts), "most": max(lens), "rows": len(slots), "seqs": frozenset(seqs)}
+                      "most_q": max(counts), "most": max(lens), "rows": len(slots), "seqs": frozenset(seqs),
+                      "held": (wide, table, small), "streams": {self._stream()}}
+
+    def _stream(self):
+        return torch.cuda.current_stream(self.device) if self.device.type == "cuda" else None
 
     @torch.no_grad()
     def append_and_attend(self, layer_idx, q, k, v, rope=None):
@@ -370,6 +374,11 @@ class PagedKV4Cache:
         s, pages = self._step, self.pages[layer_idx]
         if q.shape != (s["rows"], self.nq, HD):
             raise ValueError(f"q must be ({s['rows']}, {self.nq}, {HD}), the step's tokens, got {tuple(q.shape)}")
+        stream = self._stream()
+        if stream not in s["streams"]:      # (the next step's tensors must not take these tensors' memory before this stream is done with them)
+            for t in s["held"]:
+                t.record_stream(stream)
+            s["streams"].add(stream)
         if rope is None:
             paged_kv4_append(pages, s["slots"], k, v, status=self.status)
         else:

@@ -41,3 +41,30 @@ def test_a_result_in_other_columns_of_the_queries_buffer(rows):
             paged_kv4_prefill_attention(q, *args, out=bad)
     with pytest.raises(ValueError, match="of its own"):
         paged_kv4_prefill_attention(wide[1:], *args, out=wide[:-1])
+
+
+def test_a_step_on_another_stream_keeps_what_it_reads():
+    """The step's slots, table and lengths belong to the stream that began it; the layers run late, on another."""
+    from blockgtq_b200 import PagedKV4Cache
+    gen = torch.Generator().manual_seed(61)
+    caches = [PagedKV4Cache(1, 4, 2, n_pages=40, max_seq_len=200, page_size=16, device=DEV) for _ in range(2)]
+    tokens = [[torch.randn(n, h, 128, generator=gen).half().to(DEV) for h in (4, 2, 2)] for n in (50, 2, 2, 2)]
+    side, got = torch.cuda.Stream(DEV), ([], [])
+    torch.cuda.synchronize()
+    for cache, results, late in zip(caches, got, (False, True)):
+        a, b = cache.add_sequence(), cache.add_sequence()
+        for rows, counts in zip(tokens, ([30, 20], [1, 1], [1, 1], [1, 1])):
+            cache.begin_step([a, b], counts)
+            if late:
+                with torch.cuda.stream(side):
+                    torch.cuda._sleep(20_000_000)
+                    results.append(cache.append_and_attend(0, *rows))
+            else:
+                results.append(cache.append_and_attend(0, *rows))
+            cache.free_sequence(cache.add_sequence())
+            junk = [torch.full((1 << k,), 7, **I32) for k in range(3, 9)]         # takes what has been given back
+            del junk
+        torch.cuda.synchronize()
+        cache.check_status()
+    assert all(torch.equal(x, y) for x, y in zip(*got))
+    assert torch.equal(caches[0].pages, caches[1].pages)
