@@ -343,21 +343,26 @@ class PagedKV4Cache:
             need.append(-(-(t + c) // self.page_size) - len(held))
         if sum(need) > len(self._free):
             raise RuntimeError(f"{sum(need)} pages needed, {len(self._free)} free")
+        free = len(self._free)              # pages are taken from the end
         slots, positions, lens, ends, rows = [], [], [], [0], []
         for i, c, n in zip(seqs, counts, need):
-            s = self._seqs[i]
-            s[1].extend(self._free.pop() for _ in range(n))
-            at = range(s[0], s[0] + c)
+            t, held = self._seqs[i]
+            pages = held + [self._free[free - 1 - k] for k in range(n)]
+            free -= n
+            at = range(t, t + c)
             positions.extend(at)
-            slots.extend(s[1][t // self.page_size] * self.page_size + t % self.page_size for t in at)
-            s[0] += c
-            lens.append(s[0])
+            slots.extend(pages[t // self.page_size] * self.page_size + t % self.page_size for t in at)
+            lens.append(t + c)
             ends.append(ends[-1] + c)
-            rows.append(s[1])
+            rows.append(pages)
         width = max(len(r) for r in rows)
         wide = torch.tensor([slots, positions], dtype=torch.int64).to(self.device)
         table = torch.tensor([r + [0] * (width - len(r)) for r in rows], dtype=torch.int32).to(self.device)
         small = torch.tensor(lens + ends, dtype=torch.int32).to(self.device)
+        # (from here on nothing fails: a device without memory for the step leaves the sequences as they were)
+        for i, t, pages in zip(seqs, lens, rows):
+            self._seqs[i] = [t, pages]
+        del self._free[free:]
         self._step = {"slots": wide[0], "positions": wide[1], "table": table, "lens": small[:len(seqs)], "ends": small[len(seqs):],
                       "most_q": max(counts), "most": max(lens), "rows": len(slots), "seqs": frozenset(seqs),
                       "held": (wide, table, small), "streams": {self._stream()}}
