@@ -379,6 +379,9 @@ class PagedKV4Cache:
         s, pages = self._step, self.pages[layer_idx]
         if q.shape != (s["rows"], self.nq, HD):
             raise ValueError(f"q must be ({s['rows']}, {self.nq}, {HD}), the step's tokens, got {tuple(q.shape)}")
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a captured graph would go on reading this step's slots and lengths, which end with the step: capture "
+                               "paged_kv4_append and the attentions over tensors of your own")
         stream = self._stream()
         if stream not in s["streams"]:      # (the next step's tensors must not take these tensors' memory before this stream is done with them)
             for t in s["held"]:

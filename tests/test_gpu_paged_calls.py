@@ -68,3 +68,20 @@ def test_a_step_on_another_stream_keeps_what_it_reads():
         cache.check_status()
     assert all(torch.equal(x, y) for x, y in zip(*got))
     assert torch.equal(caches[0].pages, caches[1].pages)
+
+
+def test_a_step_is_not_captured():
+    """Replayed behind its step, the graph would store tokens in pages that are another sequence's by then."""
+    from blockgtq_b200 import PagedKV4Cache
+    cache = PagedKV4Cache(1, 4, 2, n_pages=4, max_seq_len=60, page_size=16, device=DEV)
+    cache.begin_step([cache.add_sequence()], [3])
+    q, kv = torch.ones(3, 4, 128, dtype=torch.float16, device=DEV), torch.ones(3, 2, 128, dtype=torch.float16, device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="capture"):
+            cache.append_and_attend(0, q, kv, kv)
+    assert not cache.pages.any()
+    cache.append_and_attend(0, q, kv, kv)
+    assert cache.pages.any()
+    cache.check_status()
