@@ -340,7 +340,9 @@ PyObject* paged_append(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     if (bad || !pool_ok(pages) || !half_type(k) || !rows_ok(k, k->scalar_type(), 16) || !rows_ok(v, k->scalar_type(), 16) || !status_ok(status))
         return none();
     const int64_t m = k->size(0), n_kv = pages->size(1);
-    if (k->size(1) != n_kv || v->size(0) != m || v->size(1) != n_kv || !vec_ok(slots, at::kLong, m)) return none();
+    if (k->size(1) != n_kv || v->size(0) != m || v->size(1) != n_kv || !vec_ok(slots, at::kLong, m) ||
+        !bgtq::paged_apart(pages->size(0), n_kv, pages->stride(0), pages->stride(1), pages->size(2)))
+        return none();
     if (!cs != !sn || !cs != !pos || (q && !cs)) return none();
     if (cs) {
         for (const at::Tensor* t : {cs, sn})

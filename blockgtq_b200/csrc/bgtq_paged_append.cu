@@ -5,6 +5,7 @@
 // [-7, 7].  The rotation is four fp32 products and two sums, none of them fused, and its result is quantised without another
 // rounding.  A group with a NaN gets a NaN scale; infinities and what lies beyond 65408 saturate.
 #include "bgtq_paged_common.cuh"
+#include "bgtq_paged_rows.h"
 
 namespace bgtq {
 namespace {
@@ -372,6 +373,7 @@ extern "C" __attribute__((visibility("default"))) int bgtq_paged_append(
     if (!aligned(k, 16) || !aligned(v, 16) || !aligned(q, 16) || !aligned(q_out, 16) || k_st % 8 || k_sh % 8 || v_st % 8 || v_sh % 8 ||
         q_st % 8 || q_sh % 8 || !aligned(rope_cos, 16) || !aligned(rope_sin, 16) || rope_st % 4)
         return BGTQ_E_ALIGN;
+    if (!paged_apart(n_pages, n_kv, page_stride, head_stride, (int64_t)page_tokens / kUnitTok * kUnitBytes)) return BGTQ_E_BADARG;
     // Few rows: as many warps as there are, two rows each and eight lanes to a row (32 tokens of 32 query and 8 KV heads 2.8 us, 3.0 with four).
     // Otherwise four rows and four lanes to a row (4096 tokens 3 us less, measured before the ring), as many chunks one behind the other as leave the SMs
     // one round of resident warps (6 of 12 per warp: 2 us more).

@@ -1,9 +1,10 @@
-// Whether rows of 128 elements of 16 bits, (n, h) of them at strides in elements, lie apart.
+// Whether what a call writes lies apart from itself and from what the call reads.
 #pragma once
 #include <stdint.h>
 
 namespace bgtq {
 
+// Rows of 128 elements of 16 bits, (n, h) of them at strides in elements.
 struct PagedRows {
     uintptr_t at;
     int64_t n, h, st, sh;
@@ -12,12 +13,15 @@ struct PagedRows {
     int64_t span(int dim) const { return along(dim) > 1 ? (along(dim) - 1) * bytes(dim) + 256 : 256; }      // of the rows along one dimension
 };
 
-// from one another: the rows of the dimension with the smaller stride fit between two steps of the other
-inline bool paged_rows_apart(const PagedRows& x) {
-    const int near = x.n > 1 && (x.h <= 1 || x.st < x.sh) ? 0 : 1;
-    return (x.along(near) <= 1 || x.bytes(near) >= 256) && (x.along(1 - near) <= 1 || x.bytes(1 - near) >= x.span(near));
+// Places of `row` bytes, (n, h) of them at strides st and sh in bytes, do not overlap one another: those along the smaller stride fit into a step of
+// the larger.
+inline bool paged_apart(int64_t n, int64_t h, int64_t st, int64_t sh, int64_t row) {
+    const bool rows_near = n > 1 && (h <= 1 || st < sh);
+    const int64_t near_n = rows_near ? n : h, near_st = rows_near ? st : sh, far_n = rows_near ? h : n, far_st = rows_near ? sh : st;
+    return (near_n <= 1 || near_st >= row) && (far_n <= 1 || far_st >= (near_n > 1 ? (near_n - 1) * near_st : 0) + row);
 }
-// from those of another tensor of this shape: elsewhere, or between its rows, both with the same stride along one dimension
+inline bool paged_rows_apart(const PagedRows& x) { return paged_apart(x.n, x.h, x.bytes(0), x.bytes(1), 256); }
+// The rows of two tensors of one shape lie apart: elsewhere, or between its rows, both with the same stride along one dimension
 inline bool paged_rows_apart(const PagedRows& x, const PagedRows& y) {
     auto end = [](const PagedRows& r) { return r.at + (uintptr_t)(r.span(0) + r.span(1) - 256); };
     if (end(x) <= y.at || end(y) <= x.at) return true;

@@ -68,14 +68,16 @@ def _ints(x, name, dtype, shape, device):
 
 
 def _spans(x):
-    """(rows, bytes from one to the next, bytes of all of them) along the two outer dimensions of rows (n, heads, 128) of 16 bits."""
-    return [(n, 2 * st, (max(n, 1) - 1) * 2 * st + 2 * HD) for n, st in zip(x.shape, x.stride()[:2])]
+    """(places, bytes from one to the next, bytes of all of them) along the two outer dimensions of x."""
+    row = x.shape[2] * x.element_size()
+    return [(n, x.element_size() * st, (max(n, 1) - 1) * x.element_size() * st + row) for n, st in zip(x.shape, x.stride()[:2])]
 
 
-def _rows_apart(x):
-    """The rows of x do not overlap one another: those along the smaller stride fit into a step of the larger."""
+def _apart(x):
+    """The places (i, j) of x do not overlap one another: those along the smaller stride fit into a step of the larger."""
     near, far = sorted(_spans(x), key=lambda d: (d[0] > 1, d[1]))
-    return (near[0] <= 1 or near[1] >= 2 * HD) and (far[0] <= 1 or far[1] >= near[2])
+    row = x.shape[2] * x.element_size()
+    return (near[0] <= 1 or near[1] >= row) and (far[0] <= 1 or far[1] >= near[2])
 
 
 def _rows_clear(x, y):
@@ -117,6 +119,8 @@ def _append(pages, slots, k, v, q, cos, sin, positions, status):
     """:func:`paged_kv4_append` for what the extension module leaves: tensors that have to be copied, and errors."""
     page = _pool(pages)
     dev, n_kv = pages.device, pages.shape[1]
+    if not _apart(pages):
+        raise ValueError("tokens are stored in pages of their own, apart from one another")
     flags = _type_flag(k.dtype, "k")
     k = _rows(k, "k", None, n_kv, k.dtype, dev, 16)
     n = k.shape[0]
@@ -218,7 +222,7 @@ def _attend_any(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, flags,
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1 or out.stride(0) % 4 or out.stride(1) % 4 \
             or out.data_ptr() % 8:
         raise ValueError("out must be like q, with rows of 8-byte alignment")
-    elif not _rows_apart(out) or not _rows_clear(given, out):
+    elif not _apart(out) or not _rows_clear(given, out):
         raise ValueError("out must have rows of its own, apart from one another and from q")
     lse = torch.empty(n, n_q, dtype=torch.float32, device=dev) if return_lse else None
     cap = block_table.shape[1] * page

@@ -630,7 +630,8 @@ int bgtq_decode_combined_noalloc(const BgtqDecodePlan* plan_host, const BgtqHead
                                    * merges; 14 << 8: with cu_q, tcgen05 over a workspace of unpacked tiles (many rows) */
 
 /* Quantise and store n_tok tokens.  k / v element (i, h, d) at k + i * k_st + h * k_sh + d (strides multiples of 8 elements, 16-byte
- * aligned); token i goes to slot slots[i], nowhere when that is negative; the slots of a call are distinct.  rope_cos / rope_sin (may both
+ * aligned); token i goes to slot slots[i], nowhere when that is negative; the slots of a call are distinct, and the pages' strides leave every
+ * page and head a place of its own.  rope_cos / rope_sin (may both
  * be NULL): fp32 tables, row p at + p * rope_st (a multiple of 4), 64 entries; dims d and d + 64 of k, and of q, are turned by row
  * positions[i] in fp32: x' = x cos - y sin, y' = y cos + x sin, nothing fused, K quantised from the fp32 result.  q (NULL and n_q = 0 to
  * leave it out; needs the tables): rotated queries, rounded once, to q_out (n_tok, n_q, 128) contiguous.

@@ -74,3 +74,24 @@ def test_one_token_or_one_head_has_no_stride():
         with pytest.raises(RuntimeError, match="CUDA"):
             paged_kv4_decode_attention(q, torch.zeros(3, h, page_bytes(32), dtype=torch.uint8), torch.zeros(n, 1, dtype=torch.int32),
                                        torch.ones(n, dtype=torch.int32), out=out)
+
+
+def test_pages_that_share_memory_are_not_written():
+    """Read they may be: a head's pages for all heads, for instance."""
+    from blockgtq_b200 import paged_kv4_append, paged_kv4_read
+    k, slots = torch.zeros(4, 2, ROW, dtype=torch.float16), torch.arange(4)
+    pool = torch.zeros(6, 2, page_bytes(32), dtype=torch.uint8)
+    b = page_bytes(32)
+    for pages in (pool, pool.transpose(0, 1).contiguous().transpose(0, 1), pool[::2], pool[:1], torch.zeros(2, 6, 2, b, dtype=torch.uint8)[1]):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            paged_kv4_append(pages, slots, k, k)
+    for pages in (pool[:, :1].expand(6, 2, b), pool[:1].expand(6, 2, b), pool.as_strided((3, 2, b), (b, b, 1)), pool.as_strided((3, 2, b), (2 * b, 2304, 1))):
+        with pytest.raises(ValueError, match="of their own"):
+            paged_kv4_append(pages, slots, k, k)
+        with pytest.raises(RuntimeError, match="CUDA"):
+            paged_kv4_read(pages, slots)
+    raw = C.create_string_buffer(65536)
+    p = (C.addressof(raw) + 255) & ~255
+    for page_stride, head_stride in ((4608, 0), (0, 2304), (2304, 2304), (4608, 16)):
+        rc = _lib.lib().bgtq_paged_append(p, page_stride, head_stride, 3, 16, p, p, 256, 128, p, 256, 128, 0, 0, 0, 0, 0, 0, 0, 0, 0, 1, 2, 0, 0, 0, 0)
+        assert rc == -1
