@@ -405,7 +405,7 @@ extern "C" __attribute__((visibility("default"))) int bgtq_paged_read(
     if (!aligned(k, 16) || !aligned(v, 16)) return BGTQ_E_ALIGN;
     RdParams P{{pages, page_stride, head_stride, n_pages, page_tokens / kUnitTok}, slots, k, v, n_tok, n_kv, status};
     const int64_t blocks = ((int64_t)n_tok * 2 * n_kv * 4 + 255) / 256;
-    if (blocks * 64 > INT32_MAX) return BGTQ_E_TOOBIG;
+    if (blocks * 256 > 1ll << 32) return BGTQ_E_TOOBIG;          // (threads are counted in 32 bits)
     const auto kernel = (flags & BGTQ_PAGED_F32) ? pg_read_kernel<float> : (flags & BGTQ_PAGED_BF16) ? pg_read_kernel<__nv_bfloat16> : pg_read_kernel<__half>;
     return launch_kernel(kernel, dim3((unsigned)blocks), dim3(256), 0, (cudaStream_t)stream, true, P) == cudaSuccess ? BGTQ_OK : BGTQ_E_LAUNCH;
 }

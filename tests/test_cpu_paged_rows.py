@@ -95,3 +95,11 @@ def test_pages_that_share_memory_are_not_written():
     for page_stride, head_stride in ((4608, 0), (0, 2304), (2304, 2304), (4608, 16)):
         rc = _lib.lib().bgtq_paged_append(p, page_stride, head_stride, 3, 16, p, p, 256, 128, p, 256, 128, 0, 0, 0, 0, 0, 0, 0, 0, 0, 1, 2, 0, 0, 0, 0)
         assert rc == -1
+
+
+@pytest.mark.parametrize("n,n_kv", [(1 << 28, 3), ((1 << 29) + 32, 1), (1 << 30, 1)])
+def test_reading_counts_its_rows_in_32_bits(n, n_kv):
+    """Four lanes to each of 2 n n_kv rows: beyond what 32 bits hold."""
+    raw = C.create_string_buffer(4096)
+    p = (C.addressof(raw) + 255) & ~255
+    assert _lib.lib().bgtq_paged_read(p, 2304 * n_kv, 2304, 1, 16, p, n, n_kv, p, p, 0, 0, 0) == -5
