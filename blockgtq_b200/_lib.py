@@ -149,6 +149,7 @@ _SIGNATURES = {
     "bgtq_paged_append": (C.c_int, [_vp, _i64, _i64, _i32, _i32, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp,
                                     _vp, _vp, _i64, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp]),
     "bgtq_paged_read": (C.c_int, [_vp, _i64, _i64, _i32, _i32, _vp, _i32, _i32, _vp, _vp, _i32, _vp, _vp]),
+    "bgtq_paged_launches": (C.c_int, []),
     "bgtq_paged_workspace_bytes": (C.c_int64, [_i32, _i32, _i32, _i32, _i32, _i64, _i32]),
     "bgtq_paged_attend": (C.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _i32, _i32, _vp, _i64, _i32, _vp, _vp, _i32, _i32, _i32, _i32,
                                     _i32, _i64, _f32, _i32, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp]),
@@ -200,7 +201,8 @@ def lib():
 
     module.bind(*addresses("bgtq_layer_step", "bgtq_layer_encode", "bgtq_attend", "bgtq_decode_default_splits", "bgtq_encode",
                            "bgtq_rotate_q_rows", "bgtq_prefill", "bgtq_prefill_workspace_bytes"))
-    module.bind_paged(*addresses("bgtq_paged_append", "bgtq_paged_read", "bgtq_paged_attend", "bgtq_paged_workspace_bytes"))
+    module.bind_paged(*addresses("bgtq_paged_append", "bgtq_paged_read", "bgtq_paged_attend", "bgtq_paged_workspace_bytes",
+                                 "bgtq_paged_launches"))
     native = module
     _lib = handle
     return _lib

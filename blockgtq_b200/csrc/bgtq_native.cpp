@@ -37,6 +37,7 @@ struct PagedFns {
     decltype(&bgtq_paged_read) paged_read;
     decltype(&bgtq_paged_attend) paged_attend;
     decltype(&bgtq_paged_workspace_bytes) paged_workspace;
+    decltype(&bgtq_paged_launches) paged_launches;
 } G;
 
 PyObject* none() { Py_RETURN_NONE; }
@@ -433,6 +434,9 @@ PyObject* paged_attend(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     return want_lse ? Py_BuildValue("(NN)", o, wrap(std::move(lse))) : o;
 }
 
+// paged_launched() -> kernels that this thread's last call above enqueued
+PyObject* paged_launched(PyObject*, PyObject* const*, Py_ssize_t) { return code(G.paged_launches()); }
+
 template <typename T>
 PyObject* bind_to(T& fns, PyObject* const* argv, Py_ssize_t n) {
     constexpr Py_ssize_t count = sizeof(T) / sizeof(void*);
@@ -471,7 +475,7 @@ PyObject* guarded(PyObject* self, PyObject* const* argv, Py_ssize_t n) {
 #define BGTQ_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<name>)), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {BGTQ_METHOD(bind),   BGTQ_METHOD(layer_step),  BGTQ_METHOD(layer_encode), BGTQ_METHOD(encode), BGTQ_METHOD(compress),
                           BGTQ_METHOD(attend), BGTQ_METHOD(rotate_rows), BGTQ_METHOD(prefill),      BGTQ_METHOD(paged_append), BGTQ_METHOD(paged_read),
-                          BGTQ_METHOD(paged_attend), BGTQ_METHOD(bind_paged), {nullptr, nullptr, 0, nullptr}};
+                          BGTQ_METHOD(paged_attend), BGTQ_METHOD(paged_launched), BGTQ_METHOD(bind_paged), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

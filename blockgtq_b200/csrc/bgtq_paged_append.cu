@@ -359,11 +359,14 @@ int check_pool(const void* pages, int64_t page_stride, int64_t head_stride, int3
 
 using namespace bgtq;
 
+extern "C" __attribute__((visibility("default"))) int bgtq_paged_launches(void) { return pg_launched; }
+
 extern "C" __attribute__((visibility("default"))) int bgtq_paged_append(
     uint8_t* pages, int64_t page_stride, int64_t head_stride, int32_t n_pages, int32_t page_tokens, const int64_t* slots, const void* k,
     int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, const void* q, int64_t q_st, int64_t q_sh, void* q_out,
     const float* rope_cos, const float* rope_sin, int64_t rope_st, const int64_t* positions, int32_t n_positions, int32_t n_tok,
     int32_t n_kv, int32_t n_q, int32_t flags, int32_t* status, void* stream) {
+    pg_launched = 0;
     if (n_tok < 0 || n_q < 0 || (flags & ~BGTQ_PAGED_BF16)) return BGTQ_E_BADARG;
     if (const int e = check_pool(pages, page_stride, head_stride, n_pages, page_tokens, n_kv)) return e;
     if (n_tok == 0) return BGTQ_OK;
@@ -391,13 +394,13 @@ extern "C" __attribute__((visibility("default"))) int bgtq_paged_append(
     const bool bf16 = flags & BGTQ_PAGED_BF16;
     const auto kernel = L == 8 ? bf16 ? pg_append_kernel<__nv_bfloat16, 8> : pg_append_kernel<__half, 8>
                                : bf16 ? pg_append_kernel<__nv_bfloat16, 4> : pg_append_kernel<__half, 4>;
-    return launch_kernel(kernel, dim3((unsigned)blocks), dim3(kApThreads), 0, (cudaStream_t)stream, true, P) == cudaSuccess ? BGTQ_OK
-                                                                                                                            : BGTQ_E_LAUNCH;
+    return pg_launch_ok(launch_kernel(kernel, dim3((unsigned)blocks), dim3(kApThreads), 0, (cudaStream_t)stream, true, P)) ? BGTQ_OK : BGTQ_E_LAUNCH;
 }
 
 extern "C" __attribute__((visibility("default"))) int bgtq_paged_read(
     const uint8_t* pages, int64_t page_stride, int64_t head_stride, int32_t n_pages, int32_t page_tokens, const int64_t* slots,
     int32_t n_tok, int32_t n_kv, void* k, void* v, int32_t flags, int32_t* status, void* stream) {
+    pg_launched = 0;
     if (n_tok < 0 || (flags & ~(BGTQ_PAGED_BF16 | BGTQ_PAGED_F32)) || flags == (BGTQ_PAGED_BF16 | BGTQ_PAGED_F32)) return BGTQ_E_BADARG;
     if (const int e = check_pool(pages, page_stride, head_stride, n_pages, page_tokens, n_kv)) return e;
     if (n_tok == 0) return BGTQ_OK;
@@ -407,5 +410,5 @@ extern "C" __attribute__((visibility("default"))) int bgtq_paged_read(
     const int64_t blocks = ((int64_t)n_tok * 2 * n_kv * 4 + 255) / 256;
     if (blocks * 256 > 1ll << 32) return BGTQ_E_TOOBIG;          // (threads are counted in 32 bits)
     const auto kernel = (flags & BGTQ_PAGED_F32) ? pg_read_kernel<float> : (flags & BGTQ_PAGED_BF16) ? pg_read_kernel<__nv_bfloat16> : pg_read_kernel<__half>;
-    return launch_kernel(kernel, dim3((unsigned)blocks), dim3(256), 0, (cudaStream_t)stream, true, P) == cudaSuccess ? BGTQ_OK : BGTQ_E_LAUNCH;
+    return pg_launch_ok(launch_kernel(kernel, dim3((unsigned)blocks), dim3(256), 0, (cudaStream_t)stream, true, P)) ? BGTQ_OK : BGTQ_E_LAUNCH;
 }

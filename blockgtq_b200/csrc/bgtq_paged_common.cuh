@@ -69,6 +69,13 @@ __device__ __forceinline__ void pg_pow2(int e, float& a, float& b) {
 // them at the smallest normal number either.)
 constexpr float kPgFactorMin = 1.17549435e-38f;
 
+// Kernels that this thread's last call of an entry point enqueued.
+inline thread_local int32_t pg_launched = 0;
+inline bool pg_launch_ok(cudaError_t e) {
+    pg_launched += e == cudaSuccess;
+    return e == cudaSuccess;
+}
+
 // Lets a kernel use this much dynamic shared memory, once per device.
 template <typename K>
 inline bool pg_allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {

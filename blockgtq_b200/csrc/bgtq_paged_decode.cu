@@ -880,7 +880,7 @@ int pd_launch_split(const PdParams& P, bool merge, cudaStream_t stream) {
     const auto kernel = pg_attend_kernel<NT, T, false, kStages>;
     static std::atomic<uint64_t> allowed{0};
     if (!pg_allow_smem(kernel, smem, allowed)) return BGTQ_E_LAUNCH;
-    if (launch_kernel(kernel, dim3(P.n_cta), dim3(kPdThreads), smem, stream, true, P) != cudaSuccess) return BGTQ_E_LAUNCH;
+    if (!pg_launch_ok(launch_kernel(kernel, dim3(P.n_cta), dim3(kPdThreads), smem, stream, true, P))) return BGTQ_E_LAUNCH;
     if (!merge) return BGTQ_OK;
     const int64_t triples = (int64_t)P.n_seq * P.n_kv;
     const bool by_triple = !P.cu_q && triples <= P.n_cta;
@@ -890,7 +890,7 @@ int pd_launch_split(const PdParams& P, bool merge, cudaStream_t stream) {
     const int warps = !by_triple || P.n_cta <= 4 * triples ? 2 : P.n_cta <= 16 * triples ? 8 : 16;
     const auto merging = !by_triple ? pg_merge_kernel<NT, T, false, 2>
                          : warps == 2 ? pg_merge_kernel<NT, T, true, 2> : warps == 8 ? pg_merge_kernel<NT, T, true, 8> : pg_merge_kernel<NT, T, true, 16>;
-    return launch_kernel(merging, grid, dim3(32 * warps), 0, stream, true, P) == cudaSuccess ? BGTQ_OK : BGTQ_E_LAUNCH;
+    return pg_launch_ok(launch_kernel(merging, grid, dim3(32 * warps), 0, stream, true, P)) ? BGTQ_OK : BGTQ_E_LAUNCH;
 }
 template <int NT, int kStages>
 struct ClusterLaunch {
@@ -918,7 +918,7 @@ int pd_launch_cluster(const PdParams& P, int64_t triples, int n_rank, cudaStream
     ClusterLaunch<NT, kStages> L(triples, n_rank, stream);
     static std::atomic<uint64_t> allowed{0};
     if (!pg_allow_smem(kernel, L.kBase + 8 * L.kRow, allowed)) return BGTQ_E_LAUNCH;
-    return cudaLaunchKernelEx(&L.cfg, kernel, P) == cudaSuccess && cudaGetLastError() == cudaSuccess ? BGTQ_OK : BGTQ_E_LAUNCH;
+    return pg_launch_ok(cudaLaunchKernelEx(&L.cfg, kernel, P)) && cudaGetLastError() == cudaSuccess ? BGTQ_OK : BGTQ_E_LAUNCH;
 }
 // Clusters of n_rank CTAs, each with an SM for itself, that the device runs at once (its groups of SMs are no multiples of eight).
 template <int NT, int kStages>
@@ -1008,6 +1008,7 @@ extern "C" __attribute__((visibility("default"))) int bgtq_paged_attend(
     int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv, int32_t max_q, int64_t max_tokens, float scale, int32_t flags,
     void* workspace, int64_t workspace_bytes, void* out, int64_t o_st, int64_t o_sh, float* lse, int32_t* status, void* stream) {
     const int asked = (flags & BGTQ_PAGED_FORM_MASK) >> BGTQ_PAGED_FORM_SHIFT;
+    pg_launched = 0;
     if (n_seq < 0 || n_tok < 0 || n_kv < 1 || n_q < 1 || table_cols < 0 || max_q < 1 || max_tokens < 0 ||
         (flags & ~(BGTQ_PAGED_BF16 | BGTQ_PAGED_CAUSAL | BGTQ_PAGED_FORM_MASK)) || (asked & (asked - 1) && asked < 14) || (asked == 14 && !cu_q) || asked == 13)
         return BGTQ_E_BADARG;

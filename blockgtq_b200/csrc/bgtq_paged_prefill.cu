@@ -978,9 +978,9 @@ int paged_prefill(const PagedPrefill& A, cudaStream_t stream) {
             P.max_blocks = (int32_t)blocks; P.n_cta = n_cta;
             P.q = A.q; P.q_st = A.q_st; P.q_sh = A.q_sh; P.scale_log2 = A.scale_log2;
             P.out = A.out; P.o_st = A.o_st; P.o_sh = A.o_sh; P.lse = A.lse; P.status = A.status;
-            if (launch_kernel(pg_unpack_kernel, dim3((unsigned)tiles + 1, nh, ns), dim3(256), 0, stream, true, P) != cudaSuccess) return BGTQ_E_LAUNCH;
-            if (launch_kernel(kernel, dim3(n_cta), dim3(kThreads), sizeof(PfSmem), stream, true, P) != cudaSuccess) return BGTQ_E_LAUNCH;
-            if (launch_kernel(merge, dim3(n_cta - 1, kBlockRows / (8 * kMergeRows)), dim3(256), 0, stream, true, P) != cudaSuccess) return BGTQ_E_LAUNCH;
+            if (!pg_launch_ok(launch_kernel(pg_unpack_kernel, dim3((unsigned)tiles + 1, nh, ns), dim3(256), 0, stream, true, P))) return BGTQ_E_LAUNCH;
+            if (!pg_launch_ok(launch_kernel(kernel, dim3(n_cta), dim3(kThreads), sizeof(PfSmem), stream, true, P))) return BGTQ_E_LAUNCH;
+            if (!pg_launch_ok(launch_kernel(merge, dim3(n_cta - 1, kBlockRows / (8 * kMergeRows)), dim3(256), 0, stream, true, P))) return BGTQ_E_LAUNCH;
         }
     return BGTQ_OK;
 }

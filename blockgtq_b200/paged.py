@@ -107,10 +107,11 @@ def paged_kv4_append(pages, slots, k, v, q=None, cos=None, sin=None, positions=N
     ``cos`` / ``sin`` (n_positions, 64) fp32 with ``positions`` (n,) int64: k, and ``q`` (n, n_q, 128), go through the rotary
     embedding first (dims d and d + 64 are a pair; fp32, k quantised from the unrounded result).  Returns the rotated q (n, n_q, 128),
     or None without one.  ``status``: optional int32 tensor, set to 2 where a slot or position is out of range (the token is not stored)."""
-    r = _lib.host().paged_append(pages, slots, k, v, q, cos, sin, positions, status)
+    host = _lib.host()
+    r = host.paged_append(pages, slots, k, v, q, cos, sin, positions, status)
     if r is None:
         return _append(pages, slots, k, v, q, cos, sin, positions, status)
-    _lib.done(r, "bgtq_paged_append")
+    _lib.done(r, "bgtq_paged_append", host.paged_launched())
     return None if q is None else r
 
 
@@ -155,7 +156,7 @@ def _append(pages, slots, k, v, q, cos, sin, positions, status):
             pages.data_ptr(), pages.stride(0), pages.stride(1), pages.shape[0], page, slots.data_ptr(), k.data_ptr(), *k.stride()[:2],
             v.data_ptr(), *v.stride()[:2], _lib.ptr(q), *qs, _lib.ptr(q_out) if q is not None else 0, *rope, n, n_kv, n_q, flags,
             status, _lib.stream_ptr(dev)), "bgtq_paged_append")
-    _lib.count_launch()
+    _lib.count_launch(_lib.lib().bgtq_paged_launches())
     return q_out
 
 
@@ -163,10 +164,11 @@ def paged_kv4_read(pages, slots, dtype=torch.float16, status=None):
     """The keys and values that the cache holds for ``slots`` (n,) int64: two tensors (n, n_kv, 128) of fp16 (exact), fp32
     (exact) or bf16.  A negative slot reads as zeros, and so does one out of range, with 2 in ``status``."""
     kind = _KINDS.get(dtype)
-    r = None if kind is None else _lib.host().paged_read(pages, slots, kind, status)
+    host = _lib.host()
+    r = None if kind is None else host.paged_read(pages, slots, kind, status)
     if r is None:
         return _read(pages, slots, dtype, status)
-    return _lib.done(r, "bgtq_paged_read")
+    return _lib.done(r, "bgtq_paged_read", host.paged_launched())
 
 
 @torch.no_grad()
@@ -183,17 +185,18 @@ def _read(pages, slots, dtype, status):
         _lib.check(_lib.lib().bgtq_paged_read(
             pages.data_ptr(), pages.stride(0), pages.stride(1), pages.shape[0], page, slots.data_ptr(), n, n_kv, k.data_ptr(), v.data_ptr(),
             _lib.PAGED_F32 if dtype == torch.float32 else _TYPES[dtype], status, _lib.stream_ptr(dev)), "bgtq_paged_read")
-    _lib.count_launch()
+    _lib.count_launch(_lib.lib().bgtq_paged_launches())
     return k, v
 
 
 def _attend(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, causal, scale, return_lse, status, out):
     scale = _SCALE if scale is None else float(scale)
     flags = (_lib.PAGED_CAUSAL if causal else 0) | _FORM << _lib.PAGED_FORM_SHIFT
-    r = _lib.host().paged_attend(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, scale, flags, return_lse, status, out)
+    host = _lib.host()
+    r = host.paged_attend(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, scale, flags, return_lse, status, out)
     if r is None:
         return _attend_any(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, flags, scale, return_lse, status, out)
-    return _lib.done(r, "bgtq_paged_attend", 2)
+    return _lib.done(r, "bgtq_paged_attend", host.paged_launched())
 
 
 @torch.no_grad()
@@ -242,7 +245,7 @@ def _attend_any(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, flags,
                 block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), _lib.ptr(cu_q), n_seq, n, n_q, n_kv,
                 max_q, max_tokens, scale, flags, ws.data_ptr(), need, out.data_ptr(), *out.stride()[:2], _lib.ptr(lse), status,
                 _lib.stream_ptr(dev)), "bgtq_paged_attend")
-        _lib.count_launch(2)
+        _lib.count_launch(lib.bgtq_paged_launches())
     return (out, lse) if return_lse else out
 
 

@@ -629,6 +629,10 @@ int bgtq_decode_combined_noalloc(const BgtqDecodePlan* plan_host, const BgtqHead
 #define BGTQ_PAGED_FORM_MASK 0xF00 /* head, block of query rows); 15 << 8: one list of work over all CTAs and a launch that
                                    * merges; 14 << 8: with cu_q, tcgen05 over a workspace of unpacked tiles (many rows) */
 
+/* Kernels that the calling thread's last call of one of the functions below enqueued: 1 or, where there is nothing to do, 0; an attention 1 (clusters), 2 (one
+ * list, if a part of it may have to be merged) or 3 for every workspace full of tiles (tcgen05). */
+int bgtq_paged_launches(void);
+
 /* Quantise and store n_tok tokens.  k / v element (i, h, d) at k + i * k_st + h * k_sh + d (strides multiples of 8 elements, 16-byte
  * aligned); token i goes to slot slots[i], nowhere when that is negative; the slots of a call are distinct, and the pages' strides leave every
  * page and head a place of its own.  rope_cos / rope_sin (may both

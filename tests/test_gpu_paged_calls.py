@@ -85,3 +85,44 @@ def test_a_step_is_not_captured():
     cache.append_and_attend(0, q, kv, kv)
     assert cache.pages.any()
     cache.check_status()
+
+
+def _kernels(call):
+    """Kernels in a graph of the call, by the runtime's own count."""
+    import ctypes as C
+    cudart = C.CDLL("libcudart.so.12")
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        held = call()
+    n = C.c_size_t(0)
+    assert cudart.cudaGraphGetNodes(C.c_void_p(graph.raw_cuda_graph()), None, C.byref(n)) == 0
+    del held
+    return n.value
+
+
+@pytest.mark.parametrize("form,rows,t,expected", [(0, 1, 40, 1), (15, 1, 40, 1), (15, 1, 4000, 2), (8, 1, 4000, 1), (15, 3, 700, 2), (14, 3, 700, 3), (14, 300, 700, 3)])
+def test_launches_are_counted_as_they_are_made(form, rows, t, expected, monkeypatch):
+    from blockgtq_b200 import _lib, paged, paged_kv4_append, paged_kv4_decode_attention, paged_kv4_prefill_attention, paged_kv4_read
+    monkeypatch.setattr(paged, "_FORM", form)
+    gen = torch.Generator().manual_seed(form)
+    pages, table, slots = _sequence(gen, t)
+    lens = torch.tensor([t], **I32)
+    q = torch.randn(rows, 4, 128, generator=gen).half().to(DEV)
+    odd = torch.randn(rows, 4, 129, generator=gen).half().to(DEV)[:, :, 1:]           # rows that are copied first, in the binding's other path
+    cu = torch.tensor([0, rows], **I32)
+    def attend(q):
+        return paged_kv4_decode_attention(q, pages, table, lens) if rows == 1 and form != 14 else paged_kv4_prefill_attention(q, pages, table, lens, cu)
+    def counted(call):
+        before = _lib.launches
+        call()
+        return _lib.launches - before
+    assert counted(lambda: attend(q)) == counted(lambda: attend(odd)) == expected
+    assert _kernels(lambda: attend(q)) == expected
+    kv = torch.zeros(5, 2, 128, dtype=torch.float16, device=DEV)
+    at = slots[:5].to(DEV)
+    for n in (0, 5):
+        for call in (lambda: paged_kv4_append(pages, at[:n], kv[:n], kv[:n]), lambda: paged_kv4_read(pages, at[:n]),
+                     lambda: paged_kv4_append(pages, at[:n].repeat(2)[::2], kv[:n], kv[:n])):
+            assert counted(call) == (1 if n else 0)
+    assert counted(lambda: paged_kv4_prefill_attention(q[:0], pages, table, lens, cu)) == 0
