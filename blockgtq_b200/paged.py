@@ -266,12 +266,14 @@ def paged_kv4_prefill_attention(q, pages, block_table, seq_lens, cu_q, max_q_len
     """Several query tokens of every sequence over its cached tokens, their own among them: q (n, n_q, 128), rows ``cu_q[b]`` ..
     ``cu_q[b + 1] - 1`` (``cu_q`` (B + 1,) int32) are the last positions of sequence b, and when ``causal`` each sees the tokens up to itself.
 
-    ``max_q_len``: no sequence has more query rows (default: all of them; it chooses the launch, and one that has more is attended all the
-    same).  ``max_seq_len``: sequences are held to it (default: what the table holds).  With many rows per sequence and KV head the
+    ``max_q_len``: no sequence has more query rows (default: all of them; it chooses the launch, 0 the one of 1, and one that has
+    more is attended all the same).  ``max_seq_len``: sequences are held to it (default: what the table holds).  With many rows per sequence and KV head the
     tokens are unpacked into a workspace from torch's allocator, 512 bytes per token of ``max_seq_len`` and KV head for every sequence, at
     most 2 GiB at a time.  Rows behind ``cu_q[B]`` are not written.  Otherwise as :func:`paged_kv4_decode_attention`."""
     if cu_q is None:
         raise ValueError("cu_q says which rows are whose")
+    if max_q_len is not None and max_q_len < 0:
+        raise ValueError("max_q_len must not be negative")
     rows = q.shape[0]
     max_q = max(1, rows if max_q_len is None else min(int(max_q_len), rows))
     return _attend(q, pages, block_table, seq_lens, cu_q, max_q, _most(max_seq_len), causal, scale, return_lse, status, out)

@@ -33,3 +33,13 @@ def test_a_step_that_the_device_has_no_memory_for_takes_nothing(monkeypatch, fai
     held = [p for _, pages in c._seqs.values() for p in pages]
     assert sorted(held + c._free) == list(range(6))
     assert c._step["slots"].tolist() == [c._seqs[b][1][t // 16] * 16 + t % 16 for t in range(3, 43)] + [c._seqs[a][1][1] * 16 + 1]
+
+
+def test_a_prefill_of_fewer_rows_than_none_is_refused():
+    args = dict(q=torch.zeros(4, 4, 128, dtype=torch.float16), pages=torch.zeros(3, 2, paged.page_bytes(32), dtype=torch.uint8),
+                block_table=torch.zeros(2, 1, dtype=torch.int32), seq_lens=torch.ones(2, dtype=torch.int32), cu_q=torch.tensor([0, 2, 4], dtype=torch.int32))
+    with pytest.raises(ValueError, match="max_q_len"):
+        paged.paged_kv4_prefill_attention(**args, max_q_len=-1)
+    for n in (0, 1, 2, 100, None):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            paged.paged_kv4_prefill_attention(**args, max_q_len=n)
