@@ -406,7 +406,9 @@ class PagedKV4Cache:
                                            status=self.status)
 
     def check_status(self):
-        """Raises when a launch since the last call reported an error (synchronises)."""
+        """Raises when a launch since the last call, on whatever stream, reported an error (synchronises the device)."""
+        if self.device.type == "cuda":
+            torch.cuda.synchronize(self.device)
         code = int(self.status.item())
         self.status.zero_()
         if code:

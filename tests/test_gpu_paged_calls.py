@@ -126,3 +126,20 @@ def test_launches_are_counted_as_they_are_made(form, rows, t, expected, monkeypa
                      lambda: paged_kv4_append(pages, at[:n].repeat(2)[::2], kv[:n], kv[:n])):
             assert counted(call) == (1 if n else 0)
     assert counted(lambda: paged_kv4_prefill_attention(q[:0], pages, table, lens, cu)) == 0
+
+
+def test_an_error_on_another_stream_is_told():
+    from blockgtq_b200 import PagedKV4Cache
+    cache = PagedKV4Cache(1, 4, 2, n_pages=4, max_seq_len=60, page_size=16, device=DEV)
+    cache.begin_step([cache.add_sequence()], [3])
+    q, kv = torch.ones(3, 4, 128, dtype=torch.float16, device=DEV), torch.ones(3, 2, 128, dtype=torch.float16, device=DEV)
+    cos = torch.ones(2, 64, device=DEV)                         # the third token has no angle
+    side = torch.cuda.Stream(DEV)
+    cache.append_and_attend(0, q, kv, kv)
+    cache.check_status()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        cache.append_and_attend(0, q, kv, kv, rope=(cos, cos))
+    with pytest.raises(RuntimeError, match="position"):
+        cache.check_status()
+    cache.check_status()
