@@ -26,7 +26,7 @@ struct ApParams {
     int64_t cs_st;
     const int64_t* positions;
     int32_t n_positions, n_tok, n_kv, n_q;
-    int32_t kv_chunks, q_chunks, per;                  // chunks of two K (or V) rows, of two queries; chunks of a warp's task
+    int32_t kv_chunks, q_chunks, per;                  // chunks of 16 / L heads' K (or V) rows, of queries; chunks of a warp's task
     int32_t* status;
 };
 
@@ -56,7 +56,8 @@ __device__ __forceinline__ float max_nan(float a, float b) {             // NaN 
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
     return d;
 }
-// bf16(a / 7) within the scales' range; the quotient by its remainder, as a division rounds it (an infinity ends up as the largest scale).
+// bf16(a / 7) within the scales' range; the quotient as a division rounds it, by Markstein's correction: the product with the rounded reciprocal, and
+// its remainder, both fused, on top (an infinity ends up as the largest scale).
 __device__ __forceinline__ float ap_scale(float a) {
     const float c = 1.0f / 7.0f, q0 = __fmul_rn(a, c), q = __fmaf_rn(__fmaf_rn(-7.0f, q0, a), c, q0);
     return __bfloat162float(__float2bfloat16_rn(fmaxf(fminf(q, kPgScaleMax), kPgScaleMin)));

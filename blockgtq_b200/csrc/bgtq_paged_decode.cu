@@ -24,10 +24,11 @@
 //            CTAs.  Triples cut between CTAs are merged by a second launch.  (Shares and triples of whole rounds of eight, as the warps
 //            take them: 8 sequences of 32768 tokens x 2 KV heads 27.1 us instead of 26.1, 63 short ones beside one of 30000 tokens 27.8 instead of 25.5.)
 //   cluster  a cluster of 1 to 8 CTAs per triple, which merge their shares in distributed shared memory: no list, no second launch.
-// What bounds it: with long caches the warps' instructions, 320 for a unit of 16 tokens and one column tile (128 of them make codes of 144
-// bytes' nibbles, 46 are the loop's), issued in 63 % of the cycles with the ALU half busy, 16 warps on an SM by their registers.  One sequence
-// of 131072 tokens x 8 KV heads 39.3 us, 3.8 TB/s; 64 of 4500 81.4 us, 4.1 TB/s (loads alone, nothing computed: 27.8 and 57.4).  With short ones
-// a launch and the chain length - page number - page - merging: 500 tokens 5.9 us, 4 sequences of 4099 8.4.
+// What bounds it: with long caches the warps' instructions, 339 for a unit of 16 tokens and one column tile (160 of them make operands, two for
+// a pair of codes and a third for V's scales; 46 are the loop's), issued in 62 % of the cycles with no pipe more than half busy, 16 warps on
+// an SM by their registers.  One sequence of 131072 tokens x 8 KV heads 41.0 us, 3.7 TB/s; 64 of 4500 85.0 us, 3.9 TB/s (loads alone, nothing
+// computed: 27.8 and 57.4).  With short ones a launch and the chain length - page number - page - merging: 500 tokens 6.1 us, 4 sequences of 4099
+// 8.5.  (The comparisons of forms and shares here and below were timed with V's scales in the weights, 2 to 8 % faster on either side.)
 //
 // In a CTA eight warps take batches in turn, each with a ring of bulk copies of its own (the next triple's first ones travel while this
 // one's states are merged in shared memory).
@@ -784,7 +785,7 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
 }
 
 // Block (i, col): column col of a triple that is cut.  kByTriple (one query row per sequence, no more triples than CTAs): of triple i.  Otherwise of
-// the one that the end of CTA i's share cuts, if that is its first cut.  Eight warps share the partials, four of them requested at a
+// the one that the end of CTA i's share cuts, if that is its first cut.  kWarps warps share the partials, four of a warp's requested at a
 // time.  Where the triples lie is looked up before the partials are there: the lengths were complete before the attention began.
 template <int NT, typename T, bool kByTriple, int kWarps>
 __global__ void __launch_bounds__(32 * kWarps) pg_merge_kernel(const PdParams P) {
@@ -963,7 +964,9 @@ using namespace bgtq;
 static int pd_tiles(int32_t n_q, int32_t n_kv, int32_t max_q) { return (int64_t)max_q * (n_q / n_kv) <= 8 ? 1 : 2; }
 
 // How a call is launched, from its shape: the form that the measured costs make the cheapest (in microseconds, 300 to 131072 tokens over 2 to 64
-// KV heads and sequences; a round is 256 tokens of a CTA).
+// KV heads and sequences; a round is 256 tokens of a CTA).  The lengths lie on the device: all that is known here is how many sequences there are and
+// what none of them is longer than, so a ragged batch costs what it would if all were as long, and the list, which balances it, is
+// taken later than it would pay.
 //   clusters  4.4 and 1.45 for each round while every CTA has an SM for itself, 2.1 where two share one; with 16 columns 5 and 1.95.
 //   list      5.6, the merging launch among them, and 2.25 for each round of the CTAs that are resident and one more; with 16 columns 9.
 //   tcgen05   20, unpacking at 4.2 MB (of 144 and 512 bytes per token and head) and 1.75 for each tile of a CTA.

@@ -11,14 +11,14 @@
 //               two blocks in turn, so that the tensor cores work on one block while the other's softmax runs;
 //             * 512 threads, two per query row, take S from tensor memory, apply the row's limit and put P (fp16) over S.  The value a row
 //               scales by is its maximum less 7 (P up to 2^7: what is far below it keeps its bits), and moves, with O rescaled, only
-//               when P would pass 2^15.
+//               when P would pass 2^15.  Weights below 2^-21 of the largest are subnormal in fp16, and cut at 2^-32 of it.
 //           Queries are brought to [2^13, 2^14) by a power of two per row, which makes bf16 queries exact in fp16.
 //   merge   rows of the blocks that the shares cut.
 //
 // What bounds attend: per tile 32 products of 64 cycles and 32768 exponentials at 16 a cycle, 2048 cycles each; a tile takes about 3200, the chain
-// of a block's S, its softmax (1900 cycles) and its P . vhat beside the other block's.  8192 positions x 32 query and 8 KV heads, causal: 506 us
-// in short runs, 1.09 PFLOP/s, and 562 in long ones, 0.98 PFLOP/s, where the power limit lowers the clock.  Chunks of 195 to 700 rows behind 700
-// to 9100 tokens of 2 KV heads x 8: 114 us for the three launches, every CTA's share done between 77 and 95 us.
+// of a block's S, its softmax (1900 cycles) and its P . vhat beside the other block's.  8192 positions x 32 query and 8 KV heads, causal: 493 us
+// in short runs, 1.12 PFLOP/s, and 568 in long ones, 0.97 PFLOP/s, where the power limit lowers the clock.  Chunks of 195 to 700 rows behind 700
+// to 9100 tokens of 2 KV heads x 8: 115 us for the three launches, every CTA's share done between 77 and 95 us.
 // Every wait is bounded: one that gives up is recorded in shared memory, where the others see it, and in the caller's status word; the CTA then
 // drains its copies and products, releases its tensor memory and returns.
 #include "bgtq_paged_common.cuh"
