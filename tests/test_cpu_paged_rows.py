@@ -18,7 +18,7 @@ def _view(buffer, at, st, sh, n=N, h=H):
 PLACES = [
     ((0, 512, 128), (4096, 512, 128), True),
     ((0, 512, 128), (4096, 128, 768), True),                # heads outside
-    ((0, 512, 128), (3072 + 512, 512, 128), True),
+    ((0, 512, 128), (3584, 512, 128), True),
     ((0, 512, 128), (N * 512, 512, 128), True),             # right behind q
     ((N * 512, 512, 128), (0, 512, 128), True),
     ((0, 1536, 128), (512, 1536, 128), True),               # columns of one projection
