@@ -10,8 +10,8 @@ from .packed_kv_manager import BlockGTQKVManager, decode_step
 from .production_cache import BlockGTQProductionCache
 from .production_decode import production_decode_step, production_prefill
 from .prefill import layer_major_prefill
-from .paged import (PagedKV4Cache, page_bytes, paged_kv4_append, paged_kv4_decode_attention, paged_kv4_prefill_attention,
-                    paged_kv4_read)
+from .paged import (PagedKV4Cache, page_bytes, paged_kv4_append, paged_kv4_copy, paged_kv4_decode_attention, paged_kv4_prefill_attention,
+                    paged_kv4_read, rope_axes)
 from .calibration import (bake_q_rotations, build_quantizers, collect_qk_activations, load_calib_cache,
                           save_calib_cache)
 
@@ -22,5 +22,5 @@ __all__ = [
     "BlockGTQProductionCache", "production_decode_step", "production_prefill", "collect_qk_activations",
     "build_quantizers", "bake_q_rotations", "fused_blockgtq_prefill_attention", "layer_major_prefill",
     "save_calib_cache", "load_calib_cache", "PagedKV4Cache", "page_bytes", "paged_kv4_append", "paged_kv4_read",
-    "paged_kv4_decode_attention", "paged_kv4_prefill_attention",
+    "paged_kv4_decode_attention", "paged_kv4_prefill_attention", "paged_kv4_copy", "rope_axes",
 ]

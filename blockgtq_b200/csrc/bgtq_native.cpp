@@ -10,6 +10,7 @@
 #include <Python.h>
 
 #include <cstring>
+#include <vector>
 
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAStream.h>
@@ -38,6 +39,8 @@ struct PagedFns {
     decltype(&bgtq_paged_attend) paged_attend;
     decltype(&bgtq_paged_workspace_bytes) paged_workspace;
     decltype(&bgtq_paged_launches) paged_launches;
+    decltype(&bgtq_paged_append_axes) paged_append_axes;
+    decltype(&bgtq_paged_copy) paged_copy;
 } G;
 
 PyObject* none() { Py_RETURN_NONE; }
@@ -331,9 +334,11 @@ bool half_type(const at::Tensor* x) { return x && (x->scalar_type() == at::kHalf
 bool status_ok(const at::Tensor* x) { return !x || (x->is_cuda() && here(*x) && x->scalar_type() == at::kInt && x->numel() > 0); }
 int32_t* status_ptr(const at::Tensor* x) { return x ? x->data_ptr<int32_t>() : nullptr; }
 
-// paged_append(pages, slots, k, v, q | None, cos | None, sin | None, positions | None, status | None) -> rotated q | code | None
+// paged_append(pages, slots, k, v, q | None, cos | None, sin | None, positions | None, status | None[, axes: 64 bytes]) -> rotated q | code | None
 PyObject* paged_append(PyObject*, PyObject* const* argv, Py_ssize_t n) {
-    if (n != 9) return none();
+    if (n != 9 && n != 10) return none();
+    const bool axes = n == 10;
+    if (axes && (!PyBytes_CheckExact(argv[9]) || PyBytes_GET_SIZE(argv[9]) != kHD / 2)) return none();
     const Args A{argv};
     bool bad = false;
     const at::Tensor *pages = A.tensor(0, bad), *slots = A.tensor(1, bad), *k = A.tensor(2, bad), *v = A.tensor(3, bad), *q = A.tensor(4, bad),
@@ -344,13 +349,13 @@ PyObject* paged_append(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     if (k->size(1) != n_kv || v->size(0) != m || v->size(1) != n_kv || !vec_ok(slots, at::kLong, m) ||
         !bgtq::paged_apart(pages->size(0), n_kv, pages->stride(0), pages->stride(1), pages->size(2)))
         return none();
-    if (!cs != !sn || !cs != !pos || (q && !cs)) return none();
+    if (!cs != !sn || !cs != !pos || ((q || axes) && !cs)) return none();
     if (cs) {
         for (const at::Tensor* t : {cs, sn})
             if (!is(t, 2, at::kFloat) || !here(*t) || t->size(1) != kHD / 2 || t->size(0) < 1 || t->size(0) != cs->size(0) || t->size(0) > INT32_MAX ||
                 t->stride(0) != cs->stride(0) || t->stride(0) % 4 || reinterpret_cast<uintptr_t>(t->data_ptr()) % 16)
                 return none();
-        if (!vec_ok(pos, at::kLong, m)) return none();
+        if (!axes ? !vec_ok(pos, at::kLong, m) : !is(pos, 2, at::kLong) || !here(*pos) || pos->size(0) < 1 || pos->size(0) > 4 || pos->size(1) != m) return none();
     }
     if (q && (!rows_ok(q, k->scalar_type(), 16) || q->size(0) != m || q->size(1) < 1)) return none();
     at::Tensor out;
@@ -359,13 +364,63 @@ PyObject* paged_append(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     void* const st = stream_of(*pages);
     int rc;
     Py_BEGIN_ALLOW_THREADS
-    rc = G.paged_append(pages->data_ptr<uint8_t>(), pages->stride(0), pages->stride(1), (int)pages->size(0), page_tokens(*pages),
-                        slots->data_ptr<int64_t>(), k->data_ptr(), k->stride(0), k->stride(1), v->data_ptr(), v->stride(0), v->stride(1),
-                        q ? q->data_ptr() : nullptr, q ? q->stride(0) : 0, q ? q->stride(1) : 0, q ? out.data_ptr() : nullptr,
-                        cs ? cs->data_ptr<float>() : nullptr, cs ? sn->data_ptr<float>() : nullptr, cs ? cs->stride(0) : 0,
-                        cs ? pos->data_ptr<int64_t>() : nullptr, cs ? (int)cs->size(0) : 0, (int)m, (int)n_kv, n_q, flags, status_ptr(status), st);
+    if (axes)
+        rc = G.paged_append_axes(pages->data_ptr<uint8_t>(), pages->stride(0), pages->stride(1), (int)pages->size(0), page_tokens(*pages),
+                                 slots->data_ptr<int64_t>(), k->data_ptr(), k->stride(0), k->stride(1), v->data_ptr(), v->stride(0), v->stride(1),
+                                 q ? q->data_ptr() : nullptr, q ? q->stride(0) : 0, q ? q->stride(1) : 0, q ? out.data_ptr() : nullptr,
+                                 cs->data_ptr<float>(), sn->data_ptr<float>(), cs->stride(0), pos->data_ptr<int64_t>(), pos->stride(0),
+                                 reinterpret_cast<const uint8_t*>(PyBytes_AS_STRING(argv[9])), (int)pos->size(0), (int)cs->size(0), (int)m, (int)n_kv, n_q,
+                                 flags, status_ptr(status), st);
+    else
+        rc = G.paged_append(pages->data_ptr<uint8_t>(), pages->stride(0), pages->stride(1), (int)pages->size(0), page_tokens(*pages),
+                            slots->data_ptr<int64_t>(), k->data_ptr(), k->stride(0), k->stride(1), v->data_ptr(), v->stride(0), v->stride(1),
+                            q ? q->data_ptr() : nullptr, q ? q->stride(0) : 0, q ? q->stride(1) : 0, q ? out.data_ptr() : nullptr,
+                            cs ? cs->data_ptr<float>() : nullptr, cs ? sn->data_ptr<float>() : nullptr, cs ? cs->stride(0) : 0,
+                            cs ? pos->data_ptr<int64_t>() : nullptr, cs ? (int)cs->size(0) : 0, (int)m, (int)n_kv, n_q, flags, status_ptr(status), st);
     Py_END_ALLOW_THREADS
     return rc == BGTQ_OK && q ? wrap(std::move(out)) : code(rc);
+}
+
+// The whole numbers of a list or tuple
+bool numbers(PyObject* x, std::vector<int32_t>& to) {
+    if (!PyList_CheckExact(x) && !PyTuple_CheckExact(x)) return false;
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(x);
+    PyObject** const item = PySequence_Fast_ITEMS(x);
+    to.resize((size_t)n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        if (!PyLong_CheckExact(item[i])) return false;
+        int overflow = 0;
+        const long long v = PyLong_AsLongLongAndOverflow(item[i], &overflow);
+        if (overflow || v < INT32_MIN || v > INT32_MAX) return false;
+        to[(size_t)i] = (int32_t)v;
+    }
+    return true;
+}
+
+// paged_copy(pages, src, dst, n_tokens | None, into | None) -> code | None.  Pools u8 (layers, pages, heads, page bytes), numbers in lists or tuples.
+PyObject* paged_copy(PyObject*, PyObject* const* argv, Py_ssize_t n) {
+    if (n != 5) return none();
+    const Args A{argv};
+    bool bad = false;
+    const at::Tensor *from = A.tensor(0, bad), *to = A.tensor(4, bad);
+    if (!to) to = from;
+    std::vector<int32_t> src, dst, tokens;
+    const bool whole = argv[3] == Py_None;
+    for (const at::Tensor* t : {from, to})
+        if (bad || !is(t, 4, at::kByte) || !here(*t) || t->size(0) < 1 || t->size(0) > INT32_MAX || t->size(1) < 1 || t->size(1) > INT32_MAX ||
+            t->size(2) < 1 || t->size(2) > INT32_MAX || t->size(3) < kUnit || t->size(3) % kUnit || t->size(3) / kUnit * 16 > INT32_MAX)
+            return none();
+    if (from->size(0) != to->size(0) || from->size(2) != to->size(2) || from->size(3) != to->size(3)) return none();
+    if (!numbers(argv[1], src) || !numbers(argv[2], dst) || (!whole && !numbers(argv[3], tokens))) return none();
+    if (src.size() != dst.size() || (!whole && tokens.size() != src.size()) || src.empty()) return none();
+    void* const st = stream_of(*from);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = G.paged_copy(from->data_ptr<uint8_t>(), from->stride(0), from->stride(1), from->stride(2), (int)from->size(1), to->data_ptr<uint8_t>(),
+                      to->stride(0), to->stride(1), to->stride(2), (int)to->size(1), (int)(from->size(3) / kUnit * 16), (int)from->size(0),
+                      (int)from->size(2), src.data(), dst.data(), whole ? nullptr : tokens.data(), (int)src.size(), st);
+    Py_END_ALLOW_THREADS
+    return rc == BGTQ_E_BADARG || rc == BGTQ_E_ALIGN ? none() : code(rc);         // (Python says what is wrong)
 }
 
 // paged_read(pages, slots, kind (0 fp16, 1 bf16, 2 fp32), status | None) -> (k, v) | code | None
@@ -475,7 +530,7 @@ PyObject* guarded(PyObject* self, PyObject* const* argv, Py_ssize_t n) {
 #define BGTQ_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<name>)), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {BGTQ_METHOD(bind),   BGTQ_METHOD(layer_step),  BGTQ_METHOD(layer_encode), BGTQ_METHOD(encode), BGTQ_METHOD(compress),
                           BGTQ_METHOD(attend), BGTQ_METHOD(rotate_rows), BGTQ_METHOD(prefill),      BGTQ_METHOD(paged_append), BGTQ_METHOD(paged_read),
-                          BGTQ_METHOD(paged_attend), BGTQ_METHOD(paged_launched), BGTQ_METHOD(bind_paged), {nullptr, nullptr, 0, nullptr}};
+                          BGTQ_METHOD(paged_attend), BGTQ_METHOD(paged_launched), BGTQ_METHOD(paged_copy), BGTQ_METHOD(bind_paged), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

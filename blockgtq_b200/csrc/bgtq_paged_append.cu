@@ -25,7 +25,9 @@ struct ApParams {
     const float *cos, *sin;                            // (n_positions, 64) rows, or null: no rotation
     int64_t cs_st;
     const int64_t* positions;
-    int32_t n_positions, n_tok, n_kv, n_q;
+    int64_t pos_st;                                    // from one axis to the next
+    uint32_t axis[4];                                  // the pairs' axes, two bits each (where there are several)
+    int32_t n_axes, n_positions, n_tok, n_kv, n_q;
     int32_t kv_chunks, q_chunks, per;                  // chunks of 16 / L heads' K (or V) rows, of queries; chunks of a warp's task
     int32_t* status;
 };
@@ -95,7 +97,7 @@ __device__ __forceinline__ void ap_codes(const float (&in)[E], float largest, fl
 // heads 223 us, 6.5 TB/s, and 16384 63.8 us, 5.7 TB/s, with three chunks of a warp on their way to shared memory (in registers there was room
 // for one: 289 and 82 us; three CTAs on an SM instead of two, with spills: 267 and 78).  Without queries the quantisation's
 // instructions: 16384 tokens 30.7 us, 2.8 TB/s.  32 tokens: 2.9 us, a chain of latencies.
-template <typename T, int L>
+template <typename T, int L, bool kAxes>
 __global__ void __launch_bounds__(kApThreads, L == 8 ? 4 : 2) pg_append_kernel(const ApParams P) {
     constexpr int E = 32 / L, kHeads = 16 / L;
     constexpr uint32_t kAhead = L == 4 ? 3 : 0;            // chunks of a warp on their way
@@ -154,14 +156,42 @@ __global__ void __launch_bounds__(kApThreads, L == 8 ? 4 : 2) pg_append_kernel(c
         slot = -1;
     }
     float cs[2][E] = {}, sn[2][E] = {};
-    if (P.cos && there) {
+    const bool turns = !(first >= (uint32_t)P.kv_chunks && last <= 2u * P.kv_chunks);          // (V alone needs no angle)
+    if constexpr (kAxes) {
+        if (there) {
+            int64_t p[4];
+#pragma unroll
+            for (int a = 0; a < 4; ++a) p[a] = a < P.n_axes ? P.positions[a * P.pos_st + tok] : 0;
+            const auto in = [&](int64_t x) { return x >= 0 && x < P.n_positions; };
+            if (!(in(p[0]) && in(p[1]) && in(p[2]) && in(p[3]))) {         // (as below)
+                if (P.status && slot >= 0) *P.status = kStatusOverflow;
+                slot = -1;
+                p[0] = p[1] = p[2] = p[3] = 0;
+            }
+            if (turns)
+#pragma unroll
+                for (int g = 0; g < 2; ++g)
+#pragma unroll
+                    for (int i = 0; i < E; i += 4) {
+                        const int d = 32 * g + E * j + i;
+                        const uint32_t four = P.axis[d >> 4] >> (2 * (d & 15)) & 255u;         // the axes of pairs d .. d + 3
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t a = four >> (2 * e) & 3u;
+                            const int64_t at = (a & 2 ? a & 1 ? p[3] : p[2] : a & 1 ? p[1] : p[0]) * P.cs_st + d + e;
+                            cs[g][i + e] = P.cos[at];
+                            sn[g][i + e] = P.sin[at];
+                        }
+                    }
+        }
+    } else if (P.cos && there) {
         int64_t p = P.positions[tok];
         if (p < 0 || p >= P.n_positions) { // no angle for it: the token is not stored, and the caller learns of it
             if (P.status && slot >= 0) *P.status = kStatusOverflow;
             slot = -1;
             p = 0;
         }
-        if (!(first >= (uint32_t)P.kv_chunks && last <= 2u * P.kv_chunks))         // (V alone needs none)
+        if (turns)
 #pragma unroll
             for (int g = 0; g < 2; ++g)
 #pragma unroll
@@ -362,14 +392,22 @@ using namespace bgtq;
 
 extern "C" __attribute__((visibility("default"))) int bgtq_paged_launches(void) { return pg_launched; }
 
-extern "C" __attribute__((visibility("default"))) int bgtq_paged_append(
-    uint8_t* pages, int64_t page_stride, int64_t head_stride, int32_t n_pages, int32_t page_tokens, const int64_t* slots, const void* k,
-    int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, const void* q, int64_t q_st, int64_t q_sh, void* q_out,
-    const float* rope_cos, const float* rope_sin, int64_t rope_st, const int64_t* positions, int32_t n_positions, int32_t n_tok,
-    int32_t n_kv, int32_t n_q, int32_t flags, int32_t* status, void* stream) {
+// axis_of (host, 64 entries below n_axes): the axis that each rotated pair's position is taken along; null: there is one.
+static int append(uint8_t* pages, int64_t page_stride, int64_t head_stride, int32_t n_pages, int32_t page_tokens, const int64_t* slots, const void* k,
+                  int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, const void* q, int64_t q_st, int64_t q_sh, void* q_out,
+                  const float* rope_cos, const float* rope_sin, int64_t rope_st, const int64_t* positions, int64_t pos_st, const uint8_t* axis_of,
+                  int32_t n_axes, int32_t n_positions, int32_t n_tok, int32_t n_kv, int32_t n_q, int32_t flags, int32_t* status, void* stream) {
     pg_launched = 0;
     if (n_tok < 0 || n_q < 0 || (flags & ~BGTQ_PAGED_BF16)) return BGTQ_E_BADARG;
     if (const int e = check_pool(pages, page_stride, head_stride, n_pages, page_tokens, n_kv)) return e;
+    uint32_t axis[4] = {};
+    if (axis_of) {
+        if (n_axes < 1 || n_axes > 4 || !rope_cos) return BGTQ_E_BADARG;
+        for (int d = 0; d < kHD / 2; ++d) {
+            if (axis_of[d] >= n_axes) return BGTQ_E_BADARG;
+            axis[d >> 4] |= (uint32_t)axis_of[d] << (2 * (d & 15));
+        }
+    }
     if (n_tok == 0) return BGTQ_OK;
     if (!slots || !k || !v || (q == nullptr) != (n_q == 0) || (q && !q_out) || !rope_cos != !rope_sin) return BGTQ_E_BADARG;
     if (rope_cos && (!positions || n_positions < 1)) return BGTQ_E_BADARG;
@@ -386,16 +424,38 @@ extern "C" __attribute__((visibility("default"))) int bgtq_paged_append(
     const int64_t pairs = ((int64_t)n_tok + 1) / 2;
     const int L = pairs * (n_kv + (n_q + 1) / 2 + 1) <= 8ll * sms ? 8 : 4, heads = 16 / L;
     ApParams P{pages, page_stride, head_stride, n_pages, page_tokens / kUnitTok, slots, k, v, q, k_st, k_sh, v_st, v_sh, q_st, q_sh, q_out,
-               rope_cos, rope_sin, rope_st, positions, n_positions, n_tok, n_kv, n_q, (n_kv + heads - 1) / heads, (n_q + heads - 1) / heads, 1, status};
+               rope_cos, rope_sin, rope_st, positions, pos_st, {axis[0], axis[1], axis[2], axis[3]}, n_axes, n_positions, n_tok, n_kv, n_q,
+               (n_kv + heads - 1) / heads, (n_q + heads - 1) / heads, 1, status};
     const int64_t chunks = 2 * P.kv_chunks + P.q_chunks;
     const int64_t parts = 16ll * sms / pairs;              // of a pair's chunks
     P.per = (int32_t)((chunks + (parts < 1 ? 1 : parts) - 1) / (parts < 1 ? 1 : parts));
     const int64_t tasks = pairs * ((chunks + P.per - 1) / P.per), blocks = (tasks + kApThreads / 32 - 1) / (kApThreads / 32);
     if (tasks + kApThreads / 32 > INT32_MAX) return BGTQ_E_TOOBIG;
     const bool bf16 = flags & BGTQ_PAGED_BF16;
-    const auto kernel = L == 8 ? bf16 ? pg_append_kernel<__nv_bfloat16, 8> : pg_append_kernel<__half, 8>
-                               : bf16 ? pg_append_kernel<__nv_bfloat16, 4> : pg_append_kernel<__half, 4>;
+    const auto kernel = axis_of ? L == 8 ? bf16 ? pg_append_kernel<__nv_bfloat16, 8, true> : pg_append_kernel<__half, 8, true>
+                                         : bf16 ? pg_append_kernel<__nv_bfloat16, 4, true> : pg_append_kernel<__half, 4, true>
+                        : L == 8 ? bf16 ? pg_append_kernel<__nv_bfloat16, 8, false> : pg_append_kernel<__half, 8, false>
+                                 : bf16 ? pg_append_kernel<__nv_bfloat16, 4, false> : pg_append_kernel<__half, 4, false>;
     return pg_launch_ok(launch_kernel(kernel, dim3((unsigned)blocks), dim3(kApThreads), 0, (cudaStream_t)stream, true, P)) ? BGTQ_OK : BGTQ_E_LAUNCH;
+}
+
+extern "C" __attribute__((visibility("default"))) int bgtq_paged_append(
+    uint8_t* pages, int64_t page_stride, int64_t head_stride, int32_t n_pages, int32_t page_tokens, const int64_t* slots, const void* k,
+    int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, const void* q, int64_t q_st, int64_t q_sh, void* q_out,
+    const float* rope_cos, const float* rope_sin, int64_t rope_st, const int64_t* positions, int32_t n_positions, int32_t n_tok,
+    int32_t n_kv, int32_t n_q, int32_t flags, int32_t* status, void* stream) {
+    return append(pages, page_stride, head_stride, n_pages, page_tokens, slots, k, k_st, k_sh, v, v_st, v_sh, q, q_st, q_sh, q_out, rope_cos, rope_sin,
+                  rope_st, positions, 0, nullptr, 1, n_positions, n_tok, n_kv, n_q, flags, status, stream);
+}
+
+extern "C" __attribute__((visibility("default"))) int bgtq_paged_append_axes(
+    uint8_t* pages, int64_t page_stride, int64_t head_stride, int32_t n_pages, int32_t page_tokens, const int64_t* slots, const void* k,
+    int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, const void* q, int64_t q_st, int64_t q_sh, void* q_out,
+    const float* rope_cos, const float* rope_sin, int64_t rope_st, const int64_t* positions, int64_t pos_st, const uint8_t* axis_of, int32_t n_axes,
+    int32_t n_positions, int32_t n_tok, int32_t n_kv, int32_t n_q, int32_t flags, int32_t* status, void* stream) {
+    if (!axis_of) return BGTQ_E_BADARG;
+    return append(pages, page_stride, head_stride, n_pages, page_tokens, slots, k, k_st, k_sh, v, v_st, v_sh, q, q_st, q_sh, q_out, rope_cos, rope_sin,
+                  rope_st, positions, pos_st, axis_of, n_axes, n_positions, n_tok, n_kv, n_q, flags, status, stream);
 }
 
 extern "C" __attribute__((visibility("default"))) int bgtq_paged_read(

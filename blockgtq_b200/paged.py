@@ -8,13 +8,15 @@ hands them out to sequences.
 """
 from __future__ import annotations
 
+import ctypes as C
 import math
+import operator
 
 import torch
 
 from . import _lib
 
-__all__ = ["PAGE_UNIT_BYTES", "page_bytes", "paged_kv4_append", "paged_kv4_read", "paged_kv4_decode_attention",
+__all__ = ["PAGE_UNIT_BYTES", "page_bytes", "rope_axes", "paged_kv4_append", "paged_kv4_read", "paged_kv4_copy", "paged_kv4_decode_attention",
            "paged_kv4_prefill_attention", "PagedKV4Cache"]
 
 HD = 128
@@ -100,23 +102,48 @@ def _type_flag(dtype, name):
     return _TYPES[dtype]
 
 
-def paged_kv4_append(pages, slots, k, v, q=None, cos=None, sin=None, positions=None, status=None):
+def rope_axes(sections, interleaved=False):
+    """The ``axes`` of :func:`paged_kv4_append`: the axis of each of the 64 rotated pairs, as bytes.  ``sections``: how many pairs the axes have (1 to
+    4 of them, 64 pairs in all), one axis behind the other, or ``interleaved``: the axes take turns, each while it has pairs left."""
+    left = [operator.index(n) for n in sections]
+    if not 1 <= len(left) <= 4 or min(left) < 0 or sum(left) != HD // 2:
+        raise ValueError(f"sections must be 1 to 4 numbers of pairs, {HD // 2} in all, got {left}")
+    if not interleaved:
+        return bytes(a for a, n in enumerate(left) for _ in range(n))
+    out = []
+    while len(out) < HD // 2:
+        for a in range(len(left)):
+            if left[a]:
+                out.append(a)
+                left[a] -= 1
+    return bytes(out)
+
+
+def paged_kv4_append(pages, slots, k, v, q=None, cos=None, sin=None, positions=None, status=None, axes=None):
     """Quantise k and v (n, n_kv, 128) fp16 or bf16 into the slots of ``pages`` (n_pages, n_kv, page bytes) uint8.
 
     ``slots`` (n,) int64: page * page size + place in the page, distinct; a token with a negative one is not stored.
     ``cos`` / ``sin`` (n_positions, 64) fp32 with ``positions`` (n,) int64: k, and ``q`` (n, n_q, 128), go through the rotary
     embedding first (dims d and d + 64 are a pair; fp32, k quantised from the unrounded result).  Returns the rotated q (n, n_q, 128),
-    or None without one.  ``status``: optional int32 tensor, set to 2 where a slot or position is out of range (the token is not stored)."""
+    or None without one.  ``status``: optional int32 tensor, set to 2 where a slot or position is out of range (the token is not stored).
+
+    ``axes``: positions lie along several axes, ``positions`` is (axes, n), and the pair d is turned by the angle of its token's position along axis
+    ``axes[d]``: 64 numbers of axes, as :func:`rope_axes` makes them."""
     host = _lib.host()
-    r = host.paged_append(pages, slots, k, v, q, cos, sin, positions, status)
+    if axes is None:
+        r = host.paged_append(pages, slots, k, v, q, cos, sin, positions, status)
+    else:
+        r = host.paged_append(pages, slots, k, v, q, cos, sin, positions, status, axes)
+        if type(r) is int and r < 0:        # (axes that positions do not have are named below)
+            r = None
     if r is None:
-        return _append(pages, slots, k, v, q, cos, sin, positions, status)
+        return _append(pages, slots, k, v, q, cos, sin, positions, status, axes)
     _lib.done(r, "bgtq_paged_append", host.paged_launched())
     return None if q is None else r
 
 
 @torch.no_grad()
-def _append(pages, slots, k, v, q, cos, sin, positions, status):
+def _append(pages, slots, k, v, q, cos, sin, positions, status, axes=None):
     """:func:`paged_kv4_append` for what the extension module leaves: tensors that have to be copied, and errors."""
     page = _pool(pages)
     dev, n_kv = pages.device, pages.shape[1]
@@ -129,7 +156,9 @@ def _append(pages, slots, k, v, q, cos, sin, positions, status):
     slots = _ints(slots, "slots", torch.int64, (n,), dev)
     if (cos is None) != (sin is None) or (cos is None) != (positions is None):
         raise ValueError("cos, sin and positions belong together")
-    n_q, q_out, qs, rope = 0, None, (0, 0), (None, None, 0, None, 0)
+    n_q, q_out, qs, rope, entry = 0, None, (0, 0), (None, None, 0, None, 0), "bgtq_paged_append"
+    if axes is not None and cos is None:
+        raise ValueError("axes belong to cos, sin and positions")
     if cos is not None:
         if cos.dim() != 2 or cos.shape[1] != HD // 2 or cos.shape[0] < 1 or sin.shape != cos.shape:
             raise ValueError(f"cos and sin must be (positions, {HD // 2}), got {tuple(cos.shape)} and {tuple(sin.shape)}")
@@ -139,8 +168,19 @@ def _append(pages, slots, k, v, q, cos, sin, positions, status):
             raise ValueError(f"cos and sin must be on {dev}")
         if cos.stride(1) != 1 or cos.stride(0) % 4 or sin.stride() != cos.stride() or (cos.data_ptr() | sin.data_ptr()) % 16:
             cos, sin = (x.clone(memory_format=torch.contiguous_format) for x in (cos, sin))
-        positions = _ints(positions, "positions", torch.int64, (n,), dev)
-        rope = (cos.data_ptr(), sin.data_ptr(), cos.stride(0), positions.data_ptr(), cos.shape[0])
+        if axes is None:
+            positions = _ints(positions, "positions", torch.int64, (n,), dev)
+            rope = (cos.data_ptr(), sin.data_ptr(), cos.stride(0), positions.data_ptr(), cos.shape[0])
+        else:
+            n_axes = positions.shape[0] if positions.dim() == 2 else 0
+            if not 1 <= n_axes <= 4:
+                raise ValueError(f"positions must be (axes, {n}), 1 to 4 axes, got {tuple(positions.shape)}")
+            positions = _ints(positions, "positions", torch.int64, (n_axes, n), dev)
+            axes = bytes(axes)
+            if len(axes) != HD // 2 or max(axes) >= n_axes:
+                raise ValueError(f"axes must be {HD // 2} numbers below {n_axes}, the positions' axes")
+            entry = "bgtq_paged_append_axes"
+            rope = (cos.data_ptr(), sin.data_ptr(), cos.stride(0), positions.data_ptr(), n, axes, n_axes, cos.shape[0])
     if q is not None:
         if cos is None:
             raise ValueError("q is only taken to be rotated: pass cos, sin and positions")
@@ -152,10 +192,10 @@ def _append(pages, slots, k, v, q, cos, sin, positions, status):
     status = _status(status, dev)
     _lib.require_cuda(pages, "pages")
     with torch.cuda.device(dev):
-        _lib.check(_lib.lib().bgtq_paged_append(
+        _lib.check(getattr(_lib.lib(), entry)(
             pages.data_ptr(), pages.stride(0), pages.stride(1), pages.shape[0], page, slots.data_ptr(), k.data_ptr(), *k.stride()[:2],
             v.data_ptr(), *v.stride()[:2], _lib.ptr(q), *qs, _lib.ptr(q_out) if q is not None else 0, *rope, n, n_kv, n_q, flags,
-            status, _lib.stream_ptr(dev)), "bgtq_paged_append")
+            status, _lib.stream_ptr(dev)), entry)
     _lib.count_launch(_lib.lib().bgtq_paged_launches())
     return q_out
 
@@ -187,6 +227,75 @@ def _read(pages, slots, dtype, status):
             _lib.PAGED_F32 if dtype == torch.float32 else _TYPES[dtype], status, _lib.stream_ptr(dev)), "bgtq_paged_read")
     _lib.count_launch(_lib.lib().bgtq_paged_launches())
     return k, v
+
+
+def paged_kv4_copy(pages, src, dst, n_tokens=None, into=None):
+    """Page ``dst[i]`` becomes page ``src[i]``, in every layer: ``pages`` (layers, n_pages, n_kv, page bytes) uint8, or one layer's
+    (n_pages, n_kv, page bytes).
+
+    ``src`` and ``dst`` are page numbers on the host (lists, or CPU tensors): no page is copied to twice, nor both copied to and from; one may be copied from
+    many times.  ``n_tokens``, one number for each pair: only the units of 16 tokens that hold the page's first so many tokens are copied.  ``into``:
+    another pool, of the same layers, heads and page size and apart from this one, that ``dst`` are pages of."""
+    r = None
+    host = _lib.host()
+    if pages.dim() == 4:
+        r = host.paged_copy(pages, src, dst, n_tokens, into)
+    if r is None:
+        return _copy(pages, src, dst, n_tokens, into)
+    _lib.done(r, "bgtq_paged_copy", host.paged_launched())
+
+
+def _numbers(x, name):
+    if isinstance(x, torch.Tensor):
+        if x.is_cuda:
+            raise ValueError(f"{name} must be numbers on the host: the call reads them before it returns")
+        if x.dim() != 1 or x.is_floating_point() or x.is_complex() or x.dtype == torch.bool:
+            raise ValueError(f"{name} must be whole numbers, one behind the other, got {x.dtype} {tuple(x.shape)}")
+        return x.tolist()
+    return [operator.index(i) for i in x]
+
+
+def _copy(pages, src, dst, n_tokens, into):
+    to, size = pages if into is None else into, None
+    for x in (pages, to):
+        if x.dtype != torch.uint8 or x.dim() not in (3, 4):
+            raise ValueError("pages must be uint8 (layers, n_pages, n_kv, page bytes) or (n_pages, n_kv, page bytes)")
+    if pages.dim() == 3:
+        pages = pages.unsqueeze(0)
+    to = pages if into is None else to.unsqueeze(0) if to.dim() == 3 else to
+    for x in (pages, to):
+        if x.shape[0] < 1:
+            raise ValueError("pages of no layers")
+        size = _pool(x[0])
+        if x.stride(0) % 16:
+            raise ValueError("pages must have rows whose addresses are multiples of 16 bytes")
+    if to.device != pages.device or to.shape[0] != pages.shape[0] or to.shape[2:] != pages.shape[2:]:
+        raise ValueError(f"into must have the layers, heads, page size and device of pages, got {tuple(to.shape)} on {to.device} for "
+                         f"{tuple(pages.shape)} on {pages.device}")
+    src, dst = _numbers(src, "src"), _numbers(dst, "dst")
+    if len(src) != len(dst):
+        raise ValueError(f"{len(src)} pages to copy from, {len(dst)} to copy to")
+    for x, name, n in ((src, "src", pages.shape[1]), (dst, "dst", to.shape[1])):
+        if x and not 0 <= min(x) <= max(x) < n:
+            raise ValueError(f"{name} must be numbers of the pool's {n} pages")
+    if len(set(dst)) != len(dst):
+        raise ValueError("a page is copied to once")
+    if into is None and not set(dst).isdisjoint(src):
+        raise ValueError("a page is not both copied to and from")
+    if n_tokens is not None:
+        n_tokens = _numbers(n_tokens, "n_tokens")
+        if len(n_tokens) != len(src) or (n_tokens and not 0 <= min(n_tokens) <= max(n_tokens) <= size):
+            raise ValueError(f"n_tokens must be a number of 0 to {size} tokens for each pair")
+    _lib.require_cuda(pages, "pages")
+    if not src:
+        return
+    lib, n = _lib.lib(), len(src)
+    with torch.cuda.device(pages.device):
+        _lib.check(lib.bgtq_paged_copy(
+            pages.data_ptr(), *pages.stride()[:3], pages.shape[1], to.data_ptr(), *to.stride()[:3], to.shape[1], size, pages.shape[0], pages.shape[2],
+            (C.c_int32 * n)(*src), (C.c_int32 * n)(*dst), None if n_tokens is None else (C.c_int32 * n)(*n_tokens), n,
+            _lib.stream_ptr(pages.device)), "bgtq_paged_copy")
+    _lib.count_launch(lib.bgtq_paged_launches())
 
 
 def _attend(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, causal, scale, return_lse, status, out):

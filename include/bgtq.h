@@ -647,6 +647,26 @@ int bgtq_paged_append(uint8_t* pages, int64_t page_stride, int64_t head_stride, 
                 const float* rope_cos, const float* rope_sin, int64_t rope_st, const int64_t* positions, int32_t n_positions,
                 int32_t n_tok, int32_t n_kv, int32_t n_q, int32_t flags, int32_t* status, void* stream);
 
+/* The same with positions along several axes (n_axes, at most 4): the position of token i along axis a is positions[a * pos_st + i], and dims d and
+ * d + 64 are turned by entry d of row positions[axis_of[d] * pos_st + i] (axis_of: 64 bytes on the HOST, each below n_axes).  A token of which any
+ * axis has a position outside the tables is not stored.  The tables are needed. */
+int bgtq_paged_append_axes(uint8_t* pages, int64_t page_stride, int64_t head_stride, int32_t n_pages, int32_t page_tokens, const int64_t* slots,
+                const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh,
+                const void* q, int64_t q_st, int64_t q_sh, void* q_out,
+                const float* rope_cos, const float* rope_sin, int64_t rope_st, const int64_t* positions, int64_t pos_st,
+                const uint8_t* axis_of, int32_t n_axes, int32_t n_positions,
+                int32_t n_tok, int32_t n_kv, int32_t n_q, int32_t flags, int32_t* status, void* stream);
+
+/* Page dst[i] of `to` becomes page src[i] of `from`, in every layer and KV head: n pairs of page numbers in HOST memory, read before the call
+ * returns.  n_tokens (host, or NULL: whole pages): only the units of 16 tokens that hold the pair's first n_tokens[i] tokens are copied, 0 ..
+ * page_tokens.  Page p of layer l and head h starts at l * layer_stride + p * page_stride + h * head_stride bytes (not negative, multiples of 16); the
+ * pools are one and the same (same address and strides), or apart.  No page is copied to twice, nor, in one pool, copied to and from; a page may be
+ * copied from many times.  A graph that captures the call keeps the numbers of that call. */
+int bgtq_paged_copy(const uint8_t* from, int64_t from_layer_stride, int64_t from_page_stride, int64_t from_head_stride, int32_t n_from,
+                uint8_t* to, int64_t to_layer_stride, int64_t to_page_stride, int64_t to_head_stride, int32_t n_to,
+                int32_t page_tokens, int32_t n_layers, int32_t n_kv, const int32_t* src, const int32_t* dst, const int32_t* n_tokens,
+                int32_t n, void* stream);
+
 /* The values of n_tok slots -> k, v (n_tok, n_kv, 128) contiguous, fp16 (exact), bf16 or fp32; zeros for a negative slot. */
 int bgtq_paged_read(const uint8_t* pages, int64_t page_stride, int64_t head_stride, int32_t n_pages, int32_t page_tokens,
                 const int64_t* slots, int32_t n_tok, int32_t n_kv, void* k, void* v, int32_t flags, int32_t* status, void* stream);
