@@ -71,6 +71,12 @@ class LayerStep(C.Structure):
     ]
 
 
+class PagedScores(C.Structure):
+    """Mirror of ``BgtqPagedScores``."""
+    _fields_ = [("slopes", C.c_void_p), ("prefix", C.c_void_p), ("softcap", C.c_float), ("window", C.c_int32), ("max_prefix", C.c_int32),
+                ("reserved", C.c_int32)]
+
+
 _i32, _i64, _f32, _vp = C.c_int32, C.c_int64, C.c_float, C.c_void_p
 _SIGNATURES = {
     "bgtq_abi_version": (C.c_int, []),
@@ -156,6 +162,9 @@ _SIGNATURES = {
     "bgtq_paged_workspace_bytes": (C.c_int64, [_i32, _i32, _i32, _i32, _i32, _i64, _i32]),
     "bgtq_paged_attend": (C.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _i32, _i32, _vp, _i64, _i32, _vp, _vp, _i32, _i32, _i32, _i32,
                                     _i32, _i64, _f32, _i32, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp]),
+    "bgtq_paged_scored_workspace_bytes": (C.c_int64, [_i32, _i32, _i32, _i32, _i32, _i64, _i32, C.POINTER(PagedScores)]),
+    "bgtq_paged_attend_scored": (C.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _i32, _i32, _vp, _i64, _i32, _vp, _vp, _i32, _i32, _i32, _i32,
+                                           _i32, _i64, _f32, _i32, C.POINTER(PagedScores), _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp]),
     "bgtq_combine_publish": (C.c_int, [_vp, _vp, _i32, _vp, _i32, _i32, _i32, _vp, _i64, _i64, _vp, _i32, _i32, _vp, _vp,
                                       _i32, _vp]),
     "bgtq_exchange_publish": (C.c_int, [_vp, _i64, _vp, _i64, _i64, _vp, _i32, _i32, _vp, _vp, _vp]),
@@ -205,7 +214,8 @@ def lib():
     module.bind(*addresses("bgtq_layer_step", "bgtq_layer_encode", "bgtq_attend", "bgtq_decode_default_splits", "bgtq_encode",
                            "bgtq_rotate_q_rows", "bgtq_prefill", "bgtq_prefill_workspace_bytes"))
     module.bind_paged(*addresses("bgtq_paged_append", "bgtq_paged_read", "bgtq_paged_attend", "bgtq_paged_workspace_bytes",
-                                 "bgtq_paged_launches", "bgtq_paged_append_axes", "bgtq_paged_copy"))
+                                 "bgtq_paged_launches", "bgtq_paged_append_axes", "bgtq_paged_copy", "bgtq_paged_attend_scored",
+                                 "bgtq_paged_scored_workspace_bytes"))
     native = module
     _lib = handle
     return _lib

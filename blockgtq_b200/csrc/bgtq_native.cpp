@@ -41,6 +41,8 @@ struct PagedFns {
     decltype(&bgtq_paged_launches) paged_launches;
     decltype(&bgtq_paged_append_axes) paged_append_axes;
     decltype(&bgtq_paged_copy) paged_copy;
+    decltype(&bgtq_paged_attend_scored) paged_attend_scored;
+    decltype(&bgtq_paged_scored_workspace_bytes) paged_scored_workspace;
 } G;
 
 PyObject* none() { Py_RETURN_NONE; }
@@ -446,10 +448,19 @@ PyObject* paged_read(PyObject*, PyObject* const* argv, Py_ssize_t n) {
 }
 
 // paged_attend(q, pages, block_table, seq_lens, cu_q | None, max_q, max_tokens (< 0: what the table holds), scale, flags, want_lse,
-//              status | None, out | None) -> out | (out, lse) | code | None
+//              status | None, out | None[, slopes | None, prefix lengths | None, cap or 0, window or 0, longest prefix (< 0: what the table holds)])
+//   -> out | (out, lse) | code | None
 PyObject* paged_attend(PyObject*, PyObject* const* argv, Py_ssize_t n) {
-    if (n != 12) return none();
+    if (n != 12 && n != 17) return none();
     const Args A{argv};
+    const bool scored = n == 17;
+    BgtqPagedScores sc = {};
+    int64_t most_prefix = 0;
+    if (scored) {
+        sc.softcap = A.real(14);
+        sc.window = A.i32(15);
+        most_prefix = A.num(16);
+    }
     const int64_t max_q = A.num(5);
     int64_t most = A.num(6);
     const float scale = A.real(7);
@@ -458,6 +469,7 @@ PyObject* paged_attend(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     bool bad = false;
     const at::Tensor *q = A.tensor(0, bad), *pages = A.tensor(1, bad), *table = A.tensor(2, bad), *lens = A.tensor(3, bad), *cu = A.tensor(4, bad),
                      *status = A.tensor(10, bad), *given = A.tensor(11, bad);
+    const at::Tensor *slopes = scored ? A.tensor(12, bad) : nullptr, *prefix = scored ? A.tensor(13, bad) : nullptr;
     if (bad || !pool_ok(pages) || !half_type(q) || !rows_ok(q, q->scalar_type(), 16) || !is(table, 2, at::kInt) || !here(*table) || !status_ok(status))
         return none();
     const int64_t m = q->size(0), n_q = q->size(1), n_kv = pages->size(1), n_seq = table->size(0), cap = table->size(1) * page_tokens(*pages);
@@ -469,8 +481,14 @@ PyObject* paged_attend(PyObject*, PyObject* const* argv, Py_ssize_t n) {
                   !bgtq::paged_rows_apart(rows(*q), rows(*given))))
         return none();
     if (most < 0 || most > cap) most = cap;
+    if ((slopes && !vec_ok(slopes, at::kFloat, n_q)) || (prefix && !vec_ok(prefix, at::kInt, n_seq))) return none();
+    if (scored) {
+        sc.slopes = slopes ? slopes->data_ptr<float>() : nullptr;
+        sc.prefix = prefix ? prefix->data_ptr<int32_t>() : nullptr;
+        sc.max_prefix = (int32_t)(most_prefix < 0 || most_prefix > most ? most : most_prefix);
+    }
     if (q->scalar_type() == at::kBFloat16) flags |= BGTQ_PAGED_BF16;
-    const int64_t need = G.paged_workspace((int)n_seq, (int)m, (int)n_q, (int)n_kv, (int)max_q, most, flags);
+    const int64_t need = G.paged_scored_workspace((int)n_seq, (int)m, (int)n_q, (int)n_kv, (int)max_q, most, flags, scored ? &sc : nullptr);
     if (need < 0) return code((int)need);
     at::Tensor out = given ? *given : empty(q->sizes(), q->scalar_type(), *q), ws, lse;
     if (need) ws = empty({need}, at::kByte, *q);
@@ -478,10 +496,10 @@ PyObject* paged_attend(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     void* const st = stream_of(*q);
     int rc;
     Py_BEGIN_ALLOW_THREADS
-    rc = G.paged_attend(q->data_ptr(), q->stride(0), q->stride(1), pages->data_ptr<uint8_t>(), pages->stride(0), pages->stride(1),
+    rc = G.paged_attend_scored(q->data_ptr(), q->stride(0), q->stride(1), pages->data_ptr<uint8_t>(), pages->stride(0), pages->stride(1),
                         (int)pages->size(0), page_tokens(*pages), table->data_ptr<int32_t>(), table->stride(0), (int)table->size(1),
                         lens->data_ptr<int32_t>(), cu ? cu->data_ptr<int32_t>() : nullptr, (int)n_seq, (int)m, (int)n_q, (int)n_kv, (int)max_q, most,
-                        scale, flags, need ? ws.data_ptr() : nullptr, need, out.data_ptr(), out.stride(0), out.stride(1),
+                        scale, flags, scored ? &sc : nullptr, need ? ws.data_ptr() : nullptr, need, out.data_ptr(), out.stride(0), out.stride(1),
                         want_lse ? lse.data_ptr<float>() : nullptr, status_ptr(status), st);
     Py_END_ALLOW_THREADS
     if (rc != BGTQ_OK) return code(rc);

@@ -69,6 +69,36 @@ __device__ __forceinline__ void pg_pow2(int e, float& a, float& b) {
 // them at the smallest normal number either.)
 constexpr float kPgFactorMin = 1.17549435e-38f;
 
+// What differs from plain attention: logits capped and biased by distance, tokens hidden by a window or shown by a prefix.
+struct PgScores {
+    const float* slopes;             // (n_q) or null
+    const int32_t* prefix;           // (n_seq) or null
+    float cap, cap_inv;              // of logits to the base of 2, and its reciprocal; 0: none
+    int32_t window, max_prefix;      // 0: none; what prefixes are held to
+};
+// A sequence's prefix
+__device__ __forceinline__ int pg_prefix(const PgScores& S, int seq, int len) { return S.prefix ? max(0, min(S.prefix[seq], min(S.max_prefix, len))) : 0; }
+
+__device__ __forceinline__ float pg_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// cap * tanh(x / cap), u = x / cap.  Up to 1/2 an odd polynomial of degree 9, fitted to the relative error (1.5e-8); beyond it 1 - 2 / (e^2u + 1), whose terms
+// are then of one magnitude, so that both are off by a few roundings of the result itself.
+__device__ __forceinline__ float pg_cap_near(float u, float cap) {
+    const float v = u * u;
+    float p = fmaf(v, 0.017241490183840052f, -0.05304549361635799f);
+    p = fmaf(p, v, 0.1332587894742629f);
+    p = fmaf(p, v, -0.3333314389579803f);
+    return cap * u * fmaf(p, v, 1.f);
+}
+__device__ __forceinline__ float pg_cap_far(float u, float cap) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(pg_ex2(u * 2.8853900817779268f) + 1.f));
+    return cap * fmaf(-2.f, r, 1.f);
+}
+
 // Kernels that this thread's last call of an entry point enqueued.
 inline thread_local int32_t pg_launched = 0;
 inline bool pg_launch_ok(cudaError_t e) {

@@ -38,6 +38,8 @@
 
 #include <limits.h>
 
+#include <algorithm>
+
 namespace bgtq {
 namespace {
 
@@ -68,6 +70,7 @@ struct PdParams {
     float* part_o;                   // (2 n_cta, columns, 128)
     float2* part_ml;                 // (2 n_cta, columns): reference, denominator
     int32_t* status;
+    PgScores sc;                     // (kernels of kMod read it)
 };
 
 // How a call is launched.
@@ -79,12 +82,17 @@ struct PdForm {
     bool alone;                                 // cluster: every CTA has an SM for itself
 };
 
+// kMod: a sequence's batches are counted without those between its prefix and the first that its first row's window reaches.
 struct SeqInfo {
     int len, q0, n;                  // cached tokens, first query row, query rows
+    int pre, head, skip;             // tokens and batches of the prefix, batches left out behind them
+    __device__ __forceinline__ int batch(int k) const { return k + (k >= head ? skip : 0); }
 };
 
+template <bool kMod>
 __device__ __forceinline__ SeqInfo pd_seq(const PdParams& P, int i) {
     SeqInfo s;
+    s.pre = s.head = s.skip = 0;
     s.len = max(0, min(P.lens[i], P.cap));
     if (P.cu_q) {
         s.q0 = min(max(P.cu_q[i], 0), P.n_tok);
@@ -93,9 +101,14 @@ __device__ __forceinline__ SeqInfo pd_seq(const PdParams& P, int i) {
         s.q0 = i;
         s.n = 1;
     }
+    if (kMod) {
+        s.pre = pg_prefix(P.sc, i, s.len);
+        s.head = (s.pre + kBatchTok - 1) / kBatchTok;
+        if (P.sc.window) s.skip = max(0, max(0, max(0, s.len - s.n + 1) - P.sc.window) / kBatchTok - s.head);
+    }
     return s;
 }
-__device__ __forceinline__ uint32_t pd_batches(const SeqInfo& s) { return (uint32_t)((s.len + kBatchTok - 1) / kBatchTok); }
+__device__ __forceinline__ uint32_t pd_batches(const SeqInfo& s) { return (uint32_t)((s.len + kBatchTok - 1) / kBatchTok - s.skip); }
 __device__ __forceinline__ uint32_t pd_whole(const PdParams& P, uint32_t n) { return (n + P.grain - 1) & ~(uint32_t)(P.grain - 1); }
 __device__ __forceinline__ uint32_t pd_places(const PdParams& P, const SeqInfo& s) { return s.len > 0 ? pd_whole(P, pd_batches(s)) + kTripleCost : 0u; }
 template <int NT>
@@ -133,7 +146,7 @@ __device__ __forceinline__ uint32_t block_scan(ScanSmem& S, uint32_t w) {
 
 // Total of the list and, for the position that `at` makes of it, the sequence that it lies in (-1: none) and where that one starts.  Up to 128
 // sequences are looked over by every warp for itself, without a barrier.
-template <int NT, typename At>
+template <int NT, bool kMod, typename At>
 __device__ __forceinline__ void pd_find(const PdParams& P, ScanSmem& S, uint32_t& total, int& seq, uint32_t& start, At at) {
     const int tid = threadIdx.x, step = blockDim.x;
     if (P.n_seq <= 128) {
@@ -141,7 +154,7 @@ __device__ __forceinline__ void pd_find(const PdParams& P, ScanSmem& S, uint32_t
         uint32_t w[4], mine = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            w[i] = 4 * lane + i < P.n_seq ? pd_work<NT>(P, pd_seq(P, 4 * lane + i)) : 0u;
+            w[i] = 4 * lane + i < P.n_seq ? pd_work<NT>(P, pd_seq<kMod>(P, 4 * lane + i)) : 0u;
             mine += w[i];
         }
         uint32_t before = mine;
@@ -170,7 +183,7 @@ __device__ __forceinline__ void pd_find(const PdParams& P, ScanSmem& S, uint32_t
     uint32_t sum = 0;
     for (int base = 0; base < P.n_seq; base += step) {
         const int i = base + tid;
-        block_scan(S, i < P.n_seq ? pd_work<NT>(P, pd_seq(P, i)) : 0u);
+        block_scan(S, i < P.n_seq ? pd_work<NT>(P, pd_seq<kMod>(P, i)) : 0u);
         __syncthreads();
         sum += S.total;
         __syncthreads();
@@ -180,7 +193,7 @@ __device__ __forceinline__ void pd_find(const PdParams& P, ScanSmem& S, uint32_t
     sum = 0;
     for (int base = 0; base < P.n_seq; base += step) {
         const int i = base + tid;
-        const uint32_t w = i < P.n_seq ? pd_work<NT>(P, pd_seq(P, i)) : 0u;
+        const uint32_t w = i < P.n_seq ? pd_work<NT>(P, pd_seq<kMod>(P, i)) : 0u;
         const uint32_t before = sum + block_scan(S, w);
         if (before <= want && want - before < w) {
             S.seq = i;
@@ -201,11 +214,7 @@ __device__ __forceinline__ uint32_t pd_share(const PdParams& P, uint32_t total) 
     return n <= 4 * kPdWarps ? (n + kPdWarps - 1) / kPdWarps * kPdWarps : pd_whole(P, n);
 }
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
+__device__ __forceinline__ float ex2(float x) { return pg_ex2(x); }
 // (as in bgtq_common.cuh, but not volatile: the compiler may move them among one another)
 __device__ __forceinline__ void mma_acc(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -336,9 +345,43 @@ __device__ __forceinline__ void pd_no_number(State<NT>& st, float& s0, float& s1
     }
 }
 
-// U units of 16 tokens at u in shared memory.  kEdge: some of them (tokens from len on of the sequence, from lim[] on of a column) are hidden.
-template <int NT, int U, bool kEdge>
-__device__ __forceinline__ void pd_units(const uint8_t* u, const Magic& mg, const Query<NT>& Q, State<NT>& st, int r, int c, int t0, int len, const int (&lim)[NT][2]) {
+// What a column's logits and limits are beside the plain ones (kMod).
+template <int NT>
+struct Marks {
+    int lo[NT][2], pos[NT][2];       // first token of its window, its own position
+    float slope[NT][2];              // to the base of 2
+    int pre;                         // tokens of the prefix
+    float cap, cap_inv;
+    bool biased;
+};
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 16 ? 0xffffu : (1u << n) - 1u; }
+// The tokens of a unit from t0 on that a column sees
+__device__ __forceinline__ uint32_t pd_seen(int t0, int lim, int lo, int pre) {
+    return bits_below(lim - t0) & (~bits_below(lo - t0) | bits_below(pre - t0));
+}
+// pd_no_number for columns that see what the bits in `seen` say
+template <int NT>
+__device__ __forceinline__ void pd_no_number_seen(State<NT>& st, float& s0, float& s1, int r, int c, const uint32_t (&seen)[NT][2]) {
+    const uint32_t mine = (s0 != s0 ? 1u << (2 * r) : 0u) | (s1 != s1 ? 2u << (2 * r) : 0u);
+    if (s0 != s0) s0 = 0.f;
+    if (s1 != s1) s1 = 0.f;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const uint32_t none = __reduce_or_sync(0xffffffffu, c == g ? mine : 0u);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (none & seen[nt][e])
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) st.o[nt][i][g][e] = st.o[nt][i][g][2 + e] = __uint_as_float(0x7fffffffu);
+    }
+}
+
+// U units of 16 tokens at u in shared memory.  kEdge: some of them (tokens from len on of the sequence, from lim[] on of a column, kMod: between its
+// prefix and its window) are hidden.
+template <int NT, int U, bool kEdge, bool kMod>
+__device__ __forceinline__ void pd_units(const uint8_t* u, const Magic& mg, const Query<NT>& Q, State<NT>& st, int r, int c, int t0, int len, const int (&lim)[NT][2], const Marks<NT>& mk) {
     float s[U][NT][4];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
@@ -369,6 +412,65 @@ __device__ __forceinline__ void pd_units(const uint8_t* u, const Magic& mg, cons
             }
         });
     }
+    uint32_t seen[U][NT][2];
+    if (kMod) {
+        // logits to the base of 2 in their final form
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[i][nt][e] = __fmul_rn(s[i][nt][e], Q.f[nt][e & 1]);
+        if (mk.cap > 0.f) {
+            bool far = false;
+#pragma unroll
+            for (int i = 0; i < U; ++i)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[i][nt][e] *= mk.cap_inv;
+                        far |= !(fabsf(s[i][nt][e]) <= 0.5f);
+                    }
+            if (__any_sync(0xffffffffu, far)) {
+#pragma unroll
+                for (int i = 0; i < U; ++i)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float x = s[i][nt][e], f = pg_cap_far(x, mk.cap);
+                            s[i][nt][e] = fabsf(x) <= 0.5f ? pg_cap_near(x, mk.cap) : f;
+                        }
+            } else {
+#pragma unroll
+                for (int i = 0; i < U; ++i)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[i][nt][e] = pg_cap_near(s[i][nt][e], mk.cap);
+            }
+        }
+        if (mk.biased)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float d = (float)(t0 + r - mk.pos[nt][e]);
+#pragma unroll
+                    for (int i = 0; i < U; ++i) {
+                        s[i][nt][e] = fmaf(-mk.slope[nt][e], fabsf(d + 16.f * i), s[i][nt][e]);
+                        s[i][nt][2 + e] = fmaf(-mk.slope[nt][e], fabsf(d + 16.f * i + 8.f), s[i][nt][2 + e]);
+                    }
+                }
+        if (kEdge)
+#pragma unroll
+            for (int i = 0; i < U; ++i)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) seen[i][nt][e] = pd_seen(t0 + 16 * i, lim[nt][e], mk.lo[nt][e], mk.pre);
+    }
     // V's scales of a unit's tokens 2 r, 2 r + 1, group c, exact in fp16; the lanes get theirs from one another (11 instructions; 24 if each lane converted
     // its eight pairs for itself).  All of it ahead of the weights: between them and the products it is part of the warp's chain, 55.3 us instead of
     // 52.5 (16 sequences of 8192 tokens x 8 KV heads, a CTA each).
@@ -381,7 +483,10 @@ __device__ __forceinline__ void pd_units(const uint8_t* u, const Magic& mg, cons
             const int t = t0 + 16 * i + 2 * r;
             if (t >= len) s0 = 0.f;                                             // what lies behind the sequence may be anything
             if (t + 1 >= len) s1 = 0.f;
-            if (__any_sync(0xffffffffu, s0 != s0 || s1 != s1)) pd_no_number<NT>(st, s0, s1, t, c, lim);
+            if (__any_sync(0xffffffffu, s0 != s0 || s1 != s1)) {
+                if (kMod) pd_no_number_seen<NT>(st, s0, s1, r, c, seen[i]);
+                else pd_no_number<NT>(st, s0, s1, t, c, lim);
+            }
         }
         vs[i] = pack_half2(s0, s1);
     }
@@ -394,7 +499,10 @@ __device__ __forceinline__ void pd_units(const uint8_t* u, const Magic& mg, cons
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                if (kEdge) {
+                if (kEdge && kMod) {
+                    if (!(seen[i][nt][e] >> r & 1u)) s[i][nt][e] = -INFINITY;
+                    if (!(seen[i][nt][e] >> (8 + r) & 1u)) s[i][nt][2 + e] = -INFINITY;
+                } else if (kEdge) {
                     if (t0 + 16 * i + r >= lim[nt][e]) s[i][nt][e] = -INFINITY;
                     if (t0 + 16 * i + 8 + r >= lim[nt][e]) s[i][nt][2 + e] = -INFINITY;
                 }
@@ -405,7 +513,7 @@ __device__ __forceinline__ void pd_units(const uint8_t* u, const Magic& mg, cons
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            top[nt][e] *= Q.f[nt][e];
+            if (!kMod) top[nt][e] *= Q.f[nt][e];
             move |= top[nt][e] > st.top[nt][e];
         }
     if (__any_sync(0xffffffffu, move)) {
@@ -447,8 +555,8 @@ __device__ __forceinline__ void pd_units(const uint8_t* u, const Magic& mg, cons
             for (int e = 0; e < 2; ++e) {
                 const float z = kEdge && st.m[nt][e] == -INFINITY ? 0.f : st.m[nt][e];
                 // (product and difference rounded apart, as the references were: fused, logits beyond 2^26 differ from theirs by more than a weight's range)
-                p[e] = ex2(__fmul_rn(s[i][nt][e], Q.f[nt][e]) - z);
-                p[2 + e] = ex2(__fmul_rn(s[i][nt][2 + e], Q.f[nt][e]) - z);
+                p[e] = ex2((kMod ? s[i][nt][e] : __fmul_rn(s[i][nt][e], Q.f[nt][e])) - z);
+                p[2 + e] = ex2((kMod ? s[i][nt][2 + e] : __fmul_rn(s[i][nt][2 + e], Q.f[nt][e])) - z);
                 st.l[nt][e] += p[e] + p[2 + e];
             }
             b[nt][0] = transposed(pack_half2(p[0], p[1]));
@@ -508,7 +616,7 @@ __device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {
 }
 
 // kStages 2: two CTAs on an SM hide each other's latencies.  4: one CTA on an SM, alone with them.
-template <int NT, typename T, bool kCluster, int kStages>
+template <int NT, typename T, bool kCluster, int kStages, bool kMod>
 __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(const PdParams P) {
     extern __shared__ __align__(128) uint8_t smem_raw[];
     using Smem = PdSmem<NT, kStages>;
@@ -556,7 +664,7 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
         const uint32_t in_seq = t - (uint32_t)g.seq * per_seq;
         g.cb = (int)(in_seq / P.n_kv);
         g.h = (int)(in_seq - (uint32_t)g.cb * P.n_kv);
-        g.s = pd_seq(P, g.seq);
+        g.s = pd_seq<kMod>(P, g.seq);
         if (g.cb * kCols >= g.s.n * P.gqa) {         // (the whole cluster)
             if (n_rank > 1) cluster_wait();
             return;
@@ -565,7 +673,7 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
     } else {
         // rows of sequences that have none of their tokens cached
         for (int i = blockIdx.x; i < P.n_seq; i += P.n_cta) {
-            const SeqInfo s = pd_seq(P, i);
+            const SeqInfo s = pd_seq<kMod>(P, i);
             if (s.len > 0) continue;
             for (int row = warp; row < s.n * P.n_q; row += kPdWarps) {
                 const int qp = row / P.n_q, hq = row - qp * P.n_q;
@@ -574,14 +682,14 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
             }
         }
         uint32_t total, share = 0;
-        pd_find<NT>(P, S.scan, total, g.seq, seq_start, [&](uint32_t t) {
+        pd_find<NT, kMod>(P, S.scan, total, g.seq, seq_start, [&](uint32_t t) {
             share = pd_share(P, t);
             return (uint32_t)blockIdx.x * share;
         });
         if ((uint64_t)blockIdx.x * share >= total || g.seq < 0) return;
         begin = pos = blockIdx.x * share;
         end = (uint32_t)min((uint64_t)total, (uint64_t)begin + share);
-        g.s = pd_seq(P, g.seq);
+        g.s = pd_seq<kMod>(P, g.seq);
         if (g.s.len == 0) return;                    // (row ranges that do not follow one another: the list is not one then)
         count = at_pos();
         if (g.n <= 0) return;
@@ -594,7 +702,7 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
     auto issue = [&](const Segment& sg, Copies& w, int stage) {
         const int k = w.issued++;
         if ((k & 15) == 0) {
-            const int kk = k + (lane >> 1), unit = 2 * (sg.first + warp + kPdWarps * kk) + (lane & 1);
+            const int kk = k + (lane >> 1), unit = 2 * sg.s.batch(sg.first + warp + kPdWarps * kk) + (lane & 1);
             w.from = nullptr;
             if (kk < w.n && unit < (sg.s.len + kUnitTok - 1) / kUnitTok) {
                 const int col = unit / P.pool.units, page = P.table[(int64_t)sg.seq * P.tb_st + col];
@@ -617,8 +725,9 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
         Copies w{nullptr, 0, 0, 0, false};
         // batches that no row of the block sees are left out
         const int last_row = min((sg.cb + 1) * kCols, sg.s.n * P.gqa) - 1;
-        const int lim_max = P.causal ? max(0, sg.s.len - sg.s.n + 1 + last_row / P.gqa) : sg.s.len;
-        const int n = min(sg.n, max(0, (lim_max + kBatchTok - 1) / kBatchTok - sg.first));
+        const int lim_max = P.causal ? max(kMod ? sg.s.pre : 0, sg.s.len - sg.s.n + 1 + last_row / P.gqa) : sg.s.len;
+        const int reached = (lim_max + kBatchTok - 1) / kBatchTok;
+        const int n = min(sg.n, max(0, (kMod && reached > sg.s.head ? max(sg.s.head, reached - sg.s.skip) : reached) - sg.first));
         w.n = max(0, (n - warp + kPdWarps - 1) / kPdWarps);
         if (ok)
             while (w.issued < min(w.n, kStages)) issue(sg, w, w.issued);
@@ -636,13 +745,31 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int row = row0 + 8 * nt + 2 * c + e;
-                lim[nt][e] = P.causal && row < n_rows ? max(0, behind + row / P.gqa) : g.s.len;
+                lim[nt][e] = P.causal && row < n_rows ? max(kMod ? g.s.pre : 0, behind + row / P.gqa) : g.s.len;
             }
-        const int lim_min = P.causal ? max(0, behind + row0 / P.gqa) : g.s.len;
+        const int lim_min = P.causal ? max(kMod ? g.s.pre : 0, behind + row0 / P.gqa) : g.s.len;
+        Marks<NT> mk;
+        int lo_max = 0;                                      // the last of the columns' windows begins here
+        if (kMod) {
+            mk.pre = g.s.pre;
+            mk.cap = P.sc.cap;
+            mk.cap_inv = P.sc.cap_inv;
+            mk.biased = P.sc.slopes != nullptr;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int row = row0 + 8 * nt + 2 * c + e, at = row / P.gqa;
+                    mk.pos[nt][e] = behind + at - 1;
+                    mk.lo[nt][e] = P.sc.window ? max(0, max(0, behind + at) - P.sc.window) : 0;
+                    mk.slope[nt][e] = mk.biased && row < n_rows ? P.sc.slopes[g.h * P.gqa + row - at * P.gqa] * 1.44269504088896340736f : 0.f;
+                }
+            if (P.sc.window) lo_max = max(0, max(0, behind + (min(row0 + kCols, n_rows) - 1) / P.gqa) - P.sc.window);
+        }
         State<NT> st = {};
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) st.m[nt][0] = st.m[nt][1] = st.top[nt][0] = st.top[nt][1] = -INFINITY;
-        int t0 = (g.first + warp) * kBatchTok, stage = 0;
+        int t0 = g.s.batch(g.first + warp) * kBatchTok, stage = 0;
         for (int k = 0; k < w.n && ok; ++k) {
             if (!__all_sync(0xffffffffu, mbar_wait_bounded(&S.full[warp][stage], phases >> stage & 1u))) {
                 ok = false;
@@ -651,21 +778,21 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
             phases ^= 1u << stage;
             const uint8_t* const tile = S.ring[warp][stage];
             const uint32_t there = w.have >> (2 * stage) & 3u;
-            if (there == 3u && t0 + kBatchTok <= lim_min) {
+            if (there == 3u && t0 + kBatchTok <= lim_min && (!kMod || t0 >= lo_max || t0 + kBatchTok <= g.s.pre)) {
                 if (NT == 1) {
-                    pd_units<NT, 2, false>(tile, mg, Q, st, r, c, t0, g.s.len, lim);
+                    pd_units<NT, 2, false, kMod>(tile, mg, Q, st, r, c, t0, g.s.len, lim, mk);
                 } else {
-                    pd_units<NT, 1, false>(tile, mg, Q, st, r, c, t0, g.s.len, lim);
-                    pd_units<NT, 1, false>(tile + kUnitBytes, mg, Q, st, r, c, t0 + kUnitTok, g.s.len, lim);
+                    pd_units<NT, 1, false, kMod>(tile, mg, Q, st, r, c, t0, g.s.len, lim, mk);
+                    pd_units<NT, 1, false, kMod>(tile + kUnitBytes, mg, Q, st, r, c, t0 + kUnitTok, g.s.len, lim, mk);
                 }
             } else {
 #pragma unroll 1
                 for (int i = 0; i < 2; ++i)
-                    if (there >> i & 1u) pd_units<NT, 1, true>(tile + i * kUnitBytes, mg, Q, st, r, c, t0 + i * kUnitTok, g.s.len, lim);
+                    if (there >> i & 1u) pd_units<NT, 1, true, kMod>(tile + i * kUnitBytes, mg, Q, st, r, c, t0 + i * kUnitTok, g.s.len, lim, mk);
             }
             __syncwarp();
             if (w.issued < w.n) issue(g, w, stage);
-            t0 += kPdWarps * kBatchTok;
+            t0 = kMod ? g.s.batch(g.first + warp + kPdWarps * (k + 1)) * kBatchTok : t0 + kPdWarps * kBatchTok;
             stage = stage == kStages - 1 ? 0 : stage + 1;
         }
         if (!ok)             // copies in flight land before the CTA leaves; nothing more is fetched
@@ -687,7 +814,7 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
                     break;
                 }
                 seq_start += pd_work<NT>(P, next.s);
-                next.s = pd_seq(P, ++next.seq);
+                next.s = pd_seq<kMod>(P, ++next.seq);
             }
             more = pos < end;
             if (more) {
@@ -787,7 +914,7 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
 // Block (i, col): column col of a triple that is cut.  kByTriple (one query row per sequence, no more triples than CTAs): of triple i.  Otherwise of
 // the one that the end of CTA i's share cuts, if that is its first cut.  kWarps warps share the partials, four of a warp's requested at a
 // time.  Where the triples lie is looked up before the partials are there: the lengths were complete before the attention began.
-template <int NT, typename T, bool kByTriple, int kWarps>
+template <int NT, typename T, bool kByTriple, int kWarps, bool kMod>
 __global__ void __launch_bounds__(32 * kWarps) pg_merge_kernel(const PdParams P) {
     __shared__ ScanSmem scan;
     __shared__ float4 sum_o[kWarps][32];
@@ -801,17 +928,17 @@ __global__ void __launch_bounds__(32 * kWarps) pg_merge_kernel(const PdParams P)
         const int wanted = blockIdx.x / P.n_kv;
         uint32_t before = 0;
         for (int i = 0; i < wanted; i += 32)
-            if (i + lane < wanted) before += pd_work<NT>(P, pd_seq(P, i + lane));
+            if (i + lane < wanted) before += pd_work<NT>(P, pd_seq<kMod>(P, i + lane));
         uint32_t rest = 0;
         for (int i = wanted; i < P.n_seq; i += 32)
-            if (i + lane < P.n_seq) rest += pd_work<NT>(P, pd_seq(P, i + lane));
+            if (i + lane < P.n_seq) rest += pd_work<NT>(P, pd_seq<kMod>(P, i + lane));
         seq_start = __reduce_add_sync(0xffffffffu, before);
         total = seq_start + __reduce_add_sync(0xffffffffu, rest);
         share = pd_share(P, total);
         seq = wanted;
         triple = blockIdx.x - (uint32_t)wanted * P.n_kv;
     } else {
-        pd_find<NT>(P, scan, total, seq, seq_start, [&](uint32_t t) {
+        pd_find<NT, kMod>(P, scan, total, seq, seq_start, [&](uint32_t t) {
             share = pd_share(P, t);
             return ((uint32_t)blockIdx.x + 1) * share;
         });
@@ -820,7 +947,7 @@ __global__ void __launch_bounds__(32 * kWarps) pg_merge_kernel(const PdParams P)
     }
     grid_dependency_wait();
     if (seq < 0) return;
-    const SeqInfo s = pd_seq(P, seq);
+    const SeqInfo s = pd_seq<kMod>(P, seq);
     if (s.len == 0) return;
     const uint32_t np = pd_places(P, s);
     if (!kByTriple) triple = ((blockIdx.x + 1) * share - seq_start) / np;
@@ -882,10 +1009,10 @@ __global__ void __launch_bounds__(32 * kWarps) pg_merge_kernel(const PdParams P)
     pd_write<T>(P, s, cb, kCols, col, h, lane, o, m, l);
 }
 
-template <int NT, typename T>
+template <int NT, typename T, bool kMod>
 int pd_launch_split(const PdParams& P, bool merge, cudaStream_t stream) {
     constexpr int kStages = NT == 1 ? 2 : 4, smem = (int)sizeof(PdSmem<NT, kStages>);
-    const auto kernel = pg_attend_kernel<NT, T, false, kStages>;
+    const auto kernel = pg_attend_kernel<NT, T, false, kStages, kMod>;
     static std::atomic<uint64_t> allowed{0};
     if (!pg_allow_smem(kernel, smem, allowed)) return BGTQ_E_LAUNCH;
     if (!pg_launch_ok(launch_kernel(kernel, dim3(P.n_cta), dim3(kPdThreads), smem, stream, true, P))) return BGTQ_E_LAUNCH;
@@ -896,8 +1023,8 @@ int pd_launch_split(const PdParams& P, bool merge, cudaStream_t stream) {
     // As many warps as take a triple's partials in one pass, but not more: 8 triples of 37 partials 15.3 us with 8, 14.6 with 16 (20000
     // tokens); 160 of two or three 15.5 with 8 and 19.7 with 16.
     const int warps = !by_triple || P.n_cta <= 4 * triples ? 2 : P.n_cta <= 16 * triples ? 8 : 16;
-    const auto merging = !by_triple ? pg_merge_kernel<NT, T, false, 2>
-                         : warps == 2 ? pg_merge_kernel<NT, T, true, 2> : warps == 8 ? pg_merge_kernel<NT, T, true, 8> : pg_merge_kernel<NT, T, true, 16>;
+    const auto merging = !by_triple ? pg_merge_kernel<NT, T, false, 2, kMod>
+                         : warps == 2 ? pg_merge_kernel<NT, T, true, 2, kMod> : warps == 8 ? pg_merge_kernel<NT, T, true, 8, kMod> : pg_merge_kernel<NT, T, true, 16, kMod>;
     return pg_launch_ok(launch_kernel(merging, grid, dim3(32 * warps), 0, stream, true, P)) ? BGTQ_OK : BGTQ_E_LAUNCH;
 }
 template <int NT, int kStages>
@@ -920,9 +1047,9 @@ struct ClusterLaunch {
         cfg.numAttrs = 2;
     }
 };
-template <int NT, typename T, int kStages>
+template <int NT, typename T, int kStages, bool kMod>
 int pd_launch_cluster(const PdParams& P, int64_t triples, int n_rank, cudaStream_t stream) {
-    const auto kernel = pg_attend_kernel<NT, T, true, kStages>;
+    const auto kernel = pg_attend_kernel<NT, T, true, kStages, kMod>;
     ClusterLaunch<NT, kStages> L(triples, n_rank, stream);
     static std::atomic<uint64_t> allowed{0};
     if (!pg_allow_smem(kernel, L.kBase + 8 * L.kRow, allowed)) return BGTQ_E_LAUNCH;
@@ -934,7 +1061,7 @@ int pd_clusters(int n_rank, int dev) {
     static std::atomic<int> known[64][9];
     if (dev >= 0 && dev < 64)
         if (const int n = known[dev][n_rank].load(std::memory_order_relaxed)) return n;
-    const auto kernel = pg_attend_kernel<NT, __half, true, kStages>;
+    const auto kernel = pg_attend_kernel<NT, __half, true, kStages, false>;
     ClusterLaunch<NT, kStages> L(1, n_rank, nullptr);
     L.cfg.numAttrs = 1;
     static std::atomic<uint64_t> allowed{0};
@@ -946,11 +1073,16 @@ int pd_clusters(int n_rank, int dev) {
     if (dev >= 0 && dev < 64) known[dev][n_rank].store(n, std::memory_order_relaxed);
     return n;
 }
-template <int NT, typename T>
+template <int NT, typename T, bool kMod>
 int pd_launch(const PdParams& P, const PdForm& f, cudaStream_t stream) {
-    if (!f.n_rank) return pd_launch_split<NT, T>(P, f.merge, stream);
-    if (NT == 1 && f.alone) return pd_launch_cluster<NT, T, NT == 1 ? 4 : 2>(P, f.triples, f.n_rank, stream);
-    return pd_launch_cluster<NT, T, 2>(P, f.triples, f.n_rank, stream);
+    if (!f.n_rank) return pd_launch_split<NT, T, kMod>(P, f.merge, stream);
+    if (NT == 1 && f.alone) return pd_launch_cluster<NT, T, NT == 1 ? 4 : 2, kMod>(P, f.triples, f.n_rank, stream);
+    return pd_launch_cluster<NT, T, 2, kMod>(P, f.triples, f.n_rank, stream);
+}
+template <bool kMod>
+int pd_launch(const PdParams& P, const PdForm& f, bool bf16, cudaStream_t stream) {
+    if (f.nt == 1) return bf16 ? pd_launch<1, __nv_bfloat16, kMod>(P, f, stream) : pd_launch<1, __half, kMod>(P, f, stream);
+    return bf16 ? pd_launch<2, __nv_bfloat16, kMod>(P, f, stream) : pd_launch<2, __half, kMod>(P, f, stream);
 }
 
 bool aligned(const void* p, int64_t bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
@@ -970,8 +1102,15 @@ static int pd_tiles(int32_t n_q, int32_t n_kv, int32_t max_q) { return (int64_t)
 //   clusters  4.4 and 1.45 for each round while every CTA has an SM for itself, 2.1 where two share one; with 16 columns 5 and 1.95.
 //   list      5.6, the merging launch among them, and 2.25 for each round of the CTAs that are resident and one more; with 16 columns 9.
 //   tcgen05   20, unpacking at 4.2 MB (of 144 and 512 bytes per token and head) and 1.75 for each tile of a CTA.
-static PdForm pd_form(int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv, int32_t max_q, int64_t max_tokens, int32_t flags) {
+// With a window, a sequence costs what its rows see, not what it holds.
+static PdForm pd_form(int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv, int32_t max_q, int64_t max_tokens, int32_t flags, const PgScores* sc) {
     PdForm f{};
+    int64_t block_tokens = max_tokens;           // that 256 query rows see
+    if (sc && sc->window) {
+        const int64_t beside = sc->window + (sc->prefix ? (int64_t)sc->max_prefix + kBatchTok : 0) + kBatchTok, rows = kPfBlockRows / (n_q / n_kv);
+        block_tokens = std::min(max_tokens, beside + std::min<int64_t>(max_q, rows));
+        max_tokens = std::min(max_tokens, beside + max_q);
+    }
     int dev = 0, sms = 148;
     if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     const int64_t gqa = n_q / n_kv;
@@ -995,7 +1134,7 @@ static PdForm pd_form(int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv, i
     const double cluster = (f.nt == 1 ? 4.4 : 5.0) + (f.nt > 1 ? 1.95 : f.alone ? 1.45 : 2.1) * (double)(waves * ((rounds + n - 1) / n));
     const double split = (f.nt == 1 ? 5.6 : 9.0) + 2.25 * (most + (double)resident - 1) / (double)resident;
     if (!asked && f.nt > 1) {
-        const double pairs = (double)n_seq * n_kv, tiles = pairs * (double)((max_q * gqa + 255) / 256) * (double)((max_tokens + 127) / 128);
+        const double pairs = (double)n_seq * n_kv, tiles = pairs * (double)((max_q * gqa + 255) / 256) * (double)((block_tokens + 127) / 128);
         f.prefill = 20.0 + pairs * (double)max_tokens * 656e-6 / 4.2 + 1.75 * (tiles + sms - 1) / sms < (cluster < split ? cluster : split);
         if (f.prefill) return f;
     }
@@ -1003,13 +1142,38 @@ static PdForm pd_form(int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv, i
     return f;
 }
 
-extern "C" __attribute__((visibility("default"))) int64_t bgtq_paged_workspace_bytes(int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv,
-                                                                                      int32_t max_q, int64_t max_tokens, int32_t flags) {
+// The caller's scores as the kernels take them; false: nothing of them differs from plain attention.
+static bool pd_scores(const BgtqPagedScores* s, int64_t cap_tokens, PgScores& to) {
+    if (!s) return false;
+    to.slopes = s->slopes;
+    to.prefix = s->max_prefix > 0 ? s->prefix : nullptr;
+    to.cap = s->softcap * 1.44269504088896340736f;
+    to.cap_inv = s->softcap > 0.f ? 1.0f / to.cap : 0.f;
+    to.window = s->window < cap_tokens ? s->window : 0;      // (one that no sequence is longer than hides nothing)
+    to.max_prefix = s->max_prefix;
+    return to.slopes || to.prefix || to.cap > 0.f || to.window;
+}
+static int pd_scores_error(const BgtqPagedScores* s, const void* cu_q, int32_t flags) {
+    if (!s) return BGTQ_OK;
+    if (s->reserved || s->window < 0 || s->max_prefix < 0 || (s->window && cu_q && !(flags & BGTQ_PAGED_CAUSAL))) return BGTQ_E_BADARG;
+    return s->softcap == 0.f || (s->softcap >= 7.8886090522101181e-31f && s->softcap <= 1.2676506002282294e30f) ? BGTQ_OK : BGTQ_E_BADARG;
+}
+
+extern "C" __attribute__((visibility("default"))) int64_t bgtq_paged_scored_workspace_bytes(int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv,
+                                                                                             int32_t max_q, int64_t max_tokens, int32_t flags,
+                                                                                             const BgtqPagedScores* scores) {
     if (n_seq < 0 || n_tok < 0 || n_kv < 1 || n_q < 1 || n_q % n_kv || max_q < 1 || max_tokens < 0) return BGTQ_E_BADARG;
     if (n_q / n_kv > 8) return BGTQ_E_UNSUPPORTED;
-    const PdForm f = pd_form(n_seq, n_tok, n_q, n_kv, max_q, max_tokens, flags);
-    if (f.prefill) return paged_prefill_workspace(n_seq, n_tok, n_q / n_kv, n_kv, max_tokens);
+    if (const int e = pd_scores_error(scores, nullptr, flags)) return e;
+    PgScores sc;
+    const bool mod = pd_scores(scores, max_tokens, sc);
+    const PdForm f = pd_form(n_seq, n_tok, n_q, n_kv, max_q, max_tokens, flags, mod ? &sc : nullptr);
+    if (f.prefill) return paged_prefill_workspace(n_seq, n_tok, n_q / n_kv, n_kv, max_tokens, mod);
     return f.n_rank ? 0 : (int64_t)f.n_cta * 2 * 8 * f.nt * (kHD * 4 + 8);
+}
+extern "C" __attribute__((visibility("default"))) int64_t bgtq_paged_workspace_bytes(int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv,
+                                                                                      int32_t max_q, int64_t max_tokens, int32_t flags) {
+    return bgtq_paged_scored_workspace_bytes(n_seq, n_tok, n_q, n_kv, max_q, max_tokens, flags, nullptr);
 }
 
 extern "C" __attribute__((visibility("default"))) int bgtq_paged_attend(
@@ -1017,12 +1181,22 @@ extern "C" __attribute__((visibility("default"))) int bgtq_paged_attend(
     int32_t page_tokens, const int32_t* table, int64_t table_stride, int32_t table_cols, const int32_t* seq_lens, const int32_t* cu_q,
     int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv, int32_t max_q, int64_t max_tokens, float scale, int32_t flags,
     void* workspace, int64_t workspace_bytes, void* out, int64_t o_st, int64_t o_sh, float* lse, int32_t* status, void* stream) {
+    return bgtq_paged_attend_scored(q, q_st, q_sh, pages, page_stride, head_stride, n_pages, page_tokens, table, table_stride, table_cols, seq_lens, cu_q, n_seq,
+                                    n_tok, n_q, n_kv, max_q, max_tokens, scale, flags, nullptr, workspace, workspace_bytes, out, o_st, o_sh, lse, status, stream);
+}
+
+extern "C" __attribute__((visibility("default"))) int bgtq_paged_attend_scored(
+    const void* q, int64_t q_st, int64_t q_sh, const uint8_t* pages, int64_t page_stride, int64_t head_stride, int32_t n_pages,
+    int32_t page_tokens, const int32_t* table, int64_t table_stride, int32_t table_cols, const int32_t* seq_lens, const int32_t* cu_q,
+    int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv, int32_t max_q, int64_t max_tokens, float scale, int32_t flags, const BgtqPagedScores* scores,
+    void* workspace, int64_t workspace_bytes, void* out, int64_t o_st, int64_t o_sh, float* lse, int32_t* status, void* stream) {
     const int asked = (flags & BGTQ_PAGED_FORM_MASK) >> BGTQ_PAGED_FORM_SHIFT;
     pg_launched = 0;
     if (n_seq < 0 || n_tok < 0 || n_kv < 1 || n_q < 1 || table_cols < 0 || max_q < 1 || max_tokens < 0 ||
         (flags & ~(BGTQ_PAGED_BF16 | BGTQ_PAGED_CAUSAL | BGTQ_PAGED_FORM_MASK)) || (asked & (asked - 1) && asked < 14) || (asked == 14 && !cu_q) || asked == 13)
         return BGTQ_E_BADARG;
     if (!(scale == scale) || n_q % n_kv) return BGTQ_E_BADARG;
+    if (const int e = pd_scores_error(scores, cu_q, flags)) return e;
     if (n_q / n_kv > 8) return BGTQ_E_UNSUPPORTED;
     if (!cu_q && (n_tok != n_seq || max_q != 1)) return BGTQ_E_BADARG;
     if (n_seq == 0 || n_tok == 0) return BGTQ_OK;
@@ -1037,13 +1211,15 @@ extern "C" __attribute__((visibility("default"))) int bgtq_paged_attend(
     // CTAs write rows while others read their queries
     const PagedRows q_rows{reinterpret_cast<uintptr_t>(q), n_tok, n_q, q_st, q_sh}, o_rows{reinterpret_cast<uintptr_t>(out), n_tok, n_q, o_st, o_sh};
     if (!paged_rows_apart(o_rows) || !paged_rows_apart(q_rows, o_rows)) return BGTQ_E_BADARG;
-    PdForm f = pd_form(n_seq, n_tok, n_q, n_kv, max_q, max_tokens, flags);
+    PgScores sc{};
+    const bool mod = pd_scores(scores, max_tokens, sc);
+    PdForm f = pd_form(n_seq, n_tok, n_q, n_kv, max_q, max_tokens, flags, mod ? &sc : nullptr);
     const cudaStream_t st = (cudaStream_t)stream;
     if (f.prefill) {
-        if (!workspace || workspace_bytes < paged_prefill_workspace(n_seq, n_tok, n_q / n_kv, n_kv, max_tokens)) return BGTQ_E_BADARG;
+        if (!workspace || workspace_bytes < paged_prefill_workspace(n_seq, n_tok, n_q / n_kv, n_kv, max_tokens, mod)) return BGTQ_E_BADARG;
         return paged_prefill({{pages, page_stride, head_stride, n_pages, page_tokens / kUnitTok}, table, table_stride, seq_lens, cu_q, n_seq, n_tok, n_q,
                               n_kv, n_q / n_kv, (flags & BGTQ_PAGED_CAUSAL) ? 1 : 0, (flags & BGTQ_PAGED_BF16) ? 1 : 0, max_tokens, (int32_t)cap,
-                              reinterpret_cast<uint8_t*>(workspace), q, q_st, q_sh, scale * 1.44269504088896340736f, out, o_st, o_sh, lse, status},
+                              reinterpret_cast<uint8_t*>(workspace), q, q_st, q_sh, scale * 1.44269504088896340736f, out, o_st, o_sh, lse, status, mod, sc},
                              st);
     }
     f.merge = cap > kPdWarps * kBatchTok && f.n_cta > 1;
@@ -1055,8 +1231,7 @@ extern "C" __attribute__((visibility("default"))) int bgtq_paged_attend(
     PdParams P{{pages, page_stride, head_stride, n_pages, page_tokens / kUnitTok}, q, q_st, q_sh, table, table_stride, seq_lens, cu_q,
                (int32_t)cap, n_seq, n_tok, n_q, n_kv, n_q / n_kv, !cu_q || (flags & BGTQ_PAGED_CAUSAL) ? 1 : 0, f.merge ? 1 : kPdWarps, f.n_rank ? f.blocks_of_seq : f.n_cta,
                scale * 1.44269504088896340736f, out, o_st, o_sh, lse, reinterpret_cast<float*>(workspace),
-               reinterpret_cast<float2*>(reinterpret_cast<float*>(workspace) + (int64_t)f.n_cta * 2 * cols * kHD), status};
+               reinterpret_cast<float2*>(reinterpret_cast<float*>(workspace) + (int64_t)f.n_cta * 2 * cols * kHD), status, sc};
     const bool bf16 = flags & BGTQ_PAGED_BF16;
-    if (f.nt == 1) return bf16 ? pd_launch<1, __nv_bfloat16>(P, f, st) : pd_launch<1, __half>(P, f, st);
-    return bf16 ? pd_launch<2, __nv_bfloat16>(P, f, st) : pd_launch<2, __half>(P, f, st);
+    return mod ? pd_launch<true>(P, f, bf16, st) : pd_launch<false>(P, f, bf16, st);
 }

@@ -33,6 +33,7 @@ namespace {
 constexpr int kRows = 128;                      // M of a product
 constexpr int kBlocks = 2;                      // row blocks of a CTA
 constexpr int kBlockRows = kRows * kBlocks;
+static_assert(kBlockRows == kPfBlockRows, "as the form of a call is chosen for");
 constexpr int kBlockCost = 7, kLeastCost = 8;   // halves of a tile's cost: of a block beside its tiles, of a share
 constexpr int kPart = kPfTileTok * kHD * 2;     // bytes of an operand tile (32 KB)
 static_assert(2 * kPart == kPfTileBytes, "khat and vhat");
@@ -40,7 +41,8 @@ static_assert(2 * kPart == kPfTileBytes, "khat and vhat");
 // 256 query rows of a sequence.
 struct __align__(16) Block {
     int32_t si, row0, len, q0, n;               // sequence of the launch, first row; its tokens, first query row, queries
-    int32_t tiles, sees, pad;                   // tiles that its rows see, at least one; whether they see any
+    int32_t tiles, sees, gap;                   // tiles that its rows see, at least one; 1 + those of the prefix, 0: they see none; tiles left out behind those
+    __device__ __forceinline__ int tile(int k) const { return k + (gap && k >= sees - 1 ? gap : 0); }
 };
 
 struct Pf {
@@ -67,18 +69,25 @@ struct Pf {
     int64_t o_st, o_sh;
     float* lse;
     int32_t* status;
+    PgScores sc;                                // (kernels of kMod read it)
+    uint32_t* nan_bits;                         // kMod: (n_seq, n_h, max_tiles) x 4 groups x 128 tokens: those whose V is no number
 };
 
 struct Seq {
-    int len, q0, n;
+    int len, q0, n, pre;
 };
+template <bool kMod>
 __device__ __forceinline__ Seq pf_seq(const Pf& P, int i) {
     Seq s;
+    s.pre = 0;
     s.len = max(0, min(P.lens[i], P.cap));
     s.q0 = min(max(P.cu_q[i], 0), P.n_tok);
     s.n = max(0, min(P.cu_q[i + 1], P.n_tok) - s.q0);
+    if (kMod) s.pre = pg_prefix(P.sc, i, s.len);
     return s;
 }
+// First token of the window of a sequence's row
+__device__ __forceinline__ int pf_low(const Pf& P, const Seq& s, int pos) { return P.sc.window ? max(0, max(0, s.len - s.n + 1 + pos) - P.sc.window) : 0; }
 
 // ------------------------------------------------------------------------------------------------------------------
 // unpack: a warp per unit of 16 tokens.  Operand layout (no swizzle, K-major): element (row, k) at
@@ -102,12 +111,16 @@ __device__ __forceinline__ uint32_t half2_of(float a, float b) { return pack_hal
 __device__ __forceinline__ int pf_pos(const Pf& P, int row) {      // row / gqa, rows < 2^29
     return P.gqa_inv ? (int)__umulhi((uint32_t)row, P.gqa_inv) : row;
 }
+template <bool kMod>
 __device__ __forceinline__ Block pf_block(const Pf& P, int si, const Seq& s, int j) {
     const int last_pos = (min(s.n * P.gqa, (j + 1) * kBlockRows) - 1) / P.gqa;
-    const int t_max = P.causal ? max(0, s.len - s.n + 1 + last_pos) : s.len, tiles = (t_max + kPfTileTok - 1) / kPfTileTok;
-    return Block{si, j * kBlockRows, s.len, s.q0, s.n, max(1, tiles), tiles > 0, 0};
+    const int t_max = P.causal ? max(s.pre, s.len - s.n + 1 + last_pos) : s.len, tiles = (t_max + kPfTileTok - 1) / kPfTileTok;
+    if (!kMod) return Block{si, j * kBlockRows, s.len, s.q0, s.n, max(1, tiles), tiles > 0, 0};
+    const int head = (s.pre + kPfTileTok - 1) / kPfTileTok, gap = max(0, pf_low(P, s, j * kBlockRows / P.gqa) / kPfTileTok - head);
+    return Block{si, j * kBlockRows, s.len, s.q0, s.n, max(1, tiles - gap), tiles > 0 ? 1 + head : 0, gap};
 }
 // The list of blocks and the CTAs' shares, by one CTA of 256 threads.
+template <bool kMod>
 __device__ void pf_plan(const Pf& P) {
     __shared__ int sums[8];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -133,15 +146,16 @@ __device__ void pf_plan(const Pf& P) {
     int n_blocks = 0;
     for (int base = 0; base < P.n_seq; base += 256) {
         const int i = base + tid;
-        Seq s{0, 0, 0};
-        if (i < P.n_seq) s = pf_seq(P, P.seq0 + i);
+        Seq s{0, 0, 0, 0};
+        if (i < P.n_seq) s = pf_seq<kMod>(P, P.seq0 + i);
         const int w = (s.n * P.gqa + kBlockRows - 1) / kBlockRows;
         int all;
         const int at = n_blocks + scan(w, all);
         for (int k = 0; k < 32; ++k) {           // a warp writes the blocks of its sequences one after another
             const int n = __shfl_sync(0xffffffffu, w, k), to = __shfl_sync(0xffffffffu, at, k);
-            const Seq t{__shfl_sync(0xffffffffu, s.len, k), __shfl_sync(0xffffffffu, s.q0, k), __shfl_sync(0xffffffffu, s.n, k)};
-            for (int j = lane; j < n && to + j < P.max_blocks; j += 32) P.blk[to + j] = pf_block(P, base + 32 * warp + k, t, j);
+            const Seq t{__shfl_sync(0xffffffffu, s.len, k), __shfl_sync(0xffffffffu, s.q0, k), __shfl_sync(0xffffffffu, s.n, k),
+                        kMod ? __shfl_sync(0xffffffffu, s.pre, k) : 0};
+            for (int j = lane; j < n && to + j < P.max_blocks; j += 32) P.blk[to + j] = pf_block<kMod>(P, base + 32 * warp + k, t, j);
         }
         n_blocks = min(P.max_blocks, n_blocks + all);
     }
@@ -173,18 +187,20 @@ __device__ void pf_plan(const Pf& P) {
     if (tid == 0) P.start[P.n_cta + 1] = make_int4(n_blocks, 0, 0, 0);
 }
 
+template <bool kMod>
 __global__ void __launch_bounds__(256) pg_unpack_kernel(const Pf P) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int tile = blockIdx.x, hi = blockIdx.y, si = blockIdx.z;
     grid_launch_dependents();
     grid_dependency_wait();
     if (tile == P.max_tiles) {
-        if (hi == 0 && si == 0) pf_plan(P);
+        if (hi == 0 && si == 0) pf_plan<kMod>(P);
         return;
     }
-    const Seq s = pf_seq(P, P.seq0 + si);
+    const Seq s = pf_seq<kMod>(P, P.seq0 + si);
     const int unit = tile * (kPfTileTok / kUnitTok) + warp, left = s.len - unit * kUnitTok;
     if (s.n == 0 || tile * kPfTileTok >= s.len) return;
+    if (kMod && tile * kPfTileTok >= s.pre && (tile + 1) * kPfTileTok <= pf_low(P, s, 0)) return;         // (no row sees it)
     const uint8_t* u = nullptr;
     if (left > 0) {
         const int col = unit / P.pool.units, page = P.table[(int64_t)(P.seq0 + si) * P.tb_st + col];
@@ -195,8 +211,10 @@ __global__ void __launch_bounds__(256) pg_unpack_kernel(const Pf P) {
     }
     __shared__ uint8_t there[8];
     __shared__ int first_nan[4];
+    __shared__ uint32_t all_nan[16];
     if (lane == 0) there[warp] = u || left <= 0;
     if (threadIdx.x < 4) first_nan[threadIdx.x] = INT_MAX;
+    if (kMod && threadIdx.x < 16) all_nan[threadIdx.x] = 0;
     __syncthreads();
     if (hi == 0 && threadIdx.x == 0) {
         uint32_t m = 0;
@@ -232,6 +250,7 @@ __global__ void __launch_bounds__(256) pg_unpack_kernel(const Pf P) {
         float s0 = a ? pg_lo(*reinterpret_cast<const uint16_t*>(u + kUnitVs + 16 * p + 2 * n)) : 0.f;
         float s1 = b ? pg_lo(*reinterpret_cast<const uint16_t*>(u + kUnitVs + 16 * p + 8 + 2 * n)) : 0.f;
         // A product with it would reach the rows that do not see it, too: zero here, and the rows that do are told
+        if (kMod && (s0 != s0 || s1 != s1)) atomicOr(&all_nan[4 * n + (warp >> 1)], ((s0 != s0 ? 1u : 0u) | (s1 != s1 ? 2u : 0u)) << (16 * (warp & 1) + 2 * p));
         if (s1 != s1) {
             atomicMin(&first_nan[n], unit * kUnitTok + 2 * p + 1);
             s1 = 0.f;
@@ -258,6 +277,7 @@ __global__ void __launch_bounds__(256) pg_unpack_kernel(const Pf P) {
     __syncthreads();
     if (threadIdx.x == 0)
         P.nan[((int64_t)si * P.n_h + hi) * P.max_tiles + tile] = make_int4(first_nan[0], first_nan[1], first_nan[2], first_nan[3]);
+    if (kMod && threadIdx.x < 16) P.nan_bits[16 * (((int64_t)si * P.n_h + hi) * P.max_tiles + tile) + threadIdx.x] = all_nan[threadIdx.x];
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -317,6 +337,33 @@ struct Walk {
         tiles = b.sees ? run() : 0;
     }
 };
+
+// Products of 32 tokens -> logits to the base of 2; ahead: of the first one of this row's place.
+__device__ __forceinline__ void pf_shape(const PgScores& sc, float (&x)[32], float factor, float slope, float ahead) {
+#pragma unroll
+    for (int c = 0; c < 32; ++c) x[c] *= factor;
+    if (sc.cap > 0.f) {
+        bool far = false;
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+            x[c] *= sc.cap_inv;
+            far |= !(fabsf(x[c]) <= 0.5f);
+        }
+        if (__any_sync(0xffffffffu, far)) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+                const float f = pg_cap_far(x[c], sc.cap);
+                x[c] = fabsf(x[c]) <= 0.5f ? pg_cap_near(x[c], sc.cap) : f;
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) x[c] = pg_cap_near(x[c], sc.cap);
+        }
+    }
+    if (sc.slopes)
+#pragma unroll
+        for (int c = 0; c < 32; ++c) x[c] = fmaf(-slope, fabsf(ahead + (float)c), x[c]);
+}
 
 struct PfSmem {
     __align__(128) uint8_t q[kBlocks][kPart];
@@ -401,7 +448,9 @@ __device__ __forceinline__ bool pf_wait(PfSmem& S, uint64_t* bar, uint32_t parit
     return false;
 }
 
-template <typename T>
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+
+template <typename T, bool kMod>
 __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
     extern __shared__ __align__(128) uint8_t smem_raw[];
     PfSmem& S = *reinterpret_cast<PfSmem*>(smem_raw);
@@ -436,12 +485,13 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
             asm volatile("fence.proxy.async.global;" ::: "memory");     // the tiles: another launch's stores -> bulk copies
             int n = 0;                                                  // parts so far
             for (Walk w(P); w.left > 0 && ok;) {
-                const uint8_t* src = P.tiles + (((int64_t)w.b.si * P.n_h + w.h) * P.max_tiles + w.t0) * kPfTileBytes;
+                const uint8_t* src = P.tiles + (((int64_t)w.b.si * P.n_h + w.h) * P.max_tiles + (kMod ? 0 : w.t0)) * kPfTileBytes;
                 for (int k = 0; k < 2 * w.tiles; ++k, ++n) {
                     const int slot = n % kSlots;
                     if (n >= kSlots && !pf_wait(S, &S.empty[slot], (uint32_t)(n / kSlots - 1) & 1u)) { ok = false; break; }
                     mbar_arrive_expect_tx(&S.full[slot], kPart);
-                    bulk_g2s(S.ring[slot], src + (size_t)k * kPart, kPart, &S.full[slot]);
+                    const int part = kMod ? 2 * w.b.tile(w.t0 + (k >> 1)) + (k & 1) : k;
+                    bulk_g2s(S.ring[slot], src + (size_t)part * kPart, kPart, &S.full[slot]);
                 }
                 if (!w.more()) break;
                 w.step(P.blk[w.next_g()]);
@@ -606,7 +656,7 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(&next.b) + 16 * lane),
                              "l"(reinterpret_cast<const uint8_t*>(P.blk + w.next_g()) + 16 * lane) : "memory");
             for (int t = tid & 255; t < tiles; t += 256) {
-                const int4 f = P.nan[((int64_t)w.b.si * P.n_h + w.h) * P.max_tiles + tile0 + t];
+                const int4 f = P.nan[((int64_t)w.b.si * P.n_h + w.h) * P.max_tiles + (kMod ? w.b.tile(tile0 + t) : tile0 + t)];
                 if (min(min(f.x, f.y), min(f.z, f.w)) != INT_MAX) {
                     atomicMin(&S.nan[mb][0], f.x);
                     atomicMin(&S.nan[mb][1], f.y);
@@ -615,32 +665,53 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                 }
             }
             bar_and(3 + mb, 256, true);                // (exponents are there)
-            int lim;
+            int lim, lo = 0, pre = 0, at = 0;        // tokens that this row sees: below lim, and from lo on or below pre; its own place
+            float slope = 0.f;
             {
                 // (rows behind the last one, zeros, compute what that one's limit lets them: with none of the tokens each of their tiles
                 // would be one that is cut, and these blocks, 1.6 times as long as the others, the launch's end)
                 const int g = w.b.row0 + kRows * mb + r128, pos = min(pf_pos(P, g), w.b.n - 1);
                 lim = P.causal ? max(0, min(w.b.len, w.b.len - w.b.n + 1 + pos)) : w.b.len;
+                if (kMod) {
+                    const Seq s{w.b.len, w.b.q0, w.b.n, 0};
+                    pre = pg_prefix(P.sc, P.seq0 + w.b.si, w.b.len);
+                    lim = max(lim, pre);
+                    lo = pf_low(P, s, pos);
+                    at = w.b.len - w.b.n + pos;
+                    const int g_pos = pf_pos(P, g);
+                    if (P.sc.slopes) slope = P.sc.slopes[(P.h0 + w.h) * P.gqa + g - g_pos * P.gqa] * 1.44269504088896340736f;
+                }
             }
             float down0, down1;
             pg_pow2(-S.ex[mb][r128], down0, down1);
             const float sc = fmaxf((P.scale_log2 == 0.f ? 1.f : fabsf(P.scale_log2)) * down0 * down1, kPgFactorMin);
-            const uint8_t* const valid = P.valid + (int64_t)w.b.si * P.max_tiles + tile0;
-            uint32_t units = tiles > 0 ? valid[0] : 0;
+            // kMod with a cap or slopes: logits are finished as they are loaded, and nothing is left to be multiplied by
+            const bool shaped = kMod && (P.sc.cap > 0.f || P.sc.slopes);
+            const float fac = kMod && shaped ? 1.f : sc;
+            const uint8_t* const valid = P.valid + (int64_t)w.b.si * P.max_tiles + (kMod ? 0 : tile0);
+            auto place = [&](int i) { return kMod ? w.b.tile(tile0 + i) : i; };              // of a tile among the sequence's valid[]
+            uint32_t units = tiles > 0 ? valid[place(0)] : 0;
             float m_used = -INFINITY, lsum = 0.f;    // what this row scales by (log2), this half's denominator
             bool huge = false;                       // logits whose steps in fp32 are no longer small beside a weight's range
             for (int i = 0; i < tiles; ++i) {
                 if (!__all_sync(0xffffffffu, pf_wait(S, &S.s_ready[mb], (uint32_t)(done + i) & 1u))) ok = false;
                 tc_fence_after_sync();
-                const int t0 = (tile0 + i) * kPfTileTok + 64 * hf;
+                const int t0 = (kMod ? place(i) : tile0 + i) * kPfTileTok + 64 * hf;
                 const uint32_t there = units >> (4 * hf) & 15u;
-                if (i + 1 < tiles) units = valid[i + 1];
-                const bool cut = !__all_sync(0xffffffffu, t0 + 64 <= lim) || there != 15u;     // tiles that reach a row's limit, or lack a page
+                if (i + 1 < tiles) units = valid[place(i + 1)];
+                // tiles that reach a row's limit, or lack a page
+                const bool cut = !__all_sync(0xffffffffu, t0 + 64 <= lim && (!kMod || t0 >= lo || t0 + 64 <= pre)) || there != 15u;
                 float sv[32];
                 auto load = [&](int c0) {
                     tmem_ld32(sS + (uint32_t)c0, sv);
                     tmem_ld_wait();
-                    if (cut) {
+                    if (kMod && shaped) pf_shape(P.sc, sv, sc, slope, (float)(t0 + c0 - at));
+                    if (kMod && cut) {
+                        const uint32_t seen = bits_below(lim - t0 - c0) & (~bits_below(lo - t0 - c0) | bits_below(pre - t0 - c0)) &
+                                              ((there >> (c0 >> 4) & 1u ? 0xffffu : 0u) | (there >> (c0 >> 4) & 2u ? 0xffff0000u : 0u));
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) sv[c] = seen >> c & 1u ? sv[c] : -INFINITY;
+                    } else if (cut) {
 #pragma unroll
                         for (int c = 0; c < 32; ++c) sv[c] = t0 + c0 + c < lim && (there >> ((c0 + c) >> 4) & 1u) ? sv[c] : -INFINITY;
                     }
@@ -657,7 +728,7 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                 load(32);
                 float m_half = top();
                 load(0);
-                m_half = fmaxf(m_half, top()) * sc;
+                m_half = fmaxf(m_half, top()) * fac;
                 const bool last = more && i + 1 == tiles;
                 if (last && w8 == 0) {                 // (the next block's record)
                     asm volatile("cp.async.wait_all;" ::: "memory");
@@ -689,13 +760,13 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                 }
                 if (last && w.next_tiles(next.b) > 0) fetch(next.b, w.next_h());        // (the last product with the queries is done)
                 const float z = m_used == -INFINITY ? 0.f : m_used;
-                const uint64_t nz2 = pack_f2(-z, -z), sc2 = huge ? pack_f2(1.f, 1.f) : pack_f2(sc, sc);
+                const uint64_t nz2 = pack_f2(-z, -z), sc2 = huge ? pack_f2(1.f, 1.f) : pack_f2(fac, fac);
                 uint64_t ps[2] = {0ull, 0ull};
                 auto put = [&](uint32_t c0) {       // P of the columns in sv -> 16 columns of the half's own part of S
                     uint32_t pk[16];
                     if (huge) {                     // product and difference rounded apart, as the reference was
 #pragma unroll
-                        for (int c = 0; c < 32; ++c) sv[c] = __fmul_rn(sv[c], sc);
+                        for (int c = 0; c < 32; ++c) sv[c] = __fmul_rn(sv[c], fac);
                     }
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
@@ -750,7 +821,20 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                 ok = __all_sync(0xffffffffu, pf_wait(S, &S.o_ready[mb], (uint32_t)(done - 1) & 1u));
                 tc_fence_after_sync();
             }
-            const bool bad0 = S.nan[mb][2 * hf] < lim, bad1 = S.nan[mb][2 * hf + 1] < lim;
+            bool bad0 = S.nan[mb][2 * hf] < lim, bad1 = S.nan[mb][2 * hf + 1] < lim;
+            if (kMod && (bad0 || bad1)) {              // (the first may be hidden, and a later one not)
+                bad0 = bad1 = false;
+                for (int i = 0; i < tiles; ++i) {
+                    const int tile = place(i);
+                    const uint32_t* const bits = P.nan_bits + 16 * (((int64_t)w.b.si * P.n_h + w.h) * P.max_tiles + tile) + 8 * hf;
+                    for (int k = 0; k < 4; ++k) {
+                        const int t = tile * kPfTileTok + 32 * k;
+                        const uint32_t seen = bits_below(lim - t) & (~bits_below(lo - t) | bits_below(pre - t));
+                        bad0 |= (bits[k] & seen) != 0;
+                        bad1 |= (bits[4 + k] & seen) != 0;
+                    }
+                }
+            }
             bar_and(3 + mb, 256, true);                // (maxima, and which numbers are none, are read before their places change)
             S.xch[mb][hf][r128] = lsum;
             if ((tid & 255) < 4) S.nan[mb][tid & 3] = INT_MAX;
@@ -917,14 +1001,14 @@ static void pf_parts(int n_seq, int n_kv, int64_t max_tokens, int& seqs, int& he
 
 // Where a launch's pieces lie in the workspace.
 struct PfLayout {
-    int64_t nan, part_o, part_ml, start, blk, first, valid, total;
+    int64_t nan, part_o, part_ml, start, blk, first, valid, nan_bits, total;
 };
 static int pf_ctas() {
     int dev = 0, sms = 148;
     if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     return sms;
 }
-static PfLayout pf_layout(int seqs, int heads, int64_t tiles, int64_t blocks, int n_cta) {
+static PfLayout pf_layout(int seqs, int heads, int64_t tiles, int64_t blocks, int n_cta, bool mod) {
     PfLayout L;
     L.nan = seqs * tiles * heads * (int64_t)kPfTileBytes;
     L.part_o = L.nan + seqs * tiles * heads * 16;
@@ -933,15 +1017,16 @@ static PfLayout pf_layout(int seqs, int heads, int64_t tiles, int64_t blocks, in
     L.blk = L.start + 16ll * (n_cta + 2);
     L.first = L.blk + (int64_t)sizeof(Block) * (blocks + 1);
     L.valid = L.first + 4 * (blocks + 1);
-    L.total = L.valid + seqs * tiles;
+    L.nan_bits = (L.valid + seqs * tiles + 15) / 16 * 16;
+    L.total = mod ? L.nan_bits + seqs * tiles * heads * 64 : L.valid + seqs * tiles;
     return L;
 }
 
-int64_t paged_prefill_workspace(int n_seq, int n_tok, int gqa, int n_kv, int64_t max_tokens) {
+int64_t paged_prefill_workspace(int n_seq, int n_tok, int gqa, int n_kv, int64_t max_tokens, bool mod) {
     int seqs, heads;
     int64_t tiles;
     pf_parts(n_seq, n_kv, max_tokens, seqs, heads, tiles);
-    return pf_layout(seqs, heads, tiles, (int64_t)n_tok * gqa / kBlockRows + n_seq, pf_ctas()).total;
+    return pf_layout(seqs, heads, tiles, (int64_t)n_tok * gqa / kBlockRows + n_seq, pf_ctas(), mod).total;
 }
 
 int paged_prefill(const PagedPrefill& A, cudaStream_t stream) {
@@ -952,12 +1037,14 @@ int paged_prefill(const PagedPrefill& A, cudaStream_t stream) {
     // (a launch's tiles are counted in 32 bits, rows to 2^29)
     if (2 * (double)blocks * (double)(tiles + 2) * heads > INT32_MAX || (int64_t)A.n_tok * A.gqa > 1 << 29) return BGTQ_E_TOOBIG;
     const int n_cta = pf_ctas();
-    const PfLayout L = pf_layout(seqs, heads, tiles, blocks, n_cta);
+    const PfLayout L = pf_layout(seqs, heads, tiles, blocks, n_cta, A.mod);
     uint8_t* const ws = A.workspace;
-    const auto kernel = A.bf16 ? pg_prefill_kernel<__nv_bfloat16> : pg_prefill_kernel<__half>;
+    const auto unpack = A.mod ? pg_unpack_kernel<true> : pg_unpack_kernel<false>;
+    const auto kernel = A.mod ? A.bf16 ? pg_prefill_kernel<__nv_bfloat16, true> : pg_prefill_kernel<__half, true>
+                        : A.bf16 ? pg_prefill_kernel<__nv_bfloat16, false> : pg_prefill_kernel<__half, false>;
     const auto merge = A.bf16 ? pg_prefill_merge_kernel<__nv_bfloat16> : pg_prefill_merge_kernel<__half>;
-    static std::atomic<uint64_t> allowed[2];
-    if (!pg_allow_smem(kernel, (int)sizeof(PfSmem), allowed[A.bf16])) return BGTQ_E_LAUNCH;
+    static std::atomic<uint64_t> allowed[4];
+    if (!pg_allow_smem(kernel, (int)sizeof(PfSmem), allowed[2 * A.mod + A.bf16])) return BGTQ_E_LAUNCH;
     for (int s0 = 0; s0 < A.n_seq; s0 += seqs)
         for (int h0 = 0; h0 < A.n_kv; h0 += heads) {
             const int ns = A.n_seq - s0 < seqs ? A.n_seq - s0 : seqs, nh = A.n_kv - h0 < heads ? A.n_kv - h0 : heads;
@@ -978,7 +1065,9 @@ int paged_prefill(const PagedPrefill& A, cudaStream_t stream) {
             P.max_blocks = (int32_t)blocks; P.n_cta = n_cta;
             P.q = A.q; P.q_st = A.q_st; P.q_sh = A.q_sh; P.scale_log2 = A.scale_log2;
             P.out = A.out; P.o_st = A.o_st; P.o_sh = A.o_sh; P.lse = A.lse; P.status = A.status;
-            if (!pg_launch_ok(launch_kernel(pg_unpack_kernel, dim3((unsigned)tiles + 1, nh, ns), dim3(256), 0, stream, true, P))) return BGTQ_E_LAUNCH;
+            P.sc = A.sc;
+            P.nan_bits = reinterpret_cast<uint32_t*>(ws + L.nan_bits);
+            if (!pg_launch_ok(launch_kernel(unpack, dim3((unsigned)tiles + 1, nh, ns), dim3(256), 0, stream, true, P))) return BGTQ_E_LAUNCH;
             if (!pg_launch_ok(launch_kernel(kernel, dim3(n_cta), dim3(kThreads), sizeof(PfSmem), stream, true, P))) return BGTQ_E_LAUNCH;
             if (!pg_launch_ok(launch_kernel(merge, dim3(n_cta - 1, kBlockRows / (8 * kMergeRows)), dim3(256), 0, stream, true, P))) return BGTQ_E_LAUNCH;
         }

@@ -5,6 +5,7 @@
 namespace bgtq {
 
 constexpr int kPfTileTok = 128;                             // cache tokens of a tile
+constexpr int kPfBlockRows = 256;                           // query rows that are attended together
 constexpr int kPfTileBytes = 2 * kPfTileTok * kHD * 2;      // its khat and vhat in the workspace
 
 struct PagedPrefill {
@@ -23,8 +24,10 @@ struct PagedPrefill {
     int64_t o_st, o_sh;
     float* lse;
     int32_t* status;
+    bool mod;                       // scores differ from plain ones
+    PgScores sc;
 };
-int64_t paged_prefill_workspace(int n_seq, int n_tok, int gqa, int n_kv, int64_t max_tokens);
+int64_t paged_prefill_workspace(int n_seq, int n_tok, int gqa, int n_kv, int64_t max_tokens, bool mod);
 int paged_prefill(const PagedPrefill& A, cudaStream_t stream);
 
 }  // namespace bgtq

@@ -298,18 +298,41 @@ def _copy(pages, src, dst, n_tokens, into):
     _lib.count_launch(lib.bgtq_paged_launches())
 
 
-def _attend(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, causal, scale, return_lse, status, out):
+def _attend(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, causal, scale, return_lse, status, out, softcap, slopes, window, prefix_lens, max_prefix):
     scale = _SCALE if scale is None else float(scale)
     flags = (_lib.PAGED_CAUSAL if causal else 0) | _FORM << _lib.PAGED_FORM_SHIFT
     host = _lib.host()
-    r = host.paged_attend(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, scale, flags, return_lse, status, out)
+    if softcap is None and slopes is None and window is None and prefix_lens is None:
+        scores = None
+        r = host.paged_attend(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, scale, flags, return_lse, status, out)
+    else:
+        scores = (slopes, prefix_lens, *_limits(softcap, window, causal), _most(max_prefix, "max_prefix_len"))
+        r = host.paged_attend(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, scale, flags, return_lse, status, out, *scores)
     if r is None:
-        return _attend_any(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, flags, scale, return_lse, status, out)
+        return _attend_any(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, flags, scale, return_lse, status, out, scores)
     return _lib.done(r, "bgtq_paged_attend", host.paged_launched())
 
 
+def _limits(softcap, window, causal):
+    """The cap and the window as numbers, 0 for none."""
+    if softcap is None:
+        softcap = 0.0
+    else:
+        softcap = float(softcap)
+        if not 2.0 ** -100 <= softcap <= 2.0 ** 100:
+            raise ValueError(f"softcap must be positive, 2^-100 to 2^100, got {softcap}")
+    if window is None:
+        return softcap, 0
+    window = operator.index(window)
+    if window < 1:
+        raise ValueError(f"window must be at least one token, got {window}")
+    if not causal:
+        raise ValueError("a window is counted back from a row's own position: causal attention only")
+    return softcap, min(window, 2 ** 31 - 1)
+
+
 @torch.no_grad()
-def _attend_any(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, flags, scale, return_lse, status, out):
+def _attend_any(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, flags, scale, return_lse, status, out, scores):
     """The attention for what the extension module leaves: tensors that have to be copied, empty ones, and errors."""
     page = _pool(pages)
     dev, n_kv = pages.device, pages.shape[1]
@@ -341,24 +364,33 @@ def _attend_any(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, flags,
     max_tokens = cap if max_tokens < 0 else min(max_tokens, cap)
     if math.isnan(scale):
         raise ValueError("scale is not a number")
+    sc = None
+    if scores is not None:
+        slopes, prefix, softcap, window, longest = scores
+        if slopes is not None:
+            slopes = _ints(slopes, "slopes", torch.float32, (n_q,), dev)
+        if prefix is not None:
+            prefix = _ints(prefix, "prefix_lens", torch.int32, (n_seq,), dev)
+        sc = _lib.PagedScores(_lib.ptr(slopes) or None, _lib.ptr(prefix) or None, softcap, window, max_tokens if longest < 0 else min(longest, max_tokens), 0)
     status, lib = _status(status, dev), _lib.lib()
     _lib.require_cuda(pages, "pages")
     if n and n_seq:
         with torch.cuda.device(dev):
-            need = lib.bgtq_paged_workspace_bytes(n_seq, n, n_q, n_kv, max_q, max_tokens, flags)
+            need = lib.bgtq_paged_scored_workspace_bytes(n_seq, n, n_q, n_kv, max_q, max_tokens, flags, sc)
             if need < 0:
                 _lib.check(need, "bgtq_paged_workspace_bytes")
             ws = torch.empty(need, dtype=torch.uint8, device=dev)
-            _lib.check(lib.bgtq_paged_attend(
+            _lib.check(lib.bgtq_paged_attend_scored(
                 q.data_ptr(), *q.stride()[:2], pages.data_ptr(), pages.stride(0), pages.stride(1), pages.shape[0], page,
                 block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(), _lib.ptr(cu_q), n_seq, n, n_q, n_kv,
-                max_q, max_tokens, scale, flags, ws.data_ptr(), need, out.data_ptr(), *out.stride()[:2], _lib.ptr(lse), status,
+                max_q, max_tokens, scale, flags, sc, ws.data_ptr(), need, out.data_ptr(), *out.stride()[:2], _lib.ptr(lse), status,
                 _lib.stream_ptr(dev)), "bgtq_paged_attend")
         _lib.count_launch(lib.bgtq_paged_launches())
     return (out, lse) if return_lse else out
 
 
-def paged_kv4_decode_attention(q, pages, block_table, seq_lens, scale=None, return_lse=False, status=None, out=None, max_seq_len=None):
+def paged_kv4_decode_attention(q, pages, block_table, seq_lens, scale=None, return_lse=False, status=None, out=None, max_seq_len=None, *,
+                               softcap=None, slopes=None, window=None, prefix_lens=None, max_prefix_len=None):
     """One query token of every sequence over its cached tokens: q (B, n_q, 128) fp16 or bf16 -> (B, n_q, 128) of the same type,
     with ``return_lse`` also (B, n_q) fp32, the natural logarithm of each row's sum of exponentials.
 
@@ -366,34 +398,43 @@ def paged_kv4_decode_attention(q, pages, block_table, seq_lens, scale=None, retu
     size]``; entries behind the sequence's end are not read.  A sequence without tokens gives zeros and -inf.  Query heads
     h * n_q / n_kv .. share KV head h, at most 8 of them.  ``max_seq_len``: sequences are held to it (default: what the table holds);
     a small one spares the launch what only long sequences need.  ``out``: where the result goes, like q, its rows apart from one
-    another and from q's (other columns of one buffer will do)."""
-    return _attend(q, pages, block_table, seq_lens, None, 1, _most(max_seq_len), True, scale, return_lse, status, out)
+    another and from q's (other columns of one buffer will do).
+
+    Layers that are no plain attention: ``softcap`` c: a logit x becomes c tanh(x / c).  ``slopes`` (n_q,) fp32, finite: less slope times the distance between
+    the query's position (the sequence's last) and the token's.  ``window``: of the tokens up to the query's own only the last so many are seen.
+    ``prefix_lens`` (B,) int32: a sequence's first so many tokens are seen in any case (sinks in front of a window); ``max_prefix_len``: they are held
+    to it (default: ``max_seq_len``), and with a window it chooses the launch.  Pages that no query sees are not read."""
+    return _attend(q, pages, block_table, seq_lens, None, 1, _most(max_seq_len), True, scale, return_lse, status, out, softcap, slopes, window, prefix_lens,
+                   max_prefix_len)
 
 
 def paged_kv4_prefill_attention(q, pages, block_table, seq_lens, cu_q, max_q_len=None, max_seq_len=None, causal=True, scale=None,
-                                return_lse=False, status=None, out=None):
+                                return_lse=False, status=None, out=None, *, softcap=None, slopes=None, window=None, prefix_lens=None,
+                                max_prefix_len=None):
     """Several query tokens of every sequence over its cached tokens, their own among them: q (n, n_q, 128), rows ``cu_q[b]`` ..
     ``cu_q[b + 1] - 1`` (``cu_q`` (B + 1,) int32) are the last positions of sequence b, and when ``causal`` each sees the tokens up to itself.
 
     ``max_q_len``: no sequence has more query rows (default: all of them; it chooses the launch, 0 the one of 1, and one that has
     more is attended all the same).  ``max_seq_len``: sequences are held to it (default: what the table holds).  With many rows per sequence and KV head the
     tokens are unpacked into a workspace from torch's allocator, 512 bytes per token of ``max_seq_len`` and KV head for every sequence, at
-    most 2 GiB at a time.  Rows behind ``cu_q[B]`` are not written.  Otherwise as :func:`paged_kv4_decode_attention`."""
+    most 2 GiB at a time.  Rows behind ``cu_q[B]`` are not written.  Otherwise as :func:`paged_kv4_decode_attention`: distances and the ``window``
+    (``causal`` only) count from the row's own position, and tokens of the prefix are seen by the rows in front of them too, at the distance between them."""
     if cu_q is None:
         raise ValueError("cu_q says which rows are whose")
     if max_q_len is not None and max_q_len < 0:
         raise ValueError("max_q_len must not be negative")
     rows = q.shape[0]
     max_q = max(1, rows if max_q_len is None else min(int(max_q_len), rows))
-    return _attend(q, pages, block_table, seq_lens, cu_q, max_q, _most(max_seq_len), causal, scale, return_lse, status, out)
+    return _attend(q, pages, block_table, seq_lens, cu_q, max_q, _most(max_seq_len), causal, scale, return_lse, status, out, softcap, slopes, window,
+                   prefix_lens, max_prefix_len)
 
 
-def _most(max_seq_len):
-    if max_seq_len is None:
+def _most(n, name="max_seq_len"):
+    if n is None:
         return -1
-    if max_seq_len < 0:
-        raise ValueError("max_seq_len must not be negative")
-    return int(max_seq_len)
+    if n < 0:
+        raise ValueError(f"{name} must not be negative")
+    return int(n)
 
 
 class PagedKV4Cache:

@@ -689,6 +689,26 @@ int bgtq_paged_attend(const void* q, int64_t q_st, int64_t q_sh, const uint8_t* 
                 int32_t max_q, int64_t max_tokens, float scale, int32_t flags, void* workspace, int64_t workspace_bytes,
                 void* out, int64_t o_st, int64_t o_sh, float* lse, int32_t* status, void* stream);
 
+/* What an attention does beside the plain one.  Row i of the n of a sequence is at position p = seq_lens[b] - n + i.  With x = scale * q . k its logit
+ * for token t is c tanh(x / c) - slope |p - t|, the first term x without a cap, the second none without slopes; it sees token t < seq_lens[b] if
+ * t < prefix[b], or if t <= p (any t without BGTQ_PAGED_CAUSAL) and t > p - window.  Rows that see none: zeros, lse -inf, as ever.  Of tokens that
+ * no row's window or prefix reaches, pages are not read (those beside them, in 128 tokens, may be). */
+typedef struct BgtqPagedScores {
+    const float* slopes;        /* device, (n_q), finite; NULL: no bias */
+    const int32_t* prefix;      /* device, (n_seq), held to 0 .. max_prefix; NULL: none */
+    float softcap;              /* c, 2^-100 .. 2^100; 0: no cap */
+    int32_t window;             /* tokens up to the row's own that it sees; 0: all.  Queries are causal then */
+    int32_t max_prefix;         /* it chooses the launch, too */
+    int32_t reserved;           /* 0 */
+} BgtqPagedScores;
+int64_t bgtq_paged_scored_workspace_bytes(int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv, int32_t max_q,
+                int64_t max_tokens, int32_t flags, const BgtqPagedScores* scores);
+int bgtq_paged_attend_scored(const void* q, int64_t q_st, int64_t q_sh, const uint8_t* pages, int64_t page_stride, int64_t head_stride,
+                int32_t n_pages, int32_t page_tokens, const int32_t* table, int64_t table_stride, int32_t table_cols,
+                const int32_t* seq_lens, const int32_t* cu_q, int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv,
+                int32_t max_q, int64_t max_tokens, float scale, int32_t flags, const BgtqPagedScores* scores, void* workspace,
+                int64_t workspace_bytes, void* out, int64_t o_st, int64_t o_sh, float* lse, int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
