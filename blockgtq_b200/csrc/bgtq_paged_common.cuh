@@ -86,12 +86,19 @@ __device__ __forceinline__ float pg_ex2(float x) {
 }
 // cap * tanh(x / cap), u = x / cap.  Up to 1/2 an odd polynomial of degree 9, fitted to the relative error (1.5e-8); beyond it 1 - 2 / (e^2u + 1), whose terms
 // are then of one magnitude, so that both are off by a few roundings of the result itself.
+struct CapNear {
+    static constexpr int kTerms = 5;
+    __device__ __forceinline__ static constexpr float k(int i) {
+        constexpr float c[kTerms] = {1.f, -0.3333314389579803f, 0.1332587894742629f, -0.05304549361635799f, 0.017241490183840052f};
+        return c[i];
+    }
+};
 __device__ __forceinline__ float pg_cap_near(float u, float cap) {
     const float v = u * u;
-    float p = fmaf(v, 0.017241490183840052f, -0.05304549361635799f);
-    p = fmaf(p, v, 0.1332587894742629f);
-    p = fmaf(p, v, -0.3333314389579803f);
-    return cap * u * fmaf(p, v, 1.f);
+    float p = CapNear::k(4);
+#pragma unroll
+    for (int i = 3; i >= 0; --i) p = fmaf(p, v, CapNear::k(i));
+    return cap * u * p;
 }
 __device__ __forceinline__ float pg_cap_far(float u, float cap) {
     float r;

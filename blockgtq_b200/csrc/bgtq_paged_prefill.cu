@@ -338,31 +338,86 @@ struct Walk {
     }
 };
 
-// Products of 32 tokens -> logits to the base of 2; ahead: of the first one of this row's place.
-__device__ __forceinline__ void pf_shape(const PgScores& sc, float (&x)[32], float factor, float slope, float ahead) {
+// What an attention's logits go through beside the scale.  Its rows may be masked in all forms but the plain one.
+enum Mode { kPlain, kMasked, kCapped, kBiased, kCappedBiased };
+
+// Logits under a cap, pairs at a time on the FMA pipe: u = x / cap, cap tanh(u) = u (cap + u^2 ...).  Most tiles' are small beside it: an odd polynomial of
+// degree 7 up to 5/16, of degree 19 up to 3/2, both fitted to the relative error (1.7e-8, 1.9e-8); beyond, or where products and differences have to be rounded
+// apart, one by one.  All of a warp's 32 tokens go one way.  (Two more values of the special function pipe for each logit would be twice the time of all
+// else: it makes 16 a cycle.)
+struct CapLow {
+    static constexpr int kTerms = 4;
+    static constexpr float kReach2 = 0.09765625f;
+    __device__ __forceinline__ static constexpr float k(int i) {
+        constexpr float c[kTerms] = {1.f, -0.33332987233884576f, 0.13311666824722448f, -0.0500755820287676f};
+        return c[i];
+    }
+};
+struct CapMid {
+    static constexpr int kTerms = 10;
+    static constexpr float kReach2 = 2.25f;
+    __device__ __forceinline__ static constexpr float k(int i) {
+        constexpr float c[kTerms] = {1.f, -0.3333322466769597f, 0.13331329487357702f, -0.0538386683456423f, 0.021448478261107542f, -0.00806102220738539f,
+                                     0.0026138976028419808f, -0.0006436921929764066f, 0.00010158802230323775f, -7.465266263465981e-06f};
+        return c[i];
+    }
+};
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// x[] = shape of products x[] times factor, less z; whether the polynomial reaches as far as they go (warp-wide)
+template <typename K>
+__device__ __forceinline__ bool pf_cap_pairs(float (&x)[32], float cap, float g, float z) {
+    const uint64_t g2 = pack_f2(g, g), nz = pack_f2(-z, -z);
+    float most[2] = {0.f, 0.f};
 #pragma unroll
-    for (int c = 0; c < 32; ++c) x[c] *= factor;
-    if (sc.cap > 0.f) {
-        bool far = false;
+    for (int c = 0; c < 32; c += 2) {
+        const uint64_t u = mul_f2(pack_f2(x[c], x[c + 1]), g2), v = mul_f2(u, u);
+        float v0, v1;
+        unpack_f2(v, v0, v1);
+        most[c >> 1 & 1] = max3(most[c >> 1 & 1], v0, v1);
+        uint64_t p = pack_f2(K::k(K::kTerms - 1) * cap, K::k(K::kTerms - 1) * cap);
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
-            x[c] *= sc.cap_inv;
-            far |= !(fabsf(x[c]) <= 0.5f);
+        for (int i = K::kTerms - 2; i >= 0; --i) p = fma_f2(p, v, pack_f2(K::k(i) * cap, K::k(i) * cap));
+        unpack_f2(fma_f2(u, p, nz), x[c], x[c + 1]);
+    }
+    return __all_sync(0xffffffffu, fmaxf(most[0], most[1]) <= K::kReach2);
+}
+__device__ __forceinline__ float pf_cap_any(float x, const PgScores& sc) {
+    const float u = x * sc.cap_inv, f = pg_cap_far(u, sc.cap);
+    return fabsf(u) <= 0.5f ? pg_cap_near(u, sc.cap) : f;
+}
+// x[]: 32 products, which `load` fetches anew
+template <typename Load>
+__device__ __forceinline__ void pf_cap(float (&x)[32], const PgScores& sc, bool apart, float factor, float z, Load load) {
+    if (!apart) {
+        if (pf_cap_pairs<CapLow>(x, sc.cap, factor * sc.cap_inv, z)) return;
+        load();
+        if (pf_cap_pairs<CapMid>(x, sc.cap, factor * sc.cap_inv, z)) return;
+        load();
+    }
+#pragma unroll
+    for (int c = 0; c < 32; ++c) x[c] = pf_cap_any(__fmul_rn(x[c], factor), sc) - z;
+}
+// x[] times factor less slope times the distances, the first one's `ahead` of the row's own place
+__device__ __forceinline__ void pf_bias(float (&x)[32], float factor, float slope, float ahead, bool both_sides) {
+    uint64_t d = pack_f2(ahead, ahead + 1.f);
+    const uint64_t two = pack_f2(2.f, 2.f), s2 = pack_f2(slope, slope), f2 = pack_f2(factor, factor);
+    if (both_sides) {
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+            unpack_f2(fma_f2(d | 0x8000000080000000ull, s2, mul_f2(pack_f2(x[c], x[c + 1]), f2)), x[c], x[c + 1]);
+            d = add_f2(d, two);
         }
-        if (__any_sync(0xffffffffu, far)) {
+    } else {
 #pragma unroll
-            for (int c = 0; c < 32; ++c) {
-                const float f = pg_cap_far(x[c], sc.cap);
-                x[c] = fabsf(x[c]) <= 0.5f ? pg_cap_near(x[c], sc.cap) : f;
-            }
-        } else {
-#pragma unroll
-            for (int c = 0; c < 32; ++c) x[c] = pg_cap_near(x[c], sc.cap);
+        for (int c = 0; c < 32; c += 2) {
+            unpack_f2(fma_f2(d, s2, mul_f2(pack_f2(x[c], x[c + 1]), f2)), x[c], x[c + 1]);
+            d = add_f2(d, two);
         }
     }
-    if (sc.slopes)
-#pragma unroll
-        for (int c = 0; c < 32; ++c) x[c] = fmaf(-slope, fabsf(ahead + (float)c), x[c]);
 }
 
 struct PfSmem {
@@ -422,11 +477,6 @@ __device__ __forceinline__ float max_nan(float a, float b) {             // NaN 
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
     return d;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
 __device__ __forceinline__ bool bar_or(uint32_t id, bool flag) {        // over the 256 threads of one block's rows
     uint32_t out;
     asm volatile(
@@ -450,8 +500,9 @@ __device__ __forceinline__ bool pf_wait(PfSmem& S, uint64_t* bar, uint32_t parit
 
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
-template <typename T, bool kMod>
+template <typename T, Mode kMode>
 __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
+    constexpr bool kMod = kMode != kPlain;
     extern __shared__ __align__(128) uint8_t smem_raw[];
     PfSmem& S = *reinterpret_cast<PfSmem*>(smem_raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -685,9 +736,8 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
             float down0, down1;
             pg_pow2(-S.ex[mb][r128], down0, down1);
             const float sc = fmaxf((P.scale_log2 == 0.f ? 1.f : fabsf(P.scale_log2)) * down0 * down1, kPgFactorMin);
-            // kMod with a cap or slopes: logits are finished as they are loaded, and nothing is left to be multiplied by
-            const bool shaped = kMod && (P.sc.cap > 0.f || P.sc.slopes);
-            const float fac = kMod && shaped ? 1.f : sc;
+            // kBiased: logits are finished as they are loaded, and nothing is left to be multiplied by
+            const float fac = kMode >= kBiased ? 1.f : sc;
             const uint8_t* const valid = P.valid + (int64_t)w.b.si * P.max_tiles + (kMod ? 0 : tile0);
             auto place = [&](int i) { return kMod ? w.b.tile(tile0 + i) : i; };              // of a tile among the sequence's valid[]
             uint32_t units = tiles > 0 ? valid[place(0)] : 0;
@@ -702,15 +752,18 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                 // tiles that reach a row's limit, or lack a page
                 const bool cut = !__all_sync(0xffffffffu, t0 + 64 <= lim && (!kMod || t0 >= lo || t0 + 64 <= pre)) || there != 15u;
                 float sv[32];
+                auto hide = [&](int c0) {              // kMod: what this row does not see of the tokens in sv
+                    const uint32_t seen = bits_below(lim - t0 - c0) & (~bits_below(lo - t0 - c0) | bits_below(pre - t0 - c0)) &
+                                          ((there >> (c0 >> 4) & 1u ? 0xffffu : 0u) | (there >> (c0 >> 4) & 2u ? 0xffff0000u : 0u));
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) sv[c] = seen >> c & 1u ? sv[c] : -INFINITY;
+                };
                 auto load = [&](int c0) {
                     tmem_ld32(sS + (uint32_t)c0, sv);
                     tmem_ld_wait();
-                    if (kMod && shaped) pf_shape(P.sc, sv, sc, slope, (float)(t0 + c0 - at));
+                    if (kMode >= kCapped) return;      // (made logits, and masked, elsewhere)
                     if (kMod && cut) {
-                        const uint32_t seen = bits_below(lim - t0 - c0) & (~bits_below(lo - t0 - c0) | bits_below(pre - t0 - c0)) &
-                                              ((there >> (c0 >> 4) & 1u ? 0xffffu : 0u) | (there >> (c0 >> 4) & 2u ? 0xffff0000u : 0u));
-#pragma unroll
-                        for (int c = 0; c < 32; ++c) sv[c] = seen >> c & 1u ? sv[c] : -INFINITY;
+                        hide(c0);
                     } else if (cut) {
 #pragma unroll
                         for (int c = 0; c < 32; ++c) sv[c] = t0 + c0 + c < lim && (there >> ((c0 + c) >> 4) & 1u) ? sv[c] : -INFINITY;
@@ -725,10 +778,34 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                     }
                     return max3(max3(a, c, c), sv[30], sv[31]);
                 };
-                load(32);
-                float m_half = top();
-                load(0);
-                m_half = fmaxf(m_half, top()) * fac;
+                float m_half;
+                if constexpr (kMode == kCapped) {      // caps keep the order: the largest product's logit is the largest
+                    load(32);
+                    if (cut) hide(32);
+                    m_half = top();
+                    load(0);
+                    if (cut) hide(0);
+                    m_half = fmaxf(m_half, top());
+                    if (m_half > -INFINITY) m_half = pf_cap_any(__fmul_rn(m_half, sc), P.sc);
+                } else if constexpr (kMode >= kBiased) {       // logits take their products' places
+                    m_half = -INFINITY;
+#pragma unroll 1
+                    for (int c0 = 32; c0 >= 0; c0 -= 32) {
+                        load(c0);
+                        if (kMode == kCappedBiased) pf_cap(sv, P.sc, false, sc, 0.f, [&] { load(c0); });
+                        // (tokens behind the row's own place are in its sight only where it lies in the prefix, or sees all)
+                        pf_bias(sv, kMode == kBiased ? sc : 1.f, slope, (float)(t0 + c0 - at), __any_sync(0xffffffffu, lim > at + 1 && t0 + c0 + 31 > at));
+                        if (cut) hide(c0);
+                        m_half = fmaxf(m_half, top());
+                        if (c0) tmem_st32(sS + 32u, sv);
+                    }
+                    tmem_st_wait();
+                } else {
+                    load(32);
+                    m_half = top();
+                    load(0);
+                    m_half = fmaxf(m_half, top()) * fac;
+                }
                 const bool last = more && i + 1 == tiles;
                 if (last && w8 == 0) {                 // (the next block's record)
                     asm volatile("cp.async.wait_all;" ::: "memory");
@@ -764,16 +841,25 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                 uint64_t ps[2] = {0ull, 0ull};
                 auto put = [&](uint32_t c0) {       // P of the columns in sv -> 16 columns of the half's own part of S
                     uint32_t pk[16];
-                    if (huge) {                     // product and difference rounded apart, as the reference was
+                    if constexpr (kMode == kCapped) {
+                        pf_cap(sv, P.sc, huge, sc, z, [&] { load(c0 ? 32 : 0); });
+                        if (cut) hide(c0 ? 32 : 0);
+                    }
+                    if (kMode != kCapped && huge) { // product and difference rounded apart, as the reference was
 #pragma unroll
                         for (int c = 0; c < 32; ++c) sv[c] = __fmul_rn(sv[c], fac);
                     }
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         float x0, x1, p0, p1;
-                        const uint64_t x = fma_f2(pack_f2(sv[2 * e], sv[2 * e + 1]), sc2, nz2);
-                        unpack_f2(x, x0, x1);
-                        if ((kPolyPairs >> e & 1) != 0) {
+                        if constexpr (kMode == kCapped) {
+                            x0 = sv[2 * e];
+                            x1 = sv[2 * e + 1];
+                        } else {
+                            const uint64_t x = fma_f2(pack_f2(sv[2 * e], sv[2 * e + 1]), sc2, nz2);
+                            unpack_f2(x, x0, x1);
+                        }
+                        if (kMode <= kMasked && (kPolyPairs >> e & 1) != 0) {
                             const uint64_t y = pack_f2(max_nan(x0, -125.f), max_nan(x1, -125.f));
                             pf_exp2_poly(y, p0, p1);
                             ps[e & 1] = fma_f2(y, 0ull, ps[e & 1]);      // (what is no number stays none in the denominator)
@@ -793,11 +879,20 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&S.p_ready[mb][part]);
                 };
-                put(0u);
-                tell(0);
-                load(32);
-                put(16u);
-                tell(1);
+                if constexpr (kMode >= kCapped) {      // (one piece of code for both: what it shapes logits with is long)
+#pragma unroll 1
+                    for (int part = 0; part < 2; ++part) {
+                        if (part || (kMode == kCapped && cut)) load(32 * part);
+                        put(16u * part);
+                        tell(part);
+                    }
+                } else {
+                    put(0u);
+                    tell(0);
+                    load(32);
+                    put(16u);
+                    tell(1);
+                }
                 float a0, a1;
                 unpack_f2(add_f2(ps[0], ps[1]), a0, a1);
                 lsum += a0 + a1;
@@ -1040,11 +1135,16 @@ int paged_prefill(const PagedPrefill& A, cudaStream_t stream) {
     const PfLayout L = pf_layout(seqs, heads, tiles, blocks, n_cta, A.mod);
     uint8_t* const ws = A.workspace;
     const auto unpack = A.mod ? pg_unpack_kernel<true> : pg_unpack_kernel<false>;
-    const auto kernel = A.mod ? A.bf16 ? pg_prefill_kernel<__nv_bfloat16, true> : pg_prefill_kernel<__half, true>
-                        : A.bf16 ? pg_prefill_kernel<__nv_bfloat16, false> : pg_prefill_kernel<__half, false>;
+    const int mode = !A.mod ? kPlain : A.sc.slopes ? A.sc.cap > 0.f ? kCappedBiased : kBiased : A.sc.cap > 0.f ? kCapped : kMasked;
+    constexpr decltype(&pg_prefill_kernel<__half, kPlain>) kernels[5][2] = {{pg_prefill_kernel<__half, kPlain>, pg_prefill_kernel<__nv_bfloat16, kPlain>},
+                                                                            {pg_prefill_kernel<__half, kMasked>, pg_prefill_kernel<__nv_bfloat16, kMasked>},
+                                                                            {pg_prefill_kernel<__half, kCapped>, pg_prefill_kernel<__nv_bfloat16, kCapped>},
+                                                                            {pg_prefill_kernel<__half, kBiased>, pg_prefill_kernel<__nv_bfloat16, kBiased>},
+                                                                            {pg_prefill_kernel<__half, kCappedBiased>, pg_prefill_kernel<__nv_bfloat16, kCappedBiased>}};
+    const auto kernel = kernels[mode][A.bf16];
     const auto merge = A.bf16 ? pg_prefill_merge_kernel<__nv_bfloat16> : pg_prefill_merge_kernel<__half>;
-    static std::atomic<uint64_t> allowed[4];
-    if (!pg_allow_smem(kernel, (int)sizeof(PfSmem), allowed[2 * A.mod + A.bf16])) return BGTQ_E_LAUNCH;
+    static std::atomic<uint64_t> allowed[10];
+    if (!pg_allow_smem(kernel, (int)sizeof(PfSmem), allowed[2 * mode + A.bf16])) return BGTQ_E_LAUNCH;
     for (int s0 = 0; s0 < A.n_seq; s0 += seqs)
         for (int h0 = 0; h0 < A.n_kv; h0 += heads) {
             const int ns = A.n_seq - s0 < seqs ? A.n_seq - s0 : seqs, nh = A.n_kv - h0 < heads ? A.n_kv - h0 : heads;
