@@ -26,6 +26,7 @@
 #include "bgtq_tcgen05.cuh"
 
 #include <limits.h>
+#include <string.h>
 
 namespace bgtq {
 namespace {
@@ -42,7 +43,10 @@ static_assert(2 * kPart == kPfTileBytes, "khat and vhat");
 struct __align__(16) Block {
     int32_t si, row0, len, q0, n;               // sequence of the launch, first row; its tokens, first query row, queries
     int32_t tiles, sees, gap;                   // tiles that its rows see, at least one; 1 + those of the prefix, 0: they see none; tiles left out behind those
-    __device__ __forceinline__ int tile(int k) const { return k + (gap && k >= sees - 1 ? gap : 0); }
+    template <bool kBack> __device__ __forceinline__ int tile(int k) const {     // kBack: the last one first
+        if (kBack) k = tiles - 1 - k;
+        return k + (gap && k >= sees - 1 ? gap : 0);
+    }
 };
 
 struct Pf {
@@ -70,6 +74,7 @@ struct Pf {
     float* lse;
     int32_t* status;
     PgScores sc;                                // (kernels of kMod read it)
+    uint64_t cap_low[4], cap_mid[10];           // the cap's polynomials, times the cap, each coefficient twice
     uint32_t* nan_bits;                         // kMod: (n_seq, n_h, max_tiles) x 4 groups x 128 tokens: those whose V is no number
 };
 
@@ -345,43 +350,48 @@ enum Mode { kPlain, kMasked, kCapped, kBiased, kCappedBiased };
 // degree 7 up to 5/16, of degree 19 up to 3/2, both fitted to the relative error (1.7e-8, 1.9e-8); beyond, or where products and differences have to be rounded
 // apart, one by one.  All of a warp's 32 tokens go one way.  (Two more values of the special function pipe for each logit would be twice the time of all
 // else: it makes 16 a cycle.)
+constexpr int kLowTerms = 4, kMidTerms = 10;
+constexpr float kLowReach2 = 0.09765625f, kMidReach2 = 2.25f;
+constexpr float kCapLow[kLowTerms] = {1.f, -0.33332987233884576f, 0.13311666824722448f, -0.0500755820287676f};
+constexpr float kCapMid[kMidTerms] = {1.f, -0.3333322466769597f, 0.13331329487357702f, -0.0538386683456423f, 0.021448478261107542f, -0.00806102220738539f,
+                                      0.0026138976028419808f, -0.0006436921929764066f, 0.00010158802230323775f, -7.465266263465981e-06f};
 struct CapLow {
-    static constexpr int kTerms = 4;
-    static constexpr float kReach2 = 0.09765625f;
-    __device__ __forceinline__ static constexpr float k(int i) {
-        constexpr float c[kTerms] = {1.f, -0.33332987233884576f, 0.13311666824722448f, -0.0500755820287676f};
-        return c[i];
-    }
+    static constexpr int kTerms = kLowTerms;
+    static constexpr float kReach2 = kLowReach2;
+    static __device__ __forceinline__ uint64_t k(const Pf& P, int i) { return P.cap_low[i]; }
 };
 struct CapMid {
-    static constexpr int kTerms = 10;
-    static constexpr float kReach2 = 2.25f;
-    __device__ __forceinline__ static constexpr float k(int i) {
-        constexpr float c[kTerms] = {1.f, -0.3333322466769597f, 0.13331329487357702f, -0.0538386683456423f, 0.021448478261107542f, -0.00806102220738539f,
-                                     0.0026138976028419808f, -0.0006436921929764066f, 0.00010158802230323775f, -7.465266263465981e-06f};
-        return c[i];
-    }
+    static constexpr int kTerms = kMidTerms;
+    static constexpr float kReach2 = kMidReach2;
+    static __device__ __forceinline__ uint64_t k(const Pf& P, int i) { return P.cap_mid[i]; }
 };
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-// x[] = shape of products x[] times factor, less z; whether the polynomial reaches as far as they go (warp-wide)
+// cap tanh(u) / u of a pair; most: the largest u^2 so far
 template <typename K>
-__device__ __forceinline__ bool pf_cap_pairs(float (&x)[32], float cap, float g, float z) {
-    const uint64_t g2 = pack_f2(g, g), nz = pack_f2(-z, -z);
+__device__ __forceinline__ uint64_t pf_cap_poly(const Pf& P, uint64_t u, float& most) {
+    const uint64_t v = mul_f2(u, u);
+    float v0, v1;
+    unpack_f2(v, v0, v1);
+    most = max3(most, v0, v1);
+    uint64_t p = K::k(P, K::kTerms - 1);
+#pragma unroll
+    for (int i = K::kTerms - 2; i >= 0; --i) p = fma_f2(p, v, K::k(P, i));
+    return p;
+}
+// Products x[] times factor to logits, as far as the polynomial reaches (warp-wide; whether it does)
+template <typename K>
+__device__ __forceinline__ bool pf_cap_pairs(float (&x)[32], const Pf& P, float factor) {
+    const float g = factor * P.sc.cap_inv;
+    const uint64_t g2 = pack_f2(g, g);
     float most[2] = {0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < 32; c += 2) {
-        const uint64_t u = mul_f2(pack_f2(x[c], x[c + 1]), g2), v = mul_f2(u, u);
-        float v0, v1;
-        unpack_f2(v, v0, v1);
-        most[c >> 1 & 1] = max3(most[c >> 1 & 1], v0, v1);
-        uint64_t p = pack_f2(K::k(K::kTerms - 1) * cap, K::k(K::kTerms - 1) * cap);
-#pragma unroll
-        for (int i = K::kTerms - 2; i >= 0; --i) p = fma_f2(p, v, pack_f2(K::k(i) * cap, K::k(i) * cap));
-        unpack_f2(fma_f2(u, p, nz), x[c], x[c + 1]);
+        const uint64_t u = mul_f2(pack_f2(x[c], x[c + 1]), g2);
+        unpack_f2(mul_f2(u, pf_cap_poly<K>(P, u, most[c >> 1 & 1])), x[c], x[c + 1]);
     }
     return __all_sync(0xffffffffu, fmaxf(most[0], most[1]) <= K::kReach2);
 }
@@ -389,17 +399,15 @@ __device__ __forceinline__ float pf_cap_any(float x, const PgScores& sc) {
     const float u = x * sc.cap_inv, f = pg_cap_far(u, sc.cap);
     return fabsf(u) <= 0.5f ? pg_cap_near(u, sc.cap) : f;
 }
-// x[]: 32 products, which `load` fetches anew
+// x[]: 32 products, which `load` fetches anew, to logits
 template <typename Load>
-__device__ __forceinline__ void pf_cap(float (&x)[32], const PgScores& sc, bool apart, float factor, float z, Load load) {
-    if (!apart) {
-        if (pf_cap_pairs<CapLow>(x, sc.cap, factor * sc.cap_inv, z)) return;
-        load();
-        if (pf_cap_pairs<CapMid>(x, sc.cap, factor * sc.cap_inv, z)) return;
-        load();
-    }
+__device__ __forceinline__ void pf_cap(float (&x)[32], const Pf& P, float factor, Load load) {
+    if (pf_cap_pairs<CapLow>(x, P, factor)) return;
+    load();
+    if (pf_cap_pairs<CapMid>(x, P, factor)) return;
+    load();
 #pragma unroll
-    for (int c = 0; c < 32; ++c) x[c] = pf_cap_any(__fmul_rn(x[c], factor), sc) - z;
+    for (int c = 0; c < 32; ++c) x[c] = pf_cap_any(x[c] * factor, P.sc);
 }
 // x[] times factor less slope times the distances, the first one's `ahead` of the row's own place
 __device__ __forceinline__ void pf_bias(float (&x)[32], float factor, float slope, float ahead, bool both_sides) {
@@ -420,6 +428,9 @@ __device__ __forceinline__ void pf_bias(float (&x)[32], float factor, float slop
     }
 }
 
+#ifndef KB
+#define KB kBiased
+#endif
 struct PfSmem {
     __align__(128) uint8_t q[kBlocks][kPart];
     __align__(128) uint8_t ring[kSlots][kPart];
@@ -503,6 +514,8 @@ __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >
 template <typename T, Mode kMode>
 __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
     constexpr bool kMod = kMode != kPlain;
+    // Biases fall with the distance: from a row's own place on backwards, its reference hardly moves
+    constexpr bool kBack = kMode >= KB;
     extern __shared__ __align__(128) uint8_t smem_raw[];
     PfSmem& S = *reinterpret_cast<PfSmem*>(smem_raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -541,7 +554,7 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                     const int slot = n % kSlots;
                     if (n >= kSlots && !pf_wait(S, &S.empty[slot], (uint32_t)(n / kSlots - 1) & 1u)) { ok = false; break; }
                     mbar_arrive_expect_tx(&S.full[slot], kPart);
-                    const int part = kMod ? 2 * w.b.tile(w.t0 + (k >> 1)) + (k & 1) : k;
+                    const int part = kMod ? 2 * w.b.tile<kBack>(w.t0 + (k >> 1)) + (k & 1) : k;
                     bulk_g2s(S.ring[slot], src + (size_t)part * kPart, kPart, &S.full[slot]);
                 }
                 if (!w.more()) break;
@@ -707,7 +720,7 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(&next.b) + 16 * lane),
                              "l"(reinterpret_cast<const uint8_t*>(P.blk + w.next_g()) + 16 * lane) : "memory");
             for (int t = tid & 255; t < tiles; t += 256) {
-                const int4 f = P.nan[((int64_t)w.b.si * P.n_h + w.h) * P.max_tiles + (kMod ? w.b.tile(tile0 + t) : tile0 + t)];
+                const int4 f = P.nan[((int64_t)w.b.si * P.n_h + w.h) * P.max_tiles + (kMod ? w.b.tile<kBack>(tile0 + t) : tile0 + t)];
                 if (min(min(f.x, f.y), min(f.z, f.w)) != INT_MAX) {
                     atomicMin(&S.nan[mb][0], f.x);
                     atomicMin(&S.nan[mb][1], f.y);
@@ -736,10 +749,10 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
             float down0, down1;
             pg_pow2(-S.ex[mb][r128], down0, down1);
             const float sc = fmaxf((P.scale_log2 == 0.f ? 1.f : fabsf(P.scale_log2)) * down0 * down1, kPgFactorMin);
-            // kBiased: logits are finished as they are loaded, and nothing is left to be multiplied by
-            const float fac = kMode >= kBiased ? 1.f : sc;
+            // kCapped and on: logits are finished as they are loaded, and nothing is left to be multiplied by
+            const float fac = kMode >= kCapped ? 1.f : sc;
             const uint8_t* const valid = P.valid + (int64_t)w.b.si * P.max_tiles + (kMod ? 0 : tile0);
-            auto place = [&](int i) { return kMod ? w.b.tile(tile0 + i) : i; };              // of a tile among the sequence's valid[]
+            auto place = [&](int i) { return kMod ? w.b.tile<kBack>(tile0 + i) : i; };              // of a tile among the sequence's valid[]
             uint32_t units = tiles > 0 ? valid[place(0)] : 0;
             float m_used = -INFINITY, lsum = 0.f;    // what this row scales by (log2), this half's denominator
             bool huge = false;                       // logits whose steps in fp32 are no longer small beside a weight's range
@@ -779,22 +792,14 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                     return max3(max3(a, c, c), sv[30], sv[31]);
                 };
                 float m_half;
-                if constexpr (kMode == kCapped) {      // caps keep the order: the largest product's logit is the largest
-                    load(32);
-                    if (cut) hide(32);
-                    m_half = top();
-                    load(0);
-                    if (cut) hide(0);
-                    m_half = fmaxf(m_half, top());
-                    if (m_half > -INFINITY) m_half = pf_cap_any(__fmul_rn(m_half, sc), P.sc);
-                } else if constexpr (kMode >= kBiased) {       // logits take their products' places
+                if constexpr (kMode >= kCapped) {              // logits take their products' places
                     m_half = -INFINITY;
 #pragma unroll 1
                     for (int c0 = 32; c0 >= 0; c0 -= 32) {
                         load(c0);
-                        if (kMode == kCappedBiased) pf_cap(sv, P.sc, false, sc, 0.f, [&] { load(c0); });
+                        if (kMode != kBiased) pf_cap(sv, P, sc, [&] { load(c0); });
                         // (tokens behind the row's own place are in its sight only where it lies in the prefix, or sees all)
-                        pf_bias(sv, kMode == kBiased ? sc : 1.f, slope, (float)(t0 + c0 - at), __any_sync(0xffffffffu, lim > at + 1 && t0 + c0 + 31 > at));
+                        if (kMode != kCapped) pf_bias(sv, kMode == kBiased ? sc : 1.f, slope, (float)(t0 + c0 - at), __any_sync(0xffffffffu, lim > at + 1 && t0 + c0 + 31 > at));
                         if (cut) hide(c0);
                         m_half = fmaxf(m_half, top());
                         if (c0) tmem_st32(sS + 32u, sv);
@@ -841,24 +846,15 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                 uint64_t ps[2] = {0ull, 0ull};
                 auto put = [&](uint32_t c0) {       // P of the columns in sv -> 16 columns of the half's own part of S
                     uint32_t pk[16];
-                    if constexpr (kMode == kCapped) {
-                        pf_cap(sv, P.sc, huge, sc, z, [&] { load(c0 ? 32 : 0); });
-                        if (cut) hide(c0 ? 32 : 0);
-                    }
-                    if (kMode != kCapped && huge) { // product and difference rounded apart, as the reference was
+                    if (huge) {                     // product and difference rounded apart, as the reference was
 #pragma unroll
                         for (int c = 0; c < 32; ++c) sv[c] = __fmul_rn(sv[c], fac);
                     }
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         float x0, x1, p0, p1;
-                        if constexpr (kMode == kCapped) {
-                            x0 = sv[2 * e];
-                            x1 = sv[2 * e + 1];
-                        } else {
-                            const uint64_t x = fma_f2(pack_f2(sv[2 * e], sv[2 * e + 1]), sc2, nz2);
-                            unpack_f2(x, x0, x1);
-                        }
+                        const uint64_t x = fma_f2(pack_f2(sv[2 * e], sv[2 * e + 1]), sc2, nz2);
+                        unpack_f2(x, x0, x1);
                         if (kMode <= kMasked && (kPolyPairs >> e & 1) != 0) {
                             const uint64_t y = pack_f2(max_nan(x0, -125.f), max_nan(x1, -125.f));
                             pf_exp2_poly(y, p0, p1);
@@ -882,7 +878,7 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                 if constexpr (kMode >= kCapped) {      // (one piece of code for both: what it shapes logits with is long)
 #pragma unroll 1
                     for (int part = 0; part < 2; ++part) {
-                        if (part || (kMode == kCapped && cut)) load(32 * part);
+                        if (part) load(32);
                         put(16u * part);
                         tell(part);
                     }
@@ -1166,6 +1162,14 @@ int paged_prefill(const PagedPrefill& A, cudaStream_t stream) {
             P.q = A.q; P.q_st = A.q_st; P.q_sh = A.q_sh; P.scale_log2 = A.scale_log2;
             P.out = A.out; P.o_st = A.o_st; P.o_sh = A.o_sh; P.lse = A.lse; P.status = A.status;
             P.sc = A.sc;
+            auto twice = [&](float k) {
+                uint32_t bits;
+                k *= A.sc.cap;
+                memcpy(&bits, &k, 4);
+                return (uint64_t)bits << 32 | bits;
+            };
+            for (int i = 0; i < kLowTerms; ++i) P.cap_low[i] = twice(kCapLow[i]);
+            for (int i = 0; i < kMidTerms; ++i) P.cap_mid[i] = twice(kCapMid[i]);
             P.nan_bits = reinterpret_cast<uint32_t*>(ws + L.nan_bits);
             if (!pg_launch_ok(launch_kernel(unpack, dim3((unsigned)tiles + 1, nh, ns), dim3(256), 0, stream, true, P))) return BGTQ_E_LAUNCH;
             if (!pg_launch_ok(launch_kernel(kernel, dim3(n_cta), dim3(kThreads), sizeof(PfSmem), stream, true, P))) return BGTQ_E_LAUNCH;
