@@ -26,6 +26,7 @@
 #include "bgtq_tcgen05.cuh"
 
 #include <limits.h>
+#include <math.h>
 #include <string.h>
 
 namespace bgtq {
@@ -74,7 +75,8 @@ struct Pf {
     float* lse;
     int32_t* status;
     PgScores sc;                                // (kernels of kMod read it)
-    uint64_t cap_low[4], cap_mid[10];           // the cap's polynomials, times the cap, each coefficient twice
+    uint64_t low[4], mid[10], steps[16];        // the cap's polynomials (of products, of u), each coefficient twice; 0, 1 .. 31
+    float low_reach2;                           // largest product's square that the first is for
     uint32_t* nan_bits;                         // kMod: (n_seq, n_h, max_tiles) x 4 groups x 128 tokens: those whose V is no number
 };
 
@@ -346,91 +348,87 @@ struct Walk {
 // What an attention's logits go through beside the scale.  Its rows may be masked in all forms but the plain one.
 enum Mode { kPlain, kMasked, kCapped, kBiased, kCappedBiased };
 
-// Logits under a cap, pairs at a time on the FMA pipe: u = x / cap, cap tanh(u) = u (cap + u^2 ...).  Most tiles' are small beside it: an odd polynomial of
-// degree 7 up to 5/16, of degree 19 up to 3/2, both fitted to the relative error (1.7e-8, 1.9e-8); beyond, or where products and differences have to be rounded
-// apart, one by one.  All of a warp's 32 tokens go one way.  (Two more values of the special function pipe for each logit would be twice the time of all
-// else: it makes 16 a cycle.)
+// Logits under a cap, pairs at a time on the FMA pipe, u = x / cap.  Most tiles' are small beside it: an odd polynomial of degree 7 up to 3/8, straight from the
+// products where all rows' have one factor (no row of bf16 queries was brought to another magnitude), or of degree 19 up to 3/2, both fitted to the relative
+// error (7e-8, 1.9e-8); beyond, one by one.  All of a warp's 32 tokens go one way.  (Two more values of the special function pipe for each logit would be
+// twice the time of all else: it makes 16 a cycle.)
 constexpr int kLowTerms = 4, kMidTerms = 10;
-constexpr float kLowReach2 = 0.09765625f, kMidReach2 = 2.25f;
-constexpr float kCapLow[kLowTerms] = {1.f, -0.33332987233884576f, 0.13311666824722448f, -0.0500755820287676f};
-constexpr float kCapMid[kMidTerms] = {1.f, -0.3333322466769597f, 0.13331329487357702f, -0.0538386683456423f, 0.021448478261107542f, -0.00806102220738539f,
-                                      0.0026138976028419808f, -0.0006436921929764066f, 0.00010158802230323775f, -7.465266263465981e-06f};
-struct CapLow {
-    static constexpr int kTerms = kLowTerms;
-    static constexpr float kReach2 = kLowReach2;
-    static __device__ __forceinline__ uint64_t k(const Pf& P, int i) { return P.cap_low[i]; }
-};
-struct CapMid {
-    static constexpr int kTerms = kMidTerms;
-    static constexpr float kReach2 = kMidReach2;
-    static __device__ __forceinline__ uint64_t k(const Pf& P, int i) { return P.cap_mid[i]; }
-};
+constexpr double kLowReach = 0.375;
+constexpr float kMidReach2 = 2.25f;
+constexpr double kCapLow[kLowTerms] = {1.0, -0.3333233349357446, 0.13289726163824672, -0.04848729069776324};
+constexpr double kCapMid[kMidTerms] = {1.0, -0.3333322466769597, 0.13331329487357702, -0.0538386683456423, 0.021448478261107542, -0.00806102220738539,
+                                       0.0026138976028419808, -0.0006436921929764066, 0.00010158802230323775, -7.465266263465981e-06};
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
-// cap tanh(u) / u of a pair; most: the largest u^2 so far
-template <typename K>
-__device__ __forceinline__ uint64_t pf_cap_poly(const Pf& P, uint64_t u, float& most) {
-    const uint64_t v = mul_f2(u, u);
-    float v0, v1;
-    unpack_f2(v, v0, v1);
-    most = max3(most, v0, v1);
-    uint64_t p = K::k(P, K::kTerms - 1);
-#pragma unroll
-    for (int i = K::kTerms - 2; i >= 0; --i) p = fma_f2(p, v, K::k(P, i));
-    return p;
-}
-// Products x[] times factor to logits, as far as the polynomial reaches (warp-wide; whether it does)
-template <typename K>
-__device__ __forceinline__ bool pf_cap_pairs(float (&x)[32], const Pf& P, float factor) {
-    const float g = factor * P.sc.cap_inv;
-    const uint64_t g2 = pack_f2(g, g);
-    float most[2] = {0.f, 0.f};
-#pragma unroll
-    for (int c = 0; c < 32; c += 2) {
-        const uint64_t u = mul_f2(pack_f2(x[c], x[c + 1]), g2);
-        unpack_f2(mul_f2(u, pf_cap_poly<K>(P, u, most[c >> 1 & 1])), x[c], x[c + 1]);
-    }
-    return __all_sync(0xffffffffu, fmaxf(most[0], most[1]) <= K::kReach2);
-}
 __device__ __forceinline__ float pf_cap_any(float x, const PgScores& sc) {
     const float u = x * sc.cap_inv, f = pg_cap_far(u, sc.cap);
     return fabsf(u) <= 0.5f ? pg_cap_near(u, sc.cap) : f;
 }
-// x[]: 32 products, which `load` fetches anew, to logits
-template <typename Load>
-__device__ __forceinline__ void pf_cap(float (&x)[32], const Pf& P, float factor, Load load) {
-    if (pf_cap_pairs<CapLow>(x, P, factor)) return;
-    load();
-    if (pf_cap_pairs<CapMid>(x, P, factor)) return;
-    load();
+// 32 products x[], which `load` fetches anew, to logits: times factor (even: the one that P.low is made for), capped, and less slope times the distances, of
+// which the first is `ahead` of the row's own place (both_sides: some lie behind it).
+template <bool kCap, bool kBias, typename Load>
+__device__ __forceinline__ void pf_shape(float (&x)[32], const Pf& P, float factor, bool even, float slope, float ahead, bool both_sides, Load load) {
+    const float t0 = slope * ahead;
+    const uint64_t t2 = pack_f2(t0, t0), s2 = pack_f2(slope, slope);
+    // (slopes times whole numbers below 32, on top of the first's)
+    auto bias = [&](int c) { return fma_f2(s2, P.steps[c >> 1], t2); };
+    if (kCap) {
+        bool done = false;
+        if (even) {
+            float most[2] = {0.f, 0.f};
 #pragma unroll
-    for (int c = 0; c < 32; ++c) x[c] = pf_cap_any(x[c] * factor, P.sc);
-}
-// x[] times factor less slope times the distances, the first one's `ahead` of the row's own place
-__device__ __forceinline__ void pf_bias(float (&x)[32], float factor, float slope, float ahead, bool both_sides) {
-    uint64_t d = pack_f2(ahead, ahead + 1.f);
-    const uint64_t two = pack_f2(2.f, 2.f), s2 = pack_f2(slope, slope), f2 = pack_f2(factor, factor);
-    if (both_sides) {
+            for (int c = 0; c < 32; c += 2) {
+                const uint64_t r = pack_f2(x[c], x[c + 1]), v = mul_f2(r, r);
+                float v0, v1;
+                unpack_f2(v, v0, v1);
+                most[c >> 1 & 1] = max3(most[c >> 1 & 1], v0, v1);
+                uint64_t p = fma_f2(v, P.low[kLowTerms - 1], P.low[kLowTerms - 2]);
 #pragma unroll
-        for (int c = 0; c < 32; c += 2) {
-            unpack_f2(fma_f2(d | 0x8000000080000000ull, s2, mul_f2(pack_f2(x[c], x[c + 1]), f2)), x[c], x[c + 1]);
-            d = add_f2(d, two);
+                for (int i = kLowTerms - 3; i >= 0; --i) p = fma_f2(v, p, P.low[i]);
+                unpack_f2(kBias && !both_sides ? fma_f2(r, p, bias(c)) : mul_f2(r, p), x[c], x[c + 1]);
+            }
+            done = __all_sync(0xffffffffu, fmaxf(most[0], most[1]) <= P.low_reach2);
+            if (done && (!kBias || !both_sides)) return;
+            if (!done) load();
         }
-    } else {
+        if (!done) {
+            const float g = factor * P.sc.cap_inv;
+            const uint64_t g2 = pack_f2(g, g);
+            float most[2] = {0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < 32; c += 2) {
-            unpack_f2(fma_f2(d, s2, mul_f2(pack_f2(x[c], x[c + 1]), f2)), x[c], x[c + 1]);
-            d = add_f2(d, two);
+            for (int c = 0; c < 32; c += 2) {
+                const uint64_t u = mul_f2(pack_f2(x[c], x[c + 1]), g2), v = mul_f2(u, u);
+                float v0, v1;
+                unpack_f2(v, v0, v1);
+                most[c >> 1 & 1] = max3(most[c >> 1 & 1], v0, v1);
+                uint64_t p = fma_f2(v, P.mid[kMidTerms - 1], P.mid[kMidTerms - 2]);
+#pragma unroll
+                for (int i = kMidTerms - 3; i >= 0; --i) p = fma_f2(v, p, P.mid[i]);
+                unpack_f2(mul_f2(u, p), x[c], x[c + 1]);
+            }
+            if (!__all_sync(0xffffffffu, fmaxf(most[0], most[1]) <= kMidReach2)) {
+                load();
+#pragma unroll
+                for (int c = 0; c < 32; ++c) x[c] = pf_cap_any(x[c] * factor, P.sc);
+            }
+        }
+    }
+    if (kBias) {
+        const float f = kCap ? 1.f : factor;
+        const uint64_t f2 = pack_f2(f, f);
+        if (both_sides) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) x[c] = fmaf(-slope, fabsf(ahead + (float)c), x[c] * f);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) unpack_f2(fma_f2(pack_f2(x[c], x[c + 1]), f2, bias(c)), x[c], x[c + 1]);
         }
     }
 }
 
-#ifndef KB
-#define KB kBiased
-#endif
 struct PfSmem {
     __align__(128) uint8_t q[kBlocks][kPart];
     __align__(128) uint8_t ring[kSlots][kPart];
@@ -515,7 +513,7 @@ template <typename T, Mode kMode>
 __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
     constexpr bool kMod = kMode != kPlain;
     // Biases fall with the distance: from a row's own place on backwards, its reference hardly moves
-    constexpr bool kBack = kMode >= KB;
+    constexpr bool kBack = kMode >= kBiased;
     extern __shared__ __align__(128) uint8_t smem_raw[];
     PfSmem& S = *reinterpret_cast<PfSmem*>(smem_raw);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -751,6 +749,7 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
             const float sc = fmaxf((P.scale_log2 == 0.f ? 1.f : fabsf(P.scale_log2)) * down0 * down1, kPgFactorMin);
             // kCapped and on: logits are finished as they are loaded, and nothing is left to be multiplied by
             const float fac = kMode >= kCapped ? 1.f : sc;
+            const bool even = __all_sync(0xffffffffu, S.ex[mb][r128] == 0);
             const uint8_t* const valid = P.valid + (int64_t)w.b.si * P.max_tiles + (kMod ? 0 : tile0);
             auto place = [&](int i) { return kMod ? w.b.tile<kBack>(tile0 + i) : i; };              // of a tile among the sequence's valid[]
             uint32_t units = tiles > 0 ? valid[place(0)] : 0;
@@ -797,9 +796,9 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
 #pragma unroll 1
                     for (int c0 = 32; c0 >= 0; c0 -= 32) {
                         load(c0);
-                        if (kMode != kBiased) pf_cap(sv, P, sc, [&] { load(c0); });
                         // (tokens behind the row's own place are in its sight only where it lies in the prefix, or sees all)
-                        if (kMode != kCapped) pf_bias(sv, kMode == kBiased ? sc : 1.f, slope, (float)(t0 + c0 - at), __any_sync(0xffffffffu, lim > at + 1 && t0 + c0 + 31 > at));
+                        pf_shape<kMode != kBiased, kMode != kCapped>(sv, P, sc, even, slope, (float)(t0 + c0 - at),
+                                                                     kMode != kCapped && __any_sync(0xffffffffu, lim > at + 1 && t0 + c0 + 31 > at), [&] { load(c0); });
                         if (cut) hide(c0);
                         m_half = fmaxf(m_half, top());
                         if (c0) tmem_st32(sS + 32u, sv);
@@ -846,14 +845,14 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                 uint64_t ps[2] = {0ull, 0ull};
                 auto put = [&](uint32_t c0) {       // P of the columns in sv -> 16 columns of the half's own part of S
                     uint32_t pk[16];
-                    if (huge) {                     // product and difference rounded apart, as the reference was
+                    if (kMode < kCapped && huge) {  // product and difference rounded apart, as the reference was
 #pragma unroll
                         for (int c = 0; c < 32; ++c) sv[c] = __fmul_rn(sv[c], fac);
                     }
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         float x0, x1, p0, p1;
-                        const uint64_t x = fma_f2(pack_f2(sv[2 * e], sv[2 * e + 1]), sc2, nz2);
+                        const uint64_t s2 = pack_f2(sv[2 * e], sv[2 * e + 1]), x = kMode >= kCapped ? add_f2(s2, nz2) : fma_f2(s2, sc2, nz2);
                         unpack_f2(x, x0, x1);
                         if (kMode <= kMasked && (kPolyPairs >> e & 1) != 0) {
                             const uint64_t y = pack_f2(max_nan(x0, -125.f), max_nan(x1, -125.f));
@@ -1120,6 +1119,27 @@ int64_t paged_prefill_workspace(int n_seq, int n_tok, int gqa, int n_kv, int64_t
     return pf_layout(seqs, heads, tiles, (int64_t)n_tok * gqa / kBlockRows + n_seq, pf_ctas(), mod).total;
 }
 
+// What pf_shape takes from the launch's parameters.
+static void pf_constants(Pf& P) {
+    auto pair = [](double a, double b) {
+        const float f[2] = {(float)a, (float)b};
+        uint64_t bits;
+        memcpy(&bits, f, 8);
+        return bits;
+    };
+    for (int i = 0; i < 16; ++i) P.steps[i] = pair(2 * i, 2 * i + 1);
+    for (int i = 0; i < kMidTerms; ++i) P.mid[i] = pair(kCapMid[i] * P.sc.cap, kCapMid[i] * P.sc.cap);
+    // u = product * g; where fp32 has no normal numbers for the coefficients, the polynomial is for no product
+    const double factor = P.scale_log2 == 0.f ? 1.0 : fabs((double)P.scale_log2), g = factor * P.sc.cap_inv;
+    double k = factor;
+    bool good = true;
+    for (int i = 0; i < kLowTerms; ++i, k *= g * g) {
+        P.low[i] = pair(kCapLow[i] * k, kCapLow[i] * k);
+        good = good && k > 1e-35 && k < 1e35;
+    }
+    P.low_reach2 = good ? (float)(kLowReach / g * (kLowReach / g)) : -1.f;
+}
+
 int paged_prefill(const PagedPrefill& A, cudaStream_t stream) {
     int seqs, heads;
     int64_t tiles;
@@ -1162,14 +1182,7 @@ int paged_prefill(const PagedPrefill& A, cudaStream_t stream) {
             P.q = A.q; P.q_st = A.q_st; P.q_sh = A.q_sh; P.scale_log2 = A.scale_log2;
             P.out = A.out; P.o_st = A.o_st; P.o_sh = A.o_sh; P.lse = A.lse; P.status = A.status;
             P.sc = A.sc;
-            auto twice = [&](float k) {
-                uint32_t bits;
-                k *= A.sc.cap;
-                memcpy(&bits, &k, 4);
-                return (uint64_t)bits << 32 | bits;
-            };
-            for (int i = 0; i < kLowTerms; ++i) P.cap_low[i] = twice(kCapLow[i]);
-            for (int i = 0; i < kMidTerms; ++i) P.cap_mid[i] = twice(kCapMid[i]);
+            pf_constants(P);
             P.nan_bits = reinterpret_cast<uint32_t*>(ws + L.nan_bits);
             if (!pg_launch_ok(launch_kernel(unpack, dim3((unsigned)tiles + 1, nh, ns), dim3(256), 0, stream, true, P))) return BGTQ_E_LAUNCH;
             if (!pg_launch_ok(launch_kernel(kernel, dim3(n_cta), dim3(kThreads), sizeof(PfSmem), stream, true, P))) return BGTQ_E_LAUNCH;
