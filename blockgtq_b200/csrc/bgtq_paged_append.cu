@@ -175,12 +175,18 @@ __global__ void __launch_bounds__(kApThreads, L == 8 ? 4 : 2) pg_append_kernel(c
                     for (int i = 0; i < E; i += 4) {
                         const int d = 32 * g + E * j + i;
                         const uint32_t four = P.axis[d >> 4] >> (2 * (d & 15)) & 255u;         // the axes of pairs d .. d + 3
+                        auto row = [&](uint32_t a) { return (a & 2 ? a & 1 ? p[3] : p[2] : a & 1 ? p[1] : p[0]) * P.cs_st + d; };
+                        if (four == (four & 3u) * 0x55u) {                     // (all one)
+                            const int64_t at = row(four & 3u);
+                            *reinterpret_cast<float4*>(&cs[g][i]) = *reinterpret_cast<const float4*>(P.cos + at);
+                            *reinterpret_cast<float4*>(&sn[g][i]) = *reinterpret_cast<const float4*>(P.sin + at);
+                        } else {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint32_t a = four >> (2 * e) & 3u;
-                            const int64_t at = (a & 2 ? a & 1 ? p[3] : p[2] : a & 1 ? p[1] : p[0]) * P.cs_st + d + e;
-                            cs[g][i + e] = P.cos[at];
-                            sn[g][i + e] = P.sin[at];
+                            for (int e = 0; e < 4; ++e) {
+                                const int64_t at = row(four >> (2 * e) & 3u) + e;
+                                cs[g][i + e] = P.cos[at];
+                                sn[g][i + e] = P.sin[at];
+                            }
                         }
                     }
         }
