@@ -442,7 +442,10 @@ class PagedKV4Cache:
 
     A step is :meth:`begin_step` with the sequences that get new tokens and how many each, then
     :meth:`append_and_attend` once per layer with the tokens' rows one sequence behind the other.  What a step needs on the device
-    (slots, positions, block table, lengths) is uploaded once and is the same for every layer."""
+    (slots, positions, block table, lengths) is uploaded once and is the same for every layer.
+
+    Sequences may share pages: :meth:`fork_sequence` makes one that begins with another's tokens and copies nothing.  A shared page is copied, in all
+    layers, by the step that would write into it (on the stream of :meth:`begin_step`), and goes back to the pool with the last sequence that holds it."""
 
     def __init__(self, n_layers, n_q_heads, n_kv_heads, head_dim=HD, *, n_pages, max_seq_len, page_size=64, device="cuda"):
         if head_dim != HD:
@@ -456,9 +459,12 @@ class PagedKV4Cache:
         self.pages = torch.zeros(n_layers, n_pages, n_kv_heads, page_bytes(page_size), dtype=torch.uint8, device=self.device)
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._free = list(range(n_pages - 1, -1, -1))
+        self._held = [0] * n_pages          # sequences that hold a page
         self._seqs = {}                     # id -> [tokens, [pages]]
         self._next_id = 0
         self._step = None
+        self._busy = set()                  # streams that layers have run on since pages were last copied
+        self._copied = None                 # the event behind the last copies
 
     # ---- sequences -----------------------------------------------------------
     def add_sequence(self) -> int:
@@ -468,11 +474,93 @@ class PagedKV4Cache:
         self._seqs[i] = [0, []]
         return i
 
+    def fork_sequence(self, seq: int, n_tokens=None) -> int:
+        """A new sequence that begins with the first ``n_tokens`` (default: all) of another's tokens, in the same pages."""
+        t, pages = self._seqs[seq]
+        n = t if n_tokens is None else operator.index(n_tokens)
+        if not 0 <= n <= t:
+            raise ValueError(f"sequence {seq} has {t} tokens, not {n}")
+        i = self.add_sequence()
+        self._seqs[i] = [n, pages[:-(-n // self.page_size)]]
+        for p in self._seqs[i][1]:
+            self._held[p] += 1
+        return i
+
+    def truncate_sequence(self, seq: int, n_tokens: int):
+        """Leaves the sequence its first ``n_tokens`` tokens, and gives the pages behind them back.  A step that it is part of ends with it."""
+        t, pages = self._seqs[seq]
+        n = operator.index(n_tokens)
+        if not 0 <= n <= t:
+            raise ValueError(f"sequence {seq} has {t} tokens, not {n}")
+        keep = -(-n // self.page_size)
+        self._seqs[seq] = [n, pages[:keep]]
+        self._let_go(pages[keep:])
+        self._end_step(seq)
+
     def free_sequence(self, seq: int):
         """Gives the sequence's pages back.  A step that it is part of ends with it."""
-        self._free.extend(reversed(self._seqs.pop(seq)[1]))
+        self._let_go(self._seqs.pop(seq)[1])
+        self._end_step(seq)
+
+    def _let_go(self, pages):
+        for p in reversed(pages):
+            self._held[p] -= 1
+            if self._held[p] == 0:
+                self._free.append(p)
+
+    def _end_step(self, seq):
         if self._step is not None and seq in self._step["seqs"]:
             self._step = None
+
+    def compact(self) -> int:
+        """Moves the pages that sequences hold to the front of the pool, on the current stream, and returns how many they are.  The step ends."""
+        self._not_captured()
+        n = self.n_pages - len(self._free)
+        places = sorted(p for p in self._free if p < n)
+        moved = dict(zip((p for p in range(n, self.n_pages) if self._held[p]), places))
+        if moved:
+            self._copy(list(moved), list(moved.values()))
+        self._renumber(moved, n, self.n_pages)
+        return n
+
+    def resize(self, n_pages: int):
+        """Gives the pool another number of pages, no fewer than sequences hold; those come first, as after :meth:`compact`.  The step ends.  Waits for the
+        device: nothing may be reading the old pool when it is given back."""
+        self._not_captured()
+        n, n_pages = self.n_pages - len(self._free), operator.index(n_pages)
+        if n_pages < max(1, n):
+            raise ValueError(f"{n} pages are held, more than {n_pages}" if n else "a pool has at least one page")
+        held = [p for p in range(self.n_pages) if self._held[p]]
+        pages = torch.zeros(self.n_layers, n_pages, *self.pages.shape[2:], dtype=torch.uint8, device=self.device)
+        if held:
+            self._copy(held, list(range(n)), into=pages)
+        if self.device.type == "cuda":
+            torch.cuda.synchronize(self.device)
+        self.pages = pages
+        self._renumber(dict(zip(held, range(n))), n, n_pages)
+
+    def _renumber(self, moved, n, n_pages):
+        for entry in self._seqs.values():
+            entry[1] = [moved.get(p, p) for p in entry[1]]
+        held = [0] * n_pages
+        for p, h in enumerate(self._held):
+            if h:
+                held[moved.get(p, p)] = h
+        self._held, self._free, self.n_pages, self._step = held, list(range(n_pages - 1, n - 1, -1)), n_pages, None
+
+    def _copy(self, src, dst, **kw):
+        """Copies pages on the current stream, behind the layers of every stream; layers that follow on another one wait for it."""
+        stream = self._stream()
+        for other in self._busy:
+            if other != stream:
+                stream.wait_stream(other)
+        paged_kv4_copy(self.pages, src, dst, **kw)
+        if stream is not None:
+            self._busy, self._copied = set(), stream.record_event()
+
+    def _not_captured(self):
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a captured graph would go on moving the pages that are held now")
 
     def seq_len(self, seq: int) -> int:
         return self._seqs[seq][0]
@@ -488,25 +576,31 @@ class PagedKV4Cache:
     # ---- a step --------------------------------------------------------------
     def begin_step(self, seqs, counts):
         """Makes room for ``counts[i]`` >= 1 new tokens of sequence ``seqs[i]`` (distinct); their rows follow one another in that order.
-        Either every sequence gets its room or none does."""
+        Either every sequence gets its room or none does.  Pages that others hold too and that the step would write into are copied first."""
         seqs, counts = list(seqs), [int(c) for c in counts]
         if not seqs or len(seqs) != len(counts) or len(set(seqs)) != len(seqs) or min(counts) < 1:
             raise ValueError("begin_step takes distinct sequences and a count of at least one token for each")
-        need = []
+        need, parted, left = [], [], {}     # pages; sequences that get a copy of their last one; who holds that then
         for i, c in zip(seqs, counts):
             if i not in self._seqs:
                 raise KeyError(f"no sequence {i}")
             t, held = self._seqs[i]
             if t + c > self.max_seq_len:
                 raise ValueError(f"sequence {i} would have {t + c} tokens, more than {self.max_seq_len}")
-            need.append(-(-(t + c) // self.page_size) - len(held))
+            last = held[-1] if t % self.page_size else None
+            parted.append(last is not None and left.get(last, self._held[last]) > 1)
+            if parted[-1]:
+                left[last] = left.get(last, self._held[last]) - 1
+            need.append(-(-(t + c) // self.page_size) - len(held) + parted[-1])
         if sum(need) > len(self._free):
             raise RuntimeError(f"{sum(need)} pages needed, {len(self._free)} free")
         free = len(self._free)              # pages are taken from the end
-        slots, positions, lens, ends, rows = [], [], [], [0], []
-        for i, c, n in zip(seqs, counts, need):
+        slots, positions, lens, ends, rows, copies = [], [], [], [0], [], []
+        for i, c, n, part in zip(seqs, counts, need, parted):
             t, held = self._seqs[i]
-            pages = held + [self._free[free - 1 - k] for k in range(n)]
+            pages = (held[:-1] if part else held) + [self._free[free - 1 - k] for k in range(n)]
+            if part:
+                copies.append((held[-1], pages[len(held) - 1], t % self.page_size))
             free -= n
             at = range(t, t + c)
             positions.extend(at)
@@ -518,9 +612,17 @@ class PagedKV4Cache:
         wide = torch.tensor([slots, positions], dtype=torch.int64).to(self.device)
         table = torch.tensor([r + [0] * (width - len(r)) for r in rows], dtype=torch.int32).to(self.device)
         small = torch.tensor(lens + ends, dtype=torch.int32).to(self.device)
+        if copies:
+            self._not_captured()
+            src, dst, n_tokens = (list(x) for x in zip(*copies))
+            self._copy(src, dst, n_tokens=n_tokens)
         # (from here on nothing fails: a device without memory for the step leaves the sequences as they were)
         for i, t, pages in zip(seqs, lens, rows):
             self._seqs[i] = [t, pages]
+        for p in self._free[free:]:
+            self._held[p] = 1
+        for src, _, _ in copies:
+            self._held[src] -= 1
         del self._free[free:]
         self._step = {"slots": wide[0], "positions": wide[1], "table": table, "lens": small[:len(seqs)], "ends": small[len(seqs):],
                       "most_q": max(counts), "most": max(lens), "rows": len(slots), "seqs": frozenset(seqs),
@@ -530,9 +632,12 @@ class PagedKV4Cache:
         return torch.cuda.current_stream(self.device) if self.device.type == "cuda" else None
 
     @torch.no_grad()
-    def append_and_attend(self, layer_idx, q, k, v, rope=None):
+    def append_and_attend(self, layer_idx, q, k, v, rope=None, *, positions=None, axes=None, softcap=None, slopes=None, window=None,
+                          prefix_lens=None, max_prefix_len=None):
         """The step's rows of one layer: k, v (n, n_kv, 128) are stored, q (n, n_q, 128) attends, causally, its own sequence ->
-        (n, n_q, 128).  ``rope=(cos, sin)``, tables (positions, 64) fp32: q and k go through the rotary embedding first."""
+        (n, n_q, 128).  ``rope=(cos, sin)``, tables (positions, 64) fp32: q and k go through the rotary embedding first, at the tokens' places in
+        their sequences, or at ``positions`` (n,) int64, or (axes, n) with ``axes`` as :func:`paged_kv4_append` takes them.  ``softcap``,
+        ``slopes``, ``window``, ``prefix_lens`` (one for each of the step's sequences, in its order) and ``max_prefix_len`` are the attention's."""
         if self._step is None:
             raise RuntimeError("begin_step comes first")
         s, pages = self._step, self.pages[layer_idx]
@@ -541,19 +646,31 @@ class PagedKV4Cache:
         if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("a captured graph would go on reading this step's slots and lengths, which end with the step: capture "
                                "paged_kv4_append and the attentions over tensors of your own")
+        scores = dict(softcap=softcap, slopes=slopes, window=window, prefix_lens=prefix_lens, max_prefix_len=max_prefix_len)
+        _limits(softcap, window, True)      # (nothing is stored for an attention that is refused)
+        if prefix_lens is not None and prefix_lens.shape != s["lens"].shape:
+            raise ValueError(f"prefix_lens must be ({len(s['lens'])},), one for each of the step's sequences, got {tuple(prefix_lens.shape)}")
         stream = self._stream()
         if stream not in s["streams"]:      # (the next step's tensors must not take these tensors' memory before this stream is done with them)
             for t in s["held"]:
                 t.record_stream(stream)
             s["streams"].add(stream)
+            if self._copied is not None:
+                stream.wait_event(self._copied)
+        self._busy.add(stream)
         if rope is None:
+            if positions is not None or axes is not None:
+                raise ValueError("positions and axes belong to rope")
             paged_kv4_append(pages, s["slots"], k, v, status=self.status)
         else:
-            q = paged_kv4_append(pages, s["slots"], k, v, q=q, cos=rope[0], sin=rope[1], positions=s["positions"], status=self.status)
+            if axes is not None and positions is None:
+                raise ValueError("axes belong to positions")
+            q = paged_kv4_append(pages, s["slots"], k, v, q=q, cos=rope[0], sin=rope[1], positions=s["positions"] if positions is None else positions,
+                                 status=self.status, axes=axes)
         if s["most_q"] == 1:
-            return paged_kv4_decode_attention(q, pages, s["table"], s["lens"], status=self.status)
+            return paged_kv4_decode_attention(q, pages, s["table"], s["lens"], status=self.status, **scores)
         return paged_kv4_prefill_attention(q, pages, s["table"], s["lens"], s["ends"], max_q_len=s["most_q"], max_seq_len=s["most"],
-                                           status=self.status)
+                                           status=self.status, **scores)
 
     def check_status(self):
         """Raises when a launch since the last call, on whatever stream, reported an error (synchronises the device)."""
