@@ -94,7 +94,7 @@ __device__ __forceinline__ Seq pf_seq(const Pf& P, int i) {
     return s;
 }
 // First token of the window of a sequence's row
-__device__ __forceinline__ int pf_low(const Pf& P, const Seq& s, int pos) { return P.sc.window ? max(0, max(0, s.len - s.n + 1 + pos) - P.sc.window) : 0; }
+__device__ __forceinline__ int pf_window(const Pf& P, const Seq& s, int pos) { return P.sc.window ? max(0, max(0, s.len - s.n + 1 + pos) - P.sc.window) : 0; }
 
 // ------------------------------------------------------------------------------------------------------------------
 // unpack: a warp per unit of 16 tokens.  Operand layout (no swizzle, K-major): element (row, k) at
@@ -123,7 +123,7 @@ __device__ __forceinline__ Block pf_block(const Pf& P, int si, const Seq& s, int
     const int last_pos = (min(s.n * P.gqa, (j + 1) * kBlockRows) - 1) / P.gqa;
     const int t_max = P.causal ? max(s.pre, s.len - s.n + 1 + last_pos) : s.len, tiles = (t_max + kPfTileTok - 1) / kPfTileTok;
     if (!kMod) return Block{si, j * kBlockRows, s.len, s.q0, s.n, max(1, tiles), tiles > 0, 0};
-    const int head = (s.pre + kPfTileTok - 1) / kPfTileTok, gap = max(0, pf_low(P, s, j * kBlockRows / P.gqa) / kPfTileTok - head);
+    const int head = (s.pre + kPfTileTok - 1) / kPfTileTok, gap = max(0, pf_window(P, s, j * kBlockRows / P.gqa) / kPfTileTok - head);
     return Block{si, j * kBlockRows, s.len, s.q0, s.n, max(1, tiles - gap), tiles > 0 ? 1 + head : 0, gap};
 }
 // The list of blocks and the CTAs' shares, by one CTA of 256 threads.
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(256) pg_unpack_kernel(const Pf P) {
     const Seq s = pf_seq<kMod>(P, P.seq0 + si);
     const int unit = tile * (kPfTileTok / kUnitTok) + warp, left = s.len - unit * kUnitTok;
     if (s.n == 0 || tile * kPfTileTok >= s.len) return;
-    if (kMod && tile * kPfTileTok >= s.pre && (tile + 1) * kPfTileTok <= pf_low(P, s, 0)) return;         // (no row sees it)
+    if (kMod && tile * kPfTileTok >= s.pre && (tile + 1) * kPfTileTok <= pf_window(P, s, 0)) return;         // (no row sees it)
     const uint8_t* u = nullptr;
     if (left > 0) {
         const int col = unit / P.pool.units, page = P.table[(int64_t)(P.seq0 + si) * P.tb_st + col];
@@ -367,6 +367,22 @@ __device__ __forceinline__ float pf_cap_any(float x, const PgScores& sc) {
     const float u = x * sc.cap_inv, f = pg_cap_far(u, sc.cap);
     return fabsf(u) <= 0.5f ? pg_cap_near(u, sc.cap) : f;
 }
+// A pair of products' logits by the short polynomial, over the products; v: their squares
+__device__ __forceinline__ uint64_t pf_low(const Pf& P, uint64_t v) {
+    uint64_t p = fma_f2(v, P.low[kLowTerms - 1], P.low[kLowTerms - 2]);
+#pragma unroll
+    for (int i = kLowTerms - 3; i >= 0; --i) p = fma_f2(v, p, P.low[i]);
+    return p;
+}
+__device__ __forceinline__ float abs_top(const float (&x)[32]) {
+    float a = 0.f, b = 0.f;
+#pragma unroll
+    for (int c = 0; c < 32; c += 4) {
+        a = max3(a, fabsf(x[c]), fabsf(x[c + 1]));
+        b = max3(b, fabsf(x[c + 2]), fabsf(x[c + 3]));
+    }
+    return fmaxf(a, b);
+}
 // 32 products x[], which `load` fetches anew, to logits: times factor (even: the one that P.low is made for), capped, and less slope times the distances, of
 // which the first is `ahead` of the row's own place (both_sides: some lie behind it).
 template <bool kCap, bool kBias, typename Load>
@@ -381,13 +397,10 @@ __device__ __forceinline__ void pf_shape(float (&x)[32], const Pf& P, float fact
             float most[2] = {0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < 32; c += 2) {
-                const uint64_t r = pack_f2(x[c], x[c + 1]), v = mul_f2(r, r);
+                const uint64_t r = pack_f2(x[c], x[c + 1]), v = mul_f2(r, r), p = pf_low(P, v);
                 float v0, v1;
                 unpack_f2(v, v0, v1);
                 most[c >> 1 & 1] = max3(most[c >> 1 & 1], v0, v1);
-                uint64_t p = fma_f2(v, P.low[kLowTerms - 1], P.low[kLowTerms - 2]);
-#pragma unroll
-                for (int i = kLowTerms - 3; i >= 0; --i) p = fma_f2(v, p, P.low[i]);
                 unpack_f2(kBias && !both_sides ? fma_f2(r, p, bias(c)) : mul_f2(r, p), x[c], x[c + 1]);
             }
             done = __all_sync(0xffffffffu, fmaxf(most[0], most[1]) <= P.low_reach2);
@@ -738,7 +751,7 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                     const Seq s{w.b.len, w.b.q0, w.b.n, 0};
                     pre = pg_prefix(P.sc, P.seq0 + w.b.si, w.b.len);
                     lim = max(lim, pre);
-                    lo = pf_low(P, s, pos);
+                    lo = pf_window(P, s, pos);
                     at = w.b.len - w.b.n + pos;
                     const int g_pos = pf_pos(P, g);
                     if (P.sc.slopes) slope = P.sc.slopes[(P.h0 + w.h) * P.gqa + g - g_pos * P.gqa] * 1.44269504088896340736f;
@@ -791,14 +804,37 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                     return max3(max3(a, c, c), sv[30], sv[31]);
                 };
                 float m_half;
-                if constexpr (kMode >= kCapped) {              // logits take their products' places
+                bool low = false;                      // kCapped: nothing hidden, and the short polynomial reaches: it is taken beside the exponentials
+                if constexpr (kMode == kCapped) {      // caps keep the order: the largest product's logit is the largest
+                    float far;
+                    load(32);
+                    far = abs_top(sv);
+                    if (cut) hide(32);
+                    m_half = top();
+                    load(0);
+                    far = fmaxf(far, abs_top(sv));
+                    if (cut) hide(0);
+                    m_half = fmaxf(m_half, top());
+                    if (m_half > -INFINITY) m_half = pf_cap_any(m_half * sc, P.sc);
+                    low = even && !cut && !huge && __all_sync(0xffffffffu, far * far <= P.low_reach2);
+                    if (!low) {                        // logits take their products' places
+#pragma unroll 1
+                        for (int c0 = 32; c0 >= 0; c0 -= 32) {
+                            load(c0);
+                            pf_shape<true, false>(sv, P, sc, even, 0.f, 0.f, false, [&] { load(c0); });
+                            if (cut) hide(c0);
+                            if (c0) tmem_st32(sS + 32u, sv);
+                        }
+                        tmem_st_wait();
+                    }
+                } else if constexpr (kMode >= kBiased) {       // logits take their products' places
                     m_half = -INFINITY;
 #pragma unroll 1
                     for (int c0 = 32; c0 >= 0; c0 -= 32) {
                         load(c0);
                         // (tokens behind the row's own place are in its sight only where it lies in the prefix, or sees all)
-                        pf_shape<kMode != kBiased, kMode != kCapped>(sv, P, sc, even, slope, (float)(t0 + c0 - at),
-                                                                     kMode != kCapped && __any_sync(0xffffffffu, lim > at + 1 && t0 + c0 + 31 > at), [&] { load(c0); });
+                        pf_shape<kMode == kCappedBiased, true>(sv, P, sc, even, slope, (float)(t0 + c0 - at),
+                                                               __any_sync(0xffffffffu, lim > at + 1 && t0 + c0 + 31 > at), [&] { load(c0); });
                         if (cut) hide(c0);
                         m_half = fmaxf(m_half, top());
                         if (c0) tmem_st32(sS + 32u, sv);
@@ -845,6 +881,20 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                 uint64_t ps[2] = {0ull, 0ull};
                 auto put = [&](uint32_t c0) {       // P of the columns in sv -> 16 columns of the half's own part of S
                     uint32_t pk[16];
+                    if (kMode == kCapped && low) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const uint64_t r = pack_f2(sv[2 * e], sv[2 * e + 1]);
+                            float p0, p1;
+                            unpack_f2(fma_f2(r, pf_low(P, mul_f2(r, r)), nz2), p0, p1);
+                            p0 = pf_exp2(p0);
+                            p1 = pf_exp2(p1);
+                            ps[e & 1] = add_f2(ps[e & 1], pack_f2(p0, p1));
+                            pk[e] = pack_half2(p0, p1);
+                        }
+                        tmem_st16(sS + c0, pk);
+                        return;
+                    }
                     if (kMode < kCapped && huge) {  // product and difference rounded apart, as the reference was
 #pragma unroll
                         for (int c = 0; c < 32; ++c) sv[c] = __fmul_rn(sv[c], fac);
