@@ -354,7 +354,7 @@ enum Mode { kPlain, kMasked, kCapped, kBiased, kCappedBiased };
 // twice the time of all else: it makes 16 a cycle.)
 constexpr int kLowTerms = 4, kMidTerms = 10;
 constexpr double kLowReach = 0.375;
-constexpr float kMidReach2 = 2.25f;
+constexpr float kMidReach = 1.5f;
 constexpr double kCapLow[kLowTerms] = {1.0, -0.3333233349357446, 0.13289726163824672, -0.04848729069776324};
 constexpr double kCapMid[kMidTerms] = {1.0, -0.3333322466769597, 0.13331329487357702, -0.0538386683456423, 0.021448478261107542, -0.00806102220738539,
                                        0.0026138976028419808, -0.0006436921929764066, 0.00010158802230323775, -7.465266263465981e-06};
@@ -362,6 +362,20 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
+}
+template <typename F>
+__device__ __forceinline__ void tmem_map8(uint32_t taddr, F f) {
+    uint32_t r[8];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(f(__uint_as_float(r[i])));
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
 }
 __device__ __forceinline__ float pf_cap_any(float x, const PgScores& sc) {
     const float u = x * sc.cap_inv, f = pg_cap_far(u, sc.cap);
@@ -374,6 +388,13 @@ __device__ __forceinline__ uint64_t pf_low(const Pf& P, uint64_t v) {
     for (int i = kLowTerms - 3; i >= 0; --i) p = fma_f2(v, p, P.low[i]);
     return p;
 }
+// The same by the long one; v: the squares of u
+__device__ __forceinline__ uint64_t pf_mid(const Pf& P, uint64_t v) {
+    uint64_t p = fma_f2(v, P.mid[kMidTerms - 1], P.mid[kMidTerms - 2]);
+#pragma unroll
+    for (int i = kMidTerms - 3; i >= 0; --i) p = fma_f2(v, p, P.mid[i]);
+    return p;
+}
 __device__ __forceinline__ float abs_top(const float (&x)[32]) {
     float a = 0.f, b = 0.f;
 #pragma unroll
@@ -383,10 +404,14 @@ __device__ __forceinline__ float abs_top(const float (&x)[32]) {
     }
     return fmaxf(a, b);
 }
-// 32 products x[], which `load` fetches anew, to logits: times factor (even: the one that P.low is made for), capped, and less slope times the distances, of
+// 32 products x[], in tensor memory at `from`, to logits: times factor (even: the one that P.low is made for), capped, and less slope times the distances, of
 // which the first is `ahead` of the row's own place (both_sides: some lie behind it).
-template <bool kCap, bool kBias, typename Load>
-__device__ __forceinline__ void pf_shape(float (&x)[32], const Pf& P, float factor, bool even, float slope, float ahead, bool both_sides, Load load) {
+template <bool kCap, bool kBias>
+__device__ __forceinline__ void pf_shape(float (&x)[32], const Pf& P, float factor, bool even, float slope, float ahead, bool both_sides, uint32_t from) {
+    auto load = [&]() {
+        tmem_ld32(from, x);
+        tmem_ld_wait();
+    };
     const float t0 = slope * ahead;
     const uint64_t t2 = pack_f2(t0, t0), s2 = pack_f2(slope, slope);
     // (slopes times whole numbers below 32, on top of the first's)
@@ -417,15 +442,14 @@ __device__ __forceinline__ void pf_shape(float (&x)[32], const Pf& P, float fact
                 float v0, v1;
                 unpack_f2(v, v0, v1);
                 most[c >> 1 & 1] = max3(most[c >> 1 & 1], v0, v1);
-                uint64_t p = fma_f2(v, P.mid[kMidTerms - 1], P.mid[kMidTerms - 2]);
-#pragma unroll
-                for (int i = kMidTerms - 3; i >= 0; --i) p = fma_f2(v, p, P.mid[i]);
-                unpack_f2(mul_f2(u, p), x[c], x[c + 1]);
+                unpack_f2(mul_f2(u, pf_mid(P, v)), x[c], x[c + 1]);
             }
-            if (!__all_sync(0xffffffffu, fmaxf(most[0], most[1]) <= kMidReach2)) {
+            if (!__all_sync(0xffffffffu, fmaxf(most[0], most[1]) <= kMidReach * kMidReach)) {
+                // (in place, a few at a time: what hardly ever runs is kept short)
+#pragma unroll 1
+                for (int c = 0; c < 32; c += 8) tmem_map8(from + (uint32_t)c, [&](float r) { return pf_cap_any(r * factor, P.sc); });
+                tmem_st_wait();
                 load();
-#pragma unroll
-                for (int c = 0; c < 32; ++c) x[c] = pf_cap_any(x[c] * factor, P.sc);
             }
         }
     }
@@ -480,19 +504,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
         ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
           "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
-}
-__device__ __forceinline__ void tmem_scale8(uint32_t taddr, float f) {
-    uint32_t r[8];
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                 : "r"(taddr)
-                 : "memory");
-    tmem_ld_wait();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * f);
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
-                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-                 : "memory");
 }
 __device__ __forceinline__ float max_nan(float a, float b) {             // NaN when either is
     float d;
@@ -804,7 +815,7 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                     return max3(max3(a, c, c), sv[30], sv[31]);
                 };
                 float m_half;
-                bool low = false;                      // kCapped: nothing hidden, and the short polynomial reaches: it is taken beside the exponentials
+                int way = 0;                           // kCapped, where nothing is hidden and a polynomial reaches: 1 the short one, 2 the long one, beside the exponentials
                 if constexpr (kMode == kCapped) {      // caps keep the order: the largest product's logit is the largest
                     float far;
                     load(32);
@@ -816,12 +827,13 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                     if (cut) hide(0);
                     m_half = fmaxf(m_half, top());
                     if (m_half > -INFINITY) m_half = pf_cap_any(m_half * sc, P.sc);
-                    low = even && !cut && !huge && __all_sync(0xffffffffu, far * far <= P.low_reach2);
-                    if (!low) {                        // logits take their products' places
+                    if (!cut && !huge)
+                        way = even && __all_sync(0xffffffffu, far * far <= P.low_reach2) ? 1 : __all_sync(0xffffffffu, far * (sc * P.sc.cap_inv) <= kMidReach) ? 2 : 0;
+                    if (!way) {                        // logits take their products' places
 #pragma unroll 1
                         for (int c0 = 32; c0 >= 0; c0 -= 32) {
                             load(c0);
-                            pf_shape<true, false>(sv, P, sc, even, 0.f, 0.f, false, [&] { load(c0); });
+                            pf_shape<true, false>(sv, P, sc, even, 0.f, 0.f, false, sS + (uint32_t)c0);
                             if (cut) hide(c0);
                             if (c0) tmem_st32(sS + 32u, sv);
                         }
@@ -834,7 +846,7 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                         load(c0);
                         // (tokens behind the row's own place are in its sight only where it lies in the prefix, or sees all)
                         pf_shape<kMode == kCappedBiased, true>(sv, P, sc, even, slope, (float)(t0 + c0 - at),
-                                                               __any_sync(0xffffffffu, lim > at + 1 && t0 + c0 + 31 > at), [&] { load(c0); });
+                                                               __any_sync(0xffffffffu, lim > at + 1 && t0 + c0 + 31 > at), sS + (uint32_t)c0);
                         if (cut) hide(c0);
                         m_half = fmaxf(m_half, top());
                         if (c0) tmem_st32(sS + 32u, sv);
@@ -872,7 +884,7 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                         if (!__all_sync(0xffffffffu, pf_wait(S, &S.o_ready[mb], (uint32_t)(done + i - 1) & 1u))) ok = false;   // (ends at the next tile)
                         tc_fence_after_sync();
 #pragma unroll 1
-                        for (int ch = 0; ch < 8; ++ch) tmem_scale8(colO + 8u * ch, alpha);
+                        for (int ch = 0; ch < 8; ++ch) tmem_map8(colO + 8u * ch, [&](float o) { return o * alpha; });
                     }
                 }
                 if (last && w.next_tiles(next.b) > 0) fetch(next.b, w.next_h());        // (the last product with the queries is done)
@@ -881,16 +893,27 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                 uint64_t ps[2] = {0ull, 0ull};
                 auto put = [&](uint32_t c0) {       // P of the columns in sv -> 16 columns of the half's own part of S
                     uint32_t pk[16];
-                    if (kMode == kCapped && low) {
+                    if (kMode == kCapped && way) {
+                        auto weigh = [&](auto logit) {
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const uint64_t r = pack_f2(sv[2 * e], sv[2 * e + 1]);
-                            float p0, p1;
-                            unpack_f2(fma_f2(r, pf_low(P, mul_f2(r, r)), nz2), p0, p1);
-                            p0 = pf_exp2(p0);
-                            p1 = pf_exp2(p1);
-                            ps[e & 1] = add_f2(ps[e & 1], pack_f2(p0, p1));
-                            pk[e] = pack_half2(p0, p1);
+                            for (int e = 0; e < 16; ++e) {
+                                float p0, p1;
+                                unpack_f2(logit(pack_f2(sv[2 * e], sv[2 * e + 1])), p0, p1);
+                                p0 = pf_exp2(p0);
+                                p1 = pf_exp2(p1);
+                                ps[e & 1] = add_f2(ps[e & 1], pack_f2(p0, p1));
+                                pk[e] = pack_half2(p0, p1);
+                            }
+                        };
+                        if (way == 1) {
+                            weigh([&](uint64_t r) { return fma_f2(r, pf_low(P, mul_f2(r, r)), nz2); });
+                        } else {
+                            const float g = sc * P.sc.cap_inv;
+                            const uint64_t g2 = pack_f2(g, g);
+                            weigh([&](uint64_t r) {
+                                const uint64_t u = mul_f2(r, g2);
+                                return fma_f2(u, pf_mid(P, mul_f2(u, u)), nz2);
+                            });
                         }
                         tmem_st16(sS + c0, pk);
                         return;
