@@ -75,6 +75,8 @@ struct PgScores {
     const int32_t* prefix;           // (n_seq) or null
     float cap, cap_inv;              // of logits to the base of 2, and its reciprocal; 0: none
     int32_t window, max_prefix;      // 0: none; what prefixes are held to
+    static constexpr int kNear = 5;
+    float near[kNear];               // of the cap, below
 };
 // A sequence's prefix
 __device__ __forceinline__ int pg_prefix(const PgScores& S, int seq, int len) { return S.prefix ? max(0, min(S.prefix[seq], min(S.max_prefix, len))) : 0; }
@@ -84,26 +86,24 @@ __device__ __forceinline__ float pg_ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// cap * tanh(x / cap), u = x / cap.  Up to 1/2 an odd polynomial of degree 9, fitted to the relative error (1.5e-8); beyond it 1 - 2 / (e^2u + 1), whose terms
-// are then of one magnitude, so that both are off by a few roundings of the result itself.
-struct CapNear {
-    static constexpr int kTerms = 5;
-    __device__ __forceinline__ static constexpr float k(int i) {
-        constexpr float c[kTerms] = {1.f, -0.3333314389579803f, 0.1332587894742629f, -0.05304549361635799f, 0.017241490183840052f};
-        return c[i];
-    }
-};
-__device__ __forceinline__ float pg_cap_near(float u, float cap) {
-    const float v = u * u;
-    float p = CapNear::k(4);
+// cap * tanh(x / cap), u = x / cap.  Up to 1/2 an odd polynomial of degree 9, fitted to the relative error (1.5e-8; near[]: times the cap); beyond it
+// 1 - 2 / (e^2u + 1), whose terms are then of one magnitude, so that both are off by a few roundings of the result itself.
+__device__ __forceinline__ float pg_cap_near(float u, float v, const PgScores& S) {      // v = u^2
+    float p = S.near[PgScores::kNear - 1];
 #pragma unroll
-    for (int i = 3; i >= 0; --i) p = fmaf(p, v, CapNear::k(i));
-    return cap * u * p;
+    for (int i = PgScores::kNear - 2; i >= 0; --i) p = fmaf(p, v, S.near[i]);
+    return u * p;
 }
 __device__ __forceinline__ float pg_cap_far(float u, float cap) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(pg_ex2(u * 2.8853900817779268f) + 1.f));
     return cap * fmaf(-2.f, r, 1.f);
+}
+// The factor from products to u, finite: nothing of a product of zero, and what it would take beyond has long reached the cap.
+__device__ __forceinline__ float pg_unit(float factor, const PgScores& S) { return fminf(factor * S.cap_inv, 1.329227995784916e36f); }
+__device__ __forceinline__ float pg_cap_any(float u, const PgScores& S) {
+    const float f = pg_cap_far(u, S.cap), v = u * u;
+    return v <= 0.25f ? pg_cap_near(u, v, S) : f;
 }
 
 // Kernels that this thread's last call of an entry point enqueued.

@@ -350,9 +350,10 @@ template <int NT>
 struct Marks {
     int lo[NT][2], pos[NT][2];       // first token of its window, its own position
     float slope[NT][2];              // to the base of 2
+    float unit[NT][2];               // the factor from sums to logits over the cap
     int pre;                         // tokens of the prefix
-    float cap, cap_inv;
-    bool biased;
+    float cap;
+    bool biased, both_sides;         // both_sides: some column sees tokens behind its own place
 };
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 16 ? 0xffffu : (1u << n) - 1u; }
 // The tokens of a unit from t0 on that a column sees
@@ -381,7 +382,7 @@ __device__ __forceinline__ void pd_no_number_seen(State<NT>& st, float& s0, floa
 // U units of 16 tokens at u in shared memory.  kEdge: some of them (tokens from len on of the sequence, from lim[] on of a column, kMod: between its
 // prefix and its window) are hidden.
 template <int NT, int U, bool kEdge, bool kMod>
-__device__ __forceinline__ void pd_units(const uint8_t* u, const Magic& mg, const Query<NT>& Q, State<NT>& st, int r, int c, int t0, int len, const int (&lim)[NT][2], const Marks<NT>& mk) {
+__device__ __forceinline__ void pd_units(const PdParams& P, const uint8_t* u, const Magic& mg, const Query<NT>& Q, State<NT>& st, int r, int c, int t0, int len, const int (&lim)[NT][2], const Marks<NT>& mk) {
     float s[U][NT][4];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
@@ -415,54 +416,62 @@ __device__ __forceinline__ void pd_units(const uint8_t* u, const Magic& mg, cons
     uint32_t seen[U][NT][2];
     if (kMod) {
         // logits to the base of 2 in their final form
-#pragma unroll
-        for (int i = 0; i < U; ++i)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[i][nt][e] = __fmul_rn(s[i][nt][e], Q.f[nt][e & 1]);
         if (mk.cap > 0.f) {
-            bool far = false;
+            float most = 0.f;
 #pragma unroll
             for (int i = 0; i < U; ++i)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        s[i][nt][e] *= mk.cap_inv;
-                        far |= !(fabsf(s[i][nt][e]) <= 0.5f);
+                        s[i][nt][e] *= mk.unit[nt][e & 1];
+                        most = fmaxf(most, fabsf(s[i][nt][e]));
                     }
-            if (__any_sync(0xffffffffu, far)) {
+            if (__any_sync(0xffffffffu, most > 0.5f)) {
 #pragma unroll
                 for (int i = 0; i < U; ++i)
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float x = s[i][nt][e], f = pg_cap_far(x, mk.cap);
-                            s[i][nt][e] = fabsf(x) <= 0.5f ? pg_cap_near(x, mk.cap) : f;
-                        }
+                        for (int e = 0; e < 4; ++e) s[i][nt][e] = pg_cap_any(s[i][nt][e], P.sc);
             } else {
 #pragma unroll
                 for (int i = 0; i < U; ++i)
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) s[i][nt][e] = pg_cap_near(s[i][nt][e], mk.cap);
+                        for (int e = 0; e < 4; ++e) s[i][nt][e] = pg_cap_near(s[i][nt][e], s[i][nt][e] * s[i][nt][e], P.sc);
             }
         }
-        if (mk.biased)
+        // times one with a cap, which has the factor in it
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
+            for (int e = 0; e < 2; ++e) {
+                const float f = mk.cap > 0.f ? 1.f : Q.f[nt][e];
+                if (!mk.biased) {
+                    if (mk.cap > 0.f) continue;
+#pragma unroll
+                    for (int i = 0; i < U; ++i) {
+                        s[i][nt][e] = __fmul_rn(s[i][nt][e], f);
+                        s[i][nt][2 + e] = __fmul_rn(s[i][nt][2 + e], f);
+                    }
+                } else if (mk.both_sides) {
                     const float d = (float)(t0 + r - mk.pos[nt][e]);
 #pragma unroll
                     for (int i = 0; i < U; ++i) {
-                        s[i][nt][e] = fmaf(-mk.slope[nt][e], fabsf(d + 16.f * i), s[i][nt][e]);
-                        s[i][nt][2 + e] = fmaf(-mk.slope[nt][e], fabsf(d + 16.f * i + 8.f), s[i][nt][2 + e]);
+                        s[i][nt][e] = fmaf(-mk.slope[nt][e], fabsf(d + 16.f * i), s[i][nt][e] * f);
+                        s[i][nt][2 + e] = fmaf(-mk.slope[nt][e], fabsf(d + 16.f * i + 8.f), s[i][nt][2 + e] * f);
+                    }
+                } else {                   // (the slope times whole numbers below 32, on top of the first token's)
+                    const float b = mk.slope[nt][e] * (float)(t0 + r - mk.pos[nt][e]);
+#pragma unroll
+                    for (int i = 0; i < U; ++i) {
+                        s[i][nt][e] = fmaf(s[i][nt][e], f, fmaf(mk.slope[nt][e], 16.f * i, b));
+                        s[i][nt][2 + e] = fmaf(s[i][nt][2 + e], f, fmaf(mk.slope[nt][e], 16.f * i + 8.f, b));
                     }
                 }
+            }
         if (kEdge)
 #pragma unroll
             for (int i = 0; i < U; ++i)
@@ -753,8 +762,8 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
         if (kMod) {
             mk.pre = g.s.pre;
             mk.cap = P.sc.cap;
-            mk.cap_inv = P.sc.cap_inv;
             mk.biased = P.sc.slopes != nullptr;
+            bool behind_it = false;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -762,8 +771,11 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
                     const int row = row0 + 8 * nt + 2 * c + e, at = row / P.gqa;
                     mk.pos[nt][e] = behind + at - 1;
                     mk.lo[nt][e] = P.sc.window ? max(0, max(0, behind + at) - P.sc.window) : 0;
+                    mk.unit[nt][e] = pg_unit(Q.f[nt][e], P.sc);
+                    behind_it |= lim[nt][e] > mk.pos[nt][e] + 1;
                     mk.slope[nt][e] = mk.biased && row < n_rows ? P.sc.slopes[g.h * P.gqa + row - at * P.gqa] * 1.44269504088896340736f : 0.f;
                 }
+            mk.both_sides = __any_sync(0xffffffffu, behind_it);
             if (P.sc.window) lo_max = max(0, max(0, behind + (min(row0 + kCols, n_rows) - 1) / P.gqa) - P.sc.window);
         }
         State<NT> st = {};
@@ -780,15 +792,15 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
             const uint32_t there = w.have >> (2 * stage) & 3u;
             if (there == 3u && t0 + kBatchTok <= lim_min && (!kMod || t0 >= lo_max || t0 + kBatchTok <= g.s.pre)) {
                 if (NT == 1) {
-                    pd_units<NT, 2, false, kMod>(tile, mg, Q, st, r, c, t0, g.s.len, lim, mk);
+                    pd_units<NT, 2, false, kMod>(P, tile, mg, Q, st, r, c, t0, g.s.len, lim, mk);
                 } else {
-                    pd_units<NT, 1, false, kMod>(tile, mg, Q, st, r, c, t0, g.s.len, lim, mk);
-                    pd_units<NT, 1, false, kMod>(tile + kUnitBytes, mg, Q, st, r, c, t0 + kUnitTok, g.s.len, lim, mk);
+                    pd_units<NT, 1, false, kMod>(P, tile, mg, Q, st, r, c, t0, g.s.len, lim, mk);
+                    pd_units<NT, 1, false, kMod>(P, tile + kUnitBytes, mg, Q, st, r, c, t0 + kUnitTok, g.s.len, lim, mk);
                 }
             } else {
 #pragma unroll 1
                 for (int i = 0; i < 2; ++i)
-                    if (there >> i & 1u) pd_units<NT, 1, true, kMod>(tile + i * kUnitBytes, mg, Q, st, r, c, t0 + i * kUnitTok, g.s.len, lim, mk);
+                    if (there >> i & 1u) pd_units<NT, 1, true, kMod>(P, tile + i * kUnitBytes, mg, Q, st, r, c, t0 + i * kUnitTok, g.s.len, lim, mk);
             }
             __syncwarp();
             if (w.issued < w.n) issue(g, w, stage);
@@ -1149,6 +1161,8 @@ static bool pd_scores(const BgtqPagedScores* s, int64_t cap_tokens, PgScores& to
     to.prefix = s->max_prefix > 0 ? s->prefix : nullptr;
     to.cap = s->softcap * 1.44269504088896340736f;
     to.cap_inv = s->softcap > 0.f ? 1.0f / to.cap : 0.f;
+    constexpr double near[PgScores::kNear] = {1.0, -0.3333314389579803, 0.1332587894742629, -0.05304549361635799, 0.017241490183840052};
+    for (int i = 0; i < PgScores::kNear; ++i) to.near[i] = (float)(near[i] * to.cap);
     to.window = s->window < cap_tokens ? s->window : 0;      // (one that no sequence is longer than hides nothing)
     to.max_prefix = s->max_prefix;
     return to.slopes || to.prefix || to.cap > 0.f || to.window;
@@ -1156,7 +1170,7 @@ static bool pd_scores(const BgtqPagedScores* s, int64_t cap_tokens, PgScores& to
 static int pd_scores_error(const BgtqPagedScores* s, const void* cu_q, int32_t flags) {
     if (!s) return BGTQ_OK;
     if (s->reserved || s->window < 0 || s->max_prefix < 0 || (s->window && cu_q && !(flags & BGTQ_PAGED_CAUSAL))) return BGTQ_E_BADARG;
-    return s->softcap == 0.f || (s->softcap >= 7.8886090522101181e-31f && s->softcap <= 1.2676506002282294e30f) ? BGTQ_OK : BGTQ_E_BADARG;
+    return s->softcap == 0.f || (s->softcap >= 5.42101086242752217e-20f && s->softcap <= 1.8446744073709552e19f) ? BGTQ_OK : BGTQ_E_BADARG;
 }
 
 extern "C" __attribute__((visibility("default"))) int64_t bgtq_paged_scored_workspace_bytes(int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv,

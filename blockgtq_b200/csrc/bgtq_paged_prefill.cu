@@ -377,10 +377,6 @@ __device__ __forceinline__ void tmem_map8(uint32_t taddr, F f) {
                  "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                  : "memory");
 }
-__device__ __forceinline__ float pf_cap_any(float x, const PgScores& sc) {
-    const float u = x * sc.cap_inv, f = pg_cap_far(u, sc.cap);
-    return fabsf(u) <= 0.5f ? pg_cap_near(u, sc.cap) : f;
-}
 // A pair of products' logits by the short polynomial, over the products; v: their squares
 __device__ __forceinline__ uint64_t pf_low(const Pf& P, uint64_t v) {
     uint64_t p = fma_f2(v, P.low[kLowTerms - 1], P.low[kLowTerms - 2]);
@@ -404,10 +400,10 @@ __device__ __forceinline__ float abs_top(const float (&x)[32]) {
     }
     return fmaxf(a, b);
 }
-// 32 products x[], in tensor memory at `from`, to logits: times factor (even: the one that P.low is made for), capped, and less slope times the distances, of
-// which the first is `ahead` of the row's own place (both_sides: some lie behind it).
+// 32 products x[], in tensor memory at `from`, to logits: times factor (even: the one that P.low is made for), capped (alike: by pg_cap_any, as the row's
+// reference was), and less slope times the distances, of which the first is `ahead` of the row's own place (both_sides: some lie behind it).
 template <bool kCap, bool kBias>
-__device__ __forceinline__ void pf_shape(float (&x)[32], const Pf& P, float factor, bool even, float slope, float ahead, bool both_sides, uint32_t from) {
+__device__ __forceinline__ void pf_shape(float (&x)[32], const Pf& P, float factor, bool even, bool alike, float slope, float ahead, bool both_sides, uint32_t from) {
     auto load = [&]() {
         tmem_ld32(from, x);
         tmem_ld_wait();
@@ -418,7 +414,7 @@ __device__ __forceinline__ void pf_shape(float (&x)[32], const Pf& P, float fact
     auto bias = [&](int c) { return fma_f2(s2, P.steps[c >> 1], t2); };
     if (kCap) {
         bool done = false;
-        if (even) {
+        if (even && !alike) {
             float most[2] = {0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < 32; c += 2) {
@@ -433,7 +429,7 @@ __device__ __forceinline__ void pf_shape(float (&x)[32], const Pf& P, float fact
             if (!done) load();
         }
         if (!done) {
-            const float g = factor * P.sc.cap_inv;
+            const float g = pg_unit(factor, P.sc);
             const uint64_t g2 = pack_f2(g, g);
             float most[2] = {0.f, 0.f};
 #pragma unroll
@@ -444,10 +440,10 @@ __device__ __forceinline__ void pf_shape(float (&x)[32], const Pf& P, float fact
                 most[c >> 1 & 1] = max3(most[c >> 1 & 1], v0, v1);
                 unpack_f2(mul_f2(u, pf_mid(P, v)), x[c], x[c + 1]);
             }
-            if (!__all_sync(0xffffffffu, fmaxf(most[0], most[1]) <= kMidReach * kMidReach)) {
+            if (alike || !__all_sync(0xffffffffu, fmaxf(most[0], most[1]) <= kMidReach * kMidReach)) {
                 // (in place, a few at a time: what hardly ever runs is kept short)
 #pragma unroll 1
-                for (int c = 0; c < 32; c += 8) tmem_map8(from + (uint32_t)c, [&](float r) { return pf_cap_any(r * factor, P.sc); });
+                for (int c = 0; c < 32; c += 8) tmem_map8(from + (uint32_t)c, [&](float r) { return pg_cap_any(r * g, P.sc); });
                 tmem_st_wait();
                 load();
             }
@@ -778,6 +774,8 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
             auto place = [&](int i) { return kMod ? w.b.tile<kBack>(tile0 + i) : i; };              // of a tile among the sequence's valid[]
             uint32_t units = tiles > 0 ? valid[place(0)] : 0;
             float m_used = -INFINITY, lsum = 0.f;    // what this row scales by (log2), this half's denominator
+            const float unit = kMode == kCapped ? pg_unit(sc, P.sc) : 0.f;
+            float u_lim = -INFINITY;                 // kCapped: up to here logits are within the reference's reach (they rise no faster than what is capped)
             bool huge = false;                       // logits whose steps in fp32 are no longer small beside a weight's range
             for (int i = 0; i < tiles; ++i) {
                 if (!__all_sync(0xffffffffu, pf_wait(S, &S.s_ready[mb], (uint32_t)(done + i) & 1u))) ok = false;
@@ -826,26 +824,15 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                     far = fmaxf(far, abs_top(sv));
                     if (cut) hide(0);
                     m_half = fmaxf(m_half, top());
-                    if (m_half > -INFINITY) m_half = pf_cap_any(m_half * sc, P.sc);
-                    if (!cut && !huge)
-                        way = even && __all_sync(0xffffffffu, far * far <= P.low_reach2) ? 1 : __all_sync(0xffffffffu, far * (sc * P.sc.cap_inv) <= kMidReach) ? 2 : 0;
-                    if (!way) {                        // logits take their products' places
-#pragma unroll 1
-                        for (int c0 = 32; c0 >= 0; c0 -= 32) {
-                            load(c0);
-                            pf_shape<true, false>(sv, P, sc, even, 0.f, 0.f, false, sS + (uint32_t)c0);
-                            if (cut) hide(c0);
-                            if (c0) tmem_st32(sS + 32u, sv);
-                        }
-                        tmem_st_wait();
-                    }
+                    m_half *= unit;                    // (u: capped where the reference may have to move)
+                    if (!cut) way = even && __all_sync(0xffffffffu, far * far <= P.low_reach2) ? 1 : __all_sync(0xffffffffu, far * unit <= kMidReach) ? 2 : 0;
                 } else if constexpr (kMode >= kBiased) {       // logits take their products' places
                     m_half = -INFINITY;
 #pragma unroll 1
                     for (int c0 = 32; c0 >= 0; c0 -= 32) {
                         load(c0);
                         // (tokens behind the row's own place are in its sight only where it lies in the prefix, or sees all)
-                        pf_shape<kMode == kCappedBiased, true>(sv, P, sc, even, slope, (float)(t0 + c0 - at),
+                        pf_shape<kMode == kCappedBiased, true>(sv, P, sc, even, false, slope, (float)(t0 + c0 - at),
                                                                __any_sync(0xffffffffu, lim > at + 1 && t0 + c0 + 31 > at), sS + (uint32_t)c0);
                         if (cut) hide(c0);
                         m_half = fmaxf(m_half, top());
@@ -863,12 +850,14 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                     asm volatile("cp.async.wait_all;" ::: "memory");
                     __syncwarp();
                 }
-                const bool move = bar_or(1 + mb, m_half - m_used > kReach || !ok);
+                const bool move = bar_or(1 + mb, (kMode == kCapped ? m_half > u_lim : m_half - m_used > kReach) || !ok);
                 if (move) {
                     S.xch[mb][hf][r128] = m_half;
                     const bool all_ok = bar_and(3 + mb, 256, ok);
                     if (!all_ok) { ok = false; break; }              // (the same verdict for the whole block)
-                    const float top_m = fmaxf(m_half, S.xch[mb][hf ^ 1][r128]);
+                    float top_m = fmaxf(m_half, S.xch[mb][hf ^ 1][r128]);
+                    const float top_u = top_m;
+                    if (kMode == kCapped && top_u > -INFINITY) top_m = pg_cap_any(top_u, P.sc);
                     // (where fp32's steps are wider than the distance, it becomes none)
                     const float m_new = top_m - (top_m - kLift) > kReach ? top_m : top_m - kLift;
                     float alpha = 1.f;
@@ -877,6 +866,7 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                         alpha = pf_exp2(m_used - m_new);
                         m_used = m_new;
                     }
+                    if (kMode == kCapped && top_u > -INFINITY) u_lim = top_u + (m_used + kReach - top_m) * P.sc.cap_inv;
                     huge = __any_sync(0xffffffffu, fabsf(m_used) >= kHuge && m_used > -INFINITY);
                     lsum *= alpha;
                     if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
@@ -888,6 +878,19 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                     }
                 }
                 if (last && w.next_tiles(next.b) > 0) fetch(next.b, w.next_h());        // (the last product with the queries is done)
+                if (kMode == kCapped) {
+                    if (huge) way = 0;                 // (product and difference rounded apart, as the reference was)
+                    if (!way) {                        // logits take their products' places
+#pragma unroll 1
+                        for (int c0 = 32; c0 >= 0; c0 -= 32) {
+                            load(c0);
+                            pf_shape<true, false>(sv, P, sc, even, huge, 0.f, 0.f, false, sS + (uint32_t)c0);
+                            if (cut) hide(c0);
+                            if (c0) tmem_st32(sS + 32u, sv);
+                        }
+                        tmem_st_wait();
+                    }
+                }
                 const float z = m_used == -INFINITY ? 0.f : m_used;
                 const uint64_t nz2 = pack_f2(-z, -z), sc2 = huge ? pack_f2(1.f, 1.f) : pack_f2(fac, fac);
                 uint64_t ps[2] = {0ull, 0ull};
@@ -908,8 +911,7 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                         if (way == 1) {
                             weigh([&](uint64_t r) { return fma_f2(r, pf_low(P, mul_f2(r, r)), nz2); });
                         } else {
-                            const float g = sc * P.sc.cap_inv;
-                            const uint64_t g2 = pack_f2(g, g);
+                            const uint64_t g2 = pack_f2(unit, unit);
                             weigh([&](uint64_t r) {
                                 const uint64_t u = mul_f2(r, g2);
                                 return fma_f2(u, pf_mid(P, mul_f2(u, u)), nz2);

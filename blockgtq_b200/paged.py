@@ -319,8 +319,8 @@ def _limits(softcap, window, causal):
         softcap = 0.0
     else:
         softcap = float(softcap)
-        if not 2.0 ** -100 <= softcap <= 2.0 ** 100:
-            raise ValueError(f"softcap must be positive, 2^-100 to 2^100, got {softcap}")
+        if not 2.0 ** -64 <= softcap <= 2.0 ** 64:
+            raise ValueError(f"softcap must be positive, 2^-64 to 2^64, got {softcap}")
     if window is None:
         return softcap, 0
     window = operator.index(window)

@@ -696,7 +696,7 @@ int bgtq_paged_attend(const void* q, int64_t q_st, int64_t q_sh, const uint8_t* 
 typedef struct BgtqPagedScores {
     const float* slopes;        /* device, (n_q), finite; NULL: no bias */
     const int32_t* prefix;      /* device, (n_seq), held to 0 .. max_prefix; NULL: none */
-    float softcap;              /* c, 2^-100 .. 2^100; 0: no cap */
+    float softcap;              /* c, 2^-64 .. 2^64; 0: no cap */
     int32_t window;             /* tokens up to the row's own that it sees; 0: all.  Queries are causal then */
     int32_t max_prefix;         /* it chooses the launch, too */
     int32_t reserved;           /* 0 */

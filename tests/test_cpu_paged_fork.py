@@ -193,7 +193,7 @@ def test_positions_and_axes_belong_to_rope():
         c.append_and_attend(0, *rows, causal=False)
 
 
-@pytest.mark.parametrize("change", [dict(softcap=0.0), dict(softcap=-1.0), dict(softcap=float("nan")), dict(softcap=float("inf")), dict(softcap=1e-40),
+@pytest.mark.parametrize("change", [dict(softcap=0.0), dict(softcap=-1.0), dict(softcap=float("nan")), dict(softcap=float("inf")), dict(softcap=1e-20), dict(softcap=1e20),
                                     dict(window=0), dict(window=-3), dict(max_prefix_len=-1, prefix_lens=torch.zeros(4, dtype=torch.int32)),
                                     dict(slopes=torch.zeros(3)), dict(slopes=torch.zeros(4).half()), dict(prefix_lens=torch.zeros(3, dtype=torch.int32)),
                                     dict(prefix_lens=torch.zeros(4, dtype=torch.int64))])
@@ -223,6 +223,6 @@ def test_the_library_refuses_scores():
         attend = lib.bgtq_paged_attend_scored(p, 512, 128, p, 4608, 2304, 2, 16, p, 1, 0, p, p, 0, 0, 4, 2, 1, 16, 1.0, flags, sc, p, 0, p, 512, 128, 0, 0, 0)
         return attend, lib.bgtq_paged_scored_workspace_bytes(1, 1, 4, 2, 1, 16, flags, sc)
     assert both() == (_lib.OK, 0) and both(window=5, flags=4) == (_lib.OK, 0)
-    for kw in (dict(window=-1), dict(max_prefix=-1), dict(softcap=-1.0), dict(softcap=float("nan")), dict(softcap=float("inf")), dict(softcap=1e-35), dict(reserved=1)):
+    for kw in (dict(window=-1), dict(max_prefix=-1), dict(softcap=-1.0), dict(softcap=float("nan")), dict(softcap=float("inf")), dict(softcap=5e-20), dict(softcap=2e19), dict(reserved=1)):
         assert both(**kw) == (-1, -1), kw
     assert both(window=5)[0] == -1                       # a window, and no causal queries

@@ -205,9 +205,27 @@ def test_a_cap_of_any_size_and_logits_beyond_it(rows_form):
     args = (pages, table.to(DEV), torch.tensor([200], **I32), torch.tensor([0, 5], **I32))
     for dtype, scale in ((torch.float16, 0.1), (torch.bfloat16, 0.1), (torch.float16, 100.0), (torch.float16, -3.0), (torch.float16, 0.0)):
         q = _noise(gen, 5, 4, 128).to(dtype)
-        for cap in (2.0 ** -100, 1e-3, 1.0, 60.0, 1e4, 2.0 ** 100):
+        for cap in (2.0 ** -64, 1e-3, 1.0, 60.0, 1e4, 2.0 ** 64):
             out, lse = paged_kv4_prefill_attention(q.to(DEV), *args, scale=scale, return_lse=True, softcap=cap)
             W.check(out, lse, S.attention(q, pages, slots[0], scale=scale, softcap=cap), slice(0, 5))
+    # queries of every magnitude, and keys of zeros: logits are none of fp32's, or nothing at all
+    from blockgtq_b200 import paged_kv4_append
+    zero = torch.zeros(40, 1, 128, dtype=torch.float16, device=DEV)
+    paged_kv4_append(pages, slots[0][20:60].to(DEV), zero, zero)
+    for scale in (1e30, 1.0, 1e-30):
+        for cap in (2.0 ** -64, 1.0, 2.0 ** 64):
+            for top in (3e38, 1.0, 1e-38):
+                q = (_noise(gen, 5, 4, 128).sign() * top).bfloat16()
+                q[1] = 0
+                out, lse = paged_kv4_prefill_attention(q.to(DEV), *args, scale=scale, return_lse=True, softcap=cap)
+                k, v = (x.cpu() for x in S.read(pages, slots[0]))
+                y = cap * torch.tanh(torch.einsum("nhd,td->nht", q.double(), k[:, 0]) * scale / cap)
+                for row in range(5):
+                    # a logit is off by 2^-20 of its terms' magnitudes, and the sum by what its largest ones are
+                    want = torch.logsumexp(y[row, :, :196 + row], -1)
+                    size = torch.einsum("hd,td->ht", q[row].double().abs(), k[:196 + row, 0].abs()) * scale
+                    off = 2.0 ** -20 * (torch.minimum(size, torch.tensor(cap, dtype=torch.float64)).amax(-1) + want.abs() + 1) + 1e-5
+                    assert torch.isfinite(out[row]).all() and ((lse[row].double().cpu() - want).abs() <= off).all(), (scale, cap, top, row)
     # logits far beyond fp32's range end at the cap
     q = torch.full((5, 4, 128), 3e38, dtype=torch.bfloat16)
     out, lse = paged_kv4_prefill_attention(q.to(DEV), *args, return_lse=True, softcap=20.0)
