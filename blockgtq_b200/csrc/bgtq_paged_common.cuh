@@ -78,6 +78,12 @@ struct PgScores {
     static constexpr int kNear = 5;
     float near[kNear];               // of the cap, below
 };
+// What an attention's logits go through beside the scale, each with kernels of its own: in one that asks at run time, the layers that only mask paid 7 % of
+// a decode for the others' registers.  Rows may be masked in all but the plain one.
+enum PgMode { kPlain, kMasked, kCapped, kBiased, kCappedBiased };
+inline PgMode pg_mode(const PgScores& S, bool mod) {
+    return !mod ? kPlain : S.slopes ? S.cap > 0.f ? kCappedBiased : kBiased : S.cap > 0.f ? kCapped : kMasked;
+}
 // A sequence's prefix
 __device__ __forceinline__ int pg_prefix(const PgScores& S, int seq, int len) { return S.prefix ? max(0, min(S.prefix[seq], min(S.max_prefix, len))) : 0; }
 

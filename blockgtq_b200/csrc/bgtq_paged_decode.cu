@@ -352,8 +352,7 @@ struct Marks {
     float slope[NT][2];              // to the base of 2
     float unit[NT][2];               // the factor from sums to logits over the cap
     int pre;                         // tokens of the prefix
-    float cap;
-    bool biased, both_sides;         // both_sides: some column sees tokens behind its own place
+    bool both_sides;                 // some column sees tokens behind its own place
 };
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 16 ? 0xffffu : (1u << n) - 1u; }
 // The tokens of a unit from t0 on that a column sees
@@ -381,8 +380,9 @@ __device__ __forceinline__ void pd_no_number_seen(State<NT>& st, float& s0, floa
 
 // U units of 16 tokens at u in shared memory.  kEdge: some of them (tokens from len on of the sequence, from lim[] on of a column, kMod: between its
 // prefix and its window) are hidden.
-template <int NT, int U, bool kEdge, bool kMod>
+template <int NT, int U, bool kEdge, PgMode kMode>
 __device__ __forceinline__ void pd_units(const PdParams& P, const uint8_t* u, const Magic& mg, const Query<NT>& Q, State<NT>& st, int r, int c, int t0, int len, const int (&lim)[NT][2], const Marks<NT>& mk) {
+    constexpr bool kMod = kMode != kPlain, kCap = kMode == kCapped || kMode == kCappedBiased, kBias = kMode >= kBiased, kShaped = kCap || kBias;
     float s[U][NT][4];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
@@ -415,8 +415,8 @@ __device__ __forceinline__ void pd_units(const PdParams& P, const uint8_t* u, co
     }
     uint32_t seen[U][NT][2];
     if (kMod) {
-        // logits to the base of 2 in their final form
-        if (mk.cap > 0.f) {
+        // kShaped: logits to the base of 2 in their final form
+        if (kCap) {
             float most = 0.f;
 #pragma unroll
             for (int i = 0; i < U; ++i)
@@ -427,51 +427,33 @@ __device__ __forceinline__ void pd_units(const PdParams& P, const uint8_t* u, co
                         s[i][nt][e] *= mk.unit[nt][e & 1];
                         most = fmaxf(most, fabsf(s[i][nt][e]));
                     }
-            if (__any_sync(0xffffffffu, most > 0.5f)) {
+            auto each = [&](auto f) {
 #pragma unroll
                 for (int i = 0; i < U; ++i)
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) s[i][nt][e] = pg_cap_any(s[i][nt][e], P.sc);
-            } else {
-#pragma unroll
-                for (int i = 0; i < U; ++i)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) s[i][nt][e] = pg_cap_near(s[i][nt][e], s[i][nt][e] * s[i][nt][e], P.sc);
-            }
+                        for (int e = 0; e < 4; ++e) s[i][nt][e] = f(s[i][nt][e]);
+            };
+            if (__any_sync(0xffffffffu, most > 0.5f)) each([&](float u) { return pg_cap_any(u, P.sc); });
+            else each([&](float u) { return pg_cap_near(u, u * u, P.sc); });
         }
-        // times one with a cap, which has the factor in it
+        if (kBias)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float f = mk.cap > 0.f ? 1.f : Q.f[nt][e];
-                if (!mk.biased) {
-                    if (mk.cap > 0.f) continue;
+                for (int e = 0; e < 2; ++e) {
+                    const float f = kCap ? 1.f : Q.f[nt][e], d = (float)(t0 + r - mk.pos[nt][e]), b = mk.slope[nt][e] * d;
 #pragma unroll
-                    for (int i = 0; i < U; ++i) {
-                        s[i][nt][e] = __fmul_rn(s[i][nt][e], f);
-                        s[i][nt][2 + e] = __fmul_rn(s[i][nt][2 + e], f);
-                    }
-                } else if (mk.both_sides) {
-                    const float d = (float)(t0 + r - mk.pos[nt][e]);
+                    for (int i = 0; i < U; ++i)
 #pragma unroll
-                    for (int i = 0; i < U; ++i) {
-                        s[i][nt][e] = fmaf(-mk.slope[nt][e], fabsf(d + 16.f * i), s[i][nt][e] * f);
-                        s[i][nt][2 + e] = fmaf(-mk.slope[nt][e], fabsf(d + 16.f * i + 8.f), s[i][nt][2 + e] * f);
-                    }
-                } else {                   // (the slope times whole numbers below 32, on top of the first token's)
-                    const float b = mk.slope[nt][e] * (float)(t0 + r - mk.pos[nt][e]);
-#pragma unroll
-                    for (int i = 0; i < U; ++i) {
-                        s[i][nt][e] = fmaf(s[i][nt][e], f, fmaf(mk.slope[nt][e], 16.f * i, b));
-                        s[i][nt][2 + e] = fmaf(s[i][nt][2 + e], f, fmaf(mk.slope[nt][e], 16.f * i + 8.f, b));
-                    }
+                        for (int half = 0; half < 2; ++half) {
+                            float& x = s[i][nt][2 * half + e];
+                            const float ahead = 16.f * i + 8.f * half;
+                            // (the slope times whole numbers below 32, on top of the first token's)
+                            x = mk.both_sides ? fmaf(-mk.slope[nt][e], fabsf(d + ahead), x * f) : fmaf(x, f, fmaf(mk.slope[nt][e], ahead, b));
+                        }
                 }
-            }
         if (kEdge)
 #pragma unroll
             for (int i = 0; i < U; ++i)
@@ -522,7 +504,7 @@ __device__ __forceinline__ void pd_units(const PdParams& P, const uint8_t* u, co
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            if (!kMod) top[nt][e] *= Q.f[nt][e];
+            if (!kShaped) top[nt][e] *= Q.f[nt][e];
             move |= top[nt][e] > st.top[nt][e];
         }
     if (__any_sync(0xffffffffu, move)) {
@@ -564,8 +546,8 @@ __device__ __forceinline__ void pd_units(const PdParams& P, const uint8_t* u, co
             for (int e = 0; e < 2; ++e) {
                 const float z = kEdge && st.m[nt][e] == -INFINITY ? 0.f : st.m[nt][e];
                 // (product and difference rounded apart, as the references were: fused, logits beyond 2^26 differ from theirs by more than a weight's range)
-                p[e] = ex2((kMod ? s[i][nt][e] : __fmul_rn(s[i][nt][e], Q.f[nt][e])) - z);
-                p[2 + e] = ex2((kMod ? s[i][nt][2 + e] : __fmul_rn(s[i][nt][2 + e], Q.f[nt][e])) - z);
+                p[e] = ex2((kShaped ? s[i][nt][e] : __fmul_rn(s[i][nt][e], Q.f[nt][e])) - z);
+                p[2 + e] = ex2((kShaped ? s[i][nt][2 + e] : __fmul_rn(s[i][nt][2 + e], Q.f[nt][e])) - z);
                 st.l[nt][e] += p[e] + p[2 + e];
             }
             b[nt][0] = transposed(pack_half2(p[0], p[1]));
@@ -625,9 +607,10 @@ __device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {
 }
 
 // kStages 2: two CTAs on an SM hide each other's latencies.  4: one CTA on an SM, alone with them.
-template <int NT, typename T, bool kCluster, int kStages, bool kMod>
+template <int NT, typename T, bool kCluster, int kStages, PgMode kMode>
 __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(const PdParams P) {
     extern __shared__ __align__(128) uint8_t smem_raw[];
+    constexpr bool kMod = kMode != kPlain;
     using Smem = PdSmem<NT, kStages>;
     Smem& S = *reinterpret_cast<Smem*>(smem_raw);
     constexpr int kCols = 8 * NT;
@@ -761,8 +744,6 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
         int lo_max = 0;                                      // the last of the columns' windows begins here
         if (kMod) {
             mk.pre = g.s.pre;
-            mk.cap = P.sc.cap;
-            mk.biased = P.sc.slopes != nullptr;
             bool behind_it = false;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -773,7 +754,7 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
                     mk.lo[nt][e] = P.sc.window ? max(0, max(0, behind + at) - P.sc.window) : 0;
                     mk.unit[nt][e] = pg_unit(Q.f[nt][e], P.sc);
                     behind_it |= lim[nt][e] > mk.pos[nt][e] + 1;
-                    mk.slope[nt][e] = mk.biased && row < n_rows ? P.sc.slopes[g.h * P.gqa + row - at * P.gqa] * 1.44269504088896340736f : 0.f;
+                    mk.slope[nt][e] = kMode >= kBiased && row < n_rows ? P.sc.slopes[g.h * P.gqa + row - at * P.gqa] * 1.44269504088896340736f : 0.f;
                 }
             mk.both_sides = __any_sync(0xffffffffu, behind_it);
             if (P.sc.window) lo_max = max(0, max(0, behind + (min(row0 + kCols, n_rows) - 1) / P.gqa) - P.sc.window);
@@ -792,15 +773,15 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
             const uint32_t there = w.have >> (2 * stage) & 3u;
             if (there == 3u && t0 + kBatchTok <= lim_min && (!kMod || t0 >= lo_max || t0 + kBatchTok <= g.s.pre)) {
                 if (NT == 1) {
-                    pd_units<NT, 2, false, kMod>(P, tile, mg, Q, st, r, c, t0, g.s.len, lim, mk);
+                    pd_units<NT, 2, false, kMode>(P, tile, mg, Q, st, r, c, t0, g.s.len, lim, mk);
                 } else {
-                    pd_units<NT, 1, false, kMod>(P, tile, mg, Q, st, r, c, t0, g.s.len, lim, mk);
-                    pd_units<NT, 1, false, kMod>(P, tile + kUnitBytes, mg, Q, st, r, c, t0 + kUnitTok, g.s.len, lim, mk);
+                    pd_units<NT, 1, false, kMode>(P, tile, mg, Q, st, r, c, t0, g.s.len, lim, mk);
+                    pd_units<NT, 1, false, kMode>(P, tile + kUnitBytes, mg, Q, st, r, c, t0 + kUnitTok, g.s.len, lim, mk);
                 }
             } else {
 #pragma unroll 1
                 for (int i = 0; i < 2; ++i)
-                    if (there >> i & 1u) pd_units<NT, 1, true, kMod>(P, tile + i * kUnitBytes, mg, Q, st, r, c, t0 + i * kUnitTok, g.s.len, lim, mk);
+                    if (there >> i & 1u) pd_units<NT, 1, true, kMode>(P, tile + i * kUnitBytes, mg, Q, st, r, c, t0 + i * kUnitTok, g.s.len, lim, mk);
             }
             __syncwarp();
             if (w.issued < w.n) issue(g, w, stage);
@@ -1021,10 +1002,11 @@ __global__ void __launch_bounds__(32 * kWarps) pg_merge_kernel(const PdParams P)
     pd_write<T>(P, s, cb, kCols, col, h, lane, o, m, l);
 }
 
-template <int NT, typename T, bool kMod>
+template <int NT, typename T, PgMode kMode>
 int pd_launch_split(const PdParams& P, bool merge, cudaStream_t stream) {
+    constexpr bool kMod = kMode != kPlain;
     constexpr int kStages = NT == 1 ? 2 : 4, smem = (int)sizeof(PdSmem<NT, kStages>);
-    const auto kernel = pg_attend_kernel<NT, T, false, kStages, kMod>;
+    const auto kernel = pg_attend_kernel<NT, T, false, kStages, kMode>;
     static std::atomic<uint64_t> allowed{0};
     if (!pg_allow_smem(kernel, smem, allowed)) return BGTQ_E_LAUNCH;
     if (!pg_launch_ok(launch_kernel(kernel, dim3(P.n_cta), dim3(kPdThreads), smem, stream, true, P))) return BGTQ_E_LAUNCH;
@@ -1059,9 +1041,9 @@ struct ClusterLaunch {
         cfg.numAttrs = 2;
     }
 };
-template <int NT, typename T, int kStages, bool kMod>
+template <int NT, typename T, int kStages, PgMode kMode>
 int pd_launch_cluster(const PdParams& P, int64_t triples, int n_rank, cudaStream_t stream) {
-    const auto kernel = pg_attend_kernel<NT, T, true, kStages, kMod>;
+    const auto kernel = pg_attend_kernel<NT, T, true, kStages, kMode>;
     ClusterLaunch<NT, kStages> L(triples, n_rank, stream);
     static std::atomic<uint64_t> allowed{0};
     if (!pg_allow_smem(kernel, L.kBase + 8 * L.kRow, allowed)) return BGTQ_E_LAUNCH;
@@ -1073,7 +1055,7 @@ int pd_clusters(int n_rank, int dev) {
     static std::atomic<int> known[64][9];
     if (dev >= 0 && dev < 64)
         if (const int n = known[dev][n_rank].load(std::memory_order_relaxed)) return n;
-    const auto kernel = pg_attend_kernel<NT, __half, true, kStages, false>;
+    const auto kernel = pg_attend_kernel<NT, __half, true, kStages, kPlain>;
     ClusterLaunch<NT, kStages> L(1, n_rank, nullptr);
     L.cfg.numAttrs = 1;
     static std::atomic<uint64_t> allowed{0};
@@ -1085,16 +1067,16 @@ int pd_clusters(int n_rank, int dev) {
     if (dev >= 0 && dev < 64) known[dev][n_rank].store(n, std::memory_order_relaxed);
     return n;
 }
-template <int NT, typename T, bool kMod>
+template <int NT, typename T, PgMode kMode>
 int pd_launch(const PdParams& P, const PdForm& f, cudaStream_t stream) {
-    if (!f.n_rank) return pd_launch_split<NT, T, kMod>(P, f.merge, stream);
-    if (NT == 1 && f.alone) return pd_launch_cluster<NT, T, NT == 1 ? 4 : 2, kMod>(P, f.triples, f.n_rank, stream);
-    return pd_launch_cluster<NT, T, 2, kMod>(P, f.triples, f.n_rank, stream);
+    if (!f.n_rank) return pd_launch_split<NT, T, kMode>(P, f.merge, stream);
+    if (NT == 1 && f.alone) return pd_launch_cluster<NT, T, NT == 1 ? 4 : 2, kMode>(P, f.triples, f.n_rank, stream);
+    return pd_launch_cluster<NT, T, 2, kMode>(P, f.triples, f.n_rank, stream);
 }
-template <bool kMod>
+template <PgMode kMode>
 int pd_launch(const PdParams& P, const PdForm& f, bool bf16, cudaStream_t stream) {
-    if (f.nt == 1) return bf16 ? pd_launch<1, __nv_bfloat16, kMod>(P, f, stream) : pd_launch<1, __half, kMod>(P, f, stream);
-    return bf16 ? pd_launch<2, __nv_bfloat16, kMod>(P, f, stream) : pd_launch<2, __half, kMod>(P, f, stream);
+    if (f.nt == 1) return bf16 ? pd_launch<1, __nv_bfloat16, kMode>(P, f, stream) : pd_launch<1, __half, kMode>(P, f, stream);
+    return bf16 ? pd_launch<2, __nv_bfloat16, kMode>(P, f, stream) : pd_launch<2, __half, kMode>(P, f, stream);
 }
 
 bool aligned(const void* p, int64_t bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
@@ -1247,5 +1229,11 @@ extern "C" __attribute__((visibility("default"))) int bgtq_paged_attend_scored(
                scale * 1.44269504088896340736f, out, o_st, o_sh, lse, reinterpret_cast<float*>(workspace),
                reinterpret_cast<float2*>(reinterpret_cast<float*>(workspace) + (int64_t)f.n_cta * 2 * cols * kHD), status, sc};
     const bool bf16 = flags & BGTQ_PAGED_BF16;
-    return mod ? pd_launch<true>(P, f, bf16, st) : pd_launch<false>(P, f, bf16, st);
+    switch (pg_mode(sc, mod)) {
+        case kPlain: return pd_launch<kPlain>(P, f, bf16, st);
+        case kMasked: return pd_launch<kMasked>(P, f, bf16, st);
+        case kCapped: return pd_launch<kCapped>(P, f, bf16, st);
+        case kBiased: return pd_launch<kBiased>(P, f, bf16, st);
+        default: return pd_launch<kCappedBiased>(P, f, bf16, st);
+    }
 }

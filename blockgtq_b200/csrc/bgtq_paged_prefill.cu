@@ -345,9 +345,6 @@ struct Walk {
     }
 };
 
-// What an attention's logits go through beside the scale.  Its rows may be masked in all forms but the plain one.
-enum Mode { kPlain, kMasked, kCapped, kBiased, kCappedBiased };
-
 // Logits under a cap, pairs at a time on the FMA pipe, u = x / cap.  Most tiles' are small beside it: an odd polynomial of degree 7 up to 3/8, straight from the
 // products where all rows' have one factor (no row of bf16 queries was brought to another magnitude), or of degree 19 up to 3/2, both fitted to the relative
 // error (7e-8, 1.9e-8); beyond, one by one.  All of a warp's 32 tokens go one way.  (Two more values of the special function pipe for each logit would be
@@ -529,7 +526,7 @@ __device__ __forceinline__ bool pf_wait(PfSmem& S, uint64_t* bar, uint32_t parit
 
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
-template <typename T, Mode kMode>
+template <typename T, PgMode kMode>
 __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
     constexpr bool kMod = kMode != kPlain;
     // Biases fall with the distance: from a row's own place on backwards, its reference hardly moves
@@ -1226,7 +1223,7 @@ int paged_prefill(const PagedPrefill& A, cudaStream_t stream) {
     const PfLayout L = pf_layout(seqs, heads, tiles, blocks, n_cta, A.mod);
     uint8_t* const ws = A.workspace;
     const auto unpack = A.mod ? pg_unpack_kernel<true> : pg_unpack_kernel<false>;
-    const int mode = !A.mod ? kPlain : A.sc.slopes ? A.sc.cap > 0.f ? kCappedBiased : kBiased : A.sc.cap > 0.f ? kCapped : kMasked;
+    const PgMode mode = pg_mode(A.sc, A.mod);
     constexpr decltype(&pg_prefill_kernel<__half, kPlain>) kernels[5][2] = {{pg_prefill_kernel<__half, kPlain>, pg_prefill_kernel<__nv_bfloat16, kPlain>},
                                                                             {pg_prefill_kernel<__half, kMasked>, pg_prefill_kernel<__nv_bfloat16, kMasked>},
                                                                             {pg_prefill_kernel<__half, kCapped>, pg_prefill_kernel<__nv_bfloat16, kCapped>},
