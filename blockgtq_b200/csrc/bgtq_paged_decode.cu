@@ -438,22 +438,26 @@ __device__ __forceinline__ void pd_units(const PdParams& P, const uint8_t* u, co
             if (__any_sync(0xffffffffu, most > 0.5f)) each([&](float u) { return pg_cap_any(u, P.sc); });
             else each([&](float u) { return pg_cap_near(u, u * u, P.sc); });
         }
-        if (kBias)
+        if (kBias) {
+            auto each = [&](auto f) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float f = kCap ? 1.f : Q.f[nt][e], d = (float)(t0 + r - mk.pos[nt][e]), b = mk.slope[nt][e] * d;
+                    for (int e = 0; e < 2; ++e) {
+                        const float slope = mk.slope[nt][e], d = (float)(t0 + r - mk.pos[nt][e]), first = slope * d;
 #pragma unroll
-                    for (int i = 0; i < U; ++i)
+                        for (int i = 0; i < U; ++i)
 #pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            float& x = s[i][nt][2 * half + e];
-                            const float ahead = 16.f * i + 8.f * half;
-                            // (the slope times whole numbers below 32, on top of the first token's)
-                            x = mk.both_sides ? fmaf(-mk.slope[nt][e], fabsf(d + ahead), x * f) : fmaf(x, f, fmaf(mk.slope[nt][e], ahead, b));
-                        }
-                }
+                            for (int half = 0; half < 2; ++half) {
+                                float& x = s[i][nt][2 * half + e];
+                                x = f(x, kCap ? 1.f : Q.f[nt][e], slope, d, first, 16.f * i + 8.f * half);
+                            }
+                    }
+            };
+            // (on one side, the slope times whole numbers below 32 is on top of the first token's bias)
+            if (mk.both_sides) each([](float x, float f, float slope, float d, float, float on) { return fmaf(-slope, fabsf(d + on), x * f); });
+            else each([](float x, float f, float slope, float, float first, float on) { return fmaf(x, f, fmaf(slope, on, first)); });
+        }
         if (kEdge)
 #pragma unroll
             for (int i = 0; i < U; ++i)
@@ -611,6 +615,8 @@ template <int NT, typename T, bool kCluster, int kStages, PgMode kMode>
 __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(const PdParams P) {
     extern __shared__ __align__(128) uint8_t smem_raw[];
     constexpr bool kMod = kMode != kPlain;
+    // Biases fall with the distance: a warp that takes its batches from the sequence's end backwards hardly moves its references
+    constexpr bool kBack = kMode >= kBiased;
     using Smem = PdSmem<NT, kStages>;
     Smem& S = *reinterpret_cast<Smem*>(smem_raw);
     constexpr int kCols = 8 * NT;
@@ -694,7 +700,7 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
     auto issue = [&](const Segment& sg, Copies& w, int stage) {
         const int k = w.issued++;
         if ((k & 15) == 0) {
-            const int kk = k + (lane >> 1), unit = 2 * sg.s.batch(sg.first + warp + kPdWarps * kk) + (lane & 1);
+            const int kk = k + (lane >> 1), unit = 2 * sg.s.batch(sg.first + warp + kPdWarps * (kBack ? w.n - 1 - kk : kk)) + (lane & 1);
             w.from = nullptr;
             if (kk < w.n && unit < (sg.s.len + kUnitTok - 1) / kUnitTok) {
                 const int col = unit / P.pool.units, page = P.table[(int64_t)sg.seq * P.tb_st + col];
@@ -762,7 +768,8 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
         State<NT> st = {};
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) st.m[nt][0] = st.m[nt][1] = st.top[nt][0] = st.top[nt][1] = -INFINITY;
-        int t0 = g.s.batch(g.first + warp) * kBatchTok, stage = 0;
+        auto token = [&](int k) { return g.s.batch(g.first + warp + kPdWarps * (kBack ? w.n - 1 - k : k)) * kBatchTok; };       // a batch's first
+        int t0 = token(0), stage = 0;
         for (int k = 0; k < w.n && ok; ++k) {
             if (!__all_sync(0xffffffffu, mbar_wait_bounded(&S.full[warp][stage], phases >> stage & 1u))) {
                 ok = false;
@@ -785,7 +792,7 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
             }
             __syncwarp();
             if (w.issued < w.n) issue(g, w, stage);
-            t0 = kMod ? g.s.batch(g.first + warp + kPdWarps * (k + 1)) * kBatchTok : t0 + kPdWarps * kBatchTok;
+            t0 = kMod ? token(k + 1) : t0 + kPdWarps * kBatchTok;
             stage = stage == kStages - 1 ? 0 : stage + 1;
         }
         if (!ok)             // copies in flight land before the CTA leaves; nothing more is fetched
