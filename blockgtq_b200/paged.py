@@ -236,9 +236,10 @@ def paged_kv4_copy(pages, src, dst, n_tokens=None, into=None):
     ``src`` and ``dst`` are page numbers on the host (lists, or CPU tensors): no page is copied to twice, nor both copied to and from; one may be copied from
     many times.  ``n_tokens``, one number for each pair: only the units of 16 tokens that hold the page's first so many tokens are copied.  ``into``:
     another pool, of the same layers, heads and page size and apart from this one, that ``dst`` are pages of."""
-    r = None
     host = _lib.host()
-    if pages.dim() == 4:
+    if pages.dim() == 3:
+        r = host.paged_copy(pages.unsqueeze(0), src, dst, n_tokens, into if into is None or into.dim() == 4 else into.unsqueeze(0))
+    else:
         r = host.paged_copy(pages, src, dst, n_tokens, into)
     if r is None:
         return _copy(pages, src, dst, n_tokens, into)
@@ -291,10 +292,13 @@ def _copy(pages, src, dst, n_tokens, into):
         return
     lib, n = _lib.lib(), len(src)
     with torch.cuda.device(pages.device):
-        _lib.check(lib.bgtq_paged_copy(
+        rc = lib.bgtq_paged_copy(
             pages.data_ptr(), *pages.stride()[:3], pages.shape[1], to.data_ptr(), *to.stride()[:3], to.shape[1], size, pages.shape[0], pages.shape[2],
             (C.c_int32 * n)(*src), (C.c_int32 * n)(*dst), None if n_tokens is None else (C.c_int32 * n)(*n_tokens), n,
-            _lib.stream_ptr(pages.device)), "bgtq_paged_copy")
+            _lib.stream_ptr(pages.device))
+    if rc == -1:                            # (all else has been looked at)
+        raise ValueError("the pages that are copied to must lie apart from one another, and a pool from the one that it is copied into")
+    _lib.check(rc, "bgtq_paged_copy")
     _lib.count_launch(lib.bgtq_paged_launches())
 
 

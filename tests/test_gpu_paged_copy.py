@@ -64,8 +64,10 @@ def test_pages_of_any_strides_and_of_another_pool():
         heads_first = torch.zeros(4, 2, 7, b, dtype=torch.uint8, device=DEV)              # (heads, layers, pages, bytes)
         paged_kv4_copy(dev[1:, :, 1:5, 16:16 + b], src, dst, n_tokens=t, into=heads_first.permute(1, 2, 0, 3))
         assert torch.equal(heads_first.permute(1, 2, 0, 3).cpu(), _copied(want[1:, :, 1:5, 16:16 + b], src, dst, t, torch.zeros(2, 7, 4, b, dtype=torch.uint8)))
-    with pytest.raises((ValueError, RuntimeError)):
-        paged_kv4_copy(dev[:2], src, dst, into=dev[1:])     # layers of both
+    one, rows = dev[..., :b], dev.stride()
+    for bad in (dict(pages=one[:2], into=one[1:]), dict(pages=one[:, :, :1].expand(-1, -1, 3, -1)), dict(pages=one.as_strided((3, 7, 6, b), (rows[0], 0, rows[2], 1)))):
+        with pytest.raises(ValueError, match="apart"):      # layers of both; places that are one
+            paged_kv4_copy(src=src, dst=dst if "into" in bad else [1, 2, 4], **bad)
     odd = torch.zeros(2 * 4 * b + 8, dtype=torch.uint8, device=DEV)[8:].view(1, 2, 4, b)
     with pytest.raises(ValueError, match="16 bytes"):
         paged_kv4_copy(odd, [0], [1])
