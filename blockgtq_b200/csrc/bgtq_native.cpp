@@ -9,6 +9,7 @@
 // The library is not linked: `bind` receives the addresses of its entry points from the ctypes handle.
 #include <Python.h>
 
+#include <algorithm>
 #include <cstring>
 #include <vector>
 
@@ -448,24 +449,33 @@ PyObject* paged_read(PyObject*, PyObject* const* argv, Py_ssize_t n) {
 }
 
 // paged_attend(q, pages, block_table, seq_lens, cu_q | None, max_q, max_tokens (< 0: what the table holds), scale, flags, want_lse,
-//              status | None, out | None[, slopes | None, prefix lengths | None, cap or 0, window or 0, longest prefix (< 0: what the table holds)])
+//              status | None, out | None[, slopes | None, prefix lengths | None, cap | None, window | None, longest prefix | None])
 //   -> out | (out, lse) | code | None
 PyObject* paged_attend(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     if (n != 12 && n != 17) return none();
     const Args A{argv};
-    const bool scored = n == 17;
-    BgtqPagedScores sc = {};
-    int64_t most_prefix = 0;
-    if (scored) {
-        sc.softcap = A.real(14);
-        sc.window = A.i32(15);
-        most_prefix = A.num(16);
-    }
     const int64_t max_q = A.num(5);
     int64_t most = A.num(6);
     const float scale = A.real(7);
     int flags = A.i32(8);
     const bool want_lse = A.truth(9);
+    const bool scored = n == 17;
+    BgtqPagedScores sc = {};
+    int64_t most_prefix = 0;
+    if (scored) {
+        // (what is out of range is left to Python, which names it)
+        if (argv[14] != Py_None) {
+            sc.softcap = A.real(14);
+            if (!(sc.softcap >= 0x1p-64f && sc.softcap <= 0x1p64f)) return none();
+        }
+        if (argv[15] != Py_None) {
+            const int64_t window = A.num(15);
+            if (window < 1 || !(flags & BGTQ_PAGED_CAUSAL)) return none();
+            sc.window = (int32_t)std::min<int64_t>(window, INT32_MAX);
+        }
+        most_prefix = argv[16] == Py_None ? INT64_MAX : A.num(16);
+        if (most_prefix < 0) return none();
+    }
     bool bad = false;
     const at::Tensor *q = A.tensor(0, bad), *pages = A.tensor(1, bad), *table = A.tensor(2, bad), *lens = A.tensor(3, bad), *cu = A.tensor(4, bad),
                      *status = A.tensor(10, bad), *given = A.tensor(11, bad);
@@ -485,7 +495,7 @@ PyObject* paged_attend(PyObject*, PyObject* const* argv, Py_ssize_t n) {
     if (scored) {
         sc.slopes = slopes ? slopes->data_ptr<float>() : nullptr;
         sc.prefix = prefix ? prefix->data_ptr<int32_t>() : nullptr;
-        sc.max_prefix = (int32_t)(most_prefix < 0 || most_prefix > most ? most : most_prefix);
+        sc.max_prefix = (int32_t)std::min(most_prefix, most);
     }
     if (q->scalar_type() == at::kBFloat16) flags |= BGTQ_PAGED_BF16;
     const int64_t need = G.paged_scored_workspace((int)n_seq, (int)m, (int)n_q, (int)n_kv, (int)max_q, most, flags, scored ? &sc : nullptr);

@@ -97,6 +97,8 @@ __device__ __forceinline__ void ap_codes(const float (&in)[E], float largest, fl
 // heads 223 us, 6.5 TB/s, and 16384 63.8 us, 5.7 TB/s, with three chunks of a warp on their way to shared memory (in registers there was room
 // for one: 289 and 82 us; three CTAs on an SM instead of two, with spills: 267 and 78).  Without queries the quantisation's
 // instructions: 16384 tokens 30.7 us, 2.8 TB/s.  32 tokens: 2.9 us, a chain of latencies.
+// kAxes: a pair's angle is looked up at its token's position along the pair's axis, four pairs at once where they have one axis (sections of 16, 24 and
+// 24, 16384 tokens: 66.7 us beside 63.3 with one axis; each pair by itself 78), and axes that take turns one by one (68.4).
 template <typename T, int L, bool kAxes>
 __global__ void __launch_bounds__(kApThreads, L == 8 ? 4 : 2) pg_append_kernel(const ApParams P) {
     constexpr int E = 32 / L, kHeads = 16 / L;

@@ -30,6 +30,12 @@
 // computed: 27.8 and 57.4).  With short ones a launch and the chain length - page number - page - merging: 500 tokens 6.1 us, 4 sequences of 4099
 // 8.5.  (The comparisons of forms and shares here and below were timed with V's scales in the weights, 2 to 8 % faster on either side.)
 //
+// Scores that are not plain (PgScores), each combination a kernel of its own (PgMode): logits are finished between their product and the reference.  A window
+// leaves its batches out of the list, or of the cluster's shares: what is between a sequence's prefix and the window of its first row has no place
+// there (8 sequences of 32768 tokens x 2 KV heads, the last 4096 of each and 4 in front: 11.5 us, 11.2 for sequences of 4096 tokens).  A cap costs 5 to 7 %
+// (one sequence of 131072: 43.4 us beside 40.7; 46.3 where logits lie beyond half of the cap), slopes 3 % (64 of up to 9100: 95.4 beside 92.3; from the front
+// to the end, with references that move at every step, 100.4), both 9 %.
+//
 // In a CTA eight warps take batches in turn, each with a ring of bulk copies of its own (the next triple's first ones travel while this
 // one's states are merged in shared memory).
 #include "bgtq_paged_common.cuh"

@@ -19,6 +19,12 @@
 // of a block's S, its softmax (1900 cycles) and its P . vhat beside the other block's.  8192 positions x 32 query and 8 KV heads, causal: 493 us
 // in short runs, 1.12 PFLOP/s, and 568 in long ones, 0.97 PFLOP/s, where the power limit lowers the clock.  Chunks of 195 to 700 rows behind 700
 // to 9100 tokens of 2 KV heads x 8: 115 us for the three launches, every CTA's share done between 77 and 95 us.
+//
+// Scores that are not plain (PgScores; PgMode: a kernel for each combination).  Masks: a block's tiles are those of its sequence's prefix and those from its
+// first row's window on, and only the tiles that cut a row's sight are masked, by 32 bits per row and half.  Caps and biases are made of the products by
+// the softmax's threads, and add to the chain what they take: 8192 positions as above 504 us plain, 604 with slopes, 735 to 765 with a cap that logits stay within
+// 3/8 of, 935 within 3/2, 2050 beyond; with a window of 2048 295, 325, 370 to 390.  The threads issue half of the cycles then, and no pipe is
+// busy for more than 42 %: two row blocks of two warps per scheduler each are too few to hide the latencies, and tensor memory holds no third.
 // Every wait is bounded: one that gives up is recorded in shared memory, where the others see it, and in the caller's status word; the CTA then
 // drains its copies and products, releases its tensor memory and returns.
 #include "bgtq_paged_common.cuh"

@@ -307,12 +307,14 @@ def _attend(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, causal, sc
     flags = (_lib.PAGED_CAUSAL if causal else 0) | _FORM << _lib.PAGED_FORM_SHIFT
     host = _lib.host()
     if softcap is None and slopes is None and window is None and prefix_lens is None:
-        scores = None
+        scored = False
         r = host.paged_attend(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, scale, flags, return_lse, status, out)
     else:
-        scores = (slopes, prefix_lens, *_limits(softcap, window, causal), _most(max_prefix, "max_prefix_len"))
-        r = host.paged_attend(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, scale, flags, return_lse, status, out, *scores)
+        scored = True
+        r = host.paged_attend(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, scale, flags, return_lse, status, out, slopes, prefix_lens, softcap,
+                              window, max_prefix)
     if r is None:
+        scores = (slopes, prefix_lens, *_limits(softcap, window, causal), _most(max_prefix, "max_prefix_len")) if scored else None
         return _attend_any(q, pages, block_table, seq_lens, cu_q, max_q, max_tokens, flags, scale, return_lse, status, out, scores)
     return _lib.done(r, "bgtq_paged_attend", host.paged_launched())
 

@@ -98,15 +98,12 @@ def test_decode_against_64_bits(dtype, scores, n_kv, gqa, page, lens, form):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("scores", list(SCORES))
-@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("scores,causal", [(s, c) for s in SCORES for c in (True, False) if c or "window" not in SCORES[s]])       # (windows are causal)
 @pytest.mark.parametrize("n_kv,gqa,page,seqs", [(2, 4, 16, [(1, 1), (40, 3), (33, 0), (700, 2)]), (1, 8, 64, [(400, 130), (5, 9), (1100, 1)]),
                                                 (2, 3, 32, [(333, 300), (0, 4), (129, 129)])])
 def test_prefill_against_64_bits(dtype, scores, causal, n_kv, gqa, page, seqs, rows_form):
     """(tokens, queries) of each sequence; queries beyond the tokens see what a row in front of the sequence sees: the prefix."""
     from blockgtq_b200 import paged_kv4_prefill_attention
-    if SCORES[scores].get("window") and not causal:
-        pytest.skip("windows are causal")
     gen = torch.Generator().manual_seed(len(seqs))
     lens, counts = [t for t, _ in seqs], [n for _, n in seqs]
     pages, table, slots = _case(gen, n_kv, page, lens, dtype=dtype)
