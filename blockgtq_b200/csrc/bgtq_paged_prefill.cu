@@ -900,16 +900,20 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                 auto put = [&](uint32_t c0) {       // P of the columns in sv -> 16 columns of the half's own part of S
                     uint32_t pk[16];
                     if (kMode == kCapped && way) {
+                        // (a pair is added up and packed behind the next one's exponentials: 688 us instead of 741, with a window 356 instead of 380)
+                        auto finish = [&](int e) {
+                            ps[e & 1] = add_f2(ps[e & 1], pack_f2(sv[2 * e], sv[2 * e + 1]));
+                            pk[e] = pack_half2(sv[2 * e], sv[2 * e + 1]);
+                        };
                         auto weigh = [&](auto logit) {
 #pragma unroll
                             for (int e = 0; e < 16; ++e) {
-                                float p0, p1;
-                                unpack_f2(logit(pack_f2(sv[2 * e], sv[2 * e + 1])), p0, p1);
-                                p0 = pf_exp2(p0);
-                                p1 = pf_exp2(p1);
-                                ps[e & 1] = add_f2(ps[e & 1], pack_f2(p0, p1));
-                                pk[e] = pack_half2(p0, p1);
+                                unpack_f2(logit(pack_f2(sv[2 * e], sv[2 * e + 1])), sv[2 * e], sv[2 * e + 1]);
+                                sv[2 * e] = pf_exp2(sv[2 * e]);
+                                sv[2 * e + 1] = pf_exp2(sv[2 * e + 1]);
+                                if (e > 0) finish(e - 1);
                             }
+                            finish(15);
                         };
                         if (way == 1) {
                             weigh([&](uint64_t r) { return fma_f2(r, pf_low(P, mul_f2(r, r)), nz2); });
