@@ -865,7 +865,8 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                     const float m_new = top_m - (top_m - kLift) > kReach ? top_m : top_m - kLift;
                     float alpha = 1.f;
                     if (m_used == -INFINITY) m_used = m_new;         // nothing accumulated for this row yet
-                    else if (top_m - m_used > kReach) {
+                    // (kMod: where the block's rows meet anyhow, all that have grown move: with logits of 4.8 to the base of 2, window of 2048, 373 us -> 347)
+                    else if (top_m - m_used > (kMod ? kLift + 1.f : kReach)) {
                         alpha = pf_exp2(m_used - m_new);
                         m_used = m_new;
                     }
@@ -876,8 +877,18 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                         // O is at rest between the previous tile's product and this tile's
                         if (!__all_sync(0xffffffffu, pf_wait(S, &S.o_ready[mb], (uint32_t)(done + i - 1) & 1u))) ok = false;   // (ends at the next tile)
                         tc_fence_after_sync();
+                        // (32 columns at a time, in the registers of the products, which are fetched anew: 626 to 647 us instead of 662 for logits of that size)
+                        if (kMode >= kBiased) tmem_st32(sS, sv);
 #pragma unroll 1
-                        for (int ch = 0; ch < 8; ++ch) tmem_map8(colO + 8u * ch, [&](float o) { return o * alpha; });
+                        for (int ch = 0; ch < 2; ++ch) {
+                            tmem_ld32(colO + 32u * ch, sv);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int c = 0; c < 32; ++c) sv[c] *= alpha;
+                            tmem_st32(colO + 32u * ch, sv);
+                        }
+                        if (kMode >= kBiased) tmem_st_wait();
+                        load(0);
                     }
                 }
                 if (last && w.next_tiles(next.b) > 0) fetch(next.b, w.next_h());        // (the last product with the queries is done)
