@@ -105,8 +105,9 @@ __device__ __forceinline__ float pg_cap_far(float u, float cap) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(pg_ex2(u * 2.8853900817779268f) + 1.f));
     return cap * fmaf(-2.f, r, 1.f);
 }
-// The factor from products to u, finite: nothing of a product of zero, and what it would take beyond has long reached the cap.
-__device__ __forceinline__ float pg_unit(float factor, const PgScores& S) { return fminf(factor * S.cap_inv, 1.329227995784916e36f); }
+// The factor from products to u, finite and above zero: products of zero are nothing under it and hidden ones minus infinity, and what it would take beyond has
+// long reached the cap, or is nothing beside it.
+__device__ __forceinline__ float pg_unit(float factor, const PgScores& S) { return fmaxf(fminf(factor * S.cap_inv, 1.329227995784916e36f), kPgFactorMin); }
 __device__ __forceinline__ float pg_cap_any(float u, const PgScores& S) {
     const float f = pg_cap_far(u, S.cap), v = u * u;
     return v <= 0.25f ? pg_cap_near(u, v, S) : f;

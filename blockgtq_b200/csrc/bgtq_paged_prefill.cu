@@ -870,7 +870,8 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                         alpha = pf_exp2(m_used - m_new);
                         m_used = m_new;
                     }
-                    if (kMode == kCapped && top_u > -INFINITY) u_lim = top_u + (m_used + kReach - top_m) * P.sc.cap_inv;
+                    // (a reference that is huge is looked at every time: its steps are no longer small beside the reach)
+                    if (kMode == kCapped && top_u > -INFINITY) u_lim = fabsf(m_used) < kHuge ? top_u + (m_used + kReach - top_m) * P.sc.cap_inv : -INFINITY;
                     huge = __any_sync(0xffffffffu, fabsf(m_used) >= kHuge && m_used > -INFINITY);
                     lsum *= alpha;
                     if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {

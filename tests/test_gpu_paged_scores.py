@@ -229,6 +229,42 @@ def test_a_cap_of_any_size_and_logits_beyond_it(rows_form):
     assert torch.isfinite(out).all() and (lse <= 20.0 + math.log(200) + 1e-3).all()
 
 
+@pytest.mark.parametrize("cap", [2.0 ** 64, 1e9, 1e6, 50.0, None])
+@pytest.mark.parametrize("scale", [1e-38, 1.0, 2.0 ** 20, 2.0 ** 24, 2.0 ** 30])
+def test_logits_that_grow_along_a_sequence(cap, scale, rows_form):
+    """Keys k_t = (1 + t / 64) k in steps that 4 bits hold: references follow, whatever the size of a step in fp32, and the weights stay finite and at most one.
+    Row i sees the tokens of its window; where one logit is far above the others, its value is the result."""
+    from blockgtq_b200 import page_bytes, paged_kv4_append, paged_kv4_prefill_attention
+    gen = torch.Generator().manual_seed(3)
+    t, n = 700, 300
+    pages, slots = torch.zeros(44, 1, page_bytes(16), dtype=torch.uint8, device=DEV), torch.arange(t, device=DEV)
+    k = torch.zeros(t, 1, 128)
+    k[:, 0, 0] = 7.0 * (1 + torch.arange(t) // 64)                        # one code, bf16 scales: exact
+    v = _noise(gen, t, 1, 128)
+    paged_kv4_append(pages, slots, k.half().to(DEV), v.half().to(DEV))
+    q = torch.zeros(n, 4, 128)
+    q[:, :, 0] = torch.tensor([1.0, 2.0, -1.0, 0.5])
+    for window in (None, 90):
+        out, lse = paged_kv4_prefill_attention(q.half().to(DEV), pages, torch.arange(44, **I32)[None], torch.tensor([t], **I32), torch.tensor([0, n], **I32), scale=scale,
+                                               return_lse=True, softcap=cap, window=window)
+        ks, vs = (x.cpu()[:, 0] for x in S.read(pages, slots))
+        for row in (0, 1, 63, 64, 150, 299):
+            seen = S.seen_by(t, n, row, window)
+            x = torch.einsum("hd,td->ht", q[row].double(), ks[seen]) * scale
+            y = x if cap is None else cap * torch.tanh(x / cap)
+            want = torch.logsumexp(y, -1)
+            # products are exact here: a cap's 2^-20, its base's and the reference's 2^-22, the sum's
+            off = 2.0 ** -20 * (y.abs().amax(-1) + want.abs()) + 1e-5
+            assert ((lse[row].double().cpu() - want).abs() <= off).all(), (row, lse[row], want)
+            got = out[row].double().cpu()
+            assert torch.isfinite(got).all() and (got.abs() <= vs[seen].abs().amax(0) * 1.01).all()
+            # weights and results are rounded to fp16, sums cut as in the other bounds
+            p, few = torch.softmax(y, -1), off < 1e-3
+            near = 2 * off[:, None] + 2.0 ** -10 + (t / 16 + 32) * 18 * 2.0 ** -24
+            room = near * (p @ vs[seen].abs()) + 2.0 ** -32 * vs[seen].abs().sum(0) + 2.0 ** -25
+            assert ((got - p @ vs[seen]).abs() <= room)[few].all(), row
+
+
 def test_scores_that_change_nothing_change_no_bit(rows_form):
     from blockgtq_b200 import paged_kv4_prefill_attention
     gen = torch.Generator().manual_seed(8)
