@@ -23,7 +23,7 @@
 // Scores that are not plain (PgScores; PgMode: a kernel for each combination).  Masks: a block's tiles are those of its sequence's prefix and those from its
 // first row's window on, and only the tiles that cut a row's sight are masked, by 32 bits per row and half.  Caps and biases are made of the products by
 // the softmax's threads, and add to the chain what they take: 8192 positions as above 504 us plain, 604 with slopes, 735 to 765 with a cap that logits stay within
-// 3/8 of, 935 within 3/2, 2050 beyond; with a window of 2048 295, 325, 370 to 390.  The threads issue half of the cycles then, and no pipe is
+// 3/8 of, 935 within 7/5, 2050 beyond; with a window of 2048 295, 325, 370 to 390.  The threads issue half of the cycles then, and no pipe is
 // busy for more than 42 %: two row blocks of two warps per scheduler each are too few to hide the latencies, and tensor memory holds no third.
 // Every wait is bounded: one that gives up is recorded in shared memory, where the others see it, and in the caller's status word; the CTA then
 // drains its copies and products, releases its tensor memory and returns.
@@ -81,7 +81,7 @@ struct Pf {
     float* lse;
     int32_t* status;
     PgScores sc;                                // (kernels of kMod read it)
-    uint64_t low[4], mid[10], steps[16];        // the cap's polynomials (of products, of u), each coefficient twice; 0, 1 .. 31
+    uint64_t low[4], mid[9], steps[16];        // the cap's polynomials (of products, of u), each coefficient twice; 0, 1 .. 31
     float low_reach2;                           // largest product's square that the first is for
     uint32_t* nan_bits;                         // kMod: (n_seq, n_h, max_tiles) x 4 groups x 128 tokens: those whose V is no number
 };
@@ -352,15 +352,15 @@ struct Walk {
 };
 
 // Logits under a cap, pairs at a time on the FMA pipe, u = x / cap.  Most tiles' are small beside it: an odd polynomial of degree 7 up to 3/8, straight from the
-// products where all rows' have one factor (no row of bf16 queries was brought to another magnitude), or of degree 19 up to 3/2, both fitted to the relative
-// error (7e-8, 1.9e-8); beyond, one by one.  All of a warp's 32 tokens go one way.  (Two more values of the special function pipe for each logit would be
+// products where all rows' have one factor (no row of bf16 queries was brought to another magnitude), or of degree 17 up to 7/5, both fitted to the relative
+// error (7e-8, 4.8e-8); beyond, one by one.  All of a warp's 32 tokens go one way.  (Two more values of the special function pipe for each logit would be
 // twice the time of all else: it makes 16 a cycle.)
-constexpr int kLowTerms = 4, kMidTerms = 10;
+constexpr int kLowTerms = 4, kMidTerms = 9;
 constexpr double kLowReach = 0.375;
-constexpr float kMidReach = 1.5f;
+constexpr float kMidReach = 1.4f;
 constexpr double kCapLow[kLowTerms] = {1.0, -0.3333233349357446, 0.13289726163824672, -0.04848729069776324};
-constexpr double kCapMid[kMidTerms] = {1.0, -0.3333322466769597, 0.13331329487357702, -0.0538386683456423, 0.021448478261107542, -0.00806102220738539,
-                                       0.0026138976028419808, -0.0006436921929764066, 0.00010158802230323775, -7.465266263465981e-06};
+constexpr double kCapMid[kMidTerms] = {1.0, -0.33333077724742183, 0.13328956227827346, -0.053706810286391585, 0.021092473450978352, -0.007527298246243253,
+                                       0.0021462715909971895, -0.0004054931883325217, 3.6238863462110705e-05};
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));

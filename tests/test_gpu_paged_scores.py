@@ -229,6 +229,12 @@ def test_a_cap_of_any_size_and_logits_beyond_it(rows_form):
     assert torch.isfinite(out).all() and (lse <= 20.0 + math.log(200) + 1e-3).all()
 
 
+def _near(got, p, v, off):
+    """got (h, 128) fp16 is p (h, t) times v (t, 128), each logit off by off (h,): weights and results are rounded to fp16, sums cut as in tests/paged_bounds.py."""
+    room = (2 * off[:, None] + 2.0 ** -10 + (len(v) / 16 + 32) * 18 * 2.0 ** -24) * (p @ v.abs()) + 2.0 ** -32 * v.abs().sum(0) + 2.0 ** -25
+    assert ((got - p @ v).abs() <= room).all(), ((got - p @ v).abs() / room).max()
+
+
 @pytest.mark.parametrize("cap", [2.0 ** 64, 1e9, 1e6, 50.0, None])
 @pytest.mark.parametrize("scale", [1e-38, 1.0, 2.0 ** 20, 2.0 ** 24, 2.0 ** 30])
 def test_logits_that_grow_along_a_sequence(cap, scale, rows_form):
@@ -258,11 +264,8 @@ def test_logits_that_grow_along_a_sequence(cap, scale, rows_form):
             assert ((lse[row].double().cpu() - want).abs() <= off).all(), (row, lse[row], want)
             got = out[row].double().cpu()
             assert torch.isfinite(got).all() and (got.abs() <= vs[seen].abs().amax(0) * 1.01).all()
-            # weights and results are rounded to fp16, sums cut as in the other bounds
-            p, few = torch.softmax(y, -1), off < 1e-3
-            near = 2 * off[:, None] + 2.0 ** -10 + (t / 16 + 32) * 18 * 2.0 ** -24
-            room = near * (p @ vs[seen].abs()) + 2.0 ** -32 * vs[seen].abs().sum(0) + 2.0 ** -25
-            assert ((got - p @ vs[seen]).abs() <= room)[few].all(), row
+            few = off < 1e-3
+            _near(got[few], torch.softmax(y, -1)[few], vs[seen], off[few])
 
 
 def test_scores_that_change_nothing_change_no_bit(rows_form):
@@ -335,3 +338,93 @@ def test_a_captured_call_follows_lengths_prefixes_and_slopes(rows_form):
         for i, (t, lo, hi) in enumerate(((a, 0, 4), (b, 4, 30))):
             ref = S.attention(q[lo:hi], pages, slots[i][:t], softcap=9.0, window=64, prefix=min(p[i], t), slopes=torch.full((4,), s))
             W.check(out, lse, ref, slice(lo, hi))
+
+
+@pytest.mark.parametrize("scores", ["window", "sinks", "all", "slopes"])
+def test_more_rows_and_longer_sequences_than_the_caller_said(scores, rows_form):
+    """max_q_len and max_prefix_len choose the launch; lengths are held to max_seq_len, prefixes to max_prefix_len."""
+    from blockgtq_b200 import paged_kv4_prefill_attention
+    gen = torch.Generator().manual_seed(19)
+    pages, table, slots = _case(gen, 2, 16, [600, 90])
+    q = _noise(gen, 130, 8, 128).half()
+    call, of = _arguments(SCORES[scores], [500, 90], 8, 20 if "prefix" in SCORES[scores] else None)
+    out, lse = paged_kv4_prefill_attention(q.to(DEV), pages, table.to(DEV), torch.tensor([600, 90], **I32), torch.tensor([0, 100, 130], **I32), max_q_len=2, max_seq_len=500,
+                                           return_lse=True, **call)
+    for b, (lo, hi, t) in enumerate(((0, 100, 500), (100, 130, 90))):
+        rows = [0, 1, 17, hi - lo - 1]
+        given = of(b)
+        given["prefix"] = min(given["prefix"], 20) if "prefix" in SCORES[scores] else 0
+        W.check(out, lse, S.attention(q[lo:hi], pages, slots[b][:t], rows=rows, **given), [lo + r for r in rows])
+
+
+@pytest.mark.parametrize("bad", [-1, 1 << 30, 9999])
+def test_a_page_number_outside_the_pool_leaves_its_tokens_out(bad, rows_form):
+    """Told in the status where a row's window or prefix has them, and not else."""
+    from blockgtq_b200 import paged_kv4_prefill_attention
+    gen = torch.Generator().manual_seed(29)
+    pages, table, slots = _case(gen, 1, 16, [900])
+    q = _noise(gen, 3, 4, 128).half()
+    for page, told in ((50, True), (0, True), (20, False)):      # tokens 800 .., 0 .., 320 ..
+        broken, status = table.clone(), torch.zeros(1, **I32)
+        broken[0, page] = bad
+        out, lse = paged_kv4_prefill_attention(q.to(DEV), pages, broken.to(DEV), torch.tensor([900], **I32), torch.tensor([0, 3], **I32), return_lse=True, softcap=20.0,
+                                               window=200, prefix_lens=torch.tensor([10], **I32), status=status)
+        assert status.item() == (4 if told else 0)
+        k, v = (x.cpu()[:, 0] for x in S.read(pages, slots[0]))
+        for row in range(3):
+            seen = S.seen_by(900, 3, row, 200, 10)
+            seen[16 * page:16 * page + 16] = False
+            y = 20 * torch.tanh(torch.einsum("hd,td->ht", q[row].double(), k[seen]) / math.sqrt(128) / 20)
+            # products lose 2^-20 of their terms, a cap 2^-20 of itself
+            off = 2.0 ** -20 * (torch.einsum("hd,td->ht", q[row].double().abs(), k[seen].abs()).amax(-1) / math.sqrt(128) + 20) + 1e-5
+            assert ((lse[row].double().cpu() - torch.logsumexp(y, -1)).abs() <= off + 1e-5).all()
+            _near(out[row].double().cpu(), torch.softmax(y, -1), v[seen], off)
+
+
+def test_calls_on_two_streams_at_once():
+    from blockgtq_b200 import paged_kv4_decode_attention, paged_kv4_prefill_attention
+    gen = torch.Generator().manual_seed(37)
+    pages, table, _ = _case(gen, 2, 16, [1500, 700, 30])
+    args = (pages, table.to(DEV), torch.tensor([1500, 700, 30], **I32))
+    q, few = _noise(gen, 400, 8, 128).half().to(DEV), _noise(gen, 3, 8, 128).half().to(DEV)
+    cu = torch.tensor([0, 300, 380, 400], **I32)
+    kinds = [_arguments(SCORES[k], [1500, 700, 30], 8)[0] for k in ("all", "cap", "sinks", "slopes", "prefix")]
+    calls = [lambda kw=kw: paged_kv4_prefill_attention(q, *args, cu, **kw) for kw in kinds] + [lambda kw=kw: paged_kv4_decode_attention(few, *args, **kw) for kw in kinds]
+    want = [c() for c in calls]
+    streams = [torch.cuda.Stream(DEV) for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for c in calls:
+            for s, results in zip(streams, got):
+                with torch.cuda.stream(s):
+                    results.append(c())
+    torch.cuda.synchronize()
+    for results in got:
+        assert all(torch.equal(r, want[i % len(want)]) for i, r in enumerate(results))
+
+
+def test_two_graphs_of_one_pool_of_memory(rows_form):
+    """Their workspaces may be the same memory: replayed one behind the other, each answers as it did."""
+    from blockgtq_b200 import paged_kv4_prefill_attention
+    gen = torch.Generator().manual_seed(43)
+    pages, table, _ = _case(gen, 1, 16, [800, 300])
+    args = (pages, table.to(DEV), torch.tensor([800, 300], **I32))
+    cases = []
+    for n, kind in ((40, "all"), (12, "cap")):
+        q = _noise(gen, n, 8, 128).half().to(DEV)
+        kw = _arguments(SCORES[kind], [800, 300], 8)[0]
+        cases.append((q, torch.tensor([0, n // 2, n], **I32), kw))
+    want = [paged_kv4_prefill_attention(q, *args, cu, **kw).clone() for q, cu, kw in cases]
+    torch.cuda.synchronize()
+    pool, graphs, outs = None, [], []
+    for q, cu, kw in cases:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=pool):
+            outs.append(paged_kv4_prefill_attention(q, *args, cu, **kw))
+        pool = g.pool()
+        graphs.append(g)
+    for i in (0, 1, 0, 0, 1):
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[i], want[i])
