@@ -92,13 +92,14 @@ struct PdForm {
 struct SeqInfo {
     int len, q0, n;                  // cached tokens, first query row, query rows
     int pre, head, skip;             // tokens and batches of the prefix, batches left out behind them
+    int low;                         // the first row's window begins here
     __device__ __forceinline__ int batch(int k) const { return k + (k >= head ? skip : 0); }
 };
 
 template <bool kMod>
 __device__ __forceinline__ SeqInfo pd_seq(const PdParams& P, int i) {
     SeqInfo s;
-    s.pre = s.head = s.skip = 0;
+    s.pre = s.head = s.skip = s.low = 0;
     s.len = max(0, min(P.lens[i], P.cap));
     if (P.cu_q) {
         s.q0 = min(max(P.cu_q[i], 0), P.n_tok);
@@ -110,7 +111,10 @@ __device__ __forceinline__ SeqInfo pd_seq(const PdParams& P, int i) {
     if (kMod) {
         s.pre = pg_prefix(P.sc, i, s.len);
         s.head = (s.pre + kBatchTok - 1) / kBatchTok;
-        if (P.sc.window) s.skip = max(0, max(0, max(0, s.len - s.n + 1) - P.sc.window) / kBatchTok - s.head);
+        if (P.sc.window) {
+            s.low = max(0, max(0, s.len - s.n + 1) - P.sc.window);
+            s.skip = max(0, s.low / kBatchTok - s.head);
+        }
     }
     return s;
 }
@@ -708,7 +712,9 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
         if ((k & 15) == 0) {
             const int kk = k + (lane >> 1), unit = 2 * sg.s.batch(sg.first + warp + kPdWarps * (kBack ? w.n - 1 - kk : kk)) + (lane & 1);
             w.from = nullptr;
-            if (kk < w.n && unit < (sg.s.len + kUnitTok - 1) / kUnitTok) {
+            // (nor are those units of a batch looked up that no row sees)
+            const bool hidden = kMod && unit * kUnitTok >= sg.s.pre && (unit + 1) * kUnitTok <= sg.s.low;
+            if (kk < w.n && unit < (sg.s.len + kUnitTok - 1) / kUnitTok && !hidden) {
                 const int col = unit / P.pool.units, page = P.table[(int64_t)sg.seq * P.tb_st + col];
                 if (page >= 0 && page < P.pool.n_pages)
                     w.from = P.pool.pages + (int64_t)page * P.pool.page_stride + (int64_t)sg.h * P.pool.head_stride + (unit - col * P.pool.units) * kUnitBytes;

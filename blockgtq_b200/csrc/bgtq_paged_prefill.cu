@@ -213,9 +213,11 @@ __global__ void __launch_bounds__(256) pg_unpack_kernel(const Pf P) {
     const Seq s = pf_seq<kMod>(P, P.seq0 + si);
     const int unit = tile * (kPfTileTok / kUnitTok) + warp, left = s.len - unit * kUnitTok;
     if (s.n == 0 || tile * kPfTileTok >= s.len) return;
-    if (kMod && tile * kPfTileTok >= s.pre && (tile + 1) * kPfTileTok <= pf_window(P, s, 0)) return;         // (no row sees it)
+    const int low = kMod ? pf_window(P, s, 0) : 0;
+    if (kMod && tile * kPfTileTok >= s.pre && (tile + 1) * kPfTileTok <= low) return;         // (no row sees it)
+    const bool hidden = kMod && unit * kUnitTok >= s.pre && (unit + 1) * kUnitTok <= low;     // (nor this unit of it)
     const uint8_t* u = nullptr;
-    if (left > 0) {
+    if (left > 0 && !hidden) {
         const int col = unit / P.pool.units, page = P.table[(int64_t)(P.seq0 + si) * P.tb_st + col];
         if (page >= 0 && page < P.pool.n_pages)
             u = P.pool.pages + (int64_t)page * P.pool.page_stride + (int64_t)(P.h0 + hi) * P.pool.head_stride + (unit - col * P.pool.units) * kUnitBytes;
@@ -225,7 +227,7 @@ __global__ void __launch_bounds__(256) pg_unpack_kernel(const Pf P) {
     __shared__ uint8_t there[8];
     __shared__ int first_nan[4];
     __shared__ uint32_t all_nan[16];
-    if (lane == 0) there[warp] = u || left <= 0;
+    if (lane == 0) there[warp] = u || left <= 0 || hidden;
     if (threadIdx.x < 4) first_nan[threadIdx.x] = INT_MAX;
     if (kMod && threadIdx.x < 16) all_nan[threadIdx.x] = 0;
     __syncthreads();

@@ -691,8 +691,8 @@ int bgtq_paged_attend(const void* q, int64_t q_st, int64_t q_sh, const uint8_t* 
 
 /* What an attention does beside the plain one.  Row i of the n of a sequence is at position p = seq_lens[b] - n + i.  With x = scale * q . k its logit
  * for token t is c tanh(x / c) - slope |p - t|, the first term x without a cap, the second none without slopes; it sees token t < seq_lens[b] if
- * t < prefix[b], or if t <= p (any t without BGTQ_PAGED_CAUSAL) and t > p - window.  Rows that see none: zeros, lse -inf, as ever.  Of tokens that
- * no row's window or prefix reaches, pages are not read (those beside them, in 128 tokens, may be). */
+ * t < prefix[b], or if t <= p (any t without BGTQ_PAGED_CAUSAL) and t > p - window.  Rows that see none: zeros, lse -inf, as ever.  Pages of
+ * which no row's window or prefix reaches a token are not looked up: their numbers in the table may be none. */
 typedef struct BgtqPagedScores {
     const float* slopes;        /* device, (n_q), finite; NULL: no bias */
     const int32_t* prefix;      /* device, (n_seq), held to 0 .. max_prefix; NULL: none */

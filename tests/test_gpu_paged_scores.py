@@ -316,6 +316,28 @@ def test_pages_in_front_of_the_window_need_not_be_there(form):
     W.check(out, lse, want, slice(0, 1))
 
 
+@pytest.mark.parametrize("page", [16, 48, 64])
+@pytest.mark.parametrize("rows", [1, 5])
+def test_pages_that_no_row_sees_a_token_of(page, rows, rows_form):
+    """Wherever the window begins in a page, a batch or a tile: what is hidden as a whole has no number, all else is read."""
+    from blockgtq_b200 import paged_kv4_prefill_attention
+    gen = torch.Generator().manual_seed(page)
+    pages, table, slots = _case(gen, 1, page, [500])
+    q = _noise(gen, rows, 4, 128).half()
+    for window in (1, 15, 16, 17, 31, 33, 47, 100, 127, 129, 200, 333):
+        for prefix in (0, 1, 16, 40):
+            status, part = torch.zeros(1, **I32), table.clone()
+            first = 500 - rows + 1 - window                      # the first row's window
+            for i in range(500 // page + 1):
+                if i * page >= prefix and (i + 1) * page <= first:
+                    part[0, i] = -1
+            kw = dict(window=window, prefix_lens=torch.tensor([prefix], **I32))
+            args = torch.tensor([500], **I32), torch.tensor([0, rows], **I32)
+            want = paged_kv4_prefill_attention(q.to(DEV), pages, table.to(DEV), *args, **kw)
+            got = paged_kv4_prefill_attention(q.to(DEV), pages, part.to(DEV), *args, status=status, **kw)
+            assert status.item() == 0 and torch.equal(got, want)
+
+
 def test_a_captured_call_follows_lengths_prefixes_and_slopes(rows_form):
     from blockgtq_b200 import paged_kv4_prefill_attention
     gen = torch.Generator().manual_seed(41)
