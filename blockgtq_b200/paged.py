@@ -466,7 +466,7 @@ class PagedKV4Cache:
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._free = list(range(n_pages - 1, -1, -1))
         self._held = [0] * n_pages          # sequences that hold a page
-        self._seqs = {}                     # id -> [tokens, [pages]]
+        self._seqs = {}                     # id -> [tokens, [pages, None: released]]
         self._next_id = 0
         self._step = None
         self._busy = set()                  # streams that layers have run on since pages were last copied
@@ -482,25 +482,44 @@ class PagedKV4Cache:
 
     def fork_sequence(self, seq: int, n_tokens=None) -> int:
         """A new sequence that begins with the first ``n_tokens`` (default: all) of another's tokens, in the same pages."""
-        t, pages = self._seqs[seq]
-        n = t if n_tokens is None else operator.index(n_tokens)
-        if not 0 <= n <= t:
-            raise ValueError(f"sequence {seq} has {t} tokens, not {n}")
+        n, pages = self._first(seq, self._seqs[seq][0] if n_tokens is None else n_tokens)
         i = self.add_sequence()
-        self._seqs[i] = [n, pages[:-(-n // self.page_size)]]
-        for p in self._seqs[i][1]:
-            self._held[p] += 1
+        self._seqs[i] = [n, pages]
+        for p in pages:
+            if p is not None:
+                self._held[p] += 1
         return i
 
     def truncate_sequence(self, seq: int, n_tokens: int):
         """Leaves the sequence its first ``n_tokens`` tokens, and gives the pages behind them back.  A step that it is part of ends with it."""
+        n, pages = self._first(seq, n_tokens)
+        behind = self._seqs[seq][1][len(pages):]
+        self._seqs[seq] = [n, pages]
+        self._let_go(behind)
+        self._end_step(seq)
+
+    def _first(self, seq, n_tokens):
+        """A number of a sequence's first tokens, checked, and the pages that they are in."""
         t, pages = self._seqs[seq]
         n = operator.index(n_tokens)
         if not 0 <= n <= t:
             raise ValueError(f"sequence {seq} has {t} tokens, not {n}")
-        keep = -(-n // self.page_size)
-        self._seqs[seq] = [n, pages[:keep]]
-        self._let_go(pages[keep:])
+        pages = pages[:-(-n // self.page_size)]
+        if n % self.page_size and pages[-1] is None:
+            raise ValueError(f"the page that holds token {n - 1} of sequence {seq} has been released")
+        return n, pages
+
+    def release(self, seq: int, n_tokens: int, keep: int = 0):
+        """Gives back the pages that lie as a whole behind the sequence's first ``keep`` tokens and in front of token ``n_tokens``: for models all of whose layers
+        look through a window (with a prefix of up to ``keep`` tokens) that does not reach them any more.  An attention that sees one of their tokens is told
+        of by :meth:`check_status`.  A step that the sequence is part of ends with it."""
+        t, pages = self._seqs[seq]
+        n, keep = operator.index(n_tokens), operator.index(keep)
+        if not 0 <= n <= t or keep < 0:
+            raise ValueError(f"sequence {seq} has {t} tokens: none of the first {n}, but for {keep}, can be released")
+        gone = range(-(-keep // self.page_size), n // self.page_size)
+        self._seqs[seq] = [t, [None if i in gone else p for i, p in enumerate(pages)]]
+        self._let_go([pages[i] for i in gone])
         self._end_step(seq)
 
     def free_sequence(self, seq: int):
@@ -510,6 +529,8 @@ class PagedKV4Cache:
 
     def _let_go(self, pages):
         for p in reversed(pages):
+            if p is None:
+                continue
             self._held[p] -= 1
             if self._held[p] == 0:
                 self._free.append(p)
@@ -616,7 +637,7 @@ class PagedKV4Cache:
             rows.append(pages)
         width = max(len(r) for r in rows)
         wide = torch.tensor([slots, positions], dtype=torch.int64).to(self.device)
-        table = torch.tensor([r + [0] * (width - len(r)) for r in rows], dtype=torch.int32).to(self.device)
+        table = torch.tensor([[-1 if p is None else p for p in r] + [0] * (width - len(r)) for r in rows], dtype=torch.int32).to(self.device)
         small = torch.tensor(lens + ends, dtype=torch.int32).to(self.device)
         if copies:
             self._not_captured()

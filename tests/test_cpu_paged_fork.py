@@ -27,21 +27,30 @@ class Cache(PagedKV4Cache):
                 self.tokens[b, :n] = self.tokens[a, :n]
         self.copies.append(len(src))
 
+    def resize(self, n_pages):
+        super().resize(n_pages)
+        if len(self.tokens) != n_pages:                 # (nothing was held, nothing copied)
+            self.tokens = torch.full((n_pages, self.page_size), -1, dtype=torch.int64)
+
     def store(self, rows):
         slots = self._step["slots"]
         assert len(set(slots.tolist())) == len(slots)
         self.tokens.view(-1)[slots] = rows
 
     def read(self, seq):
+        """The sequence's tokens, -1 where they have been released."""
         t, pages = self._seqs[seq]
-        return self.tokens[pages].reshape(-1)[:t] if pages else torch.zeros(0, dtype=torch.int64)
+        none = torch.full((1, self.page_size), -1, dtype=torch.int64)
+        return torch.cat([none] * (not pages) + [none if p is None else self.tokens[p:p + 1] for p in pages]).reshape(-1)[:t]
 
     def check(self):
         held = [0] * self.n_pages
         for t, pages in self._seqs.values():
-            assert len(pages) == -(-t // self.page_size) and len(set(pages)) == len(pages)
+            there = [p for p in pages if p is not None]
+            assert len(pages) == -(-t // self.page_size) and len(set(there)) == len(there)
             for p in pages:
-                held[p] += 1
+                if p is not None:
+                    held[p] += 1
         assert held == self._held and sorted(self._free) == [p for p in range(self.n_pages) if held[p] == 0]
 
 
@@ -123,13 +132,13 @@ def test_a_step_that_lacks_pages_for_its_copies_takes_nothing():
     assert c.free_pages == 0
 
 
-@pytest.mark.parametrize("seed", range(6))
+@pytest.mark.parametrize("seed", range(20))
 def test_any_order_of_calls_keeps_every_sequence_s_tokens(seed):
     rng = random.Random(seed)
     c = Cache(n_pages=40, page_size=rng.choice([16, 32]), max_seq_len=150)
     want, number = {}, 0
     for _ in range(150):
-        kind = rng.choice(["add", "step", "step", "step", "fork", "fork", "truncate", "free", "compact", "resize"])
+        kind = rng.choice(["add", "step", "step", "step", "fork", "fork", "truncate", "free", "release", "compact", "resize"])
         some = rng.sample(sorted(want), min(len(want), rng.randint(1, 5)))
         if kind == "add" or not some:
             want[c.add_sequence()] = []
@@ -147,17 +156,29 @@ def test_any_order_of_calls_keeps_every_sequence_s_tokens(seed):
                 want[i] = want[i] + r
         elif kind == "fork":
             n = rng.randint(0, len(want[some[0]]))
+            if n and want[some[0]][n - 1] == -1 and n % c.page_size:
+                with pytest.raises(ValueError, match="released"):
+                    c.fork_sequence(some[0], n)
+                continue
             want[c.fork_sequence(some[0], n)] = want[some[0]][:n]
         elif kind == "truncate":
             n = rng.randint(0, len(want[some[0]]))
+            if n and want[some[0]][n - 1] == -1 and n % c.page_size:
+                with pytest.raises(ValueError, match="released"):
+                    c.truncate_sequence(some[0], n)
+                continue
             c.truncate_sequence(some[0], n)
             want[some[0]] = want[some[0]][:n]
+        elif kind == "release":
+            n, keep, size = rng.randint(0, len(want[some[0]])), rng.choice([0, 1, 16, 40]), c.page_size
+            c.release(some[0], n, keep)
+            want[some[0]] = [-1 if -(-keep // size) <= i // size < n // size else x for i, x in enumerate(want[some[0]])]
         elif kind == "free":
             c.free_sequence(some[0])
             del want[some[0]]
         elif kind == "compact":
             n = c.compact()
-            assert sorted({p for _, pages in c._seqs.values() for p in pages}) == list(range(n)) and c._step is None
+            assert sorted({p for _, pages in c._seqs.values() for p in pages} - {None}) == list(range(n)) and c._step is None
         else:
             held = c.n_pages - c.free_pages
             c.resize(max(1, held, rng.randint(held, 40)))
@@ -165,6 +186,36 @@ def test_any_order_of_calls_keeps_every_sequence_s_tokens(seed):
         c.check()
         for i, rows in want.items():
             assert c.read(i).tolist() == rows
+
+
+def test_released_pages_are_others_and_the_table_says_so():
+    c = Cache()
+    a = c.add_sequence()
+    _step(c, [a], [70], list(range(70)))
+    b = c.fork_sequence(a)
+    c.release(a, 50, keep=4)                            # pages 1 and 2; b holds them still
+    assert c._step is None and c.free_pages == 7
+    c.release(b, 50)
+    assert c.free_pages == 9 and [p is None for p in c._seqs[a][1]] == [False, True, True, False, False] and c._seqs[b][1][:3] == [None] * 3
+    c.release(b, 50)
+    c.release(b, 0)
+    _step(c, [a, b], [1, 1], [100, 200])
+    assert c._step["table"][:, :3].tolist() == [[c._seqs[a][1][0], -1, -1], [-1, -1, -1]] and c.copies == [1]
+    assert c.read(a).tolist() == [*range(16), *[-1] * 32, *range(48, 70), 100] and c.read(b).tolist() == [*[-1] * 48, *range(48, 70), 200]
+    for n in (17, 33, 47):
+        for call in (c.truncate_sequence, c.fork_sequence):
+            with pytest.raises(ValueError, match="released"):
+                call(a, n)
+    c.truncate_sequence(a, 32)
+    _step(c, [a], [3], [7, 8, 9])
+    assert c.read(a).tolist() == [*range(16), *[-1] * 16, 7, 8, 9]
+    for bad in ((36, 0), (-1, 0), (0, -1)):
+        with pytest.raises(ValueError):
+            c.release(a, *bad)
+    c.free_sequence(a)
+    c.free_sequence(b)
+    c.check()
+    assert c.free_pages == 12
 
 
 def test_a_pool_holds_what_is_held():

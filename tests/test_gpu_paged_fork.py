@@ -108,6 +108,33 @@ def test_moved_pools_go_on_answering():
         c.check_status()
 
 
+@pytest.mark.parametrize("keep", [0, 4])
+def test_a_windowed_model_in_a_pool_that_holds_its_window(keep):
+    """200 tokens through a pool of 8 pages: released as the window leaves them behind, the answers are those of a cache that keeps everything."""
+    gen = torch.Generator().manual_seed(keep)
+    small, whole = _cache(n_pages=8), _cache()
+    score = dict(window=60, prefix_lens=torch.full((1,), keep, **I32), max_prefix_len=keep)
+    a, b = small.add_sequence(), whole.add_sequence()
+    done = 0
+    for n in (50, *[1] * 20, 30, *[4] * 25):
+        rows = [_rows(gen, n) for _ in range(2)]
+        outs = []
+        for c, s in ((small, a), (whole, b)):
+            c.begin_step([s], [n])
+            outs.append([c.append_and_attend(i, *r, **score) for i, r in enumerate(rows)])
+        assert all(torch.equal(x, y) for x, y in zip(*outs))
+        done += n
+        small.release(a, max(0, done + 1 - 60), keep)   # (the next row, at place done, sees from here on)
+    assert done == 200 and small.free_pages == 8 - 5 - (keep > 0) and whole.free_pages == 40 - 13
+    small.check_status()
+    whole.check_status()
+    small.truncate_sequence(a, 190)
+    small.begin_step([a], [1])
+    small.append_and_attend(0, *_rows(gen, 1))           # without the window: it looks for what is gone
+    with pytest.raises(RuntimeError, match="page number"):
+        small.check_status()
+
+
 def test_moving_is_not_captured():
     cache = _cache()
     cache.begin_step([cache.add_sequence()], [20])
