@@ -1183,7 +1183,7 @@ extern "C" __attribute__((visibility("default"))) int64_t bgtq_paged_scored_work
     PgScores sc;
     const bool mod = pd_scores(scores, max_tokens, sc);
     const PdForm f = pd_form(n_seq, n_tok, n_q, n_kv, max_q, max_tokens, flags, mod ? &sc : nullptr);
-    if (f.prefill) return paged_prefill_workspace(n_seq, n_tok, n_q / n_kv, n_kv, max_tokens, mod);
+    if (f.prefill) return paged_prefill_workspace(n_seq, n_tok, n_q / n_kv, n_kv, max_tokens, mod ? &sc : nullptr);
     return f.n_rank ? 0 : (int64_t)f.n_cta * 2 * 8 * f.nt * (kHD * 4 + 8);
 }
 extern "C" __attribute__((visibility("default"))) int64_t bgtq_paged_workspace_bytes(int32_t n_seq, int32_t n_tok, int32_t n_q, int32_t n_kv,
@@ -1231,7 +1231,7 @@ extern "C" __attribute__((visibility("default"))) int bgtq_paged_attend_scored(
     PdForm f = pd_form(n_seq, n_tok, n_q, n_kv, max_q, max_tokens, flags, mod ? &sc : nullptr);
     const cudaStream_t st = (cudaStream_t)stream;
     if (f.prefill) {
-        if (!workspace || workspace_bytes < paged_prefill_workspace(n_seq, n_tok, n_q / n_kv, n_kv, max_tokens, mod)) return BGTQ_E_BADARG;
+        if (!workspace || workspace_bytes < paged_prefill_workspace(n_seq, n_tok, n_q / n_kv, n_kv, max_tokens, mod ? &sc : nullptr)) return BGTQ_E_BADARG;
         return paged_prefill({{pages, page_stride, head_stride, n_pages, page_tokens / kUnitTok}, table, table_stride, seq_lens, cu_q, n_seq, n_tok, n_q,
                               n_kv, n_q / n_kv, (flags & BGTQ_PAGED_CAUSAL) ? 1 : 0, (flags & BGTQ_PAGED_BF16) ? 1 : 0, max_tokens, (int32_t)cap,
                               reinterpret_cast<uint8_t*>(workspace), q, q_st, q_sh, scale * 1.44269504088896340736f, out, o_st, o_sh, lse, status, mod, sc},

@@ -35,6 +35,8 @@
 #include <math.h>
 #include <string.h>
 
+#include <algorithm>
+
 namespace bgtq {
 namespace {
 
@@ -54,6 +56,11 @@ struct __align__(16) Block {
         if (kBack) k = tiles - 1 - k;
         return k + (gap && k >= sees - 1 ? gap : 0);
     }
+    // The same among those of its sequence that the workspace holds; first_gap: what it lacks, no more than gap
+    template <bool kBack> __device__ __forceinline__ int slot(int k, int first_gap) const {
+        if (kBack) k = tiles - 1 - k;
+        return k + (gap && k >= sees - 1 ? gap - first_gap : 0);
+    }
 };
 
 struct Pf {
@@ -63,7 +70,8 @@ struct Pf {
     const int32_t *lens, *cu_q;
     int32_t cap, n_tok, n_q, n_kv, gqa, causal;
     uint32_t gqa_inv;                           // 2^32 / gqa, rounded up; 0: gqa is 1
-    int32_t seq0, n_seq, h0, n_h, max_tiles;    // this launch's sequences and KV heads, tiles a sequence has room for
+    int32_t seq0, n_seq, h0, n_h, max_tiles;    // this launch's sequences and KV heads, tiles a sequence has room for (with a window, those that its
+                                                // prefix and its rows' windows reach, one behind the other)
     uint8_t* tiles;                             // (n_seq, n_h, max_tiles) operand tile pairs
     int4* nan;                                  // (n_seq, n_h, max_tiles): per group, the tile's first token whose V is no number (INT_MAX: none)
     Block* blk;                                 // the blocks, sequence by sequence
@@ -123,6 +131,10 @@ __device__ __forceinline__ uint32_t half2_of(float a, float b) { return pack_hal
 
 __device__ __forceinline__ int pf_pos(const Pf& P, int row) {      // row / gqa, rows < 2^29
     return P.gqa_inv ? (int)__umulhi((uint32_t)row, P.gqa_inv) : row;
+}
+// Tiles between a sequence's prefix and its first row's window: the workspace has no place for them.
+__device__ __forceinline__ int pf_gap(const Pf& P, const Seq& s) {
+    return max(0, pf_window(P, s, 0) / kPfTileTok - (s.pre + kPfTileTok - 1) / kPfTileTok);
 }
 template <bool kMod>
 __device__ __forceinline__ Block pf_block(const Pf& P, int si, const Seq& s, int j) {
@@ -203,19 +215,19 @@ __device__ void pf_plan(const Pf& P) {
 template <bool kMod>
 __global__ void __launch_bounds__(256) pg_unpack_kernel(const Pf P) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int tile = blockIdx.x, hi = blockIdx.y, si = blockIdx.z;
+    const int slot = blockIdx.x, hi = blockIdx.y, si = blockIdx.z;
     grid_launch_dependents();
     grid_dependency_wait();
-    if (tile == P.max_tiles) {
+    if (slot == P.max_tiles) {
         if (hi == 0 && si == 0) pf_plan<kMod>(P);
         return;
     }
     const Seq s = pf_seq<kMod>(P, P.seq0 + si);
+    const int tile = kMod && slot * kPfTileTok >= s.pre ? slot + pf_gap(P, s) : slot;
     const int unit = tile * (kPfTileTok / kUnitTok) + warp, left = s.len - unit * kUnitTok;
     if (s.n == 0 || tile * kPfTileTok >= s.len) return;
     const int low = kMod ? pf_window(P, s, 0) : 0;
-    if (kMod && tile * kPfTileTok >= s.pre && (tile + 1) * kPfTileTok <= low) return;         // (no row sees it)
-    const bool hidden = kMod && unit * kUnitTok >= s.pre && (unit + 1) * kUnitTok <= low;     // (nor this unit of it)
+    const bool hidden = kMod && unit * kUnitTok >= s.pre && (unit + 1) * kUnitTok <= low;     // (no row sees this unit)
     const uint8_t* u = nullptr;
     if (left > 0 && !hidden) {
         const int col = unit / P.pool.units, page = P.table[(int64_t)(P.seq0 + si) * P.tb_st + col];
@@ -235,9 +247,9 @@ __global__ void __launch_bounds__(256) pg_unpack_kernel(const Pf P) {
         uint32_t m = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) m |= (uint32_t)there[i] << i;
-        P.valid[(int64_t)si * P.max_tiles + tile] = (uint8_t)m;
+        P.valid[(int64_t)si * P.max_tiles + slot] = (uint8_t)m;
     }
-    uint8_t* const kt = P.tiles + (((int64_t)si * P.n_h + hi) * P.max_tiles + tile) * kPfTileBytes;
+    uint8_t* const kt = P.tiles + (((int64_t)si * P.n_h + hi) * P.max_tiles + slot) * kPfTileBytes;
     uint8_t* const vt = kt + kPart;
     // K: lane = (token % 8, c): dims 32 n + 8 c .. + 7 for n = 0 .. 3
 #pragma unroll
@@ -291,8 +303,8 @@ __global__ void __launch_bounds__(256) pg_unpack_kernel(const Pf P) {
     }
     __syncthreads();
     if (threadIdx.x == 0)
-        P.nan[((int64_t)si * P.n_h + hi) * P.max_tiles + tile] = make_int4(first_nan[0], first_nan[1], first_nan[2], first_nan[3]);
-    if (kMod && threadIdx.x < 16) P.nan_bits[16 * (((int64_t)si * P.n_h + hi) * P.max_tiles + tile) + threadIdx.x] = all_nan[threadIdx.x];
+        P.nan[((int64_t)si * P.n_h + hi) * P.max_tiles + slot] = make_int4(first_nan[0], first_nan[1], first_nan[2], first_nan[3]);
+    if (kMod && threadIdx.x < 16) P.nan_bits[16 * (((int64_t)si * P.n_h + hi) * P.max_tiles + slot) + threadIdx.x] = all_nan[threadIdx.x];
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -572,12 +584,13 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
             asm volatile("fence.proxy.async.global;" ::: "memory");     // the tiles: another launch's stores -> bulk copies
             int n = 0;                                                  // parts so far
             for (Walk w(P); w.left > 0 && ok;) {
+                const int first_gap = kMod ? pf_gap(P, pf_seq<true>(P, P.seq0 + w.b.si)) : 0;
                 const uint8_t* src = P.tiles + (((int64_t)w.b.si * P.n_h + w.h) * P.max_tiles + (kMod ? 0 : w.t0)) * kPfTileBytes;
                 for (int k = 0; k < 2 * w.tiles; ++k, ++n) {
                     const int slot = n % kSlots;
                     if (n >= kSlots && !pf_wait(S, &S.empty[slot], (uint32_t)(n / kSlots - 1) & 1u)) { ok = false; break; }
                     mbar_arrive_expect_tx(&S.full[slot], kPart);
-                    const int part = kMod ? 2 * w.b.tile<kBack>(w.t0 + (k >> 1)) + (k & 1) : k;
+                    const int part = kMod ? 2 * w.b.slot<kBack>(w.t0 + (k >> 1), first_gap) + (k & 1) : k;
                     bulk_g2s(S.ring[slot], src + (size_t)part * kPart, kPart, &S.full[slot]);
                 }
                 if (!w.more()) break;
@@ -742,8 +755,9 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
             if (more && w8 == 0 && lane < 2)
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(&next.b) + 16 * lane),
                              "l"(reinterpret_cast<const uint8_t*>(P.blk + w.next_g()) + 16 * lane) : "memory");
+            const int first_gap = kMod ? pf_gap(P, pf_seq<true>(P, P.seq0 + w.b.si)) : 0;
             for (int t = tid & 255; t < tiles; t += 256) {
-                const int4 f = P.nan[((int64_t)w.b.si * P.n_h + w.h) * P.max_tiles + (kMod ? w.b.tile<kBack>(tile0 + t) : tile0 + t)];
+                const int4 f = P.nan[((int64_t)w.b.si * P.n_h + w.h) * P.max_tiles + (kMod ? w.b.slot<kBack>(tile0 + t, first_gap) : tile0 + t)];
                 if (min(min(f.x, f.y), min(f.z, f.w)) != INT_MAX) {
                     atomicMin(&S.nan[mb][0], f.x);
                     atomicMin(&S.nan[mb][1], f.y);
@@ -776,7 +790,7 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
             const float fac = kMode >= kCapped ? 1.f : sc;
             const bool even = __all_sync(0xffffffffu, S.ex[mb][r128] == 0);
             const uint8_t* const valid = P.valid + (int64_t)w.b.si * P.max_tiles + (kMod ? 0 : tile0);
-            auto place = [&](int i) { return kMod ? w.b.tile<kBack>(tile0 + i) : i; };              // of a tile among the sequence's valid[]
+            auto place = [&](int i) { return kMod ? w.b.slot<kBack>(tile0 + i, first_gap) : i; };   // of a tile among the sequence's valid[]
             uint32_t units = tiles > 0 ? valid[place(0)] : 0;
             float m_used = -INFINITY, lsum = 0.f;    // what this row scales by (log2), this half's denominator
             const float unit = kMode == kCapped ? pg_unit(sc, P.sc) : 0.f;
@@ -785,7 +799,7 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
             for (int i = 0; i < tiles; ++i) {
                 if (!__all_sync(0xffffffffu, pf_wait(S, &S.s_ready[mb], (uint32_t)(done + i) & 1u))) ok = false;
                 tc_fence_after_sync();
-                const int t0 = (kMod ? place(i) : tile0 + i) * kPfTileTok + 64 * hf;
+                const int t0 = (kMod ? w.b.tile<kBack>(tile0 + i) : tile0 + i) * kPfTileTok + 64 * hf;
                 const uint32_t there = units >> (4 * hf) & 15u;
                 if (i + 1 < tiles) units = valid[place(i + 1)];
                 // tiles that reach a row's limit, or lack a page
@@ -1011,10 +1025,9 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
             if (kMod && (bad0 || bad1)) {              // (the first may be hidden, and a later one not)
                 bad0 = bad1 = false;
                 for (int i = 0; i < tiles; ++i) {
-                    const int tile = place(i);
-                    const uint32_t* const bits = P.nan_bits + 16 * (((int64_t)w.b.si * P.n_h + w.h) * P.max_tiles + tile) + 8 * hf;
+                    const uint32_t* const bits = P.nan_bits + 16 * (((int64_t)w.b.si * P.n_h + w.h) * P.max_tiles + place(i)) + 8 * hf;
                     for (int k = 0; k < 4; ++k) {
-                        const int t = tile * kPfTileTok + 32 * k;
+                        const int t = w.b.tile<kBack>(tile0 + i) * kPfTileTok + 32 * k;
                         const uint32_t seen = bits_below(lim - t) & (~bits_below(lo - t) | bits_below(pre - t));
                         bad0 |= (bits[k] & seen) != 0;
                         bad1 |= (bits[4 + k] & seen) != 0;
@@ -1175,9 +1188,12 @@ __global__ void __launch_bounds__(256) pg_prefill_merge_kernel(const Pf P) {
 }  // namespace
 
 // Sequences and KV heads of one launch's workspace: all of them, or fewer sequences, then fewer heads, so that their tiles stay within 2 GiB.
-static void pf_parts(int n_seq, int n_kv, int64_t max_tokens, int& seqs, int& heads, int64_t& tiles) {
+// With a window, a sequence of n rows has no more than its prefix's tiles and those of n - 1 + window tokens from any place on.
+static void pf_parts(int n_seq, int n_tok, int n_kv, int64_t max_tokens, const PgScores* sc, int& seqs, int& heads, int64_t& tiles) {
     constexpr int64_t kMost = 2ll << 30;
-    tiles = (max_tokens + kPfTileTok - 1) / kPfTileTok;
+    auto whole = [](int64_t tokens) { return (tokens + kPfTileTok - 1) / kPfTileTok; };
+    tiles = whole(max_tokens);
+    if (sc && sc->window) tiles = std::min(tiles, whole(sc->prefix ? sc->max_prefix : 0) + whole((int64_t)n_tok - 1 + sc->window) + 1);
     if (tiles < 1) tiles = 1;
     const int64_t pairs = kMost / (tiles * kPfTileBytes);
     heads = (int)(pairs >= n_kv ? n_kv : pairs > 1 ? pairs : 1);
@@ -1208,11 +1224,11 @@ static PfLayout pf_layout(int seqs, int heads, int64_t tiles, int64_t blocks, in
     return L;
 }
 
-int64_t paged_prefill_workspace(int n_seq, int n_tok, int gqa, int n_kv, int64_t max_tokens, bool mod) {
+int64_t paged_prefill_workspace(int n_seq, int n_tok, int gqa, int n_kv, int64_t max_tokens, const PgScores* sc) {
     int seqs, heads;
     int64_t tiles;
-    pf_parts(n_seq, n_kv, max_tokens, seqs, heads, tiles);
-    return pf_layout(seqs, heads, tiles, (int64_t)n_tok * gqa / kBlockRows + n_seq, pf_ctas(), mod).total;
+    pf_parts(n_seq, n_tok, n_kv, max_tokens, sc, seqs, heads, tiles);
+    return pf_layout(seqs, heads, tiles, (int64_t)n_tok * gqa / kBlockRows + n_seq, pf_ctas(), sc != nullptr).total;
 }
 
 // What pf_shape takes from the launch's parameters.
@@ -1239,7 +1255,7 @@ static void pf_constants(Pf& P) {
 int paged_prefill(const PagedPrefill& A, cudaStream_t stream) {
     int seqs, heads;
     int64_t tiles;
-    pf_parts(A.n_seq, A.n_kv, A.max_tokens, seqs, heads, tiles);
+    pf_parts(A.n_seq, A.n_tok, A.n_kv, A.max_tokens, A.mod ? &A.sc : nullptr, seqs, heads, tiles);
     const int64_t blocks = (int64_t)A.n_tok * A.gqa / kBlockRows + A.n_seq;
     // (a launch's tiles are counted in 32 bits, rows to 2^29)
     if (2 * (double)blocks * (double)(tiles + 2) * heads > INT32_MAX || (int64_t)A.n_tok * A.gqa > 1 << 29) return BGTQ_E_TOOBIG;

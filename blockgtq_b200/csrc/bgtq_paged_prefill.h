@@ -27,7 +27,7 @@ struct PagedPrefill {
     bool mod;                       // scores differ from plain ones
     PgScores sc;
 };
-int64_t paged_prefill_workspace(int n_seq, int n_tok, int gqa, int n_kv, int64_t max_tokens, bool mod);
+int64_t paged_prefill_workspace(int n_seq, int n_tok, int gqa, int n_kv, int64_t max_tokens, const PgScores* sc);       // null: plain ones
 int paged_prefill(const PagedPrefill& A, cudaStream_t stream);
 
 }  // namespace bgtq

@@ -424,7 +424,7 @@ def paged_kv4_prefill_attention(q, pages, block_table, seq_lens, cu_q, max_q_len
     more is attended all the same).  ``max_seq_len``: sequences are held to it (default: what the table holds).  With many rows per sequence and KV head the
     tokens are unpacked into a workspace from torch's allocator, 512 bytes per token of ``max_seq_len`` and KV head for every sequence, at
     most 2 GiB at a time.  Rows behind ``cu_q[B]`` are not written.  Otherwise as :func:`paged_kv4_decode_attention`: distances and the ``window``
-    (``causal`` only) count from the row's own position, and tokens of the prefix are seen by the rows in front of them too, at the distance between them."""
+    (``causal`` only, and the workspace has room for what it and ``max_prefix_len`` reach) count from the row's own position, and tokens of the prefix are seen by the rows in front of them too, at the distance between them."""
     if cu_q is None:
         raise ValueError("cu_q says which rows are whose")
     if max_q_len is not None and max_q_len < 0:

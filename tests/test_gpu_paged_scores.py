@@ -338,6 +338,32 @@ def test_pages_that_no_row_sees_a_token_of(page, rows, rows_form):
             assert status.item() == 0 and torch.equal(got, want)
 
 
+@pytest.mark.parametrize("scores", ["window", "sinks", "all"])
+@pytest.mark.parametrize("longest", [None, 50])
+def test_a_window_far_into_long_sequences_needs_little_room(scores, longest, monkeypatch):
+    """The workspace holds the tiles of prefixes and windows, one behind the other: rows of sequences far longer, wherever their windows begin in a tile."""
+    from blockgtq_b200 import _lib, paged, paged_kv4_prefill_attention
+    monkeypatch.setattr(paged, "_FORM", 14)
+    gen = torch.Generator().manual_seed(53)
+    lens, counts = [9000, 4096, 130, 5003, 0, 6400], [70, 1, 130, 300, 3, 64]
+    pages, table, slots = _case(gen, 1, 64, lens)
+    q = _noise(gen, sum(counts), 4, 128).half()
+    call, of = _arguments(SCORES[scores], lens, 4, longest)
+    ends = [0]
+    for c in counts:
+        ends.append(ends[-1] + c)
+    status = torch.zeros(1, **I32)
+    out, lse = paged_kv4_prefill_attention(q.to(DEV), pages, table.to(DEV), torch.tensor(lens, **I32), torch.tensor(ends, **I32), return_lse=True, status=status, **call)
+    assert status.item() == 0
+    for b, c in enumerate(counts):
+        rows = sorted({0, c // 2, c - 1})
+        W.check(out, lse, S.attention(q[ends[b]:ends[b + 1]], pages, slots[b], rows=rows, **of(b)), [ends[b] + r for r in rows])
+    def room(window):
+        sc = _lib.PagedScores(None, None, 0.0, window, 0, 0)
+        return _lib.lib().bgtq_paged_scored_workspace_bytes(2, 512, 32, 8, 256, 131072, _lib.PAGED_CAUSAL | 14 << 8, sc)
+    assert room(4096) < room(0) / 10
+
+
 def test_a_captured_call_follows_lengths_prefixes_and_slopes(rows_form):
     from blockgtq_b200 import paged_kv4_prefill_attention
     gen = torch.Generator().manual_seed(41)
