@@ -651,6 +651,8 @@ class PagedKV4Cache:
         for src, _, _ in copies:
             self._held[src] -= 1
         del self._free[free:]
+        if self._copied is not None:        # (pages may have been moved on another stream; other streams wait at their first layer)
+            self._stream().wait_event(self._copied)
         self._step = {"slots": wide[0], "positions": wide[1], "table": table, "lens": small[:len(seqs)], "ends": small[len(seqs):],
                       "most_q": max(counts), "most": max(lens), "rows": len(slots), "seqs": frozenset(seqs),
                       "held": (wide, table, small), "streams": {self._stream()}}
