@@ -576,8 +576,10 @@ class PagedKV4Cache:
         self._held, self._free, self.n_pages, self._step = held, list(range(n_pages - 1, n - 1, -1)), n_pages, None
 
     def _copy(self, src, dst, **kw):
-        """Copies pages on the current stream, behind the layers of every stream; layers that follow on another one wait for it."""
+        """Copies pages on the current stream, behind the copies and the layers of every stream; steps and layers that follow on another one wait for it."""
         stream = self._stream()
+        if self._copied is not None:        # (and so the last copies' event stands for all of them)
+            stream.wait_event(self._copied)
         for other in self._busy:
             if other != stream:
                 stream.wait_stream(other)

@@ -1,4 +1,6 @@
 """CPU: what PagedKV4Cache's copies and layers are ordered behind, whatever streams they run on: streams that record it, and do nothing else."""
+import random
+
 import pytest
 import torch
 
@@ -93,3 +95,67 @@ def test_a_step_waits_once_on_each_stream(cache):
         c.layer()
         c.layer()
         assert len(waits) == i + 1
+
+
+def _behind_all(c):
+    """The last copy is ordered behind every copy and layer before it."""
+    assert c.done[-1][0] == "copy" and c.done[-1][1] == set(range(len(c.done) - 1))
+
+
+@pytest.mark.parametrize("second", ["compact", "resize", "step"])
+def test_copies_wait_for_copies_on_another_stream(cache, second):
+    """A step's copy of a shared page, or a compact, and before any layer runs a copy on another stream."""
+    c = cache
+    a, b = _two_sequences(c)
+    d = c.fork_sequence(b)
+    if second == "step":
+        c.free_sequence(a)
+        c.now = Stream()
+        c.compact()
+        c.now = Stream()
+        c.begin_step([d], [1])
+    else:
+        c.now = Stream()
+        c.begin_step([d], [1])
+        c.free_sequence(a)
+        c.now = Stream()
+        c.compact() if second == "compact" else c.resize(9)
+    assert len(c.numbers("copy")) == 2
+    _behind_all(c)
+    c.now = third = Stream()                            # the last copy's event stands for both
+    c.begin_step([b], [1])
+    assert c.numbers("copy") <= third.behind
+
+
+@pytest.mark.parametrize("seed", range(10))
+def test_any_order_of_streams(cache, seed):
+    """Copies behind all copies and layers before them, layers behind all copies."""
+    c, rng = cache, random.Random(seed)
+    streams, seqs = [Stream() for _ in range(4)], []
+    for _ in range(120):
+        c.now = rng.choice(streams)
+        kind = rng.choice(["add", "step", "step", "layer", "layer", "fork", "free", "compact", "resize"])
+        some = rng.sample(seqs, min(len(seqs), rng.randint(1, 3)))
+        before = len(c.done)
+        if kind == "add" or not some:
+            seqs.append(c.add_sequence())
+        elif kind == "step":
+            try:
+                c.begin_step(some, [rng.randint(1, 20) for _ in some])
+            except (RuntimeError, ValueError):
+                continue
+        elif kind == "layer" and c._step is not None:
+            c.layer()
+            assert c.numbers("copy") <= c.done[-1][1]
+        elif kind == "fork":
+            seqs.append(c.fork_sequence(some[0]))
+        elif kind == "free":
+            c.free_sequence(some[0])
+            seqs.remove(some[0])
+        elif kind == "compact":
+            c.compact()
+        elif kind == "resize":
+            c.resize(max(1, c.n_pages - c.free_pages, rng.randint(10, 25)))
+        if len(c.done) > before and c.done[-1][0] == "copy":
+            _behind_all(c)
+    assert len(c.numbers("copy")) > 3

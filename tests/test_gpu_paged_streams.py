@@ -68,3 +68,30 @@ def test_pages_moved_late_and_a_step_that_copies_nothing():
     p, seqs = _beginning(1)
     assert p.late(lambda c: c.compact()) == 7
     p.check(seqs, p.step(seqs, [1, 20]))
+
+
+def test_pages_moved_late_and_a_step_that_parts_a_fork():
+    p, seqs = _beginning(2)
+    fork = p.both(lambda c: c.fork_sequence(seqs[1]))
+    assert p.late(lambda c: c.compact()) == 7
+    p.check([*seqs, fork], p.step([*seqs, fork], [1, 3, 1]))
+
+
+@pytest.mark.parametrize("n_pages", [12, 60])
+def test_pages_moved_late_and_a_pool_resized(n_pages):
+    p, seqs = _beginning(3)
+    assert p.late(lambda c: c.compact()) == 7
+    p.moved.resize(n_pages)
+    p.check(seqs, p.step(seqs, [1, 1]))
+
+
+@pytest.mark.parametrize("move", ["compact", "resize"])
+def test_a_fork_parted_late_and_its_copy_moved(move):
+    """The step that copies the shared page is taken back before a layer runs; the copy moves on the main stream."""
+    p, seqs = _beginning(4)
+    fork = p.both(lambda c: c.fork_sequence(seqs[1]))
+    p.late(lambda c: c.begin_step([fork], [2]))
+    p.plain.begin_step([fork], [2])
+    p.both(lambda c: c.truncate_sequence(fork, 60))
+    p.moved.compact() if move == "compact" else p.moved.resize(9)
+    p.check([*seqs, fork], p.step([fork, *seqs], [1, 1, 1]))
