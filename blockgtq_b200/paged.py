@@ -61,11 +61,15 @@ def _rows(x, name, n, heads, dtype, device, align):
     return x
 
 
-def _ints(x, name, dtype, shape, device):
+def _is(x, name, dtype, shape, device):
     if x.dtype != dtype or tuple(x.shape) != shape:
         raise ValueError(f"{name} must be {dtype} {shape}, got {x.dtype} {tuple(x.shape)}")
     if x.device != device:
         raise ValueError(f"{name} is on {x.device}, the pages on {device}")
+
+
+def _ints(x, name, dtype, shape, device):
+    _is(x, name, dtype, shape, device)
     return x.contiguous()
 
 
@@ -678,9 +682,18 @@ class PagedKV4Cache:
             raise RuntimeError("a captured graph would go on reading this step's slots and lengths, which end with the step: capture "
                                "paged_kv4_append and the attentions over tensors of your own")
         scores = dict(softcap=softcap, slopes=slopes, window=window, prefix_lens=prefix_lens, max_prefix_len=max_prefix_len)
-        _limits(softcap, window, True)      # (nothing is stored for an attention that is refused)
-        if prefix_lens is not None and prefix_lens.shape != s["lens"].shape:
-            raise ValueError(f"prefix_lens must be ({len(s['lens'])},), one for each of the step's sequences, got {tuple(prefix_lens.shape)}")
+        # (nothing is stored for an attention that is refused)
+        _type_flag(q.dtype, "q")
+        if q.device != self.device:
+            raise ValueError(f"q is on {q.device}, the pages on {self.device}")
+        if softcap is not None or slopes is not None or window is not None or prefix_lens is not None:
+            _limits(softcap, window, True)
+            if slopes is not None:
+                _is(slopes, "slopes", torch.float32, (self.nq,), self.device)
+            if prefix_lens is not None:     # (one for each of the step's sequences)
+                _is(prefix_lens, "prefix_lens", torch.int32, tuple(s["lens"].shape), self.device)
+            if max_prefix_len is not None:
+                _most(operator.index(max_prefix_len), "max_prefix_len")
         stream = self._stream()
         if stream not in s["streams"]:      # (the next step's tensors must not take these tensors' memory before this stream is done with them)
             for t in s["held"]:
