@@ -35,7 +35,8 @@ def test_a_step_s_operations_do_not_go_with_its_pages():
         c = _cache(2000)
         seqs = [c.add_sequence() for _ in range(3)]
         c.begin_step(seqs, [tokens] * 3)
-        counts.append(_operations(lambda: c.begin_step(seqs, [1] * 3)))
+        # (the first call that is traced tells the interpreter to, and is not counted)
+        counts.append([_operations(lambda: c.begin_step(seqs, [1] * 3)) for _ in range(2)][1])
     assert counts[0] == counts[1] > 50
 
 
