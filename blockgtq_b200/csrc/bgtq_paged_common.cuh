@@ -87,6 +87,9 @@ inline PgMode pg_mode(const PgScores& S, bool mod) {
 // A sequence's prefix
 __device__ __forceinline__ int pg_prefix(const PgScores& S, int seq, int len) { return S.prefix ? max(0, min(S.prefix[seq], min(S.max_prefix, len))) : 0; }
 
+// A slope to the base of 2, finite where it is.
+__device__ __forceinline__ float pg_slope(float s) { return fmaxf(fminf(s * 1.44269504088896340736f, 3.402823466e38f), -3.402823466e38f); }
+
 __device__ __forceinline__ float pg_ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

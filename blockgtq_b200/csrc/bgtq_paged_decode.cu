@@ -362,7 +362,6 @@ struct Marks {
     float slope[NT][2];              // to the base of 2
     float unit[NT][2];               // the factor from sums to logits over the cap
     int pre;                         // tokens of the prefix
-    bool both_sides;                 // some column sees tokens behind its own place
 };
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 16 ? 0xffffu : (1u << n) - 1u; }
 // The tokens of a unit from t0 on that a column sees
@@ -389,7 +388,7 @@ __device__ __forceinline__ void pd_no_number_seen(State<NT>& st, float& s0, floa
 }
 
 // U units of 16 tokens at u in shared memory.  kEdge: some of them (tokens from len on of the sequence, from lim[] on of a column, kMod: between its
-// prefix and its window) are hidden.
+// prefix and its window) are hidden, or lie behind a column's own place.
 template <int NT, int U, bool kEdge, PgMode kMode>
 __device__ __forceinline__ void pd_units(const PdParams& P, const uint8_t* u, const Magic& mg, const Query<NT>& Q, State<NT>& st, int r, int c, int t0, int len, const int (&lim)[NT][2], const Marks<NT>& mk) {
     constexpr bool kMod = kMode != kPlain, kCap = kMode == kCapped || kMode == kCappedBiased, kBias = kMode >= kBiased, kShaped = kCap || kBias;
@@ -454,19 +453,21 @@ __device__ __forceinline__ void pd_units(const PdParams& P, const uint8_t* u, co
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const float slope = mk.slope[nt][e], d = (float)(t0 + r - mk.pos[nt][e]), first = slope * d;
+                        constexpr float kLast = 16.f * U - 8.f;         // from the lane's first token to its last
+                        const float slope = mk.slope[nt][e], d = (float)(t0 + r - mk.pos[nt][e]), last = slope * (d + kLast);
 #pragma unroll
                         for (int i = 0; i < U; ++i)
 #pragma unroll
                             for (int half = 0; half < 2; ++half) {
                                 float& x = s[i][nt][2 * half + e];
-                                x = f(x, kCap ? 1.f : Q.f[nt][e], slope, d, first, 16.f * i + 8.f * half);
+                                x = f(x, kCap ? 1.f : Q.f[nt][e], slope, d, 16.f * i + 8.f * half, last, 16.f * i + 8.f * half - kLast);
                             }
                     }
             };
-            // (on one side, the slope times whole numbers below 32 is on top of the first token's bias)
-            if (mk.both_sides) each([](float x, float f, float slope, float d, float, float on) { return fmaf(-slope, fabsf(d + on), x * f); });
-            else each([](float x, float f, float slope, float, float first, float on) { return fmaf(x, f, fmaf(slope, on, first)); });
+            // (in front of the columns' places, the slope times whole numbers below 32 is on top of the bias of the lane's nearest token, whose rounding is no
+            // more than the others' own: two instructions for a logit instead of three.  From the farthest on, a column's own token had a bias, its rounding.)
+            if (kEdge) each([](float x, float f, float slope, float d, float on, float, float) { return fmaf(-slope, fabsf(d + on), x * f); });
+            else each([](float x, float f, float slope, float, float, float last, float back) { return fmaf(x, f, fmaf(slope, back, last)); });
         }
         if (kEdge)
 #pragma unroll
@@ -558,7 +559,7 @@ __device__ __forceinline__ void pd_units(const PdParams& P, const uint8_t* u, co
             float p[4];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const float z = kEdge && st.m[nt][e] == -INFINITY ? 0.f : st.m[nt][e];
+                const float z = (kEdge || kBias) && st.m[nt][e] == -INFINITY ? 0.f : st.m[nt][e];          // (kBias: a bias may be beyond fp32)
                 // (product and difference rounded apart, as the references were: fused, logits beyond 2^26 differ from theirs by more than a weight's range)
                 p[e] = ex2((kShaped ? s[i][nt][e] : __fmul_rn(s[i][nt][e], Q.f[nt][e])) - z);
                 p[2 + e] = ex2((kShaped ? s[i][nt][2 + e] : __fmul_rn(s[i][nt][2 + e], Q.f[nt][e])) - z);
@@ -757,12 +758,12 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
                 const int row = row0 + 8 * nt + 2 * c + e;
                 lim[nt][e] = P.causal && row < n_rows ? max(kMod ? g.s.pre : 0, behind + row / P.gqa) : g.s.len;
             }
-        const int lim_min = P.causal ? max(kMod ? g.s.pre : 0, behind + row0 / P.gqa) : g.s.len;
+        int lim_min = P.causal ? max(kMod ? g.s.pre : 0, behind + row0 / P.gqa) : g.s.len;
+        if (kMode >= kBiased) lim_min = min(lim_min, behind + row0 / P.gqa);         // (nor is a token in front of it behind a column's place)
         Marks<NT> mk;
         int lo_max = 0;                                      // the last of the columns' windows begins here
         if (kMod) {
             mk.pre = g.s.pre;
-            bool behind_it = false;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -771,10 +772,8 @@ __global__ void __launch_bounds__(kPdThreads, NT == 1 ? 2 : 1) pg_attend_kernel(
                     mk.pos[nt][e] = behind + at - 1;
                     mk.lo[nt][e] = P.sc.window ? max(0, max(0, behind + at) - P.sc.window) : 0;
                     mk.unit[nt][e] = pg_unit(Q.f[nt][e], P.sc);
-                    behind_it |= lim[nt][e] > mk.pos[nt][e] + 1;
-                    mk.slope[nt][e] = kMode >= kBiased && row < n_rows ? P.sc.slopes[g.h * P.gqa + row - at * P.gqa] * 1.44269504088896340736f : 0.f;
+                    mk.slope[nt][e] = kMode >= kBiased && row < n_rows ? pg_slope(P.sc.slopes[g.h * P.gqa + row - at * P.gqa]) : 0.f;
                 }
-            mk.both_sides = __any_sync(0xffffffffu, behind_it);
             if (P.sc.window) lo_max = max(0, max(0, behind + (min(row0 + kCols, n_rows) - 1) / P.gqa) - P.sc.window);
         }
         State<NT> st = {};

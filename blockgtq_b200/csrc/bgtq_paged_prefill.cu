@@ -89,7 +89,7 @@ struct Pf {
     float* lse;
     int32_t* status;
     PgScores sc;                                // (kernels of kMod read it)
-    uint64_t low[4], mid[9], steps[16];        // the cap's polynomials (of products, of u), each coefficient twice; 0, 1 .. 31
+    uint64_t low[4], mid[9], steps[16];        // the cap's polynomials (of products, of u), each coefficient twice; -31, -30 .. 0
     float low_reach2;                           // largest product's square that the first is for
     uint32_t* nan_bits;                         // kMod: (n_seq, n_h, max_tiles) x 4 groups x 128 tokens: those whose V is no number
 };
@@ -418,16 +418,17 @@ __device__ __forceinline__ float abs_top(const float (&x)[32]) {
     return fmaxf(a, b);
 }
 // 32 products x[], in tensor memory at `from`, to logits: times factor (even: the one that P.low is made for), capped (alike: by pg_cap_any, as the row's
-// reference was), and less slope times the distances, of which the first is `ahead` of the row's own place (both_sides: some lie behind it).
+// reference was), and less slope times the distances, of which the first is `ahead` of the row's own place (apart: each by itself, as
+// some lie behind it).
 template <bool kCap, bool kBias>
-__device__ __forceinline__ void pf_shape(float (&x)[32], const Pf& P, float factor, bool even, bool alike, float slope, float ahead, bool both_sides, uint32_t from) {
+__device__ __forceinline__ void pf_shape(float (&x)[32], const Pf& P, float factor, bool even, bool alike, float slope, float ahead, bool apart, uint32_t from) {
     auto load = [&]() {
         tmem_ld32(from, x);
         tmem_ld_wait();
     };
-    const float t0 = slope * ahead;
-    const uint64_t t2 = pack_f2(t0, t0), s2 = pack_f2(slope, slope);
-    // (slopes times whole numbers below 32, on top of the first's)
+    const float t31 = slope * (ahead + 31.f);
+    const uint64_t t2 = pack_f2(t31, t31), s2 = pack_f2(slope, slope);
+    // (slopes times whole numbers below 32, on top of the nearest token's, the last: its rounding is no more than the others' own)
     auto bias = [&](int c) { return fma_f2(s2, P.steps[c >> 1], t2); };
     if (kCap) {
         bool done = false;
@@ -439,10 +440,10 @@ __device__ __forceinline__ void pf_shape(float (&x)[32], const Pf& P, float fact
                 float v0, v1;
                 unpack_f2(v, v0, v1);
                 most[c >> 1 & 1] = max3(most[c >> 1 & 1], v0, v1);
-                unpack_f2(kBias && !both_sides ? fma_f2(r, p, bias(c)) : mul_f2(r, p), x[c], x[c + 1]);
+                unpack_f2(kBias && !apart ? fma_f2(r, p, bias(c)) : mul_f2(r, p), x[c], x[c + 1]);
             }
             done = __all_sync(0xffffffffu, fmaxf(most[0], most[1]) <= P.low_reach2);
-            if (done && (!kBias || !both_sides)) return;
+            if (done && (!kBias || !apart)) return;
             if (!done) load();
         }
         if (!done) {
@@ -469,7 +470,7 @@ __device__ __forceinline__ void pf_shape(float (&x)[32], const Pf& P, float fact
     if (kBias) {
         const float f = kCap ? 1.f : factor;
         const uint64_t f2 = pack_f2(f, f);
-        if (both_sides) {
+        if (apart) {
 #pragma unroll
             for (int c = 0; c < 32; ++c) x[c] = fmaf(-slope, fabsf(ahead + (float)c), x[c] * f);
         } else {
@@ -780,7 +781,7 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
                     lo = pf_window(P, s, pos);
                     at = w.b.len - w.b.n + pos;
                     const int g_pos = pf_pos(P, g);
-                    if (P.sc.slopes) slope = P.sc.slopes[(P.h0 + w.h) * P.gqa + g - g_pos * P.gqa] * 1.44269504088896340736f;
+                    if (P.sc.slopes) slope = pg_slope(P.sc.slopes[(P.h0 + w.h) * P.gqa + g - g_pos * P.gqa]);
                 }
             }
             float down0, down1;
@@ -850,9 +851,10 @@ __global__ void __launch_bounds__(kThreads, 1) pg_prefill_kernel(const Pf P) {
 #pragma unroll 1
                     for (int c0 = 32; c0 >= 0; c0 -= 32) {
                         load(c0);
-                        // (tokens behind the row's own place are in its sight only where it lies in the prefix, or sees all)
-                        pf_shape<kMode == kCappedBiased, true>(sv, P, sc, even, false, slope, (float)(t0 + c0 - at),
-                                                               __any_sync(0xffffffffu, lim > at + 1 && t0 + c0 + 31 > at), sS + (uint32_t)c0);
+                        // (tokens behind a row's own place are in its sight only where it lies in the prefix, or sees all; its own one has no bias)
+                        const int first = t0 + c0 - at;
+                        pf_shape<kMode == kCappedBiased, true>(sv, P, sc, even, false, slope, (float)first,
+                                                               __any_sync(0xffffffffu, first + 31 > 0 && (first <= 0 || lim > at + 1)), sS + (uint32_t)c0);
                         if (cut) hide(c0);
                         m_half = fmaxf(m_half, top());
                         if (c0) tmem_st32(sS + 32u, sv);
@@ -1239,7 +1241,7 @@ static void pf_constants(Pf& P) {
         memcpy(&bits, f, 8);
         return bits;
     };
-    for (int i = 0; i < 16; ++i) P.steps[i] = pair(2 * i, 2 * i + 1);
+    for (int i = 0; i < 16; ++i) P.steps[i] = pair(2 * i - 31, 2 * i - 30);
     for (int i = 0; i < kMidTerms; ++i) P.mid[i] = pair(kCapMid[i] * P.sc.cap, kCapMid[i] * P.sc.cap);
     // u = product * g; where fp32 has no normal numbers for the coefficients, the polynomial is for no product
     const double factor = P.scale_log2 == 0.f ? 1.0 : fabs((double)P.scale_log2), g = factor * P.sc.cap_inv;

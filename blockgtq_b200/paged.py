@@ -410,8 +410,8 @@ def paged_kv4_decode_attention(q, pages, block_table, seq_lens, scale=None, retu
     a small one spares the launch what only long sequences need.  ``out``: where the result goes, like q, its rows apart from one
     another and from q's (other columns of one buffer will do).
 
-    Layers that are no plain attention: ``softcap`` c: a logit x becomes c tanh(x / c).  ``slopes`` (n_q,) fp32, finite: less slope times the distance between
-    the query's position (the sequence's last) and the token's.  ``window``: of the tokens up to the query's own only the last so many are seen.
+    Layers that are no plain attention: ``softcap`` c: a logit x becomes c tanh(x / c).  ``slopes`` (n_q,) fp32, finite (negative ones times any
+    distance, too): less slope times the distance between the query's position (the sequence's last) and the token's.  ``window``: of the tokens up to the query's own only the last so many are seen.
     ``prefix_lens`` (B,) int32: a sequence's first so many tokens are seen in any case (sinks in front of a window); ``max_prefix_len``: they are held
     to it (default: ``max_seq_len``), and with a window it chooses the launch.  Pages that no query sees are not read."""
     return _attend(q, pages, block_table, seq_lens, None, 1, _most(max_seq_len), True, scale, return_lse, status, out, softcap, slopes, window, prefix_lens,

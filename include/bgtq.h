@@ -694,7 +694,7 @@ int bgtq_paged_attend(const void* q, int64_t q_st, int64_t q_sh, const uint8_t* 
  * t < prefix[b], or if t <= p (any t without BGTQ_PAGED_CAUSAL) and t > p - window.  Rows that see none: zeros, lse -inf, as ever.  Pages of
  * which no row's window or prefix reaches a token are not looked up: their numbers in the table may be none. */
 typedef struct BgtqPagedScores {
-    const float* slopes;        /* device, (n_q), finite; NULL: no bias */
+    const float* slopes;        /* device, (n_q), finite, negative ones times any distance too; NULL: no bias */
     const int32_t* prefix;      /* device, (n_seq), held to 0 .. max_prefix; NULL: none */
     float softcap;              /* c, 2^-64 .. 2^64; 0: no cap */
     int32_t window;             /* tokens up to the row's own that it sees; 0: all.  Queries are causal then */
