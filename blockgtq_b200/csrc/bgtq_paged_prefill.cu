@@ -22,8 +22,8 @@
 //
 // Scores that are not plain (PgScores; PgMode: a kernel for each combination).  Masks: a block's tiles are those of its sequence's prefix and those from its
 // first row's window on, and only the tiles that cut a row's sight are masked, by 32 bits per row and half.  Caps and biases are made of the products by
-// the softmax's threads, and add to the chain what they take: 8192 positions as above 504 us plain, 602 with slopes, 700 with a cap that logits stay within
-// 3/8 of, 930 within 7/5, 2060 beyond; with a window of 2048 295, 324 and, by the logits' size, 356 to 390.  The threads issue half of the cycles then, and no pipe is
+// the softmax's threads, and add to the chain what they take: 8192 positions as above 504 us plain, 609 with slopes, 677 to 692 with a cap that logits stay
+// within 3/8 of, 875 to 996 within 7/5, 2118 beyond, with both 944, 1490 and 2245; with a window of 2048 295, 326, 363 to 373, 475 to 521 and 1024, 480, 740 and 1073.  The threads issue half of the cycles then, and no pipe is
 // busy for more than 42 %: two row blocks of two warps per scheduler each are too few to hide the latencies, and tensor memory holds no third.
 // Every wait is bounded: one that gives up is recorded in shared memory, where the others see it, and in the caller's status word; the CTA then
 // drains its copies and products, releases its tensor memory and returns.

@@ -411,9 +411,11 @@ def paged_kv4_decode_attention(q, pages, block_table, seq_lens, scale=None, retu
     another and from q's (other columns of one buffer will do).
 
     Layers that are no plain attention: ``softcap`` c: a logit x becomes c tanh(x / c).  ``slopes`` (n_q,) fp32, finite (negative ones times any
-    distance, too): less slope times the distance between the query's position (the sequence's last) and the token's.  ``window``: of the tokens up to the query's own only the last so many are seen.
+    distance, too): less slope times the distance between the query's position (the sequence's last) and the token's.  ``window``: of the tokens up to the
+    query's own only the last so many are seen.
     ``prefix_lens`` (B,) int32: a sequence's first so many tokens are seen in any case (sinks in front of a window); ``max_prefix_len``: they are held
-    to it (default: ``max_seq_len``), and with a window it chooses the launch.  Pages that no query sees are not read."""
+    to it (default: ``max_seq_len``), and with a window it chooses the launch: pass it with sinks, or the call is launched as if there were no window.  Pages that
+    no query sees are not read."""
     return _attend(q, pages, block_table, seq_lens, None, 1, _most(max_seq_len), True, scale, return_lse, status, out, softcap, slopes, window, prefix_lens,
                    max_prefix_len)
 
@@ -427,8 +429,9 @@ def paged_kv4_prefill_attention(q, pages, block_table, seq_lens, cu_q, max_q_len
     ``max_q_len``: no sequence has more query rows (default: all of them; it chooses the launch, 0 the one of 1, and one that has
     more is attended all the same).  ``max_seq_len``: sequences are held to it (default: what the table holds).  With many rows per sequence and KV head the
     tokens are unpacked into a workspace from torch's allocator, 512 bytes per token of ``max_seq_len`` and KV head for every sequence, at
-    most 2 GiB at a time.  Rows behind ``cu_q[B]`` are not written.  Otherwise as :func:`paged_kv4_decode_attention`: distances and the ``window``
-    (``causal`` only, and the workspace has room for what it and ``max_prefix_len`` reach) count from the row's own position, and tokens of the prefix are seen by the rows in front of them too, at the distance between them."""
+    most 2 GiB at a time (with a ``window`` for every sequence ``max_prefix_len`` tokens and what the windows of all the call's rows together reach, where that
+    is less).  Rows behind ``cu_q[B]`` are not written.  Otherwise as :func:`paged_kv4_decode_attention`: distances and the ``window`` (``causal`` only)
+    count from the row's own position, and tokens of the prefix are seen by the rows in front of them too, at the distance between them."""
     if cu_q is None:
         raise ValueError("cu_q says which rows are whose")
     if max_q_len is not None and max_q_len < 0:
@@ -455,7 +458,10 @@ class PagedKV4Cache:
     (slots, positions, block table, lengths) is uploaded once and is the same for every layer.
 
     Sequences may share pages: :meth:`fork_sequence` makes one that begins with another's tokens and copies nothing.  A shared page is copied, in all
-    layers, by the step that would write into it (on the stream of :meth:`begin_step`), and goes back to the pool with the last sequence that holds it."""
+    layers, by the step that would write into it (on the stream of :meth:`begin_step`), and goes back to the pool with the last sequence that holds it.
+
+    Copies wait for the layers of all streams, and steps and layers for the copies, whatever streams they are on.  Layers on several streams are the caller's to
+    order otherwise, also where a page that one sequence gave back is another's next."""
 
     def __init__(self, n_layers, n_q_heads, n_kv_heads, head_dim=HD, *, n_pages, max_seq_len, page_size=64, device="cuda"):
         if head_dim != HD:
