@@ -87,8 +87,11 @@ inline PgMode pg_mode(const PgScores& S, bool mod) {
 // A sequence's prefix
 __device__ __forceinline__ int pg_prefix(const PgScores& S, int seq, int len) { return S.prefix ? max(0, min(S.prefix[seq], min(S.max_prefix, len))) : 0; }
 
-// A slope to the base of 2, finite where it is.
-__device__ __forceinline__ float pg_slope(float s) { return fmaxf(fminf(s * 1.44269504088896340736f, 3.402823466e38f), -3.402823466e38f); }
+// A slope to the base of 2, finite where it is (and none where it is none).
+__device__ __forceinline__ float pg_slope(float s) {
+    const float x = s * 1.44269504088896340736f;
+    return fabsf(x) > 3.402823466e38f ? copysignf(3.402823466e38f, x) : x;
+}
 
 __device__ __forceinline__ float pg_ex2(float x) {
     float y;

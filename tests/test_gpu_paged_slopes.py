@@ -69,3 +69,13 @@ def test_a_slope_beside_which_nothing_counts(dtype, cap, t, n, form):
     assert ((lse.double().cpu() - y).abs() <= off).all(), (lse.double().cpu() - y).abs().amax(0)
     want = v[own][:, None].expand(-1, 8, -1)
     assert ((out.double().cpu() - want).abs() <= (torch.finfo(dtype).eps / 2 + 2.0 ** -20) * want.abs() + 2.0 ** -25).all()
+
+
+def test_a_slope_that_is_no_number_shows_in_its_head_only(form):
+    gen = torch.Generator().manual_seed(5)
+    pages, table, slots = _pool(gen, 150)
+    q = torch.randn(20, 8, 128, generator=gen).half()
+    slopes = torch.tensor([0.5, math.nan, 0.25, 0.1, 0.0, 1.0, math.nan, 2.0])
+    out, lse = _attend(q, pages, table, 150, slopes=slopes.to(DEV))
+    bad = slopes.isnan().to(DEV)
+    assert out[:, bad].isnan().all() and not out[:, ~bad].isnan().any() and torch.isfinite(lse[:, ~bad]).all()
