@@ -87,10 +87,12 @@ inline PgMode pg_mode(const PgScores& S, bool mod) {
 // A sequence's prefix
 __device__ __forceinline__ int pg_prefix(const PgScores& S, int seq, int len) { return S.prefix ? max(0, min(S.prefix[seq], min(S.max_prefix, len))) : 0; }
 
-// A slope to the base of 2, finite where it is (and none where it is none).
+// A slope to the base of 2: finite where it is positive and finite, so that a row's own token has no bias; none where it is none.  (One instruction: a comparison and
+// a choice for both signs cost 64 ragged sequences 85.7 us instead of 85.1.)
 __device__ __forceinline__ float pg_slope(float s) {
-    const float x = s * 1.44269504088896340736f;
-    return fabsf(x) > 3.402823466e38f ? copysignf(3.402823466e38f, x) : x;
+    float x;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(x) : "f"(s * 1.44269504088896340736f), "f"(3.402823466e38f));
+    return x;
 }
 
 __device__ __forceinline__ float pg_ex2(float x) {

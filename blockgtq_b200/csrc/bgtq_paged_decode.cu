@@ -33,8 +33,8 @@
 // Scores that are not plain (PgScores), each combination a kernel of its own (PgMode): logits are finished between their product and the reference.  A window
 // leaves its batches out of the list, or of the cluster's shares: what is between a sequence's prefix and the window of its first row has no place
 // there (8 sequences of 32768 tokens x 2 KV heads, the last 4096 of each and 4 in front: 11.5 us, 11.2 for sequences of 4096 tokens).  A cap costs 5 to 7 %
-// (one sequence of 131072: 43.4 us beside 40.7; 46.3 where logits lie beyond half of the cap), slopes 3 % (64 of up to 9100: 95.4 beside 92.3; from the front
-// to the end, with references that move at every step, 100.4), both 9 %.
+// (one sequence of 131072: 43.4 us beside 40.7; 46.3 where logits lie beyond half of the cap), slopes 3 % (64 of up to 9100: 85.1 beside 82.3; from the front
+// to the end, with references that move at every step, 5 % more), both 11 %.
 //
 // In a CTA eight warps take batches in turn, each with a ring of bulk copies of its own (the next triple's first ones travel while this
 // one's states are merged in shared memory).
@@ -453,21 +453,21 @@ __device__ __forceinline__ void pd_units(const PdParams& P, const uint8_t* u, co
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        constexpr float kLast = 16.f * U - 8.f;         // from the lane's first token to its last
-                        const float slope = mk.slope[nt][e], d = (float)(t0 + r - mk.pos[nt][e]), last = slope * (d + kLast);
+                        constexpr int kLast = 16 * U - 8;               // from the lane's first token to its last
+                        const float slope = mk.slope[nt][e], d = (float)(t0 + r + kLast - mk.pos[nt][e]), last = slope * d;
 #pragma unroll
                         for (int i = 0; i < U; ++i)
 #pragma unroll
                             for (int half = 0; half < 2; ++half) {
                                 float& x = s[i][nt][2 * half + e];
-                                x = f(x, kCap ? 1.f : Q.f[nt][e], slope, d, 16.f * i + 8.f * half, last, 16.f * i + 8.f * half - kLast);
+                                x = f(x, kCap ? 1.f : Q.f[nt][e], slope, d, last, 16.f * i + 8.f * half - kLast);
                             }
                     }
             };
             // (in front of the columns' places, the slope times whole numbers below 32 is on top of the bias of the lane's nearest token, whose rounding is no
             // more than the others' own: two instructions for a logit instead of three.  From the farthest on, a column's own token had a bias, its rounding.)
-            if (kEdge) each([](float x, float f, float slope, float d, float on, float, float) { return fmaf(-slope, fabsf(d + on), x * f); });
-            else each([](float x, float f, float slope, float, float, float last, float back) { return fmaf(x, f, fmaf(slope, back, last)); });
+            if (kEdge) each([](float x, float f, float slope, float d, float, float back) { return fmaf(-slope, fabsf(d + back), x * f); });
+            else each([](float x, float f, float slope, float, float last, float back) { return fmaf(x, f, fmaf(slope, back, last)); });
         }
         if (kEdge)
 #pragma unroll
@@ -559,7 +559,8 @@ __device__ __forceinline__ void pd_units(const PdParams& P, const uint8_t* u, co
             float p[4];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const float z = (kEdge || kBias) && st.m[nt][e] == -INFINITY ? 0.f : st.m[nt][e];          // (kBias: a bias may be beyond fp32)
+                // (kBias: a unit's biases may all be beyond fp32)
+                const float z = kBias ? fmaxf(st.m[nt][e], -3.402823466e38f) : kEdge && st.m[nt][e] == -INFINITY ? 0.f : st.m[nt][e];
                 // (product and difference rounded apart, as the references were: fused, logits beyond 2^26 differ from theirs by more than a weight's range)
                 p[e] = ex2((kShaped ? s[i][nt][e] : __fmul_rn(s[i][nt][e], Q.f[nt][e])) - z);
                 p[2 + e] = ex2((kShaped ? s[i][nt][2 + e] : __fmul_rn(s[i][nt][2 + e], Q.f[nt][e])) - z);
